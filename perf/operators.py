@@ -1,0 +1,399 @@
+"""The paged K/V cache operators, as they are measured: their cases, plain forms and sizes.
+
+A paged cache keeps the K and V rows of many sequences in one pool of pages; a table names each sequence's pages.
+Three entry points (include/gpu.h) work on it, over a ragged batch in which sequence s brings rows starts[s]..starts[s+1]
+and has lengths[s] rows in all, the new ones last:
+
+  gpu_paged_append     rounds new FP32 K and V rows to what the pool holds (BF16, or the byte codec: int8 and a scale a row)
+  gpu_paged_read       gives those rows back as the FP32 values they stand for
+  gpu_paged_attention  grouped-query attention of the new rows' queries over the cached rows: causal, with an optional
+                       sliding window and a few first rows that stay visible
+
+With `own` false, run() computes them by elementary torch operations, else by the library's kernels.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+BF16, BYTES = 2, 3  # TcmPagedCache.kind
+
+
+def _case(name, op, kind, heads, page, seqs, new, length, window=0, sinks=0, layout=1):
+    """heads: (query heads, KV heads, head size); new, length: the smallest and largest of a sequence."""
+    return {"name": name, "op": op, "kind": kind, "qheads": heads[0], "kvheads": heads[1], "dim": heads[2], "page": page,
+            "seqs": seqs, "new_min": new[0], "new_max": new[1], "len_min": length[0], "len_max": length[1],
+            "window": window, "sinks": sinks, "layout": layout}
+
+
+def listed():
+    qwen = (12, 2, 128)  # this repository's decoder
+    return [
+        # One chat session decoding: the smallest call, append and attention of one token.
+        _case("step 1x300 bytes", "step", BYTES, qwen, 16, 1, (1, 1), (300, 300)),
+        # The batched decoder's workload: 64 sessions of 128 to 8192 rows, one token each, append and attention.
+        _case("step 64x8192 bytes", "step", BYTES, qwen, 64, 64, (1, 1), (128, 8192), layout=2),
+        # Long documents in BF16, one token each.
+        _case("decode 16x32768 bf16", "attend", BF16, qwen, 128, 16, (1, 1), (20000, 32768), layout=3),
+        # One long session alone: few rows of work, split over its length.
+        _case("decode 1x32749 bytes", "attend", BYTES, qwen, 64, 1, (1, 1), (32749, 32749)),
+        # The bounded profile's shape (64 first rows, 1024 recent ones) for sessions that ran long.
+        _case("decode 64 window bf16", "attend", BF16, qwen, 64, 64, (1, 1), (700, 32768), 1024, 64, layout=4),
+        # A drafted continuation being verified: five tokens a sequence, four query heads a KV head.
+        _case("verify 32x5 bf16", "attend", BF16, (32, 8, 128), 32, 32, (5, 5), (900, 4100), layout=5),
+        # A prompt's next chunk over what is cached already.
+        _case("chunk 512 on 4609 bytes", "attend", BYTES, qwen, 64, 1, (512, 512), (4609, 4609)),
+        # A mixed serving batch: odd chunks of many sizes, small heads of their own K and V, window and first rows.
+        _case("mixed 24 window bf16", "attend", BF16, (8, 8, 64), 48, 24, (1, 1500), (40, 6000), 2000, 4, layout=6),
+        # The largest: a long prompt's last chunk.
+        _case("chunk 4096 on 32768 bytes", "attend", BYTES, qwen, 128, 1, (4096, 4096), (32768, 32768)),
+        # One token's rows for each of 64 sessions, written and read back.
+        _case("store 64x1 bytes", "store", BYTES, qwen, 64, 64, (1, 1), (128, 8192), layout=2),
+        # Prompt chunks written and read back.
+        _case("store 16x2048 bytes", "store", BYTES, qwen, 64, 16, (1000, 2048), (1000, 8192), layout=7),
+        # Whole sequences read back (a session moved out of the pool).
+        _case("read 8x16384 bf16", "read", BF16, qwen, 128, 8, (9000, 16384), (1, 1), layout=8),
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number of [lo, hi], spread over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 0.49)))))))
+
+
+def draw(rng):
+    while True:
+        op = rng.choice(["step", "attend", "attend", "attend", "attend", "store", "store", "read"])
+        heads = rng.choice([(12, 2, 128), (12, 2, 128), (32, 8, 128), (8, 1, 128), (4, 4, 128), (8, 8, 64), (10, 2, 64), (14, 2, 64)])
+        seqs = _spread(rng, 1, 64)
+        if op == "step":
+            new = (1, 1)
+        elif op == "attend":
+            top = rng.choice([1, 1, _spread(rng, 2, 16), _spread(rng, 17, 4096)])
+            new = (rng.choice([1, top]), top)
+        else:
+            new = (1, _spread(rng, 1, 16384 if op == "read" else 4096))
+        top = _spread(rng, max(new[1], 2), 32768)
+        c = _case("", op, rng.choice([BF16, BYTES]), heads, rng.choice([16, 24, 32, 48, 64, 100, 128, 256]), seqs, new,
+                  (_spread(rng, 1, top), top), layout=rng.randrange(1 << 20))
+        if op in ("step", "attend") and rng.random() < 0.4:
+            c["window"], c["sinks"] = _spread(rng, 1, 8192), rng.choice([0, 1, 4, 64, 100])
+        del c["name"]
+        news, lengths = _extents(c)
+        rows, w = int(lengths.sum()), work(c)
+        # No dearer than the largest listed case, and within what the plain form's padding can hold.
+        padded = seqs * int(news.max()) * _width(c, news, lengths) * c["qheads"]
+        if w["flops"] < 7e11 and rows * heads[1] * heads[2] < 4e8 and padded < 1.6e9 and seqs * _width(c, news, lengths) * heads[1] * heads[2] < 1.2e9:
+            return c
+
+
+def _extents(c):
+    """Each sequence's new rows and its length, from the case alone."""
+    rng = random.Random(c["layout"])
+    news = [_spread(rng, c["new_min"], c["new_max"]) for _ in range(c["seqs"])]
+    news[rng.randrange(c["seqs"])] = c["new_max"]
+    lengths = [max(n, _spread(rng, c["len_min"], c["len_max"])) for n in news]
+    return np.array(news), np.array(lengths)
+
+
+def _width(c, news, lengths):
+    """Columns of the plain form's padded scores."""
+    if not c["window"]:
+        return int(lengths.max())
+    return min(int(lengths.max()), c["sinks"] + c["window"] + int(news.max()) - 1)
+
+
+def work(case):
+    news, lengths = _extents(case)
+    kv, d, window, sinks = case["kvheads"], case["dim"], case["window"], case["sinks"]
+    row = kv * (2 * d * 2 if case["kind"] == BF16 else 2 * (d + 4))  # a cached row's bytes, K and V
+    values = kv * d * 2 * 4
+    rows = int(news.sum())
+    if case["op"] == "store":
+        return {"bytes": rows * (2 * values + row), "flops": 0}
+    if case["op"] == "read":
+        return {"bytes": rows * (values + row), "flops": 0}
+    pairs = seen = 0
+    for n, length in zip(news.tolist(), lengths.tolist()):
+        pos = np.arange(length - n, length)
+        if window:
+            low = np.maximum(pos - window + 1, 0)
+            pairs += int((pos - low + 1).sum() + np.minimum(low, sinks).sum())
+            seen += length - int(low[0]) + min(int(low[0]), sinks)
+        else:
+            pairs += int((pos + 1).sum())
+            seen += length
+    b = seen * row + rows * case["qheads"] * d * 8
+    if case["op"] == "step":
+        b += rows * (values + row)
+    return {"bytes": b, "flops": 4 * d * case["qheads"] * pairs}
+
+
+def prepare(case, seed):
+    c = dict(case)
+    news, lengths = _extents(c)
+    seqs, page, kv, d, qh = c["seqs"], c["page"], c["kvheads"], c["dim"], c["qheads"]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    need = -(-lengths // page)
+    pages = int(need.sum()) + max(2, int(need.sum()) // 16)
+    stride = int(need.max()) + 1
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((seqs, stride), -1, dtype=torch.int32)
+    own_page = torch.zeros(seqs, stride, dtype=torch.bool)
+    for s in range(seqs):
+        own_page[s, :int(need[s])] = True
+    table, own_page = table.cuda(), own_page.cuda()
+    table[own_page] = order[:int(need.sum())]
+    starts = np.concatenate([[0], np.cumsum(news)])
+    st = {
+        "case": c, "pages": pages, "rows": int(starts[-1]), "max_new": int(news.max()), "max_length": int(lengths.max()),
+        "starts": torch.tensor(starts, dtype=torch.int32, device="cuda"),
+        "lengths": torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+        "table": table, "stride": stride, "status": torch.zeros(1, dtype=torch.int32, device="cuda"),
+    }
+    shape = (pages, kv, page, d)
+    rand = lambda *size: torch.randn(*size, generator=g, device="cuda")  # noqa: E731
+    if c["op"] == "store":  # the pool starts empty
+        pool = [torch.zeros(shape, dtype=torch.int8 if c["kind"] == BYTES else torch.bfloat16, device="cuda") for _ in range(2)]
+        scales = torch.zeros(2, pages, kv, page, device="cuda")
+    elif c["kind"] == BYTES:  # rows of unlike size, as keys and values are
+        pool = [torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2)]
+        for t in pool:
+            for a in range(0, pages, 4096):
+                t[a:a + 4096] = (rand(min(4096, pages - a), *shape[1:]) * 40).round_().clamp_(-127, 127).to(torch.int8)
+        scales = torch.exp(rand(2, pages, kv, page) * 0.3) * 0.025
+    else:
+        pool = [torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        for t in pool:
+            for a in range(0, pages, 4096):
+                n = min(4096, pages - a)
+                t[a:a + 4096] = rand(n, *shape[1:]) * torch.exp(rand(n, kv, page, 1) * 0.3)
+        scales = torch.zeros(2, 1, 1, 1, device="cuda")
+    # What no sequence holds (free pages, the rows behind a sequence's last) is never visible, whatever it contains.
+    if c["op"] != "store":
+        free = torch.ones(pages, page, dtype=torch.bool, device="cuda")
+        at = torch.arange(stride * page, device="cuda").view(1, stride, page) < st["lengths"].view(-1, 1, 1)
+        free[table[own_page].long()] = ~at.expand(seqs, stride, page)[own_page]
+        if c["kind"] == BYTES:
+            scales.masked_fill_(free.view(1, pages, 1, page), math.nan)
+        else:
+            for t in pool:
+                t.masked_fill_(free.view(pages, 1, page, 1), math.nan)
+    if c["window"]:  # pages that have left every window have been given back
+        first = (st["lengths"] - torch.tensor(news, device="cuda") - c["window"] + 1).view(-1, 1)
+        j = torch.arange(stride, device="cuda").view(1, -1) * page
+        table.masked_fill_((j >= c["sinks"]) & (j + page <= first), -1)
+    st["keys"], st["values"], st["scales"] = pool[0], pool[1], scales
+    if c["op"] in ("step", "store", "attend"):  # rows of a fused projection: queries, keys, values
+        st["qkv"] = rand(st["rows"], (qh + 2 * kv) * d) * torch.exp(rand(st["rows"], 1) * 0.2)
+    return st
+
+
+# ---------------------------------------------------------------- the plain forms
+def _new_rows(st):
+    """Of each new row: its sequence, and its place there."""
+    r = torch.arange(st["rows"], device="cuda")
+    s = torch.searchsorted(st["starts"], r, right=True, out_int32=True) - 1
+    s = s.long()
+    return s, st["lengths"].long()[s] - st["starts"].long()[s + 1] + r
+
+
+def _slots(st, s, j):
+    """Page and row in it of row j of sequence s; the page is -1 where there is none."""
+    page = st["case"]["page"]
+    return st["table"].long()[s, (j // page).clamp(0, st["stride"] - 1)], j % page
+
+
+def _plain_append(st):
+    c = st["case"]
+    kv, d, qh = c["kvheads"], c["dim"], c["qheads"]
+    p, o = _slots(st, *_new_rows(st))
+    for kind, pool in enumerate((st["keys"], st["values"])):
+        x = st["qkv"][:, (qh + kind * kv) * d:(qh + (kind + 1) * kv) * d].reshape(-1, kv, d)
+        if c["kind"] == BYTES:
+            m = x.abs().amax(-1)
+            scale = torch.where(m > 0, m / 127, torch.ones_like(m))
+            y = x / scale.unsqueeze(-1)
+            pool[p, :, o] = (torch.sign(y) * torch.floor(y.abs() + 0.5)).clamp(-127, 127).to(torch.int8)
+            st["scales"][kind][p, :, o] = scale
+        else:
+            pool[p, :, o] = x.to(torch.bfloat16)
+
+
+def _plain_rows(st, kind, p, o):
+    """FP32 values of the pool's rows (p, o): [..., kvheads, dim]."""
+    x = (st["keys"], st["values"])[kind][p, :, o].float()
+    return x * st["scales"][kind][p, :, o].unsqueeze(-1) if st["case"]["kind"] == BYTES else x
+
+
+def _plain_read(st):
+    p, o = _slots(st, *_new_rows(st))
+    return {"k": _plain_rows(st, 0, p, o), "v": _plain_rows(st, 1, p, o)}
+
+
+def _plain_attend(st):
+    c = st["case"]
+    kv, d, qh, window, sinks = c["kvheads"], c["dim"], c["qheads"], c["window"], c["sinks"]
+    n, seqs, group = st["max_new"], c["seqs"], c["qheads"] // c["kvheads"]
+    length = st["lengths"].long().view(-1, 1)
+    first = length - (st["starts"][1:] - st["starts"][:-1]).long().view(-1, 1)  # place of a sequence's first new row
+    if window:  # the columns: the first rows, then what the windows reach
+        low = (first - window + 1).clamp(min=sinks)
+        j = torch.cat([torch.arange(sinks, device="cuda").expand(seqs, sinks),
+                       low + torch.arange(min(window + n - 1, st["max_length"]), device="cuda")], 1)
+    else:
+        j = torch.arange(st["max_length"], device="cuda").expand(seqs, -1)
+    p, o = _slots(st, torch.arange(seqs, device="cuda").view(-1, 1), j)
+    there = ((j < length) & (p >= 0)).view(seqs, -1, 1, 1)
+    k, v = (torch.where(there, _plain_rows(st, kind, p.clamp(min=0), o), 0.0).permute(0, 2, 3, 1) for kind in (0, 1))
+    s, pos = _new_rows(st)
+    i = torch.arange(st["rows"], device="cuda") - st["starts"].long()[s]
+    q = torch.zeros(seqs, n, qh, d, device="cuda")
+    q[s, i] = st["qkv"][:, :qh * d].reshape(-1, qh, d)
+    q = q.view(seqs, n, kv, group, d).permute(0, 2, 3, 1, 4).reshape(seqs, kv, group * n, d)
+    at = (first + torch.arange(n, device="cuda")).unsqueeze(-1)  # [seqs, n, 1]
+    jj = j.unsqueeze(1)
+    seen = (jj <= at) & (jj < length.unsqueeze(-1))
+    if window:
+        seen &= (jj < sinks) | (jj > at - window)
+    x = torch.matmul(q, k).view(seqs, kv, group, n, -1)
+    x /= math.sqrt(d)
+    x.masked_fill_(~seen.view(seqs, 1, 1, n, -1), -math.inf)
+    m = x.amax(-1, keepdim=True)
+    x -= torch.where(m == -math.inf, torch.zeros_like(m), m)
+    x.exp_()
+    total = x.sum(-1, keepdim=True)
+    out = torch.matmul(x.view(seqs, kv, group * n, -1), v.transpose(-1, -2)).view(seqs, kv, group, n, d)
+    out = torch.where(total > 0, out / total, torch.zeros_like(out))
+    return {"out": out.permute(0, 3, 1, 2, 4).reshape(seqs, n, qh, d)[s, i]}
+
+
+# ---------------------------------------------------------------- the library's kernels
+_gpu = []  # the program's one handle: it owns the attention's workspace
+
+
+def _handles(st):
+    """The descriptors that a program keeps beside its pool and batch."""
+    if "cache" not in st:
+        import cmachine_b200 as cm
+        c = st["case"]
+        st["lib"] = cm.lib()
+        if not _gpu:
+            _gpu.append(st["lib"].gpu_open())
+        st["gpu"] = _gpu[0]
+        st["cache"] = cm.PagedCache(c["kind"], st["pages"], c["page"], c["kvheads"], c["dim"], st["keys"].data_ptr(),
+                                    st["values"].data_ptr(), st["scales"].data_ptr())
+        st["batch"] = cm.PagedBatch(c["seqs"], st["rows"], st["max_new"], st["max_length"], st["starts"].data_ptr(),
+                                    st["lengths"].data_ptr(), st["table"].data_ptr(), st["stride"])
+    return st["lib"], st["gpu"], st["cache"], st["batch"]
+
+
+def _own_append(st):
+    L, _, cache, batch = _handles(st)
+    c, qkv = st["case"], st["qkv"].data_ptr()
+    at = qkv + c["qheads"] * c["dim"] * 4
+    if L.gpu_paged_append(cache, batch, at, at + c["kvheads"] * c["dim"] * 4, st["qkv"].stride(0), st["status"].data_ptr()):
+        raise RuntimeError("gpu_paged_append refused")
+
+
+def _own_read(st):
+    L, _, cache, batch = _handles(st)
+    c = st["case"]
+    k, v = (torch.empty(st["rows"], c["kvheads"], c["dim"], device="cuda") for _ in range(2))
+    if L.gpu_paged_read(cache, batch, k.data_ptr(), v.data_ptr(), k.stride(0), st["status"].data_ptr()):
+        raise RuntimeError("gpu_paged_read refused")
+    return {"k": k, "v": v}
+
+
+def _own_attend(st):
+    L, gpu, cache, batch = _handles(st)
+    c = st["case"]
+    out = torch.empty(st["rows"], c["qheads"], c["dim"], device="cuda")
+    if L.gpu_paged_attention(gpu, out.data_ptr(), out.stride(0), st["qkv"].data_ptr(), st["qkv"].stride(0), cache, batch,
+                             c["qheads"], c["window"], c["sinks"], st["status"].data_ptr()):
+        raise RuntimeError("gpu_paged_attention refused")
+    return {"out": out}
+
+
+def run(state):
+    op = state["case"]["op"]
+    if own:
+        if op in ("step", "store"):
+            _own_append(state)
+        return _own_attend(state) if op in ("step", "attend") else _own_read(state)
+    if op in ("step", "store"):
+        _plain_append(state)
+    return _plain_attend(state) if op in ("step", "attend") else _plain_read(state)
+
+
+# ---------------------------------------------------------------- the definition in 64 bits
+def _codec64(x, kind):
+    """What rows of 64-bit values stand for once stored. The codec is defined by single-precision divisions; a 64-bit
+    quotient of single-precision numbers rounds to the same single-precision number."""
+    if kind == BF16:
+        return x.to(torch.bfloat16).double()
+    m = x.abs().amax(-1, keepdim=True)
+    scale = torch.where(m > 0, m / 127.0, torch.ones_like(m)).float().double()
+    y = (x / scale).float().double()
+    return torch.trunc(y + torch.where(y < 0, -0.5, 0.5)).clamp(-127, 127) * scale
+
+
+def _held(st, s, kind, lo, hi):
+    """Rows [lo, hi) of sequence s in 64 bits: [kvheads, hi - lo, dim]."""
+    page = st["case"]["page"]
+    a, b = lo // page, -(-hi // page)
+    ids = st["table"][s, a:b].long()
+    pool = (st["keys"], st["values"])[kind]
+    x = pool[ids].double()  # [pages, kvheads, page, dim]
+    if st["case"]["kind"] == BYTES:
+        x = x * st["scales"][kind][ids].double().unsqueeze(-1)
+    return x.transpose(0, 1).reshape(x.shape[1], -1, x.shape[3])[:, lo - a * page:hi - a * page]
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    c = st["case"]
+    kv, d, qh, window, sinks = c["kvheads"], c["dim"], c["qheads"], c["window"], c["sinks"]
+    group = qh // kv
+    starts, lengths = st["starts"].tolist(), st["lengths"].tolist()
+    if c["op"] in ("store", "read"):
+        k, v = (torch.empty(st["rows"], kv, d, dtype=torch.float64, device="cuda") for _ in range(2))
+        for kind, t in enumerate((k, v)):
+            if c["op"] == "store":
+                at = (qh + kind * kv) * d
+                t.copy_(_codec64(st["qkv"][:, at:at + kv * d].double().view(-1, kv, d), c["kind"]))
+            else:
+                for s in range(c["seqs"]):
+                    a, b = starts[s], starts[s + 1]
+                    if b > a:
+                        t[a:b] = _held(st, s, kind, lengths[s] - (b - a), lengths[s]).transpose(0, 1)
+        return {"k": k, "v": v}
+    out = torch.zeros(st["rows"], qh, d, dtype=torch.float64, device="cuda")
+    for s in range(c["seqs"]):
+        a, b, length = starts[s], starts[s + 1], lengths[s]
+        first = length - (b - a)
+        low = max(0, first - window + 1) if window else 0
+        head = min(sinks, low) if window else 0
+        rows = [torch.cat([_held(st, s, kind, 0, head), _held(st, s, kind, low, length)], 1) for kind in (0, 1)]
+        j = torch.cat([torch.arange(head, device="cuda"), torch.arange(low, length, device="cuda")])
+        if c["op"] == "step":  # the new rows as they are stored
+            for kind in (0, 1):
+                at = (qh + kind * kv) * d
+                new = _codec64(st["qkv"][a:b, at:at + kv * d].double().view(-1, kv, d), c["kind"])
+                rows[kind][:, rows[kind].shape[1] - (b - a):] = new.transpose(0, 1)
+        most = max(1, (1 << 27) // max(1, j.numel()))
+        for h in range(qh):
+            keys, values = rows[0][h // group], rows[1][h // group]
+            for r in range(a, b, most):
+                e = min(b, r + most)
+                pos = (first + torch.arange(r - a, e - a, device="cuda")).view(-1, 1)
+                hide = j > pos
+                if window:
+                    hide |= (j >= sinks) & (j <= pos - window)
+                x = st["qkv"][r:e, h * d:(h + 1) * d].double() @ keys.T / math.sqrt(d)
+                out[r:e, h] = torch.softmax(x.masked_fill_(hide, -math.inf), -1) @ values
+    return {"out": out}
