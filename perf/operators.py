@@ -216,7 +216,7 @@ def _plain_append(st):
         x = st["qkv"][:, (qh + kind * kv) * d:(qh + (kind + 1) * kv) * d].reshape(-1, kv, d)
         if c["kind"] == BYTES:
             m = x.abs().amax(-1)
-            scale = torch.where(m > 0, m / 127, torch.ones_like(m))
+            scale = torch.where(m > 0, m / torch.full_like(m, 127), torch.ones_like(m))  # by a number, torch multiplies by 1/127
             y = x / scale.unsqueeze(-1)
             pool[p, :, o] = (torch.sign(y) * torch.floor(y.abs() + 0.5)).clamp(-127, 127).to(torch.int8)
             st["scales"][kind][p, :, o] = scale
