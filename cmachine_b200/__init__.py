@@ -11,7 +11,7 @@ fallback: a missing library raises at import of `lib()`.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, Structure, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, Structure, c_float, c_int, c_longlong, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 import numpy as np
@@ -53,6 +53,18 @@ class SessionView(Structure):
         ("checkpoint_serial", c_uint64), ("top_frame", c_uint64), ("top", Top2), ("keys", c_void_p),
         ("values", c_void_p), ("x", c_void_p), ("logits", c_void_p), ("allocated_bytes", c_size_t),
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("attention", c_void_p)]
+
+
+class PagedCache(Structure):
+    """TcmPagedCache (include/gpu.h): kind 2 BF16 or 3 bytes; keys, values and scales are device pointers."""
+    _fields_ = [(n, c_int) for n in ("kind", "pages", "page", "kvheads", "dim")] + [
+        ("keys", c_void_p), ("values", c_void_p), ("scales", c_void_p)]
+
+
+class PagedBatch(Structure):
+    """TcmPagedBatch (include/gpu.h): starts, lengths and table are device pointers to int32."""
+    _fields_ = [(n, c_int) for n in ("sequences", "rows", "max_new", "max_length")] + [
+        ("starts", c_void_p), ("lengths", c_void_p), ("table", c_void_p), ("table_stride", c_int)]
 
 
 def qwen_shape(layers: int = 28, max_position: int = 32768) -> Shape:
@@ -132,6 +144,10 @@ def _declare(L, strict: bool = True):
         "gpu_byte_attention": (None, [P, P, P, P, P, P, P, P, c_int, c_int]),
         "gpu_ring_attention": (None, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int]),
         "gpu_attention_static": (c_int, [P, P, P, P, c_int, c_int, c_int, c_int, c_int]),
+        "gpu_paged_append": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), P, P, c_longlong, P]),
+        "gpu_paged_read": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), P, P, c_longlong, P]),
+        "gpu_paged_attention": (c_int, [P, P, c_longlong, P, c_longlong, POINTER(PagedCache), POINTER(PagedBatch), c_int,
+                                        c_int, c_int, P]),
         # include/bounded_cache.h
         "ring_open": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int]),
         "ring_begin": (c_int, [P, c_int]), "ring_abort": (c_int, [P]), "ring_finish": (c_int, [P]),

@@ -1,0 +1,291 @@
+// Paged K/V cache: append, read back and attention of ragged batches.
+//
+// The reference's caches are one session's: dense FP32 slabs and the byte-codec
+// ring. Here many sequences share one pool of pages (include/gpu.h); rows are
+// addressed only through csrc/paged_index.h.
+#include "common.cuh"
+#include "paged.cuh"
+#include "kernels.h"
+#include "../../include/gpu.h"
+#include "../../include/tcm_seeded.h"
+#include <math.h>
+
+namespace tcm {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+// ---------------------------------------------------------------- append, read back
+// One warp per (new row, KV head), K and V together: DIM / 32 elements a lane.
+// Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x /
+// scale), +-127), the divisions IEEE as in byte_cache.cu, so codes and scales are
+// the ring's bit for bit.
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, const float *k, const float *vals,
+                                                                   long long stride, int *status) {
+    constexpr int E = DIM / 32;
+    const int lane = threadIdx.x & 31, s = blockIdx.y;
+    PagedExtent e;
+    int bad = paged_extent(&v, s, &e);
+    const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
+    for (int item = (blockIdx.x * kRowThreads + threadIdx.x) >> 5; item < items; item += warps) {
+        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
+        if (j < 0) continue;
+        const int64_t row = paged_slot(&v, s, j, h);
+        if (row < 0) {
+            bad |= kPagedBadPage;
+            continue;
+        }
+#pragma unroll
+        for (int kind = 0; kind < 2; kind++) {
+            const float *src = (kind ? vals : k) + (long long)(e.start + i) * stride + h * DIM + lane * E;
+            float x[E], m = 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int c = 0; c < E; c++) {
+                x[c] = src[c];
+                finite &= isfinite(x[c]);
+                m = fmaxf(m, fabsf(x[c]));
+            }
+            if (!__all_sync(0xffffffffu, finite)) {
+                bad |= kPagedNonFinite;
+                m = 0.f;
+#pragma unroll
+                for (int c = 0; c < E; c++) x[c] = 0.f;
+            }
+            void *dst = kind ? v.values : v.keys;
+            if constexpr (KIND == kPagedBytes) {
+                m = warp_max(m);
+                const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
+                // A row so small that m / 127 underflows stands for zeros (scale 0, codes 0).
+                int8_t q[E];
+#pragma unroll
+                for (int c = 0; c < E; c++)
+                    q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(x[c], scale)))) : (int8_t)0;
+                if constexpr (E == 4)
+                    *reinterpret_cast<char4 *>(static_cast<int8_t *>(dst) + row * DIM + lane * E) = make_char4(q[0], q[1], q[2], q[3]);
+                else
+                    *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + row * DIM + lane * E) = make_char2(q[0], q[1]);
+                if (lane == 0) v.scales[(int64_t)kind * v.pages * v.kvheads * v.page + row] = scale;
+            } else {
+                uint16_t *d = static_cast<uint16_t *>(dst) + row * DIM + lane * E;
+                uint32_t w[E / 2];
+#pragma unroll
+                for (int c = 0; c < E; c += 2) w[c / 2] = (uint32_t)tcm_bf16_rne(x[c]) | ((uint32_t)tcm_bf16_rne(x[c + 1]) << 16);
+                if constexpr (E == 4) *reinterpret_cast<uint2 *>(d) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t *>(d) = w[0];
+            }
+        }
+    }
+    if (lane == 0) paged_report(status, bad);
+}
+
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, float *k, float *vals, long long stride,
+                                                                 int *status) {
+    constexpr int L = DIM / 4, R = 32 / L;  // lanes a row, rows a warp
+    const int lane = threadIdx.x & 31, s = blockIdx.y, c = (lane % L) * 4;
+    PagedExtent e;
+    int bad = paged_extent(&v, s, &e);
+    const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
+    const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
+    for (int item = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R + lane / L; item < items; item += warps * R) {
+        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
+        int64_t row = -1;
+        if (j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
+        const long long at = (long long)(e.start + i) * stride + h * DIM + c;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (row >= 0) {
+            a = paged_load4<KIND>(v.keys, row * DIM + c);
+            b = paged_load4<KIND>(v.values, row * DIM + c);
+            if constexpr (KIND == kPagedBytes) {
+                const float sk = v.scales[row], sv = v.scales[half + row];
+                a = make_float4(a.x * sk, a.y * sk, a.z * sk, a.w * sk);
+                b = make_float4(b.x * sv, b.y * sv, b.z * sv, b.w * sv);
+            }
+        }
+        *reinterpret_cast<float4 *>(k + at) = a;
+        *reinterpret_cast<float4 *>(vals + at) = b;
+    }
+    paged_report(status, bad);
+}
+
+// ---------------------------------------------------------------- attention
+// One warp per (new row, query head): the online softmax over the rows it sees,
+// row by row, FP32 throughout.
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(kRowThreads) paged_attention_kernel(PagedView v, float *out, long long out_stride,
+                                                                      const float *q, long long q_stride, int qheads,
+                                                                      int window, int sinks, float scale2, int *status) {
+    constexpr int E = DIM / 32;
+    const int lane = threadIdx.x & 31, s = blockIdx.y, group = qheads / v.kvheads;
+    PagedExtent e;
+    int bad = paged_extent(&v, s, &e);
+    const int items = e.count * qheads, warps = gridDim.x * (kRowThreads / 32);
+    const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
+    for (int item = (blockIdx.x * kRowThreads + threadIdx.x) >> 5; item < items; item += warps) {
+        const int i = item / qheads, h = item - i * qheads, at = e.length - e.count + i;
+        float x[E], acc[E], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < E; c++) {
+            x[c] = q[(long long)(e.start + i) * q_stride + h * DIM + lane * E + c];
+            acc[c] = 0.f;
+        }
+        const PagedTiles t = paged_tiles(at, at, window, sinks, 4);
+        for (int n = 0; n < t.count; n++)
+            for (int j = paged_tile(t, n) * 16, end = min(j + 16, at + 1); j < end; j++) {
+                if (!paged_sees(at, j, window, sinks)) continue;
+                const int64_t row = paged_slot(&v, s, j, h / group);
+                if (row < 0) {
+                    bad |= kPagedBadPage;
+                    continue;
+                }
+                float kx[E], vx[E];
+                if constexpr (KIND == kPagedBytes) {
+                    const float sk = v.scales[row], sv = v.scales[half + row];
+#pragma unroll
+                    for (int c = 0; c < E; c++) {
+                        kx[c] = sk * (float)static_cast<const int8_t *>(v.keys)[row * DIM + lane * E + c];
+                        vx[c] = sv * (float)static_cast<const int8_t *>(v.values)[row * DIM + lane * E + c];
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < E; c++) {
+                        kx[c] = bf16_lo(static_cast<const uint16_t *>(v.keys)[row * DIM + lane * E + c]);
+                        vx[c] = bf16_lo(static_cast<const uint16_t *>(v.values)[row * DIM + lane * E + c]);
+                    }
+                }
+                float d = 0.f;
+#pragma unroll
+                for (int c = 0; c < E; c++) d = fmaf(x[c], kx[c], d);
+                d = warp_sum(d) * scale2;
+                const float top = fmaxf(m, d), keep = exp2f(m - top), p = exp2f(d - top);
+                l = fmaf(l, keep, p);
+                m = top;
+#pragma unroll
+                for (int c = 0; c < E; c++) acc[c] = fmaf(acc[c], keep, p * vx[c]);
+            }
+#pragma unroll
+        for (int c = 0; c < E; c++)
+            out[(long long)(e.start + i) * out_stride + h * DIM + lane * E + c] = l > 0.f ? acc[c] / l : (l == l ? 0.f : l);
+    }
+    if (lane == 0) paged_report(status, bad);
+}
+
+// ---------------------------------------------------------------- host
+int refuse(const char *call, const char *why) {
+    fprintf(stderr, "%s: %s\n", call, why);
+    return -1;
+}
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// The call's descriptors as a view; 0, or -1 with a message.
+int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, PagedView *v) {
+    if (!c || !b) return refuse(call, "no cache or no batch");
+    if (c->kind != kPagedBf16 && c->kind != kPagedBytes) return refuse(call, "kind is 2 (BF16) or 3 (bytes)");
+    if (c->dim != 64 && c->dim != 128) return refuse(call, "dim is 64 or 128");
+    if (c->pages < 1 || c->page < 1 || c->page > 65536 || c->kvheads < 1 || c->kvheads > 1024)
+        return refuse(call, "pages, page or kvheads out of range");
+    if (!c->keys || !c->values || !aligned16(c->keys) || !aligned16(c->values))
+        return refuse(call, "keys and values are 16-byte aligned device memory");
+    if (c->kind == kPagedBytes && (!c->scales || ((uintptr_t)c->scales & 3))) return refuse(call, "a byte cache has scales");
+    if (b->sequences < 0 || b->sequences > 65535 || b->rows < 0 || b->max_new < 0 || b->max_length < 0)
+        return refuse(call, "sequences, rows, max_new or max_length out of range");
+    if (b->sequences && (!b->starts || !b->lengths || !b->table || b->table_stride < 1))
+        return refuse(call, "a batch has starts, lengths and a table");
+    if (((uintptr_t)b->starts | (uintptr_t)b->lengths | (uintptr_t)b->table) & 3)
+        return refuse(call, "starts, lengths and table are 4-byte aligned");
+    const int max_new = b->max_new < b->rows ? b->max_new : b->rows;
+    if ((long long)max_new * c->kvheads > 0x7fffffff / 8) return refuse(call, "too many new rows for one call");
+    *v = PagedView{c->kind, c->pages, c->page, c->kvheads, c->dim, c->keys, c->values, c->scales, b->sequences, b->rows,
+                   max_new, b->max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0};
+    paged_divider(v);
+    return 0;
+}
+int check_rows(const char *call, const void *p, long long stride, int heads, int dim) {
+    if (!p || !aligned16(p)) return refuse(call, "row buffers are 16-byte aligned device memory");
+    if (stride < (long long)heads * dim || stride % 4) return refuse(call, "a row stride is a multiple of 4 and holds a row");
+    return 0;
+}
+// Nothing to do: no sequence, or none that may have a new row.
+bool nothing(const PagedView &v) { return !v.sequences || !v.rows || !v.max_new; }
+
+unsigned blocks_of(long long items, int a_block) {
+    const long long blocks = (items + a_block - 1) / a_block;
+    return (unsigned)(blocks < 4096 ? blocks : 4096);
+}
+
+}  // namespace
+}  // namespace tcm
+
+using namespace tcm;
+
+#define PAGED_DISPATCH(view, call)                                      \
+    do {                                                                \
+        if ((view).kind == kPagedBf16) {                                \
+            if ((view).dim == 64) { call(kPagedBf16, 64); }             \
+            else { call(kPagedBf16, 128); }                             \
+        } else {                                                        \
+            if ((view).dim == 64) { call(kPagedBytes, 64); }            \
+            else { call(kPagedBytes, 128); }                            \
+        }                                                               \
+    } while (0)
+
+extern "C" {
+
+int gpu_paged_append(const TcmPagedCache *cache, const TcmPagedBatch *batch, const float *k, const float *v,
+                     long long stride, int *status) {
+    PagedView view;
+    if (open_view("gpu_paged_append", cache, batch, &view)) return -1;
+    if (nothing(view)) return 0;
+    if (check_rows("gpu_paged_append", k, stride, view.kvheads, view.dim) ||
+        check_rows("gpu_paged_append", v, stride, view.kvheads, view.dim))
+        return -1;
+    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32), view.sequences);
+#define CALL(K, D) paged_append_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, k, v, stride, status)
+    PAGED_DISPATCH(view, CALL);
+#undef CALL
+    TCM_CUDA(cudaGetLastError());
+    return 0;
+}
+
+int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float *k, float *v, long long stride,
+                   int *status) {
+    PagedView view;
+    if (open_view("gpu_paged_read", cache, batch, &view)) return -1;
+    if (nothing(view)) return 0;
+    if (check_rows("gpu_paged_read", k, stride, view.kvheads, view.dim) ||
+        check_rows("gpu_paged_read", v, stride, view.kvheads, view.dim))
+        return -1;
+    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32), view.sequences);
+#define CALL(K, D) paged_read_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, k, v, stride, status)
+    PAGED_DISPATCH(view, CALL);
+#undef CALL
+    TCM_CUDA(cudaGetLastError());
+    return 0;
+}
+
+int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const float *q, long long q_stride,
+                        const TcmPagedCache *cache, const TcmPagedBatch *batch, int qheads, int window, int sinks,
+                        int *status) {
+    const char *name = "gpu_paged_attention";
+    PagedView view;
+    if (!gpu) return refuse(name, "no handle");
+    if (open_view(name, cache, batch, &view)) return -1;
+    if (qheads < 1 || qheads % view.kvheads || qheads / view.kvheads > 8)
+        return refuse(name, "qheads is 1 to 8 times kvheads");
+    if (window < 0 || sinks < 0) return refuse(name, "window and sinks are not negative");
+    if (nothing(view)) return 0;
+    if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
+    const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
+    const dim3 grid(blocks_of((long long)view.max_new * qheads, kRowThreads / 32), view.sequences);
+#define CALL(K, D)                                                                                                 \
+    paged_attention_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, out, out_stride, q, q_stride, qheads, window, \
+                                                                     sinks, scale2, status)
+    PAGED_DISPATCH(view, CALL);
+#undef CALL
+    TCM_CUDA(cudaGetLastError());
+    return 0;
+}
+
+}  // extern "C"

@@ -123,6 +123,64 @@ void gpu_ring_attention(TcmGpu *, float *out, const float *q, const signed char 
                         const float *scales, float *scores, float *workspace, const int *order,
                         const float *weights, int capacity, int length, int weighted);
 
+/* ---- Paged K/V cache of many sequences (no counterpart in the reference) ----
+ * One pool of fixed-size pages holds the K and V rows of every sequence; a table
+ * names each sequence's pages, so sequences grow, end and share prefixes without
+ * copies. The pool, the table and the extents are device memory of the caller;
+ * the descriptors are host structures read during the call.
+ *
+ * keys and values are [pages][kvheads][page][dim]: BF16 (kind 2, round to nearest
+ * even), or the byte codec above (kind 3: int8 codes, with scales [2][pages]
+ * [kvheads][page], K's then V's). Limits: dim 64 or 128; 1 <= page <= 65536;
+ * keys and values 16-byte aligned; kvheads <= 1024. */
+typedef struct {
+    int kind, pages, page, kvheads, dim;
+    void *keys, *values;
+    float *scales; /* kind 3 only */
+} TcmPagedCache;
+/* A ragged batch: sequence s brings the rows starts[s] .. starts[s + 1] - 1 of the
+ * callers' row buffers (which have `rows` rows in all) and has lengths[s] rows in
+ * the cache counting them, so new row i stands at place lengths[s] - count + i.
+ * table[s * table_stride + p] is the page of places p * page .. p * page + page - 1;
+ * entries of places that nothing reads or writes may hold anything. max_new and
+ * max_length are upper bounds of the new rows and the length of any sequence. */
+typedef struct {
+    int sequences, rows, max_new, max_length; /* sequences <= 65535 */
+    const int *starts;  /* [sequences + 1] */
+    const int *lengths; /* [sequences] */
+    const int *table;   /* [sequences][table_stride] */
+    int table_stride;
+} TcmPagedBatch;
+/* All three return 0 when launched, or -1 with a message on stderr for sizes,
+ * strides or alignment they do not take, and launch nothing; they never wait for
+ * the device. What only the device can see is reported in *status (a device word
+ * the kernels OR into and never clear; may be NULL): 1 a non-finite row was
+ * appended, 2 a page id outside the pool for a row that was needed, 4 extents that
+ * do not fit rows, max_new, max_length or the table. A row without a page is not
+ * written, reads as zeros and is visible to no query; a sequence with bad extents
+ * is left out, its rows of the outputs untouched. Row buffers are FP32, strides
+ * count floats from one row to the next (multiples of 4), buffers are 16-byte
+ * aligned; rows of no sequence are neither read nor written.
+ *
+ * Write the new rows: k and v hold [kvheads][dim] a row, `stride` apart (both). A
+ * row of one KV head with a non-finite value is stored as zeros. New rows at
+ * negative places (count > length) are skipped. Two sequences that write the same
+ * row of a shared page leave either's. */
+int gpu_paged_append(const TcmPagedCache *, const TcmPagedBatch *, const float *k, const float *v, long long stride,
+                     int *status);
+/* Read the same rows back as the FP32 values they stand for. */
+int gpu_paged_read(const TcmPagedCache *, const TcmPagedBatch *, float *k, float *v, long long stride, int *status);
+/* Grouped-query attention of the new rows' queries over the cache: the query at
+ * place p sees rows j <= p with window == 0, j > p - window or j < sinks, scores
+ * q . k / sqrt(dim). q and out hold [qheads][dim] a row; query head h reads KV head
+ * h / (qheads / kvheads); at most 8 query heads per KV head. A query that sees no
+ * row gets zeros. Outputs that see a row with a non-finite value are unspecified;
+ * no other output is touched by it. Deterministic. Scratch belongs to the handle and grows on
+ * demand (the growing call allocates): calls with one handle follow one another on
+ * the library's stream, and another thread needs a handle of its own. */
+int gpu_paged_attention(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
+                        const TcmPagedCache *, const TcmPagedBatch *, int qheads, int window, int sinks, int *status);
+
 #ifdef __cplusplus
 }
 #endif
