@@ -5,6 +5,7 @@
 // addressed only through csrc/paged_index.h.
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_decode.cuh"
 #include "kernels.h"
 #include "../../include/gpu.h"
 #include "../../include/tcm_seeded.h"
@@ -116,11 +117,13 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kRowThreads) paged_attention_kernel(PagedView v, float *out, long long out_stride,
                                                                       const float *q, long long q_stride, int qheads,
-                                                                      int window, int sinks, float scale2, int *status) {
+                                                                      int window, int sinks, float scale2, int few,
+                                                                      int *status) {
     constexpr int E = DIM / 32;
     const int lane = threadIdx.x & 31, s = blockIdx.y, group = qheads / v.kvheads;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
+    if (e.count <= few) return;
     const int items = e.count * qheads, warps = gridDim.x * (kRowThreads / 32);
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     for (int item = (blockIdx.x * kRowThreads + threadIdx.x) >> 5; item < items; item += warps) {
@@ -210,6 +213,34 @@ int check_rows(const char *call, const void *p, long long stride, int heads, int
 // Nothing to do: no sequence, or none that may have a new row.
 bool nothing(const PagedView &v) { return !v.sequences || !v.rows || !v.max_new; }
 
+constexpr int kFewRows = 32;  // sequences with at most this many query rows a KV head are the decode kernel's
+
+// Most rows of one sequence that the queries of one tile can see.
+long long visible_rows(const PagedView &v, int window, int sinks) {
+    const long long most = window ? (long long)window + sinks + v.max_new + 32 : v.max_length;
+    return most < v.max_length ? most : v.max_length;
+}
+
+template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) {
+    const PagedView &v = a.v;
+    const int rows = (v.max_new < a.few ? v.max_new : a.few) * a.group, r = rows <= 8 ? 8 : 16;
+    a.row_tiles = (rows + r - 1) / r;
+    // Splits: enough items to fill the GPU several times over, whole steps for each of the four
+    // warps, and no more than the merge holds.
+    const long long steps = (visible_rows(v, a.window, a.sinks) + 15) / 16 + 2;
+    const long long items = (long long)v.sequences * v.kvheads * a.row_tiles;
+    long long per = (steps * items + sm_count() * 32 - 1) / (sm_count() * 32);
+    if (per < kPdWarps) per = kPdWarps;
+    if (per * kPdSplitsMax < steps) per = (steps + kPdSplitsMax - 1) / kPdSplitsMax;
+    per = (per + kPdWarps - 1) / kPdWarps * kPdWarps;
+    a.tiles_per_item = (int)per;
+    a.splits = (int)((steps + per - 1) / per);
+    paged_scratch(gpu, a.splits > 1 ? items * a.splits * r : 0, DIM, items, &a.part, &a.ml, &a.counters);
+    const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
+    if (r == 8) launch(paged_decode_kernel<KIND, DIM, 8>, grid, dim3(kPdThreads), 0, stream(), true, a);
+    else launch(paged_decode_kernel<KIND, DIM, 16>, grid, dim3(kPdThreads), 0, stream(), true, a);
+}
+
 unsigned blocks_of(long long items, int a_block) {
     const long long blocks = (items + a_block - 1) / a_block;
     return (unsigned)(blocks < 4096 ? blocks : 4096);
@@ -278,10 +309,17 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     if (nothing(view)) return 0;
     if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
     const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
+    const int group = qheads / view.kvheads, few = kFewRows / group;
+    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, 1, 1, 1, scale2, nullptr, nullptr,
+                         nullptr, status};
+#define CALL(K, D) decode_launch<K, D>(gpu, d)
+    PAGED_DISPATCH(view, CALL);
+#undef CALL
+    if (view.max_new <= few) return 0;
     const dim3 grid(blocks_of((long long)view.max_new * qheads, kRowThreads / 32), view.sequences);
 #define CALL(K, D)                                                                                                 \
     paged_attention_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, out, out_stride, q, q_stride, qheads, window, \
-                                                                     sinks, scale2, status)
+                                                                     sinks, scale2, few, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
     TCM_CUDA(cudaGetLastError());

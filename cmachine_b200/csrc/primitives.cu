@@ -17,6 +17,9 @@ struct TcmGpu {
     unsigned *attn_counters;
     size_t attn_part_floats;
     int attn_kv;
+    float *paged_part;   // the paged attention's split partials and arrival counters (grown on demand)
+    unsigned *paged_counters;
+    size_t paged_floats, paged_count;
 };
 
 namespace tcm {
@@ -370,6 +373,24 @@ void attention_scratch(TcmGpu *g, int kvheads, float **part, unsigned **counters
     *part = g->attn_part;
     *counters = g->attn_counters;
 }
+
+void paged_scratch(TcmGpu *g, long long rows, int dim, long long counters, float **part, float2 **ml, unsigned **count) {
+    const size_t floats = (size_t)rows * (dim + 2);
+    if (g->paged_floats < floats) {
+        gpu_free(g->paged_part);
+        g->paged_part = (float *)gpu_alloc(floats * sizeof(float));
+        g->paged_floats = floats;
+    }
+    if (g->paged_count < (size_t)counters) {
+        gpu_free(g->paged_counters);
+        g->paged_counters = (unsigned *)gpu_alloc((size_t)counters * sizeof(unsigned));
+        gpu_zero(g->paged_counters, (size_t)counters * sizeof(unsigned));
+        g->paged_count = (size_t)counters;
+    }
+    *part = g->paged_part;
+    *ml = reinterpret_cast<float2 *>(g->paged_part + (size_t)rows * dim);
+    *count = g->paged_counters;
+}
 }  // namespace tcm
 
 extern "C" {
@@ -393,6 +414,8 @@ void gpu_close(TcmGpu *g) {
     gpu_free(g->result);
     gpu_free(g->attn_part);
     gpu_free(g->attn_counters);
+    gpu_free(g->paged_part);
+    gpu_free(g->paged_counters);
     free(g);
 }
 
