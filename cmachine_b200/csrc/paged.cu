@@ -6,6 +6,7 @@
 #include "common.cuh"
 #include "paged.cuh"
 #include "paged_decode.cuh"
+#include "paged_chunk.cuh"
 #include "kernels.h"
 #include "../../include/gpu.h"
 #include "../../include/tcm_seeded.h"
@@ -111,70 +112,6 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
     paged_report(status, bad);
 }
 
-// ---------------------------------------------------------------- attention
-// One warp per (new row, query head): the online softmax over the rows it sees,
-// row by row, FP32 throughout.
-template <int KIND, int DIM>
-__global__ void __launch_bounds__(kRowThreads) paged_attention_kernel(PagedView v, float *out, long long out_stride,
-                                                                      const float *q, long long q_stride, int qheads,
-                                                                      int window, int sinks, float scale2, int few,
-                                                                      int *status) {
-    constexpr int E = DIM / 32;
-    const int lane = threadIdx.x & 31, s = blockIdx.y, group = qheads / v.kvheads;
-    PagedExtent e;
-    int bad = paged_extent(&v, s, &e);
-    if (e.count <= few) return;
-    const int items = e.count * qheads, warps = gridDim.x * (kRowThreads / 32);
-    const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
-    for (int item = (blockIdx.x * kRowThreads + threadIdx.x) >> 5; item < items; item += warps) {
-        const int i = item / qheads, h = item - i * qheads, at = e.length - e.count + i;
-        float x[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int c = 0; c < E; c++) {
-            x[c] = q[(long long)(e.start + i) * q_stride + h * DIM + lane * E + c];
-            acc[c] = 0.f;
-        }
-        const PagedTiles t = paged_tiles(at, at, window, sinks, 4);
-        for (int n = 0; n < t.count; n++)
-            for (int j = paged_tile(t, n) * 16, end = min(j + 16, at + 1); j < end; j++) {
-                if (!paged_sees(at, j, window, sinks)) continue;
-                const int64_t row = paged_slot(&v, s, j, h / group);
-                if (row < 0) {
-                    bad |= kPagedBadPage;
-                    continue;
-                }
-                float kx[E], vx[E];
-                if constexpr (KIND == kPagedBytes) {
-                    const float sk = v.scales[row], sv = v.scales[half + row];
-#pragma unroll
-                    for (int c = 0; c < E; c++) {
-                        kx[c] = sk * (float)static_cast<const int8_t *>(v.keys)[row * DIM + lane * E + c];
-                        vx[c] = sv * (float)static_cast<const int8_t *>(v.values)[row * DIM + lane * E + c];
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < E; c++) {
-                        kx[c] = bf16_lo(static_cast<const uint16_t *>(v.keys)[row * DIM + lane * E + c]);
-                        vx[c] = bf16_lo(static_cast<const uint16_t *>(v.values)[row * DIM + lane * E + c]);
-                    }
-                }
-                float d = 0.f;
-#pragma unroll
-                for (int c = 0; c < E; c++) d = fmaf(x[c], kx[c], d);
-                d = warp_sum(d) * scale2;
-                const float top = fmaxf(m, d), keep = exp2f(m - top), p = exp2f(d - top);
-                l = fmaf(l, keep, p);
-                m = top;
-#pragma unroll
-                for (int c = 0; c < E; c++) acc[c] = fmaf(acc[c], keep, p * vx[c]);
-            }
-#pragma unroll
-        for (int c = 0; c < E; c++)
-            out[(long long)(e.start + i) * out_stride + h * DIM + lane * E + c] = l > 0.f ? acc[c] / l : (l == l ? 0.f : l);
-    }
-    if (lane == 0) paged_report(status, bad);
-}
-
 // ---------------------------------------------------------------- host
 int refuse(const char *call, const char *why) {
     fprintf(stderr, "%s: %s\n", call, why);
@@ -235,10 +172,44 @@ template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) 
     per = (per + kPdWarps - 1) / kPdWarps * kPdWarps;
     a.tiles_per_item = (int)per;
     a.splits = (int)((steps + per - 1) / per);
-    paged_scratch(gpu, a.splits > 1 ? items * a.splits * r : 0, DIM, items, &a.part, &a.ml, &a.counters);
+    unsigned *count;  // [0] takes the chunk kernel's wait errors when there is no status word
+    paged_scratch(gpu, a.splits > 1 ? items * a.splits * r : 0, DIM, items + 1, &a.part, &a.ml, &count);
+    a.counters = count + 1;
     const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
     if (r == 8) launch(paged_decode_kernel<KIND, DIM, 8>, grid, dim3(kPdThreads), 0, stream(), true, a);
     else launch(paged_decode_kernel<KIND, DIM, 16>, grid, dim3(kPdThreads), 0, stream(), true, a);
+}
+
+template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
+    const PagedView &v = a.v;
+    static PerDeviceOnce once;
+    once.run([] {
+        TCM_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<KIND, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)PcGeo<DIM>::kSmem));
+        // The warpgroups' register shares are taken from what the launch allots.
+        cudaFuncAttributes attr;
+        TCM_CUDA(cudaFuncGetAttributes(&attr, paged_chunk_kernel<KIND, DIM>));
+        if (attr.numRegs != kPcRegs) TCM_FATAL("paged attention: built with %d registers, not %d", attr.numRegs, kPcRegs);
+    });
+    a.row_tiles = (int)(((long long)v.max_new * a.group + kPcRows - 1) / kPcRows);
+    // Splits: the fewest rounds of the SMs, counting an item's start and end as three tiles.
+    const long long items = (long long)v.sequences * v.kvheads * a.row_tiles;
+    const long long tiles = (visible_rows(v, a.window, a.sinks) + kPcTile - 1) / kPcTile + 2;
+    a.splits = 1;
+    double best = 0;
+    for (int k = 1; k <= kPcSplitsMax && k * 2 <= tiles; k++) {
+        const double cost = (double)((items * k + sm_count() - 1) / sm_count()) * ((double)tiles / k + 3);
+        if (k == 1 || cost < 0.97 * best) {
+            best = cost;
+            a.splits = k;
+        }
+    }
+    unsigned *count;
+    paged_scratch(gpu, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, items + 1, &a.part, &a.ml, &count);
+    a.counters = count + 1;
+    a.err = a.status ? reinterpret_cast<unsigned *>(a.status) : count;
+    const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
+    launch(paged_chunk_kernel<KIND, DIM>, grid, dim3(kPcThreads), PcGeo<DIM>::kSmem, stream(), true, a);
 }
 
 unsigned blocks_of(long long items, int a_block) {
@@ -316,13 +287,11 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     PAGED_DISPATCH(view, CALL);
 #undef CALL
     if (view.max_new <= few) return 0;
-    const dim3 grid(blocks_of((long long)view.max_new * qheads, kRowThreads / 32), view.sequences);
-#define CALL(K, D)                                                                                                 \
-    paged_attention_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, out, out_stride, q, q_stride, qheads, window, \
-                                                                     sinks, scale2, few, status)
+    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, few, 1, 1, scale2, nullptr, nullptr,
+                        nullptr, status, nullptr};
+#define CALL(K, D) chunk_launch<K, D>(gpu, c)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
-    TCM_CUDA(cudaGetLastError());
     return 0;
 }
 

@@ -1,0 +1,594 @@
+// Attention of chunks of new rows over a paged K/V cache on the tcgen05 tensor
+// cores: prompts and long drafted runs, 256 query rows of one KV head a CTA.
+//
+// Row r of the KV head's chunk is new row r / group, query head r % group, so grouped
+// heads fill the tile whatever the group. Per tile of 128 cached rows
+//   S = Q K^T (tcgen05.mma, M = 128 twice, N = 128), P = exp2(S - m) (registers),
+//   O_t = P V (P from tensor memory), O = O c + O_t (registers).
+//
+// Four warpgroups: two for the softmax, one per 128 query rows (one row a thread, with
+// its output row in registers), one that turns stored rows into FP16 operand tiles in
+// shared memory (pages end anywhere, so rows are fetched by address), and one of which
+// a single thread issues the MMAs. While one warpgroup computes weights
+// the tensor cores run the other's products. A ring of three operand tiles holds
+// K(t + 1), V(t) and the next.
+//
+// Precision. Results are FP32, so a 16-bit rounding of Q or P would be visible:
+// both enter as two FP16 parts (22 bits) after scaling into FP16's range by powers
+// of two, against operands that are exact: a byte row is its codes, with the row's
+// scale applied to the column of S and to the weight; a BF16 row is the row divided
+// by the power of two below its largest element (2^-39 of that element at worst).
+// That doubles the products: half of the FP16 rate is the ceiling. The tensor cores
+// truncate when they add (measured: 4e-8 of the sum a step, 9e-6 after 8192
+// products), so every tile's P V starts from zero and is added in FP32 registers,
+// smaller parts first, instead of one long accumulation in tensor memory.
+#pragma once
+#include "paged_decode.cuh"
+#include "stream.cuh"
+#include "tc_gemm.cuh"
+
+namespace tcm {
+
+constexpr int kPcRows = 256, kPcTile = 128;   // query rows a CTA, cached rows a tile
+constexpr int kPcThreads = 512;
+constexpr int kPcSlots = 3;
+constexpr int kPcSplitsMax = 32;
+// Registers: four warpgroups are launched with 128 a thread; what the converters and the
+// issuing warp's group give away lets the softmax threads hold an output row. Each of the
+// SM's four register files holds one warp of each group: 200 + 200 + 64 + 48 = 4 x 128.
+constexpr int kPcRegs = 128, kPcSoftmaxRegs = 200, kPcConvertRegs = 64, kPcIssueRegs = 48;
+static_assert(2 * kPcSoftmaxRegs + kPcConvertRegs + kPcIssueRegs <= 4 * kPcRegs, "register split");
+constexpr unsigned kPagedWaitRanOut = 8u;     // status bit
+
+struct PagedChunkArgs {
+    PagedView v;
+    float *out;
+    const float *q;
+    long long out_stride, q_stride;
+    int group, window, sinks, few;
+    int row_tiles, splits;   // splits: of the tiles that a row tile sees
+    float scale2;
+    float *part;             // [item][256][DIM]
+    float2 *ml;              // [item][256]
+    unsigned *counters;      // [sequence][KV head][row tile]
+    int *status;
+    unsigned *err;           // where waits that run out are recorded (status, or scratch)
+};
+
+template <int DIM> struct PcGeo {
+    static constexpr uint32_t kHalf = 128 * 128;                  // bytes: 128 rows of 64 FP16 in the 128-byte swizzle
+    static constexpr int kHalves = DIM / 64;
+    static constexpr uint32_t kOperand = kHalves * kHalf;         // one 128-row operand tile
+    static constexpr uint32_t kQ = 4 * kOperand;                  // [row half][part]
+    static constexpr uint32_t kScales = kQ + kPcSlots * kOperand; // float [2 K|V][2][128]
+    static constexpr uint32_t kMisc = kScales + 2 * 2 * 128 * 4;
+    static constexpr size_t kSmem = kMisc + 256;
+    static constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | (8u << 24);                     // FP16, K-major
+    static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(DIM >> 3) << 17) | (8u << 24);  // B MN-major
+};
+struct PcMisc {  // in shared memory behind the scales
+    uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
+    uint32_t tmem;
+    int last;
+    uint32_t there[2][4];
+    float v_scale[2];
+    float vmax[2][4];
+};
+static_assert(sizeof(PcMisc) <= 256, "misc area");
+
+// B operand descriptor of a V tile (rows are keys, 128 bytes of 64 dims a row): MN-major
+// in the 128-byte swizzle, 8-key groups 1024 bytes apart, the next 64 dims one half on.
+__device__ __forceinline__ uint64_t pc_desc_v(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(PcGeo<128>::kHalf >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// 32 columns of this thread's tensor-memory lane, and the same back (16 columns).
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {  // results below 2^-126 are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Bounded wait of a whole warp, which leaves it converged: all lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsigned *err) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kPagedWaitRanOut));
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Byte offset of 16-byte piece `piece` of row `row` inside a 128-byte-swizzled half tile.
+__device__ __forceinline__ uint32_t pc_swizzle(int row, int piece) {
+    return (uint32_t)(row * 128 + ((piece ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void st_smem16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void st_smem8(uint32_t a, uint32_t x, uint32_t y) {
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+// Bits [0, n) of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Eight stored elements of a BF16 row (16 bytes), scaled, as FP16 pairs.
+__device__ __forceinline__ uint32_t bf16_pair_f16(uint32_t w, float scale) {
+    return pack_f16(bf16_lo(w) * scale, bf16_hi(w) * scale);
+}
+
+// The converters: operand tile `which` (0 K, 1 V) of 128 rows from `base` into the
+// shared-memory tile at `dst`, with its row scales. Warp w of the group takes rows
+// 32 w .. 32 w + 31, LPR lanes a row.
+template <int KIND, int DIM>
+struct PcConvert {
+    static constexpr int ES = KIND == kPagedBytes ? 1 : 2;
+    static constexpr int LPR = DIM * ES / 16;   // 16-byte pieces a row
+    static constexpr int RPL = 32 / LPR;        // rows a load instruction covers
+    static constexpr int LOADS = 32 / RPL;
+    static constexpr int BATCH = LOADS < 8 ? LOADS : 8;
+};
+
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedChunkArgs a) {
+    using G = PcGeo<DIM>;
+    constexpr bool kBytes = KIND == kPagedBytes;
+    extern __shared__ __align__(1024) unsigned char pc_smem[];
+    unsigned char *smem = pc_smem;
+    PcMisc &x = *reinterpret_cast<PcMisc *>(smem + G::kMisc);
+    float *scales = reinterpret_cast<float *>(smem + G::kScales);  // [K|V][tile parity][128]
+    const PagedView &v = a.v;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int s = blockIdx.z, h = blockIdx.y;
+    // The longest row tiles (the last ones) start first.
+    const int rt = a.row_tiles - 1 - (int)blockIdx.x / a.splits, sp = (int)blockIdx.x % a.splits;
+    pdl_wait();
+    PagedExtent e;
+    const int bad_extent = paged_extent(&v, s, &e);
+    if (bad_extent && !blockIdx.x && !h && !tid) paged_report(a.status, bad_extent);
+    if (e.count <= a.few) return;
+    const int rows = e.count * a.group, r0 = rt * kPcRows;
+    if (r0 >= rows) return;
+    const int origin = e.length - e.count;  // place of the first new row
+    const int live = min(kPcRows, rows - r0), halves = live > 128 ? 2 : 1;
+    const int first = origin + r0 / a.group, last = origin + (r0 + live - 1) / a.group;
+    const PagedTiles tiles = paged_tiles(first, last, a.window, a.sinks, 7);
+    const int splits = max(1, min(a.splits, tiles.count));
+    if (sp >= splits) return;
+    const int k0 = (int)((int64_t)tiles.count * sp / splits), n = (int)((int64_t)tiles.count * (sp + 1) / splits) - k0;
+
+    const uint32_t base_s = smem_addr(smem);
+    if (base_s & 1023u) {  // the swizzled tiles need it; a launch without static shared memory starts there
+        if (!tid) atomicOr(a.err, kPagedWaitRanOut);
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kPcSlots; i++) {
+            mbar_init(&x.full[i], 128);
+            mbar_init(&x.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&x.s_full[i], 1);
+            mbar_init(&x.p_full[i], 128);
+            mbar_init(&x.o_full[i], 1);
+            mbar_init(&x.ks_full[i], 128);
+            mbar_init(&x.vm_full[i], 4);
+            mbar_init(&x.vs_full[i], 128);
+        }
+        mbar_init(&x.q_full, halves * 128);
+        mbar_init(&x.done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&x.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = x.tmem;  // columns: S and P of half i at 128 i, O at 256 + 128 i
+
+    if (warp < 8) {
+        // ================================================================ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPcSoftmaxRegs));
+        const int i = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + i * 128 + row;
+        if (i < halves) {
+            // ---- Q: this warp's 32 rows as two FP16 parts, scaled by the row's power of two
+            float mine = 0.f;
+            for (int k = 0; k < 32; k++) {
+                const int rr = (warp & 3) * 32 + k, rg = r0 + i * 128 + rr;
+                constexpr int E = DIM / 32;
+                float f[E], m = 0.f;
+#pragma unroll
+                for (int c = 0; c < E; c++) f[c] = 0.f;
+                if (rg < rows) {
+                    const float *src = a.q + (long long)(e.start + rg / a.group) * a.q_stride +
+                                       (h * a.group + rg % a.group) * DIM + lane * E;
+                    if constexpr (E == 4) {
+                        const float4 t = *reinterpret_cast<const float4 *>(src);
+                        f[0] = t.x, f[1] = t.y, f[2] = t.z, f[3] = t.w;
+                    } else {
+                        const float2 t = *reinterpret_cast<const float2 *>(src);
+                        f[0] = t.x, f[1] = t.y;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(f[c]));
+                const int ex = exponent_of(warp_max(m)) - 14;
+                const float up = power_of_two(-ex);
+                if (lane == k) mine = a.scale2 * power_of_two(ex);
+                uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+                for (int c = 0; c < E; c += 2) {
+                    uint32_t p[2];
+                    split_pair<kPagedBytes>(f[c] * up, f[c + 1] * up, p);
+                    hi[c / 2] = p[0];
+                    lo[c / 2] = p[1];
+                }
+                const int d = lane * E;  // half tile, 16-byte piece, offset inside it
+                const uint32_t at = base_s + (uint32_t)(2 * i) * G::kOperand + (uint32_t)(d / 64) * G::kHalf +
+                                    pc_swizzle(rr, (d % 64) / 8) + (uint32_t)(d % 8) * 2;
+                if constexpr (E == 4) {
+                    st_smem8(at, hi[0], hi[1]);
+                    st_smem8(at + G::kOperand, lo[0], lo[1]);
+                } else {
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi[0]) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + G::kOperand), "r"(lo[0]) : "memory");
+                }
+            }
+            fence_async_smem();
+            mbar_arrive(&x.q_full);
+
+            const float qs = mine;
+            const int at = r < rows ? origin + r / a.group : -1;  // a row behind the last sees nothing
+            const int top_row = min(live, (i + 1) * 128) - 1;
+            const int first_i = origin + (r0 + i * 128) / a.group, last_i = origin + (r0 + top_row) / a.group;
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t ts = tmem + lanes + (uint32_t)(128 * i), to = tmem + lanes + 256u + (uint32_t)(128 * i);
+            float o[DIM], m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int c = 0; c < DIM; c++) o[c] = 0.f;
+            for (int t = 0; t < n; t++) {
+                const int base = paged_tile(tiles, k0 + t) * kPcTile, par = t & 1;
+                const float *ks = scales + par * 128, *vs = scales + 256 + par * 128;
+                if (!warp_wait(&x.ks_full[par], (t >> 1) & 1, a.err)) break;
+                if (!warp_wait(&x.s_full[i], t & 1, a.err)) break;
+                tc_fence_after();
+                uint32_t vis[4];
+#pragma unroll
+                for (int w = 0; w < 4; w++) vis[w] = x.there[par][w];
+                // Every row of this half sees the whole tile?
+                const bool full = (vis[0] & vis[1] & vis[2] & vis[3]) == 0xffffffffu && base + 127 <= first_i &&
+                                  (a.window == 0 || base + 127 < a.sinks || base > last_i - a.window);
+                if (!full) {
+                    const int hi = at - base + 1, lo = a.window == 0 || a.window > at ? 0 : at - a.window - base + 1,
+                              sk = a.sinks - base;
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        vis[w] &= bits_below(hi - 32 * w) & (~bits_below(lo - 32 * w) | bits_below(sk - 32 * w));
+                }
+                // ---- the row's maximum
+                float2 mx = make_float2(-INFINITY, -INFINITY);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float f[32];
+                    tc_ld32(ts + 32 * c, f);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                        float2 y0 = __fmul2_rn(make_float2(f[j], f[j + 1]), make_float2(k4.x, k4.y));
+                        float2 y1 = __fmul2_rn(make_float2(f[j + 2], f[j + 3]), make_float2(k4.z, k4.w));
+                        if (!full) {
+                            y0.x = (vis[c] >> j) & 1 ? y0.x : -INFINITY;
+                            y0.y = (vis[c] >> (j + 1)) & 1 ? y0.y : -INFINITY;
+                            y1.x = (vis[c] >> (j + 2)) & 1 ? y1.x : -INFINITY;
+                            y1.y = (vis[c] >> (j + 3)) & 1 ? y1.y : -INFINITY;
+                        }
+                        mx.x = fmaxf(mx.x, fmaxf(y0.x, y0.y));
+                        mx.y = fmaxf(mx.y, fmaxf(y1.x, y1.y));
+                    }
+                }
+                const float m_new = fmaxf(m, fmaxf(mx.x, mx.y) * qs);
+                const float mr = m_new == -INFINITY ? 0.f : m_new;
+                const float keep = m == -INFINITY ? 0.f : ex2(m - mr);
+                m = m_new;
+                if (!warp_wait(&x.vs_full[par], (t >> 1) & 1, a.err)) break;
+                const float v_scale = x.v_scale[par];
+                // ---- weights, over the scores they come from: 32 columns of S become two MMA k-steps
+                // of first parts and two of second parts
+                float2 sum = make_float2(0.f, 0.f);
+                const float2 qs2 = make_float2(qs, qs), mr2 = make_float2(-mr, -mr);
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float f[32];
+                    uint32_t hi[16], lo[16];
+                    tc_ld32(ts + 32 * c, f);
+                    const uint32_t seen = vis[0];
+                    vis[0] = vis[1], vis[1] = vis[2], vis[2] = vis[3];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
+                        const float4 v4 = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float2 kk = u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
+                            const float2 vv = u ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                            const int b = j + 2 * u;
+                            const float2 y = __ffma2_rn(__fmul2_rn(make_float2(f[b], f[b + 1]), kk), qs2, mr2);
+                            float2 p = make_float2(ex2(y.x), ex2(y.y));
+                            if (!full) {
+                                p.x = (seen >> b) & 1 ? p.x : 0.f;
+                                p.y = (seen >> (b + 1)) & 1 ? p.y : 0.f;
+                            }
+                            sum = __fadd2_rn(sum, p);
+                            float2 w = __fmul2_rn(p, vv);
+                            if (!full) {  // a non-finite scale of a row not seen
+                                w.x = (seen >> b) & 1 ? w.x : 0.f;
+                                w.y = (seen >> (b + 1)) & 1 ? w.y : 0.f;
+                            }
+                            uint32_t parts[2];
+                            split_pair<kPagedBytes>(w.x, w.y, parts);
+                            hi[b / 2] = parts[0];
+                            lo[b / 2] = parts[1];
+                        }
+                    }
+                    tc_st16(ts + 32 * c, hi);
+                    tc_st16(ts + 32 * c + 16, lo);
+                }
+                l = fmaf(l, keep, sum.x + sum.y);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                mbar_arrive(&x.p_full[i]);
+                // ---- this tile's output
+                if (!warp_wait(&x.o_full[i], t & 1, a.err)) break;
+                tc_fence_after();
+                const float2 keep2 = make_float2(keep, keep), vsc2 = make_float2(v_scale, v_scale);
+#pragma unroll
+                for (int c = 0; c < DIM / 32; c++) {
+                    float f[32];
+                    tc_ld32(to + 32 * c, f);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 y = __ffma2_rn(make_float2(f[j], f[j + 1]), vsc2,
+                                                    __fmul2_rn(make_float2(o[32 * c + j], o[32 * c + j + 1]), keep2));
+                        o[32 * c + j] = y.x;
+                        o[32 * c + j + 1] = y.y;
+                    }
+                }
+                tc_fence_before();
+            }
+            if (r < rows) {
+                float *dst;
+                float f = 1.f;
+                if (splits == 1) {
+                    dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM;
+                    f = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
+                } else {
+                    const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits + sp;
+                    dst = a.part + (item * kPcRows + (r - r0)) * DIM;
+                    a.ml[item * kPcRows + (r - r0)] = make_float2(m, l);
+                }
+#pragma unroll
+                for (int c = 0; c < DIM; c += 4)
+                    *reinterpret_cast<float4 *>(dst + c) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+            }
+        }
+    } else if (warp < 12) {
+        // ================================================================ stored rows -> operand tiles
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcConvertRegs));
+        using C = PcConvert<KIND, DIM>;
+        const int w = warp - 8, piece = lane % C::LPR, sub = lane / C::LPR;
+        const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
+        int bad = 0;
+        bool ok = true;
+        for (int t = 0; t < n && ok; t++) {
+            const int base = paged_tile(tiles, k0 + t) * kPcTile, par = t & 1;
+            // This lane's row: place base + 32 w + lane.
+            const int j = base + 32 * w + lane;
+            int64_t mine = -1;
+            if (j <= last) {
+                const int pg = paged_div(&v, j);
+                mine = paged_row(&v, v.table[(int64_t)s * v.table_stride + pg], j, pg, h);
+                // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
+                if (mine < 0 && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) bad |= kPagedBadPage;
+            }
+            const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0);
+#pragma unroll 1
+            for (int which = 0; which < 2; which++) {
+                const char *pool = static_cast<const char *>(which ? v.values : v.keys);
+                const int use = 2 * t + which, slot = use % kPcSlots;
+                const uint32_t dst = base_s + G::kQ + (uint32_t)slot * G::kOperand;
+                float scale = 0.f;
+                if (kBytes && mine >= 0) scale = __ldcg(v.scales + (which ? half : 0) + mine);
+#pragma unroll 1
+                for (int b = 0; b < C::LOADS; b += C::BATCH) {
+                    uint4 in[C::BATCH];
+#pragma unroll
+                    for (int k = 0; k < C::BATCH; k++) {
+                        const int64_t rk = __shfl_sync(0xffffffffu, mine, (b + k) * C::RPL + sub);
+                        in[k] = rk >= 0 ? ld_row16(pool + rk * (DIM * C::ES) + piece * 16) : make_uint4(0, 0, 0, 0);
+                    }
+                    if (b == 0 && use >= kPcSlots) {  // the slot's last use is over
+                        ok = warp_wait(&x.empty[slot], ((use / kPcSlots) & 1) ^ 1, a.err);
+                        if (!ok) break;
+                    }
+#pragma unroll
+                    for (int k = 0; k < C::BATCH; k++) {
+                        const int rl = (b + k) * C::RPL + sub, rr = 32 * w + rl;
+                        uint4 y = in[k];
+                        if constexpr (kBytes) {
+                            // 16 codes: dims 16 piece ..: two 16-byte pieces of FP16.
+                            const int d = piece * 16;
+                            const uint32_t at = dst + (uint32_t)(d / 64) * G::kHalf;
+                            const uint32_t q0 = y.x ^ 0x80808080u, q1 = y.y ^ 0x80808080u, q2 = y.z ^ 0x80808080u,
+                                           q3 = y.w ^ 0x80808080u;
+                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8), codes_f16(q0, 0x4140), codes_f16(q0, 0x4342),
+                                      codes_f16(q1, 0x4140), codes_f16(q1, 0x4342));
+                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8 + 1), codes_f16(q2, 0x4140), codes_f16(q2, 0x4342),
+                                      codes_f16(q3, 0x4140), codes_f16(q3, 0x4342));
+                        } else {
+                            // The row's largest magnitude as bits, over its lanes.
+                            uint32_t mb = __vmaxu2(__vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu),
+                                                   __vmaxu2(y.z & 0x7fff7fffu, y.w & 0x7fff7fffu));
+                            mb = max(mb & 0xffffu, mb >> 16);
+#pragma unroll
+                            for (int off = C::LPR / 2; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
+                            const int ef = (int)(mb >> 7);
+                            int ex = (ef == 0 || ef == 255 ? 0 : ef - 127) - 14;
+                            ex = max(-126, min(126, ex));
+                            const float up = power_of_two(-ex);
+                            // A non-finite V row enters as zeros with a NaN weight: only who sees it is touched.
+                            if (ef == 255 && which) y = make_uint4(0, 0, 0, 0);
+                            const float rs = __shfl_sync(0xffffffffu, ef == 255 && which ? __uint_as_float(0x7fc00000u) : power_of_two(ex),
+                                                         (lane % C::RPL) * C::LPR);
+                            if (lane / C::RPL == b + k) scale = rs;  // row rl = (b + k) RPL + lane % RPL is this lane's
+                            const int d = piece * 8;
+                            st_smem16(dst + (uint32_t)(d / 64) * G::kHalf + pc_swizzle(rr, (d % 64) / 8),
+                                      bf16_pair_f16(y.x, up), bf16_pair_f16(y.y, up), bf16_pair_f16(y.z, up),
+                                      bf16_pair_f16(y.w, up));
+                        }
+                    }
+                }
+                if (!ok) break;
+                fence_async_smem();
+                mbar_arrive(&x.full[slot]);
+                if (!which) {
+                    scales[par * 128 + 32 * w + lane] = mine >= 0 ? scale : 0.f;
+                    if (lane == 0) x.there[par][w] = there;
+                    mbar_arrive(&x.ks_full[par]);
+                } else {
+                    // Weights are scaled by the tile's largest V scale: p s 2^14 / R < 2^14.
+                    if (mine < 0) scale = 0.f;
+                    const float top = warp_max(isfinite(scale) ? scale : 0.f);
+                    if (lane == 0) {
+                        x.vmax[par][w] = top;
+                        mbar_arrive(&x.vm_full[par]);
+                    }
+                    ok = warp_wait(&x.vm_full[par], (t >> 1) & 1, a.err);
+                    if (!ok) break;
+                    const float vmax = fmaxf(fmaxf(x.vmax[par][0], x.vmax[par][1]), fmaxf(x.vmax[par][2], x.vmax[par][3]));
+                    const int er = max(-100, exponent_of(vmax) + 1) - 14;
+                    scales[256 + par * 128 + 32 * w + lane] = scale * power_of_two(-er);
+                    if (w == 0 && lane == 0) x.v_scale[par] = power_of_two(er);
+                    mbar_arrive(&x.vs_full[par]);
+                }
+            }
+        }
+        if (bad) paged_report(a.status, bad);
+    } else {
+        // ================================================================ MMA
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcIssueRegs));
+    }
+    if (warp == 12 && lane == 0) {
+        const uint32_t ring = base_s + G::kQ;
+        bool ok = mbar_wait(&x.q_full, 0, a.err, kPagedWaitRanOut);
+        auto scores = [&](int t, int i) {  // S_i = Q_i K(t)^T
+            const int use = 2 * t, slot = use % kPcSlots;
+            if (!mbar_wait(&x.full[slot], (use / kPcSlots) & 1, a.err, kPagedWaitRanOut)) return false;
+            // P_i(t - 1) lies in the same columns: its product must be over.
+            if (t && !mbar_wait(&x.o_full[i], (t - 1) & 1, a.err, kPagedWaitRanOut)) return false;
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(128 * i);
+#pragma unroll
+            for (int part = 1; part >= 0; part--)
+#pragma unroll
+                for (int ks = 0; ks < DIM / 16; ks++) {
+                    const uint32_t off = (uint32_t)(ks / 4) * G::kHalf;
+                    tc_mma(d, tc_desc(base_s + (uint32_t)(2 * i + part) * G::kOperand + off) + 2 * (ks % 4),
+                           tc_desc(ring + (uint32_t)slot * G::kOperand + off) + 2 * (ks % 4), G::kIdescS,
+                           part == 1 && ks == 0 ? 0u : 1u);
+                }
+            tc_commit(&x.s_full[i]);
+            if (i == halves - 1) tc_commit(&x.empty[slot]);
+            return true;
+        };
+        for (int i = 0; i < halves && ok && n > 0; i++) ok = scores(0, i);
+        for (int t = 0; t < n && ok; t++)
+            for (int i = 0; i < halves && ok; i++) {
+                const int use = 2 * t + 1, slot = use % kPcSlots;
+                if (!mbar_wait(&x.full[slot], (use / kPcSlots) & 1, a.err, kPagedWaitRanOut) ||
+                    !mbar_wait(&x.p_full[i], t & 1, a.err, kPagedWaitRanOut)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem + 256u + (uint32_t)(128 * i), p = tmem + (uint32_t)(128 * i);
+                const uint64_t vd = pc_desc_v(ring + (uint32_t)slot * G::kOperand);
+#pragma unroll
+                for (int part = 1; part >= 0; part--)
+#pragma unroll
+                    for (int ks = 0; ks < kPcTile / 16; ks++)  // 16 keys: 2048 bytes on in V, 8 columns on in P
+                        tc_mma_ts(d, p + 32 * (ks / 2) + 8 * (ks % 2) + 16 * part, vd + (uint64_t)(128 * ks), G::kIdescO,
+                                  part == 1 && ks == 0 ? 0u : 1u);
+                tc_commit(&x.o_full[i]);
+                if (i == halves - 1) tc_commit(&x.empty[slot]);
+                if (t + 1 < n) ok = scores(t + 1, i);
+            }
+        // Every product and arrival is over before tensor memory and the barriers are given back.
+        tc_commit(&x.done);
+        mbar_wait(&x.done, 0, a.err, kPagedWaitRanOut);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+    if (splits == 1) return;
+
+    // ---- the last split of the row tile to arrive adds all of them, in order
+    __threadfence();
+    __syncthreads();
+    unsigned *counter = &a.counters[((int64_t)s * v.kvheads + h) * a.row_tiles + rt];
+    if (tid == 0) x.last = atomicAdd(counter, 1u) == (unsigned)(splits - 1);
+    __syncthreads();
+    if (!x.last) return;
+    __threadfence();
+    if (tid == 0) *counter = 0u;
+    const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits;
+    for (int rr = warp; rr < live; rr += kPcThreads / 32) {
+        float top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < splits; w++) top = fmaxf(top, __ldcg(&a.ml[(item + w) * kPcRows + rr]).x);
+        constexpr int E = DIM / 32;
+        float y[E];
+#pragma unroll
+        for (int c = 0; c < E; c++) y[c] = 0.f;
+        for (int w = 0; w < splits; w++) {
+            const float2 ml = __ldcg(&a.ml[(item + w) * kPcRows + rr]);
+            const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            const float *src = a.part + ((item + w) * kPcRows + rr) * DIM + lane * E;
+#pragma unroll
+            for (int c = 0; c < E; c++) y[c] = fmaf(__ldcg(src + c), f, y[c]);
+        }
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+        const int r = r0 + rr;
+        float *dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
+#pragma unroll
+        for (int c = 0; c < E; c++) dst[c] = y[c] * inv;
+    }
+}
+
+}  // namespace tcm
