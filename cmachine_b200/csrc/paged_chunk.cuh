@@ -82,42 +82,76 @@ __device__ __forceinline__ uint64_t pc_desc_v(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(PcGeo<128>::kHalf >> 4) << 16) |
            ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// MMAs issued by one elected thread of a converged warp (their operands stay in uniform
+// registers; issued from a one-lane branch they took 87 cycles each instead of 64). A from
+// shared memory, and from tensor memory.
+__device__ __forceinline__ void pc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-// 32 columns of this thread's tensor-memory lane, and the same back (16 columns).
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+__device__ __forceinline__ void pc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pc_commit(uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+        : "memory");
+}
+// 16 columns of this thread's tensor-memory lane: the load (complete after tc_wait_ld), and
+// eight columns back.
+__device__ __forceinline__ void tc_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// The registers pass through the wait, so nothing reads them before it.
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ float2 as_pair(uint32_t x, uint32_t y) {
+    return make_float2(__uint_as_float(x), __uint_as_float(y));
 }
 __device__ __forceinline__ float ex2(float x) {  // results below 2^-126 are zero
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Bounded wait of a whole warp, which leaves it converged: all lanes go on, or none.
+// Bounded wait. The timer is read once in 256 tries: reading it takes longer than these
+// waits usually last, and the barrier completing meanwhile would go unnoticed.
+__device__ __forceinline__ bool pc_wait(uint64_t *bar, uint32_t parity, unsigned *err) {
+    unsigned long long start = 0;
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 256; i++)
+            if (mbar_try(bar, parity)) return true;
+        const unsigned long long now = global_ns();
+        if (!start) start = now;
+        if (wait_expired(now - start)) {
+            atomicOr(err, kPagedWaitRanOut);
+            return false;
+        }
+    }
+}
+// The same of a whole warp, which leaves it converged: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, unsigned *err) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, kPagedWaitRanOut));
+    return __all_sync(0xffffffffu, pc_wait(bar, parity, err));
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Byte offset of 16-byte piece `piece` of row `row` inside a 128-byte-swizzled half tile.
@@ -149,6 +183,84 @@ struct PcConvert {
     static constexpr int LOADS = 32 / RPL;
     static constexpr int BATCH = LOADS < 8 ? LOADS : 8;
 };
+
+// The largest of a row's 128 scores times their K scales; MASKED leaves out columns whose
+// bit of vis is clear. Each 16 columns are loaded while the ones before are used.
+template <bool MASKED> __device__ __forceinline__ float pc_row_max(uint32_t ts, const float *ks, const uint32_t (&vis)[4]) {
+    uint32_t buf[2][16];
+    float a = -INFINITY, b = -INFINITY;
+    tc_ld16_async(ts, buf[0]);
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        uint32_t(&f)[16] = buf[c & 1];
+        tc_wait_ld(f);
+        if (c < 7) tc_ld16_async(ts + 16 * (c + 1), buf[(c + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + j);
+            float2 y0 = __fmul2_rn(as_pair(f[j], f[j + 1]), make_float2(k4.x, k4.y));
+            float2 y1 = __fmul2_rn(as_pair(f[j + 2], f[j + 3]), make_float2(k4.z, k4.w));
+            if (MASKED) {
+                const uint32_t seen = vis[c / 2] >> (16 * (c & 1) + j);
+                y0.x = seen & 1 ? y0.x : -INFINITY;
+                y0.y = seen & 2 ? y0.y : -INFINITY;
+                y1.x = seen & 4 ? y1.x : -INFINITY;
+                y1.y = seen & 8 ? y1.y : -INFINITY;
+            }
+            a = fmaxf(a, fmaxf(y0.x, y0.y));
+            b = fmaxf(b, fmaxf(y1.x, y1.y));
+        }
+    }
+    return fmaxf(a, b);
+}
+// The row's weights over the scores they come from, and their sum before the V scales: the 16
+// columns of an MMA k-step become eight of first parts and eight of second parts.
+template <bool MASKED>
+__device__ __forceinline__ float pc_row_weights(uint32_t ts, const float *ks, const float *vs, float qs, float m,
+                                                const uint32_t (&vis)[4]) {
+    uint32_t buf[2][16];
+    float2 sum = make_float2(0.f, 0.f);
+    const float2 qs2 = make_float2(qs, qs), m2 = make_float2(-m, -m);
+    tc_ld16_async(ts, buf[0]);
+#pragma unroll
+    for (int c = 0; c < 8; c++) {
+        uint32_t(&f)[16] = buf[c & 1];
+        uint32_t hi[8], lo[8];
+        tc_wait_ld(f);
+        if (c < 7) tc_ld16_async(ts + 16 * (c + 1), buf[(c + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + j);
+            const float4 v4 = *reinterpret_cast<const float4 *>(vs + 16 * c + j);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int b = j + 2 * u;
+                const float2 kk = u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
+                const float2 vv = u ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                const float2 y = __ffma2_rn(__fmul2_rn(as_pair(f[b], f[b + 1]), kk), qs2, m2);
+                float2 p = make_float2(ex2(y.x), ex2(y.y)), w;
+                const uint32_t seen = vis[c / 2] >> (16 * (c & 1) + b);
+                if (MASKED) {
+                    p.x = seen & 1 ? p.x : 0.f;
+                    p.y = seen & 2 ? p.y : 0.f;
+                }
+                sum = __fadd2_rn(sum, p);
+                w = __fmul2_rn(p, vv);
+                if (MASKED) {  // the scale of a row not seen may be anything
+                    w.x = seen & 1 ? w.x : 0.f;
+                    w.y = seen & 2 ? w.y : 0.f;
+                }
+                uint32_t parts[2];
+                split_pair<kPagedBytes>(w.x, w.y, parts);
+                hi[b / 2] = parts[0];
+                lo[b / 2] = parts[1];
+            }
+        }
+        tc_st8(ts + 16 * c, hi);
+        tc_st8(ts + 16 * c + 8, lo);
+    }
+    return sum.x + sum.y;
+}
 
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedChunkArgs a) {
@@ -216,45 +328,53 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         if (i < halves) {
             // ---- Q: this warp's 32 rows as two FP16 parts, scaled by the row's power of two
             float mine = 0.f;
-            for (int k = 0; k < 32; k++) {
-                const int rr = (warp & 3) * 32 + k, rg = r0 + i * 128 + rr;
-                constexpr int E = DIM / 32;
-                float f[E], m = 0.f;
+            constexpr int E = DIM / 32, QB = 16;  // rows whose loads are in flight together
+            const long long q_at = r < rows ? (long long)(e.start + r / a.group) * a.q_stride + (h * a.group + r % a.group) * DIM : -1;
+#pragma unroll 1
+            for (int first_k = 0; first_k < 32; first_k += QB) {
+                float f[QB][E];
 #pragma unroll
-                for (int c = 0; c < E; c++) f[c] = 0.f;
-                if (rg < rows) {
-                    const float *src = a.q + (long long)(e.start + rg / a.group) * a.q_stride +
-                                       (h * a.group + rg % a.group) * DIM + lane * E;
-                    if constexpr (E == 4) {
-                        const float4 t = *reinterpret_cast<const float4 *>(src);
-                        f[0] = t.x, f[1] = t.y, f[2] = t.z, f[3] = t.w;
-                    } else {
-                        const float2 t = *reinterpret_cast<const float2 *>(src);
-                        f[0] = t.x, f[1] = t.y;
+                for (int k = 0; k < QB; k++) {
+                    const long long at = __shfl_sync(0xffffffffu, q_at, first_k + k);
+#pragma unroll
+                    for (int c = 0; c < E; c++) f[k][c] = 0.f;
+                    if (at >= 0) {
+                        const float *src = a.q + at + lane * E;
+                        if constexpr (E == 4) {
+                            const float4 t = *reinterpret_cast<const float4 *>(src);
+                            f[k][0] = t.x, f[k][1] = t.y, f[k][2] = t.z, f[k][3] = t.w;
+                        } else {
+                            const float2 t = *reinterpret_cast<const float2 *>(src);
+                            f[k][0] = t.x, f[k][1] = t.y;
+                        }
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(f[c]));
-                const int ex = exponent_of(warp_max(m)) - 14;
-                const float up = power_of_two(-ex);
-                if (lane == k) mine = a.scale2 * power_of_two(ex);
-                uint32_t hi[E / 2], lo[E / 2];
+                for (int k = 0; k < QB; k++) {
+                    float m = 0.f;
 #pragma unroll
-                for (int c = 0; c < E; c += 2) {
-                    uint32_t p[2];
-                    split_pair<kPagedBytes>(f[c] * up, f[c + 1] * up, p);
-                    hi[c / 2] = p[0];
-                    lo[c / 2] = p[1];
-                }
-                const int d = lane * E;  // half tile, 16-byte piece, offset inside it
-                const uint32_t at = base_s + (uint32_t)(2 * i) * G::kOperand + (uint32_t)(d / 64) * G::kHalf +
-                                    pc_swizzle(rr, (d % 64) / 8) + (uint32_t)(d % 8) * 2;
-                if constexpr (E == 4) {
-                    st_smem8(at, hi[0], hi[1]);
-                    st_smem8(at + G::kOperand, lo[0], lo[1]);
-                } else {
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi[0]) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + G::kOperand), "r"(lo[0]) : "memory");
+                    for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(f[k][c]));
+                    const int ex = exponent_of(warp_max(m)) - 14;
+                    const float up = power_of_two(-ex);
+                    if (lane == first_k + k) mine = a.scale2 * power_of_two(ex);
+                    uint32_t hi[E / 2], lo[E / 2];
+#pragma unroll
+                    for (int c = 0; c < E; c += 2) {
+                        uint32_t p[2];
+                        split_pair<kPagedBytes>(f[k][c] * up, f[k][c + 1] * up, p);
+                        hi[c / 2] = p[0];
+                        lo[c / 2] = p[1];
+                    }
+                    const int d = lane * E, rr = (warp & 3) * 32 + first_k + k;  // half tile, 16-byte piece, offset inside it
+                    const uint32_t at = base_s + (uint32_t)(2 * i) * G::kOperand + (uint32_t)(d / 64) * G::kHalf +
+                                        pc_swizzle(rr, (d % 64) / 8) + (uint32_t)(d % 8) * 2;
+                    if constexpr (E == 4) {
+                        st_smem8(at, hi[0], hi[1]);
+                        st_smem8(at + G::kOperand, lo[0], lo[1]);
+                    } else {
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi[0]) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + G::kOperand), "r"(lo[0]) : "memory");
+                    }
                 }
             }
             fence_async_smem();
@@ -288,75 +408,15 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     for (int w = 0; w < 4; w++)
                         vis[w] &= bits_below(hi - 32 * w) & (~bits_below(lo - 32 * w) | bits_below(sk - 32 * w));
                 }
-                // ---- the row's maximum
-                float2 mx = make_float2(-INFINITY, -INFINITY);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float f[32];
-                    tc_ld32(ts + 32 * c, f);
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                        float2 y0 = __fmul2_rn(make_float2(f[j], f[j + 1]), make_float2(k4.x, k4.y));
-                        float2 y1 = __fmul2_rn(make_float2(f[j + 2], f[j + 3]), make_float2(k4.z, k4.w));
-                        if (!full) {
-                            y0.x = (vis[c] >> j) & 1 ? y0.x : -INFINITY;
-                            y0.y = (vis[c] >> (j + 1)) & 1 ? y0.y : -INFINITY;
-                            y1.x = (vis[c] >> (j + 2)) & 1 ? y1.x : -INFINITY;
-                            y1.y = (vis[c] >> (j + 3)) & 1 ? y1.y : -INFINITY;
-                        }
-                        mx.x = fmaxf(mx.x, fmaxf(y0.x, y0.y));
-                        mx.y = fmaxf(mx.y, fmaxf(y1.x, y1.y));
-                    }
-                }
-                const float m_new = fmaxf(m, fmaxf(mx.x, mx.y) * qs);
+                const float top = full ? pc_row_max<false>(ts, ks, vis) : pc_row_max<true>(ts, ks, vis);
+                const float m_new = fmaxf(m, top * qs);
                 const float mr = m_new == -INFINITY ? 0.f : m_new;
                 const float keep = m == -INFINITY ? 0.f : ex2(m - mr);
                 m = m_new;
                 if (!warp_wait(&x.vs_full[par], (t >> 1) & 1, a.err)) break;
                 const float v_scale = x.v_scale[par];
-                // ---- weights, over the scores they come from: 32 columns of S become two MMA k-steps
-                // of first parts and two of second parts
-                float2 sum = make_float2(0.f, 0.f);
-                const float2 qs2 = make_float2(qs, qs), mr2 = make_float2(-mr, -mr);
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    float f[32];
-                    uint32_t hi[16], lo[16];
-                    tc_ld32(ts + 32 * c, f);
-                    const uint32_t seen = vis[0];
-                    vis[0] = vis[1], vis[1] = vis[2], vis[2] = vis[3];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4 *>(ks + 32 * c + j);
-                        const float4 v4 = *reinterpret_cast<const float4 *>(vs + 32 * c + j);
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const float2 kk = u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
-                            const float2 vv = u ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
-                            const int b = j + 2 * u;
-                            const float2 y = __ffma2_rn(__fmul2_rn(make_float2(f[b], f[b + 1]), kk), qs2, mr2);
-                            float2 p = make_float2(ex2(y.x), ex2(y.y));
-                            if (!full) {
-                                p.x = (seen >> b) & 1 ? p.x : 0.f;
-                                p.y = (seen >> (b + 1)) & 1 ? p.y : 0.f;
-                            }
-                            sum = __fadd2_rn(sum, p);
-                            float2 w = __fmul2_rn(p, vv);
-                            if (!full) {  // a non-finite scale of a row not seen
-                                w.x = (seen >> b) & 1 ? w.x : 0.f;
-                                w.y = (seen >> (b + 1)) & 1 ? w.y : 0.f;
-                            }
-                            uint32_t parts[2];
-                            split_pair<kPagedBytes>(w.x, w.y, parts);
-                            hi[b / 2] = parts[0];
-                            lo[b / 2] = parts[1];
-                        }
-                    }
-                    tc_st16(ts + 32 * c, hi);
-                    tc_st16(ts + 32 * c + 16, lo);
-                }
-                l = fmaf(l, keep, sum.x + sum.y);
+                const float sum = full ? pc_row_weights<false>(ts, ks, vs, qs, mr, vis) : pc_row_weights<true>(ts, ks, vs, qs, mr, vis);
+                l = fmaf(l, keep, sum);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 mbar_arrive(&x.p_full[i]);
@@ -364,34 +424,47 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                 if (!warp_wait(&x.o_full[i], t & 1, a.err)) break;
                 tc_fence_after();
                 const float2 keep2 = make_float2(keep, keep), vsc2 = make_float2(v_scale, v_scale);
+                uint32_t buf[2][16];
+                tc_ld16_async(to, buf[0]);
 #pragma unroll
-                for (int c = 0; c < DIM / 32; c++) {
-                    float f[32];
-                    tc_ld32(to + 32 * c, f);
+                for (int c = 0; c < DIM / 16; c++) {
+                    uint32_t(&f)[16] = buf[c & 1];
+                    tc_wait_ld(f);
+                    if (c + 1 < DIM / 16) tc_ld16_async(to + 16 * (c + 1), buf[(c + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 y = __ffma2_rn(make_float2(f[j], f[j + 1]), vsc2,
-                                                    __fmul2_rn(make_float2(o[32 * c + j], o[32 * c + j + 1]), keep2));
-                        o[32 * c + j] = y.x;
-                        o[32 * c + j + 1] = y.y;
+                    for (int j = 0; j < 16; j += 2) {
+                        const float2 y = __ffma2_rn(as_pair(f[j], f[j + 1]), vsc2,
+                                                    __fmul2_rn(make_float2(o[16 * c + j], o[16 * c + j + 1]), keep2));
+                        o[16 * c + j] = y.x;
+                        o[16 * c + j + 1] = y.y;
                     }
                 }
                 tc_fence_before();
             }
-            if (r < rows) {
-                float *dst;
-                float f = 1.f;
-                if (splits == 1) {
-                    dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM;
-                    f = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
-                } else {
-                    const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits + sp;
-                    dst = a.part + (item * kPcRows + (r - r0)) * DIM;
-                    a.ml[item * kPcRows + (r - r0)] = make_float2(m, l);
-                }
+            // ---- rows out, through this half's part of the Q area (its products are over) so that a
+            // warp writes whole rows
+            const float f = splits > 1 ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
+            const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits + sp;
+            if (splits > 1 && r < rows) a.ml[item * kPcRows + (r - r0)] = make_float2(m, l);
+            constexpr int PR = DIM / 4;  // 16-byte pieces a row
+            const uint32_t area = base_s + (uint32_t)(2 * i) * G::kOperand + (uint32_t)((warp & 3) * 32 * DIM * 4);
 #pragma unroll
-                for (int c = 0; c < DIM; c += 4)
-                    *reinterpret_cast<float4 *>(dst + c) = make_float4(o[c] * f, o[c + 1] * f, o[c + 2] * f, o[c + 3] * f);
+            for (int c = 0; c < PR; c++)
+                st_smem16(area + (uint32_t)(lane * PR + (c ^ (lane & (PR - 1)))) * 16, __float_as_uint(o[4 * c] * f),
+                          __float_as_uint(o[4 * c + 1] * f), __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f));
+            __syncwarp();
+            const long long mine_at = splits > 1 ? (item * kPcRows + (r - r0)) * DIM
+                                                 : (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM;
+            float *dst = splits > 1 ? a.part : a.out;
+#pragma unroll 4
+            for (int k = 0; k < 32; k += 32 / PR) {
+                const int rr = k + lane / PR, c = lane % PR;
+                const long long at_row = __shfl_sync(0xffffffffu, mine_at, rr);
+                uint4 y;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                             : "r"(area + (uint32_t)(rr * PR + (c ^ (rr & (PR - 1)))) * 16));
+                if (r - lane + rr < rows) *reinterpret_cast<uint4 *>(dst + at_row + c * 4) = y;
             }
         }
     } else if (warp < 12) {
@@ -500,14 +573,14 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         // ================================================================ MMA
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPcIssueRegs));
     }
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
         const uint32_t ring = base_s + G::kQ;
-        bool ok = mbar_wait(&x.q_full, 0, a.err, kPagedWaitRanOut);
+        bool ok = warp_wait(&x.q_full, 0, a.err);
         auto scores = [&](int t, int i) {  // S_i = Q_i K(t)^T
             const int use = 2 * t, slot = use % kPcSlots;
-            if (!mbar_wait(&x.full[slot], (use / kPcSlots) & 1, a.err, kPagedWaitRanOut)) return false;
+            if (!warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err)) return false;
             // P_i(t - 1) lies in the same columns: its product must be over.
-            if (t && !mbar_wait(&x.o_full[i], (t - 1) & 1, a.err, kPagedWaitRanOut)) return false;
+            if (t && !warp_wait(&x.o_full[i], (t - 1) & 1, a.err)) return false;
             tc_fence_after();
             const uint32_t d = tmem + (uint32_t)(128 * i);
 #pragma unroll
@@ -515,20 +588,20 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
 #pragma unroll
                 for (int ks = 0; ks < DIM / 16; ks++) {
                     const uint32_t off = (uint32_t)(ks / 4) * G::kHalf;
-                    tc_mma(d, tc_desc(base_s + (uint32_t)(2 * i + part) * G::kOperand + off) + 2 * (ks % 4),
+                    pc_mma_ss(d, tc_desc(base_s + (uint32_t)(2 * i + part) * G::kOperand + off) + 2 * (ks % 4),
                            tc_desc(ring + (uint32_t)slot * G::kOperand + off) + 2 * (ks % 4), G::kIdescS,
                            part == 1 && ks == 0 ? 0u : 1u);
                 }
-            tc_commit(&x.s_full[i]);
-            if (i == halves - 1) tc_commit(&x.empty[slot]);
+            pc_commit(&x.s_full[i]);
+            if (i == halves - 1) pc_commit(&x.empty[slot]);
             return true;
         };
         for (int i = 0; i < halves && ok && n > 0; i++) ok = scores(0, i);
         for (int t = 0; t < n && ok; t++)
             for (int i = 0; i < halves && ok; i++) {
                 const int use = 2 * t + 1, slot = use % kPcSlots;
-                if (!mbar_wait(&x.full[slot], (use / kPcSlots) & 1, a.err, kPagedWaitRanOut) ||
-                    !mbar_wait(&x.p_full[i], t & 1, a.err, kPagedWaitRanOut)) {
+                if (!warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err) ||
+                    !warp_wait(&x.p_full[i], t & 1, a.err)) {
                     ok = false;
                     break;
                 }
@@ -538,16 +611,16 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
 #pragma unroll
                 for (int part = 1; part >= 0; part--)
 #pragma unroll
-                    for (int ks = 0; ks < kPcTile / 16; ks++)  // 16 keys: 2048 bytes on in V, 8 columns on in P
-                        tc_mma_ts(d, p + 32 * (ks / 2) + 8 * (ks % 2) + 16 * part, vd + (uint64_t)(128 * ks), G::kIdescO,
+                    for (int ks = 0; ks < kPcTile / 16; ks++)  // 16 keys: 2048 bytes on in V, 16 columns on in P
+                        pc_mma_ts(d, p + 16 * ks + 8 * part, vd + (uint64_t)(128 * ks), G::kIdescO,
                                   part == 1 && ks == 0 ? 0u : 1u);
-                tc_commit(&x.o_full[i]);
-                if (i == halves - 1) tc_commit(&x.empty[slot]);
+                pc_commit(&x.o_full[i]);
+                if (i == halves - 1) pc_commit(&x.empty[slot]);
                 if (t + 1 < n) ok = scores(t + 1, i);
             }
         // Every product and arrival is over before tensor memory and the barriers are given back.
-        tc_commit(&x.done);
-        mbar_wait(&x.done, 0, a.err, kPagedWaitRanOut);
+        pc_commit(&x.done);
+        warp_wait(&x.done, 0, a.err);
     }
     __syncwarp();
     tc_fence_before();
@@ -568,26 +641,43 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     __threadfence();
     if (tid == 0) *counter = 0u;
     const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits;
+    static_assert(kPcSplitsMax <= 32, "a lane for each split");
     for (int rr = warp; rr < live; rr += kPcThreads / 32) {
-        float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < splits; w++) top = fmaxf(top, __ldcg(&a.ml[(item + w) * kPcRows + rr]).x);
         constexpr int E = DIM / 32;
+        // Lane w holds split w's maximum and sum; every lane a piece of the row of each split.
+        const float2 ml = lane < splits ? __ldcg(&a.ml[(item + lane) * kPcRows + rr]) : make_float2(-INFINITY, 0.f);
+        const float top = warp_max(ml.x);
+        const float mine = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top);
+        const float sum = warp_sum(ml.y * mine);
         float y[E];
 #pragma unroll
         for (int c = 0; c < E; c++) y[c] = 0.f;
-        for (int w = 0; w < splits; w++) {
-            const float2 ml = __ldcg(&a.ml[(item + w) * kPcRows + rr]);
-            const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            const float *src = a.part + ((item + w) * kPcRows + rr) * DIM + lane * E;
+        for (int w0 = 0; w0 < splits; w0 += 8) {
+            float z[8][E];
 #pragma unroll
-            for (int c = 0; c < E; c++) y[c] = fmaf(__ldcg(src + c), f, y[c]);
+            for (int w = 0; w < 8; w++) {
+                const float *src = a.part + ((item + min(w0 + w, splits - 1)) * kPcRows + rr) * DIM + lane * E;
+                if constexpr (E == 4) {
+                    const float4 t = __ldcg(reinterpret_cast<const float4 *>(src));
+                    z[w][0] = t.x, z[w][1] = t.y, z[w][2] = t.z, z[w][3] = t.w;
+                } else {
+                    const float2 t = __ldcg(reinterpret_cast<const float2 *>(src));
+                    z[w][0] = t.x, z[w][1] = t.y;
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                const float f = __shfl_sync(0xffffffffu, mine, (w0 + w) & 31);
+                if (w0 + w < splits)
+#pragma unroll
+                    for (int c = 0; c < E; c++) y[c] = fmaf(z[w][c], f, y[c]);
+            }
         }
         const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
         const int r = r0 + rr;
         float *dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
-#pragma unroll
-        for (int c = 0; c < E; c++) dst[c] = y[c] * inv;
+        if constexpr (E == 4) *reinterpret_cast<float4 *>(dst) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        else *reinterpret_cast<float2 *>(dst) = make_float2(y[0] * inv, y[1] * inv);
     }
 }
 
