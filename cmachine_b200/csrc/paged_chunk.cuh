@@ -76,33 +76,34 @@ struct PcMisc {  // in shared memory behind the scales
 };
 static_assert(sizeof(PcMisc) <= 256, "misc area");
 
-// B operand descriptor of a V tile (rows are keys, 128 bytes of 64 dims a row): MN-major
-// in the 128-byte swizzle, 8-key groups 1024 bytes apart, the next 64 dims one half on.
-__device__ __forceinline__ uint64_t pc_desc_v(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(PcGeo<128>::kHalf >> 4) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory operand descriptors, in halves: bits 0-13 the address / 16 with the stride of
+// 64-dim halves above it, and for both operands 8-row groups 1024 bytes apart in the 128-byte
+// swizzle. K and Q are K-major; V (rows are keys, 128 bytes of 64 dims a row) is MN-major, the
+// next 64 dims one half on.
+constexpr uint32_t kPcDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t pc_desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t pc_desc_v(uint32_t saddr) { return (saddr >> 4) | ((PcGeo<128>::kHalf >> 4) << 16); }
+// One thread of a converged warp. MMAs issued inside `if (pc_elect())`, their descriptors built
+// from 32-bit halves, go out at the tensor cores' own rate (64 cycles for 128 x 128 x 16); from
+// an ordinary one-lane branch they took 87 to 130.
+__device__ __forceinline__ bool pc_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(one));
+    return one != 0;
 }
-// MMAs issued by one elected thread of a converged warp (their operands stay in uniform
-// registers; issued from a one-lane branch they took 87 cycles each instead of 64). A from
-// shared memory, and from tensor memory.
-__device__ __forceinline__ void pc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+template <bool ACC> __device__ __forceinline__ void pc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(kPcDescHigh), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
 }
-__device__ __forceinline__ void pc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A from tensor memory.
+template <bool ACC> __device__ __forceinline__ void pc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void pc_commit(uint64_t *bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(kPcDescHigh), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
 }
 // 16 columns of this thread's tensor-memory lane: the load (complete after tc_wait_ld), and
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     PcMisc &x = *reinterpret_cast<PcMisc *>(smem + G::kMisc);
     float *scales = reinterpret_cast<float *>(smem + G::kScales);  // [K|V][tile parity][128]
     const PagedView &v = a.v;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int s = blockIdx.z, h = blockIdx.y;
     // The longest row tiles (the last ones) start first.
     const int rt = a.row_tiles - 1 - (int)blockIdx.x / a.splits, sp = (int)blockIdx.x % a.splits;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = x.tmem;  // columns: S and P of half i at 128 i, O at 256 + 128 i
+    const uint32_t tmem = __shfl_sync(0xffffffffu, x.tmem, 0);  // columns: S and P of half i at 128 i, O at 256 + 128 i
 
     if (warp < 8) {
         // ================================================================ softmax
@@ -582,44 +583,53 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
             // P_i(t - 1) lies in the same columns: its product must be over.
             if (t && !warp_wait(&x.o_full[i], (t - 1) & 1, a.err)) return false;
             tc_fence_after();
-            const uint32_t d = tmem + (uint32_t)(128 * i);
+            if (pc_elect()) {
+                const uint32_t d = tmem + (uint32_t)(128 * i), kd = pc_desc_k(ring + (uint32_t)slot * G::kOperand);
 #pragma unroll
-            for (int part = 1; part >= 0; part--)
+                for (int part = 1; part >= 0; part--) {
+                    const uint32_t qd = pc_desc_k(base_s + (uint32_t)(2 * i + part) * G::kOperand);
 #pragma unroll
-                for (int ks = 0; ks < DIM / 16; ks++) {
-                    const uint32_t off = (uint32_t)(ks / 4) * G::kHalf;
-                    pc_mma_ss(d, tc_desc(base_s + (uint32_t)(2 * i + part) * G::kOperand + off) + 2 * (ks % 4),
-                           tc_desc(ring + (uint32_t)slot * G::kOperand + off) + 2 * (ks % 4), G::kIdescS,
-                           part == 1 && ks == 0 ? 0u : 1u);
+                    for (int ks = 0; ks < DIM / 16; ks++) {  // 32 bytes on in a row of 128, then the next half
+                        const uint32_t off = (uint32_t)(ks / 4) * (G::kHalf >> 4) + 2 * (ks % 4);
+                        if (part == 1 && ks == 0) pc_mma_ss<false>(d, qd + off, kd + off, G::kIdescS);
+                        else pc_mma_ss<true>(d, qd + off, kd + off, G::kIdescS);
+                    }
                 }
-            pc_commit(&x.s_full[i]);
-            if (i == halves - 1) pc_commit(&x.empty[slot]);
+                tc_commit(&x.s_full[i]);
+                if (i == halves - 1) tc_commit(&x.empty[slot]);
+            }
+            __syncwarp();
             return true;
         };
         for (int i = 0; i < halves && ok && n > 0; i++) ok = scores(0, i);
         for (int t = 0; t < n && ok; t++)
             for (int i = 0; i < halves && ok; i++) {
                 const int use = 2 * t + 1, slot = use % kPcSlots;
-                if (!warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err) ||
-                    !warp_wait(&x.p_full[i], t & 1, a.err)) {
+                if (!warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err) || !warp_wait(&x.p_full[i], t & 1, a.err)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem + 256u + (uint32_t)(128 * i), p = tmem + (uint32_t)(128 * i);
-                const uint64_t vd = pc_desc_v(ring + (uint32_t)slot * G::kOperand);
+                if (pc_elect()) {
+                    const uint32_t d = tmem + 256u + (uint32_t)(128 * i), p = tmem + (uint32_t)(128 * i),
+                                   vd = pc_desc_v(ring + (uint32_t)slot * G::kOperand);
 #pragma unroll
-                for (int part = 1; part >= 0; part--)
+                    for (int part = 1; part >= 0; part--)
 #pragma unroll
-                    for (int ks = 0; ks < kPcTile / 16; ks++)  // 16 keys: 2048 bytes on in V, 16 columns on in P
-                        pc_mma_ts(d, p + 16 * ks + 8 * part, vd + (uint64_t)(128 * ks), G::kIdescO,
-                                  part == 1 && ks == 0 ? 0u : 1u);
-                pc_commit(&x.o_full[i]);
-                if (i == halves - 1) pc_commit(&x.empty[slot]);
+                        for (int ks = 0; ks < kPcTile / 16; ks++) {  // 16 keys: 2048 bytes on in V, 16 columns on in P
+                            const uint32_t pa = p + 16 * ks + 8 * part, vb = vd + (uint32_t)(128 * ks);
+                            if (part == 1 && ks == 0) pc_mma_ts<false>(d, pa, vb, G::kIdescO);
+                            else pc_mma_ts<true>(d, pa, vb, G::kIdescO);
+                        }
+                    tc_commit(&x.o_full[i]);
+                    if (i == halves - 1) tc_commit(&x.empty[slot]);
+                }
+                __syncwarp();
                 if (t + 1 < n) ok = scores(t + 1, i);
             }
         // Every product and arrival is over before tensor memory and the barriers are given back.
-        pc_commit(&x.done);
+        if (pc_elect()) tc_commit(&x.done);
+        __syncwarp();
         warp_wait(&x.done, 0, a.err);
     }
     __syncwarp();
