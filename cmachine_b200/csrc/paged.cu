@@ -158,26 +158,39 @@ long long visible_rows(const PagedView &v, int window, int sinks) {
     return most < v.max_length ? most : v.max_length;
 }
 
+// Most steps one sequence of the decode kernel can have: rows below the length, and for each KV
+// head and row tile.
+long long decode_steps(const PagedView &v, int few, int group) {
+    const long long rows = (long long)(v.max_new < few ? v.max_new : few) * group;
+    return ((long long)v.max_length / 16 + 2) * v.kvheads * ((rows + 7) / 8);
+}
+template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDecodeArgs a) {
+    constexpr size_t smem = kPdSmem<KIND, DIM, R>;
+    static PerDeviceOnce once;
+    once.run([] {
+        TCM_CUDA(cudaFuncSetAttribute(paged_decode_kernel<KIND, DIM, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    });
+    const int ctas = sm_count() * PdGeo<KIND, DIM>::kCtas;
+    unsigned *count;
+    paged_scratch(gpu, 2ll * ctas * R, DIM, ctas + 1, &a.part, &a.ml, &count);
+    a.counters = count + 1;  // [0] takes the chunk kernel's wait errors when there is no status word
+    // As many sequences a launch as it counts, and steps below 2^31 (paged_attention refuses a
+    // sequence that alone has more).
+    const PagedView all = a.v;
+    long long most = 0x7fffffff / decode_steps(all, a.few, a.group);
+    if (most > kPdSequences) most = kPdSequences;
+    for (int s = 0; s < all.sequences; s += (int)most) {
+        a.v.sequences = all.sequences - s < most ? all.sequences - s : (int)most;
+        a.v.starts = all.starts + s;
+        a.v.lengths = all.lengths + s;
+        a.v.table = all.table + (int64_t)s * all.table_stride;
+        launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
+    }
+}
 template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) {
-    const PagedView &v = a.v;
-    const int rows = (v.max_new < a.few ? v.max_new : a.few) * a.group, r = rows <= 8 ? 8 : 16;
-    a.row_tiles = (rows + r - 1) / r;
-    // Splits: enough items to fill the GPU several times over, whole steps for each of the four
-    // warps, and no more than the merge holds.
-    const long long steps = (visible_rows(v, a.window, a.sinks) + 15) / 16 + 2;
-    const long long items = (long long)v.sequences * v.kvheads * a.row_tiles;
-    long long per = (steps * items + sm_count() * 32 - 1) / (sm_count() * 32);
-    if (per < kPdWarps) per = kPdWarps;
-    if (per * kPdSplitsMax < steps) per = (steps + kPdSplitsMax - 1) / kPdSplitsMax;
-    per = (per + kPdWarps - 1) / kPdWarps * kPdWarps;
-    a.tiles_per_item = (int)per;
-    a.splits = (int)((steps + per - 1) / per);
-    unsigned *count;  // [0] takes the chunk kernel's wait errors when there is no status word
-    paged_scratch(gpu, a.splits > 1 ? items * a.splits * r : 0, DIM, items + 1, &a.part, &a.ml, &count);
-    a.counters = count + 1;
-    const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
-    if (r == 8) launch(paged_decode_kernel<KIND, DIM, 8>, grid, dim3(kPdThreads), 0, stream(), true, a);
-    else launch(paged_decode_kernel<KIND, DIM, 16>, grid, dim3(kPdThreads), 0, stream(), true, a);
+    const int rows = (a.v.max_new < a.few ? a.v.max_new : a.few) * a.group;
+    if (rows <= 8) decode_launch_rows<KIND, DIM, 8>(gpu, a);
+    else decode_launch_rows<KIND, DIM, 16>(gpu, a);
 }
 
 template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
@@ -279,10 +292,11 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     if (window < 0 || sinks < 0) return refuse(name, "window and sinks are not negative");
     if (nothing(view)) return 0;
     if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
-    const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
     const int group = qheads / view.kvheads, few = kFewRows / group;
-    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, 1, 1, 1, scale2, nullptr, nullptr,
-                         nullptr, status};
+    if (decode_steps(view, few, group) > 0x7fffffff) return refuse(name, "max_length times kvheads is too large");
+    const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
+    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
+                         status};
 #define CALL(K, D) decode_launch<K, D>(gpu, d)
     PAGED_DISPATCH(view, CALL);
 #undef CALL

@@ -119,20 +119,14 @@ __device__ __forceinline__ void tc_ld16_async(uint32_t taddr, uint32_t (&r)[16])
 __device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 __device__ __forceinline__ void tc_st8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]));
 }
 __device__ __forceinline__ float2 as_pair(uint32_t x, uint32_t y) {
     return make_float2(__uint_as_float(x), __uint_as_float(y));
-}
-__device__ __forceinline__ float ex2(float x) {  // results below 2^-126 are zero
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 // Bounded wait. The timer is read once in 256 tries: reading it takes longer than these
 // waits usually last, and the barrier completing meanwhile would go unnoticed.
@@ -512,15 +506,17 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                         const int rl = (b + k) * C::RPL + sub, rr = 32 * w + rl;
                         uint4 y = in[k];
                         if constexpr (kBytes) {
-                            // 16 codes: dims 16 piece ..: two 16-byte pieces of FP16.
-                            const int d = piece * 16;
+                            // 16 codes: dims 16 piece ..: two 16-byte pieces of FP16. The lanes of a row's
+                            // second 64 dims store their pieces in the other order: eight lanes, all banks.
+                            const int d = piece * 16, other = d / 64;
                             const uint32_t at = dst + (uint32_t)(d / 64) * G::kHalf;
+                            if (other) y = make_uint4(y.z, y.w, y.x, y.y);
                             const uint32_t q0 = y.x ^ 0x80808080u, q1 = y.y ^ 0x80808080u, q2 = y.z ^ 0x80808080u,
                                            q3 = y.w ^ 0x80808080u;
-                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8), codes_f16(q0, 0x4140), codes_f16(q0, 0x4342),
+                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8 + other), codes_f16(q0, 0x4140), codes_f16(q0, 0x4342),
                                       codes_f16(q1, 0x4140), codes_f16(q1, 0x4342));
-                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8 + 1), codes_f16(q2, 0x4140), codes_f16(q2, 0x4342),
-                                      codes_f16(q3, 0x4140), codes_f16(q3, 0x4342));
+                            st_smem16(at + pc_swizzle(rr, (d % 64) / 8 + 1 - other), codes_f16(q2, 0x4140),
+                                      codes_f16(q2, 0x4342), codes_f16(q3, 0x4140), codes_f16(q3, 0x4342));
                         } else {
                             // The row's largest magnitude as bits, over its lanes.
                             uint32_t mb = __vmaxu2(__vmaxu2(y.x & 0x7fff7fffu, y.y & 0x7fff7fffu),
@@ -657,7 +653,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         // Lane w holds split w's maximum and sum; every lane a piece of the row of each split.
         const float2 ml = lane < splits ? __ldcg(&a.ml[(item + lane) * kPcRows + rr]) : make_float2(-INFINITY, 0.f);
         const float top = warp_max(ml.x);
-        const float mine = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top);
+        const float mine = pd_factor(ml, top);
         const float sum = warp_sum(ml.y * mine);
         float y[E];
 #pragma unroll

@@ -1,17 +1,23 @@
 // Attention of few query rows over a paged K/V cache: single tokens and short
 // drafted runs, at most R = 8 or 16 query rows of one KV head at a time.
 //
-// Work items are (sequence, KV head, row tile, split of the visible rows); the
-// four warps of a CTA take the item's 16-row steps in turn, each with its own
-// online softmax, and merge at the end. Memory bound: a cached row is read once
-// from HBM (row tiles of one sequence are neighbours in the grid and meet in L2)
-// and never staged: every lane loads 16-byte pieces of K and V rows straight into
-// the registers it needs as tensor-core fragments (mma.sync m16n8k16; a tile of 8
-// rows cannot fill a tcgen05 tile of 128), one step ahead of their use.
+// The work is a line of steps: 16 cached rows against one row tile, ordered by
+// sequence, KV head, row tile and place. Every CTA of a grid that fills the GPU once
+// counts the steps of all sequences (their lengths are on the device), takes an equal
+// stretch of the line, and works through the one to few (sequence, KV head, row tile)
+// segments in it; its warps take a segment's steps in turn, each with its own online
+// softmax, and merge at the segment's end. A segment that began or goes on in another CTA
+// leaves a partial result, and the last of its CTAs to arrive adds the partials in order.
+// Memory bound: a cached row is read once from HBM (row tiles of one KV head meet in L2).
+// Every warp copies its own steps into its own ring of three stages (cp.async, 16 bytes a
+// lane, rows found by address), two steps ahead, and waits for no other warp; the products
+// are mma.sync m16n8k16 (a tile of 8 rows cannot fill a tcgen05 tile of 128). Loading
+// straight into registers instead left the compiler spilling loads in flight, which made
+// every one of them a wait: 64 sessions of up to 8192 byte rows took 66 us so.
 //
 // Fragments. The order of the dims inside a k-step and of the output columns is
 // free as long as both operands agree, so it follows the memory layout: lane
-// (g = lane / 4, t = lane % 4) holds 16-byte pieces of key g's row for Q K^T, and
+// (g = lane / 4, t = lane % 4) reads 16-byte pieces of key g's row for Q K^T, and
 // dims [g DIM / 8, (g + 1) DIM / 8) of keys 2t, 2t + 1, 8 + 2t, 9 + 2t for P V, whose
 // pairs of keys meet by byte permutes.
 //
@@ -23,12 +29,12 @@
 // step): chains stay as short as one warp's share of an item.
 #pragma once
 #include "paged.cuh"
+#include "stream.cuh"
 #include <cuda_fp16.h>
 
 namespace tcm {
 
-constexpr int kPdWarps = 4, kPdThreads = kPdWarps * 32;
-constexpr int kPdSplitsMax = 128;  // splits of one (sequence, KV head, row tile)
+constexpr int kPdSequences = 512;  // sequences a launch counts in shared memory
 
 struct PagedDecodeArgs {
     PagedView v;
@@ -37,13 +43,45 @@ struct PagedDecodeArgs {
     long long out_stride, q_stride;
     int group, window, sinks;
     int few;              // sequences of at most this many new rows are this kernel's
-    int row_tiles, splits, tiles_per_item;
     float scale2;         // log2(e) / sqrt(dim): base-2 scores
-    float *part;          // [item][R][DIM]
-    float2 *ml;           // [item][R]: running maximum and sum
-    unsigned *counters;   // [sequence][KV head][row tile], zero between calls
+    float *part;          // [CTA][2][R][DIM]: the first and the last segment of a CTA's stretch
+    float2 *ml;           // [CTA][2][R]: running maximum and sum
+    unsigned *counters;   // [CTA], of the segment that begins there and goes on; zero between calls
     int *status;
 };
+
+// Eight warps a CTA; two CTAs an SM where their rings fit.
+constexpr int kPdWarps = 8, kPdThreads = kPdWarps * 32, kPdStages = 3;
+template <int KIND, int DIM> struct PdGeo {
+    static constexpr int kRow = DIM * (KIND == kPagedBytes ? 1 : 2);          // bytes a stored row
+    static constexpr int kStage = 32 * kRow + (KIND == kPagedBytes ? 128 : 0);  // 16 K rows, 16 V rows, their scales
+    static constexpr int kCtas = kRow <= 128 ? 2 : 1;
+    static constexpr size_t kRing = (size_t)kPdWarps * kPdStages * kStage;
+};
+// The warps' outputs meet in the rings' memory.
+template <int KIND, int DIM, int R> constexpr size_t kPdSmem =
+    PdGeo<KIND, DIM>::kRing > (size_t)kPdWarps * R * DIM * 4 ? PdGeo<KIND, DIM>::kRing : (size_t)kPdWarps * R * DIM * 4;
+
+// The 16-byte piece of a stored row of ROW bytes where its piece `piece` lies in a stage: the
+// eight lanes that read together (keys 2j, 2j + 1 and four pieces; or four even or odd keys
+// and two pieces) meet eight bank groups.
+template <int ROW> __device__ __forceinline__ int pd_swizzle(int row, int piece) {
+    if (ROW == 64) return piece ^ ((row >> 1) & 3);
+    const int far = (((row >> 2) ^ row) & 1) << 2;
+    return piece ^ (ROW == 128 ? (row & 2) | far : ((row >> 1) & 1) | far);
+}
+__device__ __forceinline__ void pd_copy16(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pd_copy4(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+
+// Where the 16-byte piece d4 of merge row r lies, in pieces of the row: the eight lanes that
+// store together (two rows, four stretches of dims) meet eight different bank groups.
+template <int DIM> __device__ __forceinline__ int pd_piece(int r, int d4) {
+    return DIM == 128 ? d4 ^ ((d4 >> 3) + 4 * (r & 1)) : d4 ^ ((d4 >> 3) | ((r & 1) << 1));
+}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -112,6 +150,15 @@ __device__ __forceinline__ float power_of_two(int e) {
 
 // Rows are read past L1, which keeps nothing that an append may have changed.
 __device__ __forceinline__ uint4 ld_row16(const void *p) { return __ldcg(static_cast<const uint4 *>(p)); }
+__device__ __forceinline__ float ex2(float x) {  // results below 2^-126 are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// What a partial result with maximum and sum ml counts for under the maximum `top`; NaN stays NaN.
+__device__ __forceinline__ float pd_factor(float2 ml, float top) {
+    return ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : ex2(ml.x - top);
+}
 __device__ __forceinline__ float quad_max(float x) {  // over the four lanes of a fragment row
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
     return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -126,9 +173,20 @@ __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 
 
 constexpr float kPdWeightTop = 14.f;  // byte rows' weights are scaled to at most 2^14
 
+// A CTA's present segment; read again after the loop, so that the loop keeps its registers.
+struct PdSegment {
+    PagedExtent e;
+    PagedTiles tiles;
+    int s, h, r0;
+    int k0;        // the segment's first step of the row tile's
+    int from, to;  // all of the row tile's steps in the line
+};
+
 template <int KIND, int DIM, int R>
-__global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) paged_decode_kernel(const PagedDecodeArgs a) {
+__global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_decode_kernel(const PagedDecodeArgs a) {
     constexpr bool kBytes = KIND == kPagedBytes;
+    using G = PdGeo<KIND, DIM>;
+    constexpr int W = kPdWarps, T = kPdThreads;
     constexpr int ES = kBytes ? 1 : 2;              // bytes an element
     constexpr int KP = DIM * ES / 64;               // 16-byte pieces of a key a lane holds for Q K^T
     constexpr int KS = DIM / 16;                    // k-steps of Q K^T
@@ -137,32 +195,89 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
     constexpr int P = kPdParts<KIND>;
     constexpr int NA = R == 8 ? (P + 1) / 2 : P;    // A tiles a product takes
     constexpr int RW = R / 8;                       // query rows a lane holds scores of
+    extern __shared__ __align__(1024) unsigned char pc_smem[];
+    float4(*wo)[R][DIM / 4] = reinterpret_cast<float4(*)[R][DIM / 4]>(pc_smem);  // the warps' outputs
     __shared__ __align__(16) uint4 qf[NA][KS][32];  // Q's fragments
     __shared__ float qs[R];                         // scale2 times the row's power of two
-    __shared__ __align__(16) float wo[kPdWarps][R][DIM];
-    __shared__ float2 wml[kPdWarps][R];
+    __shared__ float2 wml[W][R];
+    __shared__ int upto[kPdSequences + 1];    // steps before each sequence
     __shared__ int last_s;
+    __shared__ PdSegment seg;
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int s = blockIdx.z, h = blockIdx.y, rt = blockIdx.x % a.row_tiles, sp = blockIdx.x / a.row_tiles;
     pdl_wait();
-    PagedExtent e;
-    const int bad_extent = paged_extent(&v, s, &e);
-    if (e.count > a.few || !e.count) {
-        if (bad_extent && !blockIdx.x && !h && !tid) paged_report(a.status, bad_extent);
-        return;
+
+    // ---- this CTA's stretch of the line of steps
+    auto tiles_of = [&](const PagedExtent &e, int rt) {
+        const int origin = e.length - e.count, r0 = rt * R, r1 = min(e.count * a.group, r0 + R) - 1;
+        return paged_tiles(origin + r0 / a.group, origin + r1 / a.group, a.window, a.sinks, 4);
+    };
+    for (int i = tid; i < v.sequences; i += T) {
+        PagedExtent e;
+        const int bad = paged_extent(&v, i, &e);
+        if (bad && !blockIdx.x) paged_report(a.status, bad);
+        int steps = 0;  // the host keeps a launch's sum below 2^31
+        if (e.count <= a.few)
+            for (int rt = 0; rt * R < e.count * a.group; rt++) steps += max(1, tiles_of(e, rt).count);
+        upto[i + 1] = steps * v.kvheads;
     }
-    const int rows = e.count * a.group, r0 = rt * R;  // row r of the KV head: new row r / group, head r % group
-    if (r0 >= rows) return;
+    __syncthreads();
+    if (warp == 0) {
+        int before = 0;
+        for (int i0 = 0; i0 < v.sequences; i0 += 32) {
+            int x = i0 + lane < v.sequences ? upto[i0 + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (i0 + lane < v.sequences) upto[i0 + lane + 1] = before + x;
+            before += __shfl_sync(0xffffffffu, x, 31);
+        }
+        if (lane == 0) upto[0] = 0;
+    }
+    __syncthreads();
+    const int steps = upto[v.sequences];
+    const int share = (int)(((unsigned)steps + gridDim.x - 1) / gridDim.x + W - 1) / W * W;
+    const int begin = (int)min((long long)steps, (long long)share * blockIdx.x), end = (int)min((long long)steps, begin + (long long)share);
+    const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
+    int bad = 0;
+    for (int pos = begin; pos < end;) {
+    // ---- the segment at pos
+    if (tid == 0) {
+        PdSegment z;
+        z.s = 0;
+        for (int top = v.sequences - 1; z.s < top;) {  // the last sequence that begins at or before pos
+            const int mid = (z.s + top + 1) >> 1;
+            if (upto[mid] <= pos) z.s = mid;
+            else top = mid - 1;
+        }
+        paged_extent(&v, z.s, &z.e);
+        const int in_seq = pos - upto[z.s], a_head = (upto[z.s + 1] - upto[z.s]) / v.kvheads;
+        z.h = in_seq / a_head;
+        int in_tile = in_seq - z.h * a_head, rt = 0;
+        z.tiles = tiles_of(z.e, 0);
+        while (in_tile >= max(1, z.tiles.count)) {
+            in_tile -= max(1, z.tiles.count);
+            z.tiles = tiles_of(z.e, ++rt);
+        }
+        z.r0 = rt * R;
+        z.k0 = in_tile;
+        z.from = pos - in_tile;
+        z.to = z.from + max(1, z.tiles.count);
+        seg = z;
+    }
+    __syncthreads();
+    const int s = seg.s, h = seg.h;
+    const PagedExtent e = seg.e;
+    const PagedTiles tiles = seg.tiles;
+    const int k0 = seg.k0, k1 = min(tiles.count, k0 + (end - pos)), r0 = seg.r0;
+    const int rows = e.count * a.group;  // row r of the KV head: new row r / group, head r % group
     const int first = e.length - e.count + r0 / a.group;
     const int last = e.length - e.count + (min(rows, r0 + R) - 1) / a.group;
-    const PagedTiles tiles = paged_tiles(first, last, a.window, a.sinks, 4);
-    const int splits = max(1, (tiles.count + a.tiles_per_item - 1) / a.tiles_per_item);
-    if (sp >= splits) return;
-    const int k0 = sp * a.tiles_per_item, k1 = min(tiles.count, k0 + a.tiles_per_item);
 
-    // ---- this item's queries as fragments: warp w prepares rows w, w + 4, ...
-    for (int r = warp; r < R; r += kPdWarps) {
+    // ---- its queries as fragments: warp w prepares rows w, w + W, ...
+    for (int r = warp; r < R; r += W) {
         float x[DIM / 32], m = 0.f;
         const bool on = r0 + r < rows;
         if (on) {
@@ -210,7 +325,6 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
 
     // ---- the loop over this warp's 16-row steps
     const bool whole = v.page % 16 == 0;  // a step lies inside one page
-    const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     float o[DV][4], m[RW], mu[RW], l[RW], sc[RW];
 #pragma unroll
     for (int j = 0; j < DV; j++)
@@ -219,76 +333,77 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
 #pragma unroll
     for (int r = 0; r < RW; r++) m[r] = mu[r] = -INFINITY, l[r] = 0.f, sc[r] = qs[g + 8 * r];
 
-    int bad = 0;
-    // The row of place j; -1 where there is none (behind the last query, or no page).
     auto page_of = [&](int k) -> int {  // the page id of lane % 16's row of step k
         if (k >= k1) return -1;
         const int j = min(paged_tile(tiles, k) * 16 + (whole ? 0 : lane & 15), last);
         return v.table[(int64_t)s * v.table_stride + paged_div(&v, j)];
     };
-    auto row_of = [&](int k, int id) -> int64_t {  // of lane % 16's place
-        if (k >= k1) return -1;
-        const int j = paged_tile(tiles, k) * 16 + (lane & 15);
-        const int64_t row = j <= last ? paged_row(&v, id, j, paged_div(&v, j), h) : -1;
-        // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
-        if (row < 0 && j <= last && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) bad |= kPagedBadPage;
-        return row;
-    };
-    uint4 kr[2][KP];
-    uint4 vr[4][VW / 4 > 0 ? VW / 4 : 1];  // DIM 64 bytes: half a piece is used
-    float scales = 0.f;                    // lanes 0-15: the K scale of the lane's row, 16-31 V's
-    auto load_k = [&](int64_t row) {
-#pragma unroll
-        for (int gr = 0; gr < 2; gr++) {
-            const int64_t rk = __shfl_sync(0xffffffffu, row, gr * 8 + g);
-            const char *p = static_cast<const char *>(v.keys) + rk * (DIM * ES) + t * 16;
-#pragma unroll
-            for (int c = 0; c < KP; c++) kr[gr][c] = rk >= 0 ? ld_row16(p + c * 64) : make_uint4(0, 0, 0, 0);
-        }
-        if constexpr (kBytes) scales = row >= 0 ? __ldcg(v.scales + (lane >= 16 ? half : 0) + row) : 1.f;
-    };
-    auto load_v = [&](int64_t row) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int64_t rv = __shfl_sync(0xffffffffu, row, (i >> 1) * 8 + 2 * t + (i & 1));
-            const char *p = static_cast<const char *>(v.values) + rv * (DIM * ES) + g * (DV * ES);
-            if constexpr (VW == 2) {
-                const uint2 w = rv >= 0 ? __ldcg(reinterpret_cast<const uint2 *>(p)) : make_uint2(0, 0);
-                vr[i][0] = make_uint4(w.x, w.y, 0, 0);
-            } else {
-#pragma unroll
-                for (int c = 0; c < VW / 4; c++) vr[i][c] = rv >= 0 ? ld_row16(p + c * 16) : make_uint4(0, 0, 0, 0);
+    // Copies step k into its stage; returns which of its 16 places have a row. One copy group a
+    // call, empty behind the last step.
+    const uint32_t ring = smem_addr(pc_smem) + (uint32_t)warp * kPdStages * G::kStage;
+    auto fetch = [&](int k, int id, int stage) -> unsigned {
+        int64_t row = -1;  // lane % 16's
+        if (k < k1) {
+            const int j = paged_tile(tiles, k) * 16 + (lane & 15);
+            if (j <= last) {
+                row = paged_row(&v, id, j, paged_div(&v, j), h);
+                // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
+                if (row < 0 && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) bad |= kPagedBadPage;
             }
+            const uint32_t dst = ring + (uint32_t)stage * G::kStage;
+            constexpr int LPR = G::kRow / 16, RPL = 32 / LPR;  // lanes a row, rows at a time
+#pragma unroll
+            for (int i = 0; i < 16 / RPL; i++) {
+                const int rr = i * RPL + lane / LPR, piece = lane % LPR;
+                const int64_t r = __shfl_sync(0xffffffffu, row, rr);
+                const int64_t at = r < 0 ? 0 : r * G::kRow + piece * 16;
+                const uint32_t to = dst + (uint32_t)(rr * G::kRow + pd_swizzle<G::kRow>(rr, piece) * 16);
+                pd_copy16(to, static_cast<const char *>(v.keys) + at, r >= 0);
+                pd_copy16(to + 16 * G::kRow, static_cast<const char *>(v.values) + at, r >= 0);
+            }
+            if constexpr (kBytes)
+                pd_copy4(dst + 32 * G::kRow + lane * 4, v.scales + (row < 0 ? 0 : (lane >= 16 ? half : 0) + row), row >= 0);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
     };
 
     int k = k0 + warp;
-    int64_t row = row_of(k, page_of(k));
-    int id_next = page_of(k + kPdWarps);
-    load_k(row);
-    load_v(row);
-    for (; k < k1; k += kPdWarps) {
-        const int64_t next = row_of(k + kPdWarps, id_next);
-        const unsigned there = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-        id_next = page_of(k + 2 * kPdWarps);
+    unsigned there = fetch(k, page_of(k), 0), there1 = fetch(k + W, page_of(k + W), 1);
+    int id_next = page_of(k + 2 * W);
+    for (int stage = 0; k < k1; k += W, stage = stage == kPdStages - 1 ? 0 : stage + 1) {
+        const int ahead = stage == 0 ? kPdStages - 1 : stage - 1;  // the stage read in the step before
+        const unsigned there2 = fetch(k + 2 * W, id_next, ahead);
+        id_next = page_of(k + 3 * W);
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        __syncwarp();
+        const unsigned char *st = pc_smem + (size_t)warp * kPdStages * G::kStage + (size_t)stage * G::kStage;
         // Scores of 16 places: S[gr] columns 2t, 2t + 1 are places base + 8 gr + 2t, + 1.
         float sf[2][4];
 #pragma unroll
         for (int gr = 0; gr < 2; gr++)
 #pragma unroll
             for (int c = 0; c < 4; c++) sf[gr][c] = 0.f;
+        uint4 kr[2];
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
+            constexpr int KPP = KS / KP;  // k-steps a 16-byte piece of a key feeds
+            if (ks % KPP == 0)
+#pragma unroll
+                for (int gr = 0; gr < 2; gr++) {
+                    const int key = gr * 8 + g;
+                    kr[gr] = *reinterpret_cast<const uint4 *>(st + key * G::kRow + pd_swizzle<G::kRow>(key, (ks / KPP) * 4 + t) * 16);
+                }
             uint32_t b0[2], b1[2];
 #pragma unroll
             for (int gr = 0; gr < 2; gr++) {
                 if constexpr (kBytes) {
-                    const uint32_t w = word(kr[gr][ks / 4], ks % 4) ^ 0x80808080u;
+                    const uint32_t w = word(kr[gr], ks % 4) ^ 0x80808080u;
                     b0[gr] = codes_f16(w, 0x4140);
                     b1[gr] = codes_f16(w, 0x4342);
                 } else {
-                    b0[gr] = word(kr[gr][ks / 2], (ks % 2) * 2);
-                    b1[gr] = word(kr[gr][ks / 2], (ks % 2) * 2 + 1);
+                    b0[gr] = word(kr[gr], (ks % 2) * 2);
+                    b1[gr] = word(kr[gr], (ks % 2) * 2 + 1);
                 }
             }
 #pragma unroll
@@ -302,12 +417,11 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
         if constexpr (kBytes) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int at = (i >> 1) * 8 + 2 * t + (i & 1);
-                ks4[i] = __shfl_sync(0xffffffffu, scales, at);
-                vs4[i] = __shfl_sync(0xffffffffu, scales, 16 + at);
+                const float *sc4 = reinterpret_cast<const float *>(st + 32 * G::kRow) + (i >> 1) * 8 + 2 * t + (i & 1);
+                ks4[i] = sc4[0];
+                vs4[i] = sc4[16];
             }
         }
-        load_k(next);
 
         const int base = paged_tile(tiles, k) * 16;
         // Every query of the tile sees every place of the step?
@@ -335,11 +449,11 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
             }
             const float m_new = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
             const float mr = m_new == -INFINITY ? 0.f : m_new;
-            l[r] *= m[r] == -INFINITY ? 0.f : exp2f(m[r] - mr);
+            l[r] *= m[r] == -INFINITY ? 0.f : ex2(m[r] - mr);
             m[r] = m_new;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                w[i] = exp2f(x[i] - mr);
+                w[i] = ex2(x[i] - mr);
                 l[r] += w[i];
             }
             float mu_new = m_new;
@@ -351,11 +465,11 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
 #pragma unroll
                 for (int i = 0; i < 4; i++) u = fmaxf(u, x[i] + __log2f(vs4[i]));
                 mu_new = fmaxf(fmaxf(mu[r], quad_max(u)), m_new - 113.f);
-                const float f = mu_new == -INFINITY ? 0.f : exp2f(mr - mu_new + kPdWeightTop);
+                const float f = mu_new == -INFINITY ? 0.f : ex2(mr - mu_new + kPdWeightTop);
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[i] = x[i] == -INFINITY ? 0.f : w[i] * (vs4[i] * f);
             }
-            keep[r] = mu[r] == -INFINITY ? 0.f : exp2f(mu[r] - mu_new);
+            keep[r] = mu[r] == -INFINITY ? 0.f : ex2(mu[r] - mu_new);
             moved |= mu_new != mu[r];
             mu[r] = mu_new;
             split_pair<KIND>(w[0], w[1], pa[r][0]);
@@ -370,17 +484,6 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
                 o[j][3] *= keep[RW - 1];
             }
         }
-        if constexpr (!kBytes) {
-            // A weight of 0 times a non-finite value would spoil queries that do not see it.
-            if (!full) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int c = 0; c < VW / 4; c++)
-                        vr[i][c] = make_uint4(finite_pair(vr[i][c].x), finite_pair(vr[i][c].y), finite_pair(vr[i][c].z),
-                                              finite_pair(vr[i][c].w));
-            }
-        }
         auto pv = [&](float(&acc)[4], uint32_t b0, uint32_t b1) {
             if constexpr (R == 8) {
                 if constexpr (P == 3) mma_kind<KIND>(acc, pa[0][0][2], 0u, pa[0][1][2], 0u, b0, b1);
@@ -391,11 +494,27 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
                     mma_kind<KIND>(acc, pa[0][0][p], pa[RW - 1][0][p], pa[0][1][p], pa[RW - 1][1][p], b0, b1);
             }
         };
+        uint4 vr[4];
 #pragma unroll
         for (int c = 0; c < VW; c++) {
+            if (c % 4 == 0)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = (i >> 1) * 8 + 2 * t + (i & 1), byte = g * (DV * ES) + c * 4;
+                    const unsigned char *p = st + (16 + key) * G::kRow + pd_swizzle<G::kRow>(key, byte / 16) * 16;
+                    if constexpr (VW == 2) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(p + byte % 16);
+                        vr[i] = make_uint4(w.x, w.y, 0, 0);
+                    } else {
+                        vr[i] = *reinterpret_cast<const uint4 *>(p);
+                    }
+                    // A weight of 0 times a non-finite value would spoil queries that do not see it.
+                    if (!kBytes && !full)
+                        vr[i] = make_uint4(finite_pair(vr[i].x), finite_pair(vr[i].y), finite_pair(vr[i].z), finite_pair(vr[i].w));
+                }
             uint32_t x[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = word(vr[i][c / 4], c % 4);
+            for (int i = 0; i < 4; i++) x[i] = word(vr[i], c % 4);
             if constexpr (kBytes) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] ^= 0x80808080u;
@@ -410,106 +529,145 @@ __global__ void __launch_bounds__(kPdThreads, (KIND == kPagedBytes ? 4 : 3)) pag
                 pv(o[2 * c + 1], __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
             }
         }
-        load_v(next);
-        row = next;
+        there = there1;
+        there1 = there2;
+        __syncwarp();  // every lane has read the stage before it is copied into again
     }
-    if (bad || bad_extent) paged_report(a.status, bad | bad_extent);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // no copy is left in flight, and the rings' memory is free for the outputs
 
-    // ---- the four warps' states: lane (g, t) holds dims [2 t DV, (2 t + 2) DV) of row g (+ 8)
+    // ---- the warps' states: lane (g, t) holds dims [2 t DV, (2 t + 2) DV) of row g (+ 8)
 #pragma unroll
     for (int r = 0; r < RW; r++) {
         float sum = l[r];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (t == 0) wml[warp][g + 8 * r] = make_float2(m[r], sum);
-        const float f = kBytes ? (mu[r] == -INFINITY ? 0.f : exp2f(mu[r] - m[r] - kPdWeightTop)) : 1.f;
+        const float f = kBytes ? (mu[r] == -INFINITY ? 0.f : ex2(mu[r] - m[r] - kPdWeightTop)) : 1.f;
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            float *dst = &wo[warp][g + 8 * r][(2 * t + c) * DV];
+        for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int j = 0; j < DV; j += 4) {
                 float y[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[i] = f * (R == 8 ? o[j + i][c] + o[j + i][2 + c] : o[j + i][2 * r + c]);
-                *reinterpret_cast<float4 *>(dst + j) = make_float4(y[0], y[1], y[2], y[3]);
+                wo[warp][g + 8 * r][pd_piece<DIM>(g + 8 * r, ((2 * t + c) * DV + j) / 4)] = make_float4(y[0], y[1], y[2], y[3]);
+            }
+    }
+    __syncthreads();
+    {
+    const volatile PdSegment &z = seg;
+    const int from = z.from, to = z.to, r0 = z.r0, rows = z.e.count * a.group, start = z.e.start, h = z.h;
+    auto store_out = [&](int r, int d4, float4 y, float sum) {
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);  // nothing seen: zeros
+        *reinterpret_cast<float4 *>(a.out + (long long)(start + (r0 + r) / a.group) * a.out_stride +
+                                    (h * a.group + (r0 + r) % a.group) * DIM + d4 * 4) =
+            make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+    };
+    const int live = min(R, rows - r0);
+    const bool alone = from >= begin && to <= end;
+    const int slot = 2 * blockIdx.x + (pos == begin ? 0 : 1);
+    for (int i = tid; i < live * (DIM / 4); i += T) {
+        const int r = i / (DIM / 4), d4 = i % (DIM / 4);
+        float top = -INFINITY, sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; w++) top = fmaxf(top, wml[w][r].x);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float2 ml = wml[w][r];
+            const float f = pd_factor(ml, top);
+            const float4 x = wo[w][r][pd_piece<DIM>(r, d4)];
+            sum = fmaf(ml.y, f, sum);
+            y.x = fmaf(x.x, f, y.x);
+            y.y = fmaf(x.y, f, y.y);
+            y.z = fmaf(x.z, f, y.z);
+            y.w = fmaf(x.w, f, y.w);
+        }
+        if (alone) {
+            store_out(r, d4, y, sum);
+        } else {
+            reinterpret_cast<float4 *>(a.part)[((int64_t)slot * R + r) * (DIM / 4) + d4] = y;
+            if (d4 == 0) a.ml[slot * R + r] = make_float2(top, sum);
+        }
+    }
+    pos += to <= end ? to - pos : end - pos;
+    if (!alone) {
+        // ---- the last CTA of the row tile to arrive adds all their partials, in order
+        const int c0 = (int)(from / share), pieces = (int)((to - 1) / share) - c0 + 1;
+        auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 && from != c0 * share ? 1 : 0); };
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) last_s = atomicAdd(&a.counters[c0], 1u) == (unsigned)(pieces - 1);
+        __syncthreads();
+        if (last_s) {
+            __threadfence();
+            if (tid == 0) a.counters[c0] = 0u;
+            // Warp w sums pieces w, w + W, ... of every row; then the warps are added as above.
+            constexpr int L = DIM / 4, PR = 32 / L;  // lanes a row, rows at a time
+            for (int rb = 0; rb < live; rb += PR) {
+                const int r = rb + lane / L, d4 = lane % L;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                float top = -INFINITY, sum = 0.f;
+                if (r < live)
+                    for (int i0 = warp; i0 < pieces; i0 += 8 * W) {
+                        float2 ml[8];
+                        float4 x[8];
+#pragma unroll
+                        for (int u = 0; u < 8; u++) {
+                            const int i = i0 + u * W, sl = slot_of(min(i, pieces - 1));
+                            ml[u] = i < pieces ? __ldcg(&a.ml[sl * R + r]) : make_float2(-INFINITY, 0.f);
+                            x[u] = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((int64_t)sl * R + r) * (DIM / 4) + d4);
+                        }
+                        float now = top;
+#pragma unroll
+                        for (int u = 0; u < 8; u++) now = fmaxf(now, ml[u].x);
+                        const float keep = pd_factor(make_float2(top, sum), now);
+                        y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
+                        sum *= keep;
+                        top = now;
+#pragma unroll
+                        for (int u = 0; u < 8; u++)
+                            if (i0 + u * W < pieces) {
+                                const float f = pd_factor(ml[u], now);
+                                sum = fmaf(ml[u].y, f, sum);
+                                y.x = fmaf(x[u].x, f, y.x);
+                                y.y = fmaf(x[u].y, f, y.y);
+                                y.z = fmaf(x[u].z, f, y.z);
+                                y.w = fmaf(x[u].w, f, y.w);
+                            }
+                    }
+                if (r < live) {
+                    wo[warp][r][pd_piece<DIM>(r, d4)] = y;
+                    if (d4 == 0) wml[warp][r] = make_float2(top, sum);
+                }
+            }
+            __syncthreads();
+            for (int i = tid; i < live * (DIM / 4); i += T) {
+                const int r = i / (DIM / 4), d4 = i % (DIM / 4);
+                float top = -INFINITY, sum = 0.f;
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < W; w++) top = fmaxf(top, wml[w][r].x);
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const float2 ml = wml[w][r];
+                    const float f = pd_factor(ml, top);
+                    const float4 x = wo[w][r][pd_piece<DIM>(r, d4)];
+                    sum = fmaf(ml.y, f, sum);
+                    y.x = fmaf(x.x, f, y.x);
+                    y.y = fmaf(x.y, f, y.y);
+                    y.z = fmaf(x.z, f, y.z);
+                    y.w = fmaf(x.w, f, y.w);
+                }
+                store_out(r, d4, y, sum);
             }
         }
     }
-    __syncthreads();
-    auto store_out = [&](int r, int d, float4 y, float sum) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);  // nothing seen: zeros
-        *reinterpret_cast<float4 *>(a.out + (long long)(e.start + (r0 + r) / a.group) * a.out_stride +
-                                    (h * a.group + (r0 + r) % a.group) * DIM + d) =
-            make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-    };
-    const int64_t base_item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits;
-    const int live = min(R, rows - r0);
-    for (int i = tid; i < live * (DIM / 4); i += kPdThreads) {
-        const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-        float top = -INFINITY, sum = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kPdWarps; w++) top = fmaxf(top, wml[w][r].x);
-#pragma unroll
-        for (int w = 0; w < kPdWarps; w++) {
-            const float2 ml = wml[w][r];
-            const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - top);
-            const float4 x = *reinterpret_cast<const float4 *>(&wo[w][r][d]);
-            sum = fmaf(ml.y, f, sum);
-            y.x = fmaf(x.x, f, y.x);
-            y.y = fmaf(x.y, f, y.y);
-            y.z = fmaf(x.z, f, y.z);
-            y.w = fmaf(x.w, f, y.w);
-        }
-        if (splits == 1) {
-            store_out(r, d, y, sum);
-        } else {
-            *reinterpret_cast<float4 *>(a.part + ((base_item + sp) * R + r) * DIM + d) = y;
-            if (d == 0) a.ml[(base_item + sp) * R + r] = make_float2(top, sum);
-        }
     }
-    if (splits == 1) return;
-
-    // ---- the last split of the row tile to arrive adds all of them, in order
-    __threadfence();
-    __syncthreads();
-    unsigned *counter = &a.counters[((int64_t)s * v.kvheads + h) * a.row_tiles + rt];
-    if (tid == 0) last_s = atomicAdd(counter, 1u) == (unsigned)(splits - 1);
-    __syncthreads();
-    if (!last_s) return;
-    __threadfence();
-    if (tid == 0) *counter = 0u;
-    float *factor = &wo[0][0][0];  // [row][split]
-    static_assert(R * kPdSplitsMax <= kPdWarps * R * DIM, "factors fit the merge buffer");
-    __shared__ float total[R];
-    for (int r = warp; r < live; r += kPdWarps) {
-        float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < splits; i += 32) top = fmaxf(top, __ldcg(&a.ml[(base_item + i) * R + r]).x);
-        top = warp_max(top);
-        for (int i = lane; i < splits; i += 32) {
-            const float2 ml = __ldcg(&a.ml[(base_item + i) * R + r]);
-            const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - top);
-            factor[r * kPdSplitsMax + i] = f;
-            sum = fmaf(ml.y, f, sum);
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) total[r] = sum;
+    __syncthreads();  // the merge buffer, the fragments and the segment are free for the next
     }
-    __syncthreads();
-    for (int i = tid; i < live * (DIM / 4); i += kPdThreads) {
-        const int r = i / (DIM / 4), d = i % (DIM / 4) * 4;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int w = 0; w < splits; w++) {
-            const float f = factor[r * kPdSplitsMax + w];
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.part + ((base_item + w) * R + r) * DIM + d));
-            y.x = fmaf(x.x, f, y.x);
-            y.y = fmaf(x.y, f, y.y);
-            y.z = fmaf(x.z, f, y.z);
-            y.w = fmaf(x.w, f, y.w);
-        }
-        store_out(r, d, y, total[r]);
-    }
+    if (bad) paged_report(a.status, bad);
 }
 
 }  // namespace tcm
