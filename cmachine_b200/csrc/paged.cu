@@ -170,7 +170,7 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
     once.run([] {
         TCM_CUDA(cudaFuncSetAttribute(paged_decode_kernel<KIND, DIM, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     });
-    const int ctas = sm_count() * PdGeo<KIND, DIM>::kCtas;
+    const int ctas = sm_count() * kPdCtas<KIND, DIM, R>;
     unsigned *count;
     paged_scratch(gpu, 2ll * ctas * R, DIM, ctas + 1, &a.part, &a.ml, &count);
     a.counters = count + 1;  // [0] takes the chunk kernel's wait errors when there is no status word
@@ -190,7 +190,8 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
 template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) {
     const int rows = (a.v.max_new < a.few ? a.v.max_new : a.few) * a.group;
     if (rows <= 8) decode_launch_rows<KIND, DIM, 8>(gpu, a);
-    else decode_launch_rows<KIND, DIM, 16>(gpu, a);
+    else if (rows <= 16) decode_launch_rows<KIND, DIM, 16>(gpu, a);
+    else decode_launch_rows<KIND, DIM, 32>(gpu, a);
 }
 
 template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {

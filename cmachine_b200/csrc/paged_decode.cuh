@@ -21,12 +21,14 @@
 // dims [g DIM / 8, (g + 1) DIM / 8) of keys 2t, 2t + 1, 8 + 2t, 9 + 2t for P V, whose
 // pairs of keys meet by byte permutes.
 //
-// Precision. FP32 queries and weights enter as sums of 16-bit parts whose products
-// with the stored rows are exact: byte codes are FP16 integers, and two FP16 parts
-// of a value scaled into FP16's range carry 22 bits; BF16 rows take three BF16
-// parts (24 bits). With R = 8 the A tile of 16 rows is [first parts; second parts],
-// so one MMA forms both. Sums in the tensor core truncate (about 4e-8 of the sum a
-// step): chains stay as short as one warp's share of an item.
+// Precision. FP32 queries and weights enter as sums of parts whose products with the stored
+// rows are exact. Byte rows meet the queries as integers: a query scaled to 23 bits and its
+// sign is three signed bytes, the products are exact in 32-bit integers, and codes need no
+// conversion (as FP16 they took 84 of a step's 600 instructions); weights meet them in
+// FP16, two parts of 22 bits together. BF16 rows take three BF16 parts (24 bits) both times.
+// With R = 8 a tile of 16 rows is [first parts; second parts], so one MMA forms both.
+// Floating-point sums in the tensor core truncate (about 4e-8 of the sum a step): chains
+// stay as short as one warp's share of a segment.
 #pragma once
 #include "paged.cuh"
 #include "stream.cuh"
@@ -34,7 +36,7 @@
 
 namespace tcm {
 
-constexpr int kPdSequences = 512;  // sequences a launch counts in shared memory
+constexpr int kPdSequences = 128;  // sequences a launch counts in shared memory (two CTAs an SM still fit)
 
 struct PagedDecodeArgs {
     PagedView v;
@@ -55,9 +57,10 @@ constexpr int kPdWarps = 8, kPdThreads = kPdWarps * 32, kPdStages = 3;
 template <int KIND, int DIM> struct PdGeo {
     static constexpr int kRow = DIM * (KIND == kPagedBytes ? 1 : 2);          // bytes a stored row
     static constexpr int kStage = 32 * kRow + (KIND == kPagedBytes ? 128 : 0);  // 16 K rows, 16 V rows, their scales
-    static constexpr int kCtas = kRow <= 128 ? 2 : 1;
     static constexpr size_t kRing = (size_t)kPdWarps * kPdStages * kStage;
 };
+// With 32 rows a thread holds 128 sums: one CTA an SM.
+template <int KIND, int DIM, int R> constexpr int kPdCtas = PdGeo<KIND, DIM>::kRow <= 128 && R <= 16 ? 2 : 1;
 // The warps' outputs meet in the rings' memory.
 template <int KIND, int DIM, int R> constexpr size_t kPdSmem =
     PdGeo<KIND, DIM>::kRing > (size_t)kPdWarps * R * DIM * 4 ? PdGeo<KIND, DIM>::kRing : (size_t)kPdWarps * R * DIM * 4;
@@ -95,11 +98,10 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int KIND>
-__device__ __forceinline__ void mma_kind(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    if constexpr (KIND == kPagedBytes) mma_f16(c, a0, a1, a2, a3, b0, b1);
-    else mma_bf16(c, a0, a1, a2, a3, b0, b1);
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -112,7 +114,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two values as the parts of a pair of 16-bit operands: parts[0] + parts[1] (+ parts[2])
+// Two weights as the parts of a pair of 16-bit operands: parts[0] + parts[1] (+ parts[2])
 // is the value to 22 (FP16) or 24 (BF16) bits.
 template <int KIND> constexpr int kPdParts = KIND == kPagedBytes ? 2 : 3;
 template <int KIND> __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&parts)[kPdParts<KIND>]) {
@@ -171,7 +173,8 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-constexpr float kPdWeightTop = 14.f;  // byte rows' weights are scaled to at most 2^14
+constexpr float kPdSlack = 3.f;   // log2 of how far a row's weights may pass 1 before its reference moves
+constexpr int kPdWeightTop = 12;  // log2 of the largest byte row's weight at 1: 2^15 with the slack, inside FP16
 
 // A CTA's present segment; read again after the loop, so that the loop keeps its registers.
 struct PdSegment {
@@ -183,24 +186,25 @@ struct PdSegment {
 };
 
 template <int KIND, int DIM, int R>
-__global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_decode_kernel(const PagedDecodeArgs a) {
+__global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_decode_kernel(const PagedDecodeArgs a) {
     constexpr bool kBytes = KIND == kPagedBytes;
     using G = PdGeo<KIND, DIM>;
     constexpr int W = kPdWarps, T = kPdThreads;
-    constexpr int ES = kBytes ? 1 : 2;              // bytes an element
-    constexpr int KP = DIM * ES / 64;               // 16-byte pieces of a key a lane holds for Q K^T
-    constexpr int KS = DIM / 16;                    // k-steps of Q K^T
-    constexpr int DV = DIM / 8;                     // dims of a key a lane holds for P V
-    constexpr int VW = DV * ES / 4;                 // the same in words
-    constexpr int P = kPdParts<KIND>;
-    constexpr int NA = R == 8 ? (P + 1) / 2 : P;    // A tiles a product takes
-    constexpr int RW = R / 8;                       // query rows a lane holds scores of
+    constexpr int ES = kBytes ? 1 : 2;         // bytes an element
+    constexpr int KS = DIM * ES / 32;          // k-steps of Q K^T: 8 bytes of a key a lane
+    constexpr int DV = DIM / 8;                // dims of a key a lane holds for P V
+    constexpr int VW = DV * ES / 4;            // the same in words
+    constexpr int P = kPdParts<KIND>;          // parts of a weight; a query has three
+    constexpr int M = R == 32 ? 2 : 1;         // tiles of 16 MMA rows
+    constexpr int NA = R == 8 ? 2 : 3;         // of each, the A operands a query product takes
+    constexpr int RL = R == 8 ? 1 : 2;         // query rows of a tile a lane holds scores of
     extern __shared__ __align__(1024) unsigned char pc_smem[];
     float4(*wo)[R][DIM / 4] = reinterpret_cast<float4(*)[R][DIM / 4]>(pc_smem);  // the warps' outputs
-    __shared__ __align__(16) uint4 qf[NA][KS][32];  // Q's fragments
+    __shared__ __align__(16) uint4 qf[M * NA][KS][32];  // Q's fragments
     __shared__ float qs[R];                         // scale2 times the row's power of two
     __shared__ float2 wml[W][R];
     __shared__ int upto[kPdSequences + 1];    // steps before each sequence
+    __shared__ PagedExtent extents[kPdSequences];
     __shared__ int last_s;
     __shared__ PdSegment seg;
     const PagedView &v = a.v;
@@ -215,6 +219,7 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
     for (int i = tid; i < v.sequences; i += T) {
         PagedExtent e;
         const int bad = paged_extent(&v, i, &e);
+        extents[i] = e;
         if (bad && !blockIdx.x) paged_report(a.status, bad);
         int steps = 0;  // the host keeps a launch's sum below 2^31
         if (e.count <= a.few)
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
             if (upto[mid] <= pos) z.s = mid;
             else top = mid - 1;
         }
-        paged_extent(&v, z.s, &z.e);
+        z.e = extents[z.s];
         const int in_seq = pos - upto[z.s], a_head = (upto[z.s + 1] - upto[z.s]) / v.kvheads;
         z.h = in_seq / a_head;
         int in_tile = in_seq - z.h * a_head, rt = 0;
@@ -276,64 +281,9 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
     const int first = e.length - e.count + r0 / a.group;
     const int last = e.length - e.count + (min(rows, r0 + R) - 1) / a.group;
 
-    // ---- its queries as fragments: warp w prepares rows w, w + W, ...
-    for (int r = warp; r < R; r += W) {
-        float x[DIM / 32], m = 0.f;
-        const bool on = r0 + r < rows;
-        if (on) {
-            const float *src = a.q + (long long)(e.start + (r0 + r) / a.group) * a.q_stride +
-                               (h * a.group + (r0 + r) % a.group) * DIM;
-            if constexpr (DIM == 128) {
-                const float4 f = reinterpret_cast<const float4 *>(src)[lane];
-                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-            } else {
-                const float2 f = reinterpret_cast<const float2 *>(src)[lane];
-                x[0] = f.x, x[1] = f.y;
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < DIM / 32; c++) x[c] = 0.f;
-        }
-        float up = 1.f, down = 1.f;
-        if constexpr (kBytes) {  // into FP16's range: the largest element in [2^14, 2^15)
-#pragma unroll
-            for (int c = 0; c < DIM / 32; c++) m = fmaxf(m, fabsf(x[c]));
-            const int ex = exponent_of(warp_max(m)) - 14;
-            up = power_of_two(-ex);
-            down = power_of_two(ex);
-        }
-        if (lane == 0) qs[r] = a.scale2 * down;
-#pragma unroll
-        for (int c = 0; c < DIM / 32; c += 2) {
-            uint32_t parts[P];
-            split_pair<KIND>(x[c] * up, x[c + 1] * up, parts);
-            // Dims d, d + 1 -> k-step, lane and half of the fragment.
-            const int d = lane * (DIM / 32) + c;
-            int ks, ft, fh;
-            if constexpr (kBytes) ks = (d / 64) * 4 + (d % 16) / 4, ft = (d % 64) / 16, fh = (d % 4) / 2;
-            else ks = (d / 32) * 2 + (d % 8) / 4, ft = (d % 32) / 8, fh = (d % 4) / 2;
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                // R = 8: part p is rows 8 (p % 2) + r of tile p / 2; R = 16: row r of tile p.
-                const int tile = R == 8 ? p / 2 : p, row = R == 8 ? (p % 2) * 8 + r : r;
-                reinterpret_cast<uint32_t *>(&qf[tile][ks][(row % 8) * 4 + ft])[2 * fh + row / 8] = parts[p];
-            }
-            if (R == 8 && P % 2) reinterpret_cast<uint32_t *>(&qf[NA - 1][ks][r * 4 + ft])[2 * fh + 1] = 0u;
-        }
-    }
-    __syncthreads();
-
-    // ---- the loop over this warp's 16-row steps
-    const bool whole = v.page % 16 == 0;  // a step lies inside one page
-    float o[DV][4], m[RW], mu[RW], l[RW], sc[RW];
-#pragma unroll
-    for (int j = 0; j < DV; j++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) o[j][c] = 0.f;
-#pragma unroll
-    for (int r = 0; r < RW; r++) m[r] = mu[r] = -INFINITY, l[r] = 0.f, sc[r] = qs[g + 8 * r];
-
-    auto page_of = [&](int k) -> int {  // the page id of lane % 16's row of step k
+    // ---- the copies of this warp's steps
+    const bool whole = v.page % 16 == 0;  // a step lies inside one page, 16 rows of one stretch of memory
+    auto page_of = [&](int k) -> int {    // the page id of step k, or (pages that end inside steps) of lane % 16's row
         if (k >= k1) return -1;
         const int j = min(paged_tile(tiles, k) * 16 + (whole ? 0 : lane & 15), last);
         return v.table[(int64_t)s * v.table_stride + paged_div(&v, j)];
@@ -342,156 +292,326 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
     // call, empty behind the last step.
     const uint32_t ring = smem_addr(pc_smem) + (uint32_t)warp * kPdStages * G::kStage;
     auto fetch = [&](int k, int id, int stage) -> unsigned {
-        int64_t row = -1;  // lane % 16's
+        constexpr int LPR = G::kRow / 16, RPL = 32 / LPR;  // lanes a row, rows at a time
+        unsigned there = 0;
         if (k < k1) {
-            const int j = paged_tile(tiles, k) * 16 + (lane & 15);
-            if (j <= last) {
-                row = paged_row(&v, id, j, paged_div(&v, j), h);
-                // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
-                if (row < 0 && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) bad |= kPagedBadPage;
-            }
+            const int j0 = paged_tile(tiles, k) * 16;
             const uint32_t dst = ring + (uint32_t)stage * G::kStage;
-            constexpr int LPR = G::kRow / 16, RPL = 32 / LPR;  // lanes a row, rows at a time
+            // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
+            auto needed = [&](int j) { return a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window; };
+            if (whole) {
+                const int64_t row = paged_row(&v, id, j0, paged_div(&v, j0), h);
+                const int rows_there = row < 0 ? 0 : min(16, last - j0 + 1);
+                if (row < 0)
+                    for (int j = j0; j < j0 + 16; j++)
+                        if (j <= last && needed(j)) bad |= kPagedBadPage;
+                there = (1u << rows_there) - 1u;
+                const int64_t at = (row < 0 ? 0 : row) * G::kRow + lane * 16;
 #pragma unroll
-            for (int i = 0; i < 16 / RPL; i++) {
-                const int rr = i * RPL + lane / LPR, piece = lane % LPR;
-                const int64_t r = __shfl_sync(0xffffffffu, row, rr);
-                const int64_t at = r < 0 ? 0 : r * G::kRow + piece * 16;
-                const uint32_t to = dst + (uint32_t)(rr * G::kRow + pd_swizzle<G::kRow>(rr, piece) * 16);
-                pd_copy16(to, static_cast<const char *>(v.keys) + at, r >= 0);
-                pd_copy16(to + 16 * G::kRow, static_cast<const char *>(v.values) + at, r >= 0);
+                for (int i = 0; i < 16 / RPL; i++) {
+                    const int rr = i * RPL + lane / LPR;
+                    const uint32_t to = dst + (uint32_t)(rr * G::kRow + pd_swizzle<G::kRow>(rr, lane % LPR) * 16);
+                    pd_copy16(to, static_cast<const char *>(v.keys) + at + i * 512, rr < rows_there);
+                    pd_copy16(to + 16 * G::kRow, static_cast<const char *>(v.values) + at + i * 512, rr < rows_there);
+                }
+                if constexpr (kBytes)
+                    pd_copy4(dst + 32 * G::kRow + lane * 4, v.scales + ((lane & 15) < rows_there ? (lane >= 16 ? half : 0) + row + (lane & 15) : 0),
+                             (lane & 15) < rows_there);
+            } else {
+                const int j = j0 + (lane & 15);
+                int64_t row = -1;  // lane % 16's
+                if (j <= last) {
+                    row = paged_row(&v, id, j, paged_div(&v, j), h);
+                    if (row < 0 && needed(j)) bad |= kPagedBadPage;
+                }
+                there = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+#pragma unroll
+                for (int i = 0; i < 16 / RPL; i++) {
+                    const int rr = i * RPL + lane / LPR, piece = lane % LPR;
+                    const int64_t r = __shfl_sync(0xffffffffu, row, rr);
+                    const int64_t at = r < 0 ? 0 : r * G::kRow + piece * 16;
+                    const uint32_t to = dst + (uint32_t)(rr * G::kRow + pd_swizzle<G::kRow>(rr, piece) * 16);
+                    pd_copy16(to, static_cast<const char *>(v.keys) + at, r >= 0);
+                    pd_copy16(to + 16 * G::kRow, static_cast<const char *>(v.values) + at, r >= 0);
+                }
+                if constexpr (kBytes)
+                    pd_copy4(dst + 32 * G::kRow + lane * 4, v.scales + (row < 0 ? 0 : (lane >= 16 ? half : 0) + row), row >= 0);
             }
-            if constexpr (kBytes)
-                pd_copy4(dst + 32 * G::kRow + lane * 4, v.scales + (row < 0 ? 0 : (lane >= 16 ? half : 0) + row), row >= 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+        return there;
     };
-
     int k = k0 + warp;
     unsigned there = fetch(k, page_of(k), 0), there1 = fetch(k + W, page_of(k + W), 1);
     int id_next = page_of(k + 2 * W);
+
+    // ---- the queries as fragments: warp w prepares rows w, w + W, ...
+    for (int r = warp; r < R; r += W) {
+        constexpr int E = DIM / 32;
+        float x[E];
+#pragma unroll
+        for (int c = 0; c < E; c++) x[c] = 0.f;
+        if (r0 + r < rows) {
+            const float *src = a.q + (long long)(e.start + (r0 + r) / a.group) * a.q_stride +
+                               (h * a.group + (r0 + r) % a.group) * DIM;
+            if constexpr (E == 4) {
+                const float4 f = reinterpret_cast<const float4 *>(src)[lane];
+                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+            } else {
+                const float2 f = reinterpret_cast<const float2 *>(src)[lane];
+                x[0] = f.x, x[1] = f.y;
+            }
+        }
+        // R = 8: part p is rows 8 (p % 2) + r of operand p / 2; else row r % 16 of operand 3 (r / 16) + p.
+        auto place = [&](int p, int ks, int ft, int fh) {
+            const int tile = R == 8 ? p / 2 : r / 16 * 3 + p, row = R == 8 ? (p % 2) * 8 + r : r % 16;
+            return &reinterpret_cast<uint32_t *>(&qf[tile][ks][(row % 8) * 4 + ft])[2 * fh + row / 8];
+        };
+        const int d = lane * E;
+        if constexpr (kBytes) {
+            // The row as integers up to 127 x 65536, each three signed bytes: 65536 a + 256 b + c, off by at
+            // most half of 2^-23 of the row's largest element.
+            constexpr float kMost = 127.f * 65536.f;
+            float m = 0.f;
+            bool finite = true;
+#pragma unroll
+            for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(x[c])), finite &= isfinite(x[c]);
+            finite = __all_sync(0xffffffffu, finite);
+            m = warp_max(m);
+            const bool any = finite && m >= 1e-30f;  // smaller queries see every row alike
+            const float up = any ? kMost / m : 0.f;
+            if (lane == 0) qs[r] = finite ? a.scale2 * (m * (1.f / kMost)) : __uint_as_float(0x7fc00000u);
+            uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < E; c++) {
+                int n = any ? __float2int_rn(x[c] * up) : 0;
+                const int lo = (int)(signed char)n;
+                n = (n - lo) >> 8;
+                const int mid = (int)(signed char)n;
+                n = (n - mid) >> 8;
+                w[0] |= (uint32_t)(n & 0xff) << (8 * c);
+                w[1] |= (uint32_t)(mid & 0xff) << (8 * c);
+                w[2] |= (uint32_t)(lo & 0xff) << (8 * c);
+            }
+            // Dims 4n .. 4n + 3 of a 16-dim piece: k-step n / 2 of the piece's two, half n % 2.
+            const int ks = (d / 64) * 2 + (d % 16) / 8, ft = (d % 64) / 16, fh = (d % 8) / 4;
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                if constexpr (E == 4) *place(p, ks, ft, fh) = w[p];
+                else reinterpret_cast<uint16_t *>(place(p, ks, ft, fh))[(d % 4) / 2] = (uint16_t)w[p];
+            }
+            if (R == 8) *place(3, ks, ft, fh) = 0u;
+        } else {
+            if (lane == 0) qs[r] = a.scale2;
+#pragma unroll
+            for (int c = 0; c < E; c += 2) {
+                uint32_t w[3];
+                split_pair<kPagedBf16>(x[c], x[c + 1], w);
+                const int dd = d + c, ks = (dd / 32) * 2 + (dd % 8) / 4, ft = (dd % 32) / 8, fh = (dd % 4) / 2;
+#pragma unroll
+                for (int p = 0; p < 3; p++) *place(p, ks, ft, fh) = w[p];
+                if (R == 8) *place(3, ks, ft, fh) = 0u;
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- the loop over this warp's 16-row steps
+    float o[M][DV][4], m[M][RL], l[M][RL], sc[M][RL];
+#pragma unroll
+    for (int mt = 0; mt < M; mt++) {
+#pragma unroll
+        for (int j = 0; j < DV; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[mt][j][c] = 0.f;
+#pragma unroll
+        for (int r = 0; r < RL; r++) m[mt][r] = -INFINITY, l[mt][r] = 0.f, sc[mt][r] = qs[16 * mt + 8 * r + g];
+    }
+    // Byte rows: weights carry the rows' scales, times 2^12 over a power of two above the largest
+    // scale so far (v_top, exponent v_exp).
+    float v_top = 0.f, v_factor = 0.f;
+    int v_exp = 0;
+    const int see_all = a.window == 0 || a.window > last ? 0 : last - a.window + 1;  // every query sees from here to `first`
     for (int stage = 0; k < k1; k += W, stage = stage == kPdStages - 1 ? 0 : stage + 1) {
         const int ahead = stage == 0 ? kPdStages - 1 : stage - 1;  // the stage read in the step before
         const unsigned there2 = fetch(k + 2 * W, id_next, ahead);
         id_next = page_of(k + 3 * W);
         asm volatile("cp.async.wait_group 2;" ::: "memory");
         __syncwarp();
-        const unsigned char *st = pc_smem + (size_t)warp * kPdStages * G::kStage + (size_t)stage * G::kStage;
-        // Scores of 16 places: S[gr] columns 2t, 2t + 1 are places base + 8 gr + 2t, + 1.
-        float sf[2][4];
+        const unsigned char *st = pc_smem + ((size_t)warp * kPdStages + stage) * G::kStage;
+        const int base = paged_tile(tiles, k) * 16;
+        const bool full = there == 0xffffu && base + 15 <= first && (base >= see_all || base + 15 < a.sinks);
+
+        // ---- scores of 16 places: x[..][i] is place base + 8 (i / 2) + 2t + i % 2
+        float x[M][RL][4];
+        {
+            int ci[kBytes ? M * NA : 1][2][4];
+            float cf[kBytes ? 1 : M][2][4];
 #pragma unroll
-        for (int gr = 0; gr < 2; gr++)
+            for (int gr = 0; gr < 2; gr++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) sf[gr][c] = 0.f;
-        uint4 kr[2];
+                for (int c = 0; c < 4; c++) {
+                    if constexpr (kBytes)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            constexpr int KPP = KS / KP;  // k-steps a 16-byte piece of a key feeds
-            if (ks % KPP == 0)
+                        for (int n = 0; n < M * NA; n++) ci[n][gr][c] = 0;
+                    else
 #pragma unroll
-                for (int gr = 0; gr < 2; gr++) {
-                    const int key = gr * 8 + g;
-                    kr[gr] = *reinterpret_cast<const uint4 *>(st + key * G::kRow + pd_swizzle<G::kRow>(key, (ks / KPP) * 4 + t) * 16);
+                        for (int mt = 0; mt < M; mt++) cf[mt][gr][c] = 0.f;
                 }
-            uint32_t b0[2], b1[2];
+            uint4 kr[2];
 #pragma unroll
-            for (int gr = 0; gr < 2; gr++) {
-                if constexpr (kBytes) {
-                    const uint32_t w = word(kr[gr], ks % 4) ^ 0x80808080u;
-                    b0[gr] = codes_f16(w, 0x4140);
-                    b1[gr] = codes_f16(w, 0x4342);
-                } else {
-                    b0[gr] = word(kr[gr], (ks % 2) * 2);
-                    b1[gr] = word(kr[gr], (ks % 2) * 2 + 1);
+            for (int ks = 0; ks < KS; ks++) {
+                if (ks % 2 == 0)
+#pragma unroll
+                    for (int gr = 0; gr < 2; gr++) {
+                        const int key = gr * 8 + g;
+                        kr[gr] = *reinterpret_cast<const uint4 *>(st + key * G::kRow + pd_swizzle<G::kRow>(key, (ks / 2) * 4 + t) * 16);
+                    }
+#pragma unroll
+                for (int n = M * NA - 1; n >= 0; n--) {
+                    const uint4 f = qf[n][ks][lane];
+#pragma unroll
+                    for (int gr = 0; gr < 2; gr++) {
+                        const uint32_t b0 = ks % 2 ? kr[gr].z : kr[gr].x, b1 = ks % 2 ? kr[gr].w : kr[gr].y;
+                        if constexpr (kBytes) mma_s8(ci[n][gr], f, b0, b1);
+                        else mma_bf16(cf[n / NA][gr], f.x, f.y, f.z, f.w, b0, b1);
+                    }
                 }
             }
 #pragma unroll
-            for (int n = NA - 1; n >= 0; n--) {
-                const uint4 f = qf[n][ks][lane];
+            for (int mt = 0; mt < M; mt++)
 #pragma unroll
-                for (int gr = 0; gr < 2; gr++) mma_kind<KIND>(sf[gr], f.x, f.y, f.z, f.w, b0[gr], b1[gr]);
+                for (int r = 0; r < RL; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int gr = i >> 1, c = i & 1;
+                        if constexpr (kBytes) {
+                            // Each sum is below 2^21, the lower two together below 2^30.
+                            const int top = R == 8 ? ci[0][gr][c] : ci[mt * NA][gr][2 * r + c];
+                            const int mid = R == 8 ? ci[0][gr][2 + c] : ci[mt * NA + 1][gr][2 * r + c];
+                            const int low = R == 8 ? ci[1][gr][c] : ci[mt * NA + NA - 1][gr][2 * r + c];
+                            x[mt][r][i] = fmaf((float)top, 65536.f, (float)(mid * 256 + low));
+                        } else {
+                            x[mt][r][i] = R == 8 ? cf[0][gr][c] + cf[0][gr][2 + c] : cf[mt][gr][2 * r + c];
+                        }
+                    }
+        }
+        float vs[4];
+        if constexpr (kBytes) {
+            const float *ks4 = reinterpret_cast<const float *>(st + 32 * G::kRow);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = (i >> 1) * 8 + 2 * t + (i & 1);
+                vs[i] = ks4[16 + at];
+#pragma unroll
+                for (int mt = 0; mt < M; mt++)
+#pragma unroll
+                    for (int r = 0; r < RL; r++) x[mt][r][i] *= ks4[at];
             }
         }
-        float ks4[4], vs4[4];
+        bool moves = false;
+        float top[M][RL];
+#pragma unroll
+        for (int mt = 0; mt < M; mt++)
+#pragma unroll
+            for (int r = 0; r < RL; r++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[mt][r][i] *= sc[mt][r];
+                if (!full) {
+                    const int at = e.length - e.count + min(r0 + 16 * mt + 8 * r + g, rows - 1) / a.group;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int c = (i >> 1) * 8 + 2 * t + (i & 1);
+                        if (!((there >> c) & 1) || !paged_sees(at, base + c, a.window, a.sinks)) x[mt][r][i] = -INFINITY;
+                    }
+                }
+                top[mt][r] = quad_max(fmaxf(fmaxf(x[mt][r][0], x[mt][r][1]), fmaxf(x[mt][r][2], x[mt][r][3])));
+                moves |= top[mt][r] > m[mt][r] + kPdSlack;
+            }
+        float v_most = 0.f;
+        if constexpr (kBytes) {
+            v_most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+            if (!full) {  // the scale of a row that some query does not see may be anything
+                v_most = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) v_most = fmaxf(v_most, vs[i] < INFINITY ? vs[i] : 0.f);
+            }
+            v_most = quad_max(v_most);
+            moves |= v_most > v_top;
+        }
+        // References move rarely: a row's when its maximum has passed it by 2^3 (weights have that
+        // much room), the scale's when a larger one turns up.
+        if (__any_sync(0xffffffffu, moves)) {
+            float shrink = 1.f;
+            if constexpr (kBytes) {
+                if (v_most > v_top) {  // the same in every lane
+                    const int was = v_exp;
+                    v_exp = max(-100, exponent_of(v_most) + 1);
+                    shrink = v_top == 0.f ? 0.f : power_of_two(was - v_exp);
+                    v_top = power_of_two(v_exp);
+                    v_factor = power_of_two(kPdWeightTop - v_exp);
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < M; mt++) {
+                float keep[RL];
+#pragma unroll
+                for (int r = 0; r < RL; r++) {
+                    keep[r] = shrink;
+                    if (top[mt][r] > m[mt][r] + kPdSlack) {
+                        const float c = m[mt][r] == -INFINITY ? 0.f : ex2(m[mt][r] - top[mt][r]);
+                        m[mt][r] = top[mt][r];
+                        l[mt][r] *= c;
+                        keep[r] *= c;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < DV; j++) {
+                    o[mt][j][0] *= keep[0];
+                    o[mt][j][1] *= keep[0];
+                    o[mt][j][2] *= keep[RL - 1];
+                    o[mt][j][3] *= keep[RL - 1];
+                }
+            }
+        }
         if constexpr (kBytes) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float *sc4 = reinterpret_cast<const float *>(st + 32 * G::kRow) + (i >> 1) * 8 + 2 * t + (i & 1);
-                ks4[i] = sc4[0];
-                vs4[i] = sc4[16];
-            }
+            for (int i = 0; i < 4; i++) vs[i] *= v_factor;
         }
-
-        const int base = paged_tile(tiles, k) * 16;
-        // Every query of the tile sees every place of the step?
-        const bool full = there == 0xffffu && base + 15 <= first &&
-                          (a.window == 0 || base + 15 < a.sinks || (int64_t)base > (int64_t)last - a.window);
-        uint32_t pa[RW][2][P];  // weights as fragments' parts: [row][group of 8 places][part]
-        float keep[RW];         // what this step's new reference leaves of the sums so far
-        bool moved = false;
+        uint32_t pa[M][RL][2][P];  // weights as fragments' parts: [tile][row][group of 8 places][part]
 #pragma unroll
-        for (int r = 0; r < RW; r++) {
-            float x[4], w[4];
+        for (int mt = 0; mt < M; mt++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[i] = R == 8 ? sf[i >> 1][i & 1] + sf[i >> 1][2 + (i & 1)] : sf[i >> 1][2 * r + (i & 1)];
-                if constexpr (kBytes) x[i] *= ks4[i];
-                x[i] *= sc[r];
-            }
-            if (!full) {
-                const int at = e.length - e.count + min(r0 + g + 8 * r, rows - 1) / a.group;
+            for (int r = 0; r < RL; r++) {
+                float w[4];
+                const float mr = m[mt][r] == -INFINITY ? 0.f : m[mt][r];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int c = (i >> 1) * 8 + 2 * t + (i & 1);
-                    if (!((there >> c) & 1) || !paged_sees(at, base + c, a.window, a.sinks)) x[i] = -INFINITY;
+                    w[i] = ex2(x[mt][r][i] - mr);
+                    l[mt][r] += w[i];
+                    if constexpr (kBytes) w[i] *= vs[i];
+                    if (kBytes && !full && x[mt][r][i] == -INFINITY) w[i] = 0.f;
                 }
+                split_pair<KIND>(w[0], w[1], pa[mt][r][0]);
+                split_pair<KIND>(w[2], w[3], pa[mt][r][1]);
             }
-            const float m_new = fmaxf(m[r], quad_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
-            const float mr = m_new == -INFINITY ? 0.f : m_new;
-            l[r] *= m[r] == -INFINITY ? 0.f : ex2(m[r] - mr);
-            m[r] = m_new;
+        auto pv = [&](int j, uint32_t b0, uint32_t b1) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w[i] = ex2(x[i] - mr);
-                l[r] += w[i];
-            }
-            float mu_new = m_new;
-            if constexpr (kBytes) {
-                // The weight of a row is p_j s_j. mu follows log2 of the largest, so that 2^14 of the
-                // FP16 range goes to whatever carries the sum, however unlike the rows' scales are;
-                // at most 2^113 from m, so that the factor is a number.
-                float u = -INFINITY;
+            for (int mt = 0; mt < M; mt++) {
+                float(&acc)[4] = o[mt][j];
+                const auto &w = pa[mt];
+                if constexpr (kBytes) {
+                    if constexpr (R == 8) mma_f16(acc, w[0][0][0], w[0][0][1], w[0][1][0], w[0][1][1], b0, b1);
+                    else
 #pragma unroll
-                for (int i = 0; i < 4; i++) u = fmaxf(u, x[i] + __log2f(vs4[i]));
-                mu_new = fmaxf(fmaxf(mu[r], quad_max(u)), m_new - 113.f);
-                const float f = mu_new == -INFINITY ? 0.f : ex2(mr - mu_new + kPdWeightTop);
+                        for (int p = 1; p >= 0; p--) mma_f16(acc, w[0][0][p], w[RL - 1][0][p], w[0][1][p], w[RL - 1][1][p], b0, b1);
+                } else if constexpr (R == 8) {
+                    mma_bf16(acc, w[0][0][P - 1], 0u, w[0][1][P - 1], 0u, b0, b1);
+                    mma_bf16(acc, w[0][0][0], w[0][0][1], w[0][1][0], w[0][1][1], b0, b1);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = x[i] == -INFINITY ? 0.f : w[i] * (vs4[i] * f);
-            }
-            keep[r] = mu[r] == -INFINITY ? 0.f : ex2(mu[r] - mu_new);
-            moved |= mu_new != mu[r];
-            mu[r] = mu_new;
-            split_pair<KIND>(w[0], w[1], pa[r][0]);
-            split_pair<KIND>(w[2], w[3], pa[r][1]);
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int j = 0; j < DV; j++) {
-                o[j][0] *= keep[0];
-                o[j][1] *= keep[0];
-                o[j][2] *= keep[RW - 1];
-                o[j][3] *= keep[RW - 1];
-            }
-        }
-        auto pv = [&](float(&acc)[4], uint32_t b0, uint32_t b1) {
-            if constexpr (R == 8) {
-                if constexpr (P == 3) mma_kind<KIND>(acc, pa[0][0][2], 0u, pa[0][1][2], 0u, b0, b1);
-                mma_kind<KIND>(acc, pa[0][0][0], pa[0][0][1], pa[0][1][0], pa[0][1][1], b0, b1);
-            } else {
-#pragma unroll
-                for (int p = P - 1; p >= 0; p--)
-                    mma_kind<KIND>(acc, pa[0][0][p], pa[RW - 1][0][p], pa[0][1][p], pa[RW - 1][1][p], b0, b1);
+                    for (int p = P - 1; p >= 0; p--) mma_bf16(acc, w[0][0][p], w[RL - 1][0][p], w[0][1][p], w[RL - 1][1][p], b0, b1);
+                }
             }
         };
         uint4 vr[4];
@@ -512,21 +632,19 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
                     if (!kBytes && !full)
                         vr[i] = make_uint4(finite_pair(vr[i].x), finite_pair(vr[i].y), finite_pair(vr[i].z), finite_pair(vr[i].w));
                 }
-            uint32_t x[4];
+            uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = word(vr[i], c % 4);
+            for (int i = 0; i < 4; i++) y[i] = word(vr[i], c % 4);
             if constexpr (kBytes) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] ^= 0x80808080u;
-                const uint32_t lo0 = __byte_perm(x[0], x[1], 0x5140), hi0 = __byte_perm(x[0], x[1], 0x7362);
-                const uint32_t lo1 = __byte_perm(x[2], x[3], 0x5140), hi1 = __byte_perm(x[2], x[3], 0x7362);
-                pv(o[4 * c], codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140));
-                pv(o[4 * c + 1], codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342));
-                pv(o[4 * c + 2], codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140));
-                pv(o[4 * c + 3], codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342));
+                const uint32_t lo0 = __byte_perm(y[0], y[1], 0x5140) ^ 0x80808080u, hi0 = __byte_perm(y[0], y[1], 0x7362) ^ 0x80808080u;
+                const uint32_t lo1 = __byte_perm(y[2], y[3], 0x5140) ^ 0x80808080u, hi1 = __byte_perm(y[2], y[3], 0x7362) ^ 0x80808080u;
+                pv(4 * c, codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140));
+                pv(4 * c + 1, codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342));
+                pv(4 * c + 2, codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140));
+                pv(4 * c + 3, codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342));
             } else {
-                pv(o[2 * c], __byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410));
-                pv(o[2 * c + 1], __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
+                pv(2 * c, __byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410));
+                pv(2 * c + 1, __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
             }
         }
         there = there1;
@@ -537,23 +655,27 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
     __syncthreads();  // no copy is left in flight, and the rings' memory is free for the outputs
 
     // ---- the warps' states: lane (g, t) holds dims [2 t DV, (2 t + 2) DV) of row g (+ 8)
+    const float unscale = kBytes ? power_of_two(v_exp - kPdWeightTop) : 1.f;
 #pragma unroll
-    for (int r = 0; r < RW; r++) {
-        float sum = l[r];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (t == 0) wml[warp][g + 8 * r] = make_float2(m[r], sum);
-        const float f = kBytes ? (mu[r] == -INFINITY ? 0.f : ex2(mu[r] - m[r] - kPdWeightTop)) : 1.f;
+    for (int mt = 0; mt < M; mt++)
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int r = 0; r < RL; r++) {
+            float sum = l[mt][r];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int row = 16 * mt + 8 * r + g;
+            if (t == 0) wml[warp][row] = make_float2(m[mt][r], sum);
 #pragma unroll
-            for (int j = 0; j < DV; j += 4) {
-                float y[4];
+            for (int c = 0; c < 2; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = f * (R == 8 ? o[j + i][c] + o[j + i][2 + c] : o[j + i][2 * r + c]);
-                wo[warp][g + 8 * r][pd_piece<DIM>(g + 8 * r, ((2 * t + c) * DV + j) / 4)] = make_float4(y[0], y[1], y[2], y[3]);
-            }
-    }
+                for (int j = 0; j < DV; j += 4) {
+                    float y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        y[i] = unscale * (R == 8 ? o[mt][j + i][c] + o[mt][j + i][2 + c] : o[mt][j + i][2 * r + c]);
+                    wo[warp][row][pd_piece<DIM>(row, ((2 * t + c) * DV + j) / 4)] = make_float4(y[0], y[1], y[2], y[3]);
+                }
+        }
     __syncthreads();
     {
     const volatile PdSegment &z = seg;
@@ -603,43 +725,40 @@ __global__ void __launch_bounds__(kPdThreads, (PdGeo<KIND, DIM>::kCtas)) paged_d
         if (last_s) {
             __threadfence();
             if (tid == 0) a.counters[c0] = 0u;
-            // Warp w sums pieces w, w + W, ... of every row; then the warps are added as above.
-            constexpr int L = DIM / 4, PR = 32 / L;  // lanes a row, rows at a time
-            for (int rb = 0; rb < live; rb += PR) {
-                const int r = rb + lane / L, d4 = lane % L;
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                float top = -INFINITY, sum = 0.f;
-                if (r < live)
-                    for (int i0 = warp; i0 < pieces; i0 += 8 * W) {
-                        float2 ml[8];
-                        float4 x[8];
+            // Warp w sums pieces w, w + W, ..., eight rows' loads in flight; then the warps are added
+            // as above.
+            constexpr int L = DIM / 4, PR = 32 / L, B = 8;  // lanes a row, rows a load, loads in flight
+            for (int rb = 0; rb < live; rb += PR * B) {
+                const int d4 = lane % L;
+                float4 y[B];
+                float2 state[B];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) {
-                            const int i = i0 + u * W, sl = slot_of(min(i, pieces - 1));
-                            ml[u] = i < pieces ? __ldcg(&a.ml[sl * R + r]) : make_float2(-INFINITY, 0.f);
-                            x[u] = __ldcg(reinterpret_cast<const float4 *>(a.part) + ((int64_t)sl * R + r) * (DIM / 4) + d4);
-                        }
-                        float now = top;
+                for (int u = 0; u < B; u++) y[u] = make_float4(0.f, 0.f, 0.f, 0.f), state[u] = make_float2(-INFINITY, 0.f);
+                for (int i = warp; i < pieces; i += W) {
+                    const int64_t at = (int64_t)slot_of(i) * R;
+                    float2 ml[B];
+                    float4 x[B];
 #pragma unroll
-                        for (int u = 0; u < 8; u++) now = fmaxf(now, ml[u].x);
-                        const float keep = pd_factor(make_float2(top, sum), now);
-                        y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
-                        sum *= keep;
-                        top = now;
-#pragma unroll
-                        for (int u = 0; u < 8; u++)
-                            if (i0 + u * W < pieces) {
-                                const float f = pd_factor(ml[u], now);
-                                sum = fmaf(ml[u].y, f, sum);
-                                y.x = fmaf(x[u].x, f, y.x);
-                                y.y = fmaf(x[u].y, f, y.y);
-                                y.z = fmaf(x[u].z, f, y.z);
-                                y.w = fmaf(x[u].w, f, y.w);
-                            }
+                    for (int u = 0; u < B; u++) {
+                        const int r = min(rb + u * PR + lane / L, live - 1);
+                        ml[u] = __ldcg(&a.ml[at + r]);
+                        x[u] = __ldcg(reinterpret_cast<const float4 *>(a.part) + (at + r) * L + d4);
                     }
-                if (r < live) {
-                    wo[warp][r][pd_piece<DIM>(r, d4)] = y;
-                    if (d4 == 0) wml[warp][r] = make_float2(top, sum);
+#pragma unroll
+                    for (int u = 0; u < B; u++) {
+                        const float now = fmaxf(state[u].x, ml[u].x), keep = pd_factor(state[u], now), f = pd_factor(ml[u], now);
+                        state[u] = make_float2(now, fmaf(ml[u].y, f, state[u].y * keep));
+                        y[u] = make_float4(fmaf(x[u].x, f, y[u].x * keep), fmaf(x[u].y, f, y[u].y * keep),
+                                           fmaf(x[u].z, f, y[u].z * keep), fmaf(x[u].w, f, y[u].w * keep));
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < B; u++) {
+                    const int r = rb + u * PR + lane / L;
+                    if (r < live) {
+                        wo[warp][r][pd_piece<DIM>(r, d4)] = y[u];
+                        if (d4 == 0) wml[warp][r] = state[u];
+                    }
                 }
             }
             __syncthreads();

@@ -3,12 +3,14 @@
 The oracle reads the pool's own bytes, so attention is held to its arithmetic
 alone, element by element, by
 
-    |out - exact| <= 2^-23 (64 S + 128 + n / 8) sum_j p_j |v_j|,   S = max_j sum_c |q_c k_jc| / sqrt(dim)
+    |out - exact| <= 2^-23 (64 S + 128 + n / 8) sum_j p_j |v_j|,   S = max_j sum_c max(|q_c|, |q|max / 16) |k_jc| / sqrt(dim)
 
-over the n rows a query sees. A score q.k is a sum of dim products carried to 22
-bits or more, in FP32 with truncating additions: at most dim / 16 + 1 <= 9 steps a
-half, two halves, below 2^-23 * 20 S in all, and the factor log2(e) and the scale
-add 4 roundings, so 24 S. Both numerator and denominator of the softmax carry it,
+over the n rows a query sees. A score q.k is a sum of dim products. Either each is
+carried to 22 bits or more and they are added in FP32 with truncation, at most
+dim / 16 + 1 <= 9 steps a half, two halves, below 2^-23 * 20 S in all; or q_c is off by
+2^-24 of the largest |q| plus a rounding of its own (2^-24 |q|max = 2^-23 * 8 |q|max / 16,
+so below 2^-23 * 9 S) and the products are exact. The factor log2(e) and the scale add 4
+roundings, so 24 S. Both numerator and denominator of the softmax carry it,
 as a factor: 2 * 24 S < 64 S with the base-2 subtraction's rounding (at most S) and
 the running maximum's. exp2, the 22-bit weights, their scales, partial sums of at
 most 64 truncating steps and the merge: below 128. Adding n / 16 partial results in
@@ -169,7 +171,7 @@ class Pool:
                 x = q[a:b, h * d:(h + 1) * d].astype(np.float64)
                 with np.errstate(invalid="ignore"):
                     t = np.where(seen, x @ np.where(seen.any(0)[:, None], k[h // group], 0).T / np.sqrt(d), -np.inf)
-                    big = np.where(seen, np.abs(x) @ np.abs(np.where(seen.any(0)[:, None], k[h // group], 0)).T / np.sqrt(d), 0)
+                    big = np.where(seen, np.maximum(np.abs(x), np.abs(x).max(1, keepdims=True, initial=0) / 16) @ np.abs(np.where(seen.any(0)[:, None], k[h // group], 0)).T / np.sqrt(d), 0)
                 m = t.max(1, keepdims=True, initial=-np.inf)
                 p = np.where(seen, np.exp(t - np.where(np.isfinite(m), m, 0)), 0)
                 total = p.sum(1, keepdims=True)
