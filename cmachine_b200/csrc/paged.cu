@@ -162,7 +162,7 @@ long long visible_rows(const PagedView &v, int window, int sinks) {
 // head and row tile.
 long long decode_steps(const PagedView &v, int few, int group) {
     const long long rows = (long long)(v.max_new < few ? v.max_new : few) * group;
-    return ((long long)v.max_length / 16 + 2) * v.kvheads * ((rows + 7) / 8);
+    return ((long long)v.max_length / 16 + 2 + kPdSegmentCost) * v.kvheads * ((rows + 7) / 8);
 }
 template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDecodeArgs a) {
     constexpr size_t smem = kPdSmem<KIND, DIM, R>;

@@ -6,7 +6,9 @@
 // counts the steps of all sequences (their lengths are on the device), takes an equal
 // stretch of the line, and works through the one to few (sequence, KV head, row tile)
 // segments in it; its warps take a segment's steps in turn, each with its own online
-// softmax, and merge at the segment's end. A segment that began or goes on in another CTA
+// softmax, and merge at the segment's end. A segment's start and end take as long as
+// kPdSegmentCost steps, so each has that many empty steps before its own: without them a
+// CTA that met seven short sequences took 20 us longer than the others. A segment that began or goes on in another CTA
 // leaves a partial result, and the last of its CTAs to arrive adds the partials in order.
 // Memory bound: a cached row is read once from HBM (row tiles of one KV head meet in L2).
 // Every warp copies its own steps into its own ring of three stages (cp.async, 16 bytes a
@@ -36,6 +38,7 @@
 
 namespace tcm {
 
+constexpr int kPdSegmentCost = 32;   // empty steps a segment counts for
 constexpr int kPdSequences = 128;  // sequences a launch counts in shared memory (two CTAs an SM still fit)
 
 struct PagedDecodeArgs {
@@ -176,13 +179,14 @@ __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 
 constexpr float kPdSlack = 3.f;   // log2 of how far a row's weights may pass 1 before its reference moves
 constexpr int kPdWeightTop = 12;  // log2 of the largest byte row's weight at 1: 2^15 with the slack, inside FP16
 
-// A CTA's present segment; read again after the loop, so that the loop keeps its registers.
+// A CTA's present segment, kept by thread 0; read again after the loop, so that the loop
+// keeps its registers.
 struct PdSegment {
     PagedExtent e;
     PagedTiles tiles;
-    int s, h, r0;
-    int k0;        // the segment's first step of the row tile's
-    int from, to;  // all of the row tile's steps in the line
+    int s, h, rt;
+    int from;  // the row tile's first own step in the line
+    int n;     // its own steps: one at least, so that queries that see nothing get their zeros
 };
 
 template <int KIND, int DIM, int R>
@@ -203,7 +207,8 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __shared__ __align__(16) uint4 qf[M * NA][KS][32];  // Q's fragments
     __shared__ float qs[R];                         // scale2 times the row's power of two
     __shared__ float2 wml[W][R];
-    __shared__ int upto[kPdSequences + 1];    // steps before each sequence
+    __shared__ __align__(16) int units[kPdSequences];  // each sequence's stretch of the line
+    __shared__ int longest;
     __shared__ PagedExtent extents[kPdSequences];
     __shared__ int last_s;
     __shared__ PdSegment seg;
@@ -216,70 +221,79 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
         const int origin = e.length - e.count, r0 = rt * R, r1 = min(e.count * a.group, r0 + R) - 1;
         return paged_tiles(origin + r0 / a.group, origin + r1 / a.group, a.window, a.sinks, 4);
     };
-    for (int i = tid; i < v.sequences; i += T) {
-        PagedExtent e;
-        const int bad = paged_extent(&v, i, &e);
-        extents[i] = e;
-        if (bad && !blockIdx.x) paged_report(a.status, bad);
-        int steps = 0;  // the host keeps a launch's sum below 2^31
-        if (e.count <= a.few)
-            for (int rt = 0; rt * R < e.count * a.group; rt++) steps += max(1, tiles_of(e, rt).count);
-        upto[i + 1] = steps * v.kvheads;
-    }
+    static_assert(T >= kPdSequences && kPdSequences == 128, "a thread a sequence, four sequences a lane");
+    if (tid == 0) longest = 0;
     __syncthreads();
-    if (warp == 0) {
-        int before = 0;
-        for (int i0 = 0; i0 < v.sequences; i0 += 32) {
-            int x = i0 + lane < v.sequences ? upto[i0 + lane + 1] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            if (i0 + lane < v.sequences) upto[i0 + lane + 1] = before + x;
-            before += __shfl_sync(0xffffffffu, x, 31);
+    if (tid < kPdSequences) {
+        PagedExtent e = {0, 0, 0};
+        int steps = 0, most = 0;  // the host keeps a launch's sum below 2^31
+        if (tid < v.sequences) {
+            const int bad = paged_extent(&v, tid, &e);
+            if (bad && !blockIdx.x) paged_report(a.status, bad);
+            if (e.count <= a.few)
+                for (int rt = 0; rt * R < e.count * a.group; rt++) {
+                    const int n = max(1, tiles_of(e, rt).count);
+                    steps += kPdSegmentCost + n;
+                    most = max(most, n);
+                }
         }
-        if (lane == 0) upto[0] = 0;
+        extents[tid] = e;
+        units[tid] = steps * v.kvheads;
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) atomicMax(&longest, most);
     }
     __syncthreads();
-    const int steps = upto[v.sequences];
-    const int share = (int)(((unsigned)steps + gridDim.x - 1) / gridDim.x + W - 1) / W * W;
+    // Every warp adds the stretches up, four sequences a lane.
+    const int4 u4 = *reinterpret_cast<const int4 *>(&units[4 * lane]);
+    int mine = u4.x + u4.y + u4.z + u4.w, upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    const int steps = __shfl_sync(0xffffffffu, upto, 31);
+    // An equal share, in whole rounds of the warps. A share of s steps ends after s / W rounds of
+    // about 1000 cycles, and a row tile of n steps then has n / s partials to add, 16 in about 800
+    // cycles: the sum is least at s = sqrt(0.4 n).
+    int share = max((int)(((unsigned)steps + gridDim.x - 1) / gridDim.x), (int)sqrtf(0.4f * (float)longest));
+    share = (share + W - 1) / W * W;
     const int begin = (int)min((long long)steps, (long long)share * blockIdx.x), end = (int)min((long long)steps, begin + (long long)share);
+    if (begin >= end) return;
+    // The sequence, and by thread 0 the segment, that `begin` lies in.
+    {
+        const int holder = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
+        int s = 4 * holder, before = __shfl_sync(0xffffffffu, upto - mine, holder);
+        if (tid == 0) {
+            while (before + units[s] <= begin) before += units[s++];
+            PdSegment z;
+            z.s = s;
+            z.e = extents[s];
+            const int a_head = units[s] / v.kvheads;
+            z.h = (begin - before) / a_head;
+            z.rt = 0;
+            z.tiles = tiles_of(z.e, 0);
+            z.n = max(1, z.tiles.count);
+            z.from = before + z.h * a_head + kPdSegmentCost;
+            while (z.from + z.n <= begin && (z.rt + 1) * R < z.e.count * a.group) {
+                z.tiles = tiles_of(z.e, ++z.rt);
+                z.from += z.n + kPdSegmentCost;
+                z.n = max(1, z.tiles.count);
+            }
+            seg = z;
+        }
+    }
+    __syncthreads();
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     int bad = 0;
-    for (int pos = begin; pos < end;) {
-    // ---- the segment at pos
-    if (tid == 0) {
-        PdSegment z;
-        z.s = 0;
-        for (int top = v.sequences - 1; z.s < top;) {  // the last sequence that begins at or before pos
-            const int mid = (z.s + top + 1) >> 1;
-            if (upto[mid] <= pos) z.s = mid;
-            else top = mid - 1;
-        }
-        z.e = extents[z.s];
-        const int in_seq = pos - upto[z.s], a_head = (upto[z.s + 1] - upto[z.s]) / v.kvheads;
-        z.h = in_seq / a_head;
-        int in_tile = in_seq - z.h * a_head, rt = 0;
-        z.tiles = tiles_of(z.e, 0);
-        while (in_tile >= max(1, z.tiles.count)) {
-            in_tile -= max(1, z.tiles.count);
-            z.tiles = tiles_of(z.e, ++rt);
-        }
-        z.r0 = rt * R;
-        z.k0 = in_tile;
-        z.from = pos - in_tile;
-        z.to = z.from + max(1, z.tiles.count);
-        seg = z;
-    }
-    __syncthreads();
+    for (;;) {
     const int s = seg.s, h = seg.h;
     const PagedExtent e = seg.e;
     const PagedTiles tiles = seg.tiles;
-    const int k0 = seg.k0, k1 = min(tiles.count, k0 + (end - pos)), r0 = seg.r0;
-    const int rows = e.count * a.group;  // row r of the KV head: new row r / group, head r % group
+    const int r0 = seg.rt * R, rows = e.count * a.group;  // row r of the KV head: new row r / group, head r % group
     const int first = e.length - e.count + r0 / a.group;
     const int last = e.length - e.count + (min(rows, r0 + R) - 1) / a.group;
+    const int k0 = max(0, begin - seg.from), k1 = min(tiles.count, end - seg.from);
+    if (seg.from < end && seg.from + seg.n > begin) {
 
     // ---- the copies of this warp's steps
     const bool whole = v.page % 16 == 0;  // a step lies inside one page, 16 rows of one stretch of memory
@@ -341,27 +355,36 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
         asm volatile("cp.async.commit_group;" ::: "memory");
         return there;
     };
+    // Page ids and queries are asked for together, before the first copy waits for an id. Warp w
+    // prepares query rows w, w + W, ...
     int k = k0 + warp;
-    unsigned there = fetch(k, page_of(k), 0), there1 = fetch(k + W, page_of(k + W), 1);
+    const int id0 = page_of(k), id1 = page_of(k + W);
     int id_next = page_of(k + 2 * W);
-
-    // ---- the queries as fragments: warp w prepares rows w, w + W, ...
-    for (int r = warp; r < R; r += W) {
-        constexpr int E = DIM / 32;
-        float x[E];
+    constexpr int E = DIM / 32;
+    float qx[R / W][E];
 #pragma unroll
-        for (int c = 0; c < E; c++) x[c] = 0.f;
-        if (r0 + r < rows) {
-            const float *src = a.q + (long long)(e.start + (r0 + r) / a.group) * a.q_stride +
-                               (h * a.group + (r0 + r) % a.group) * DIM;
+    for (int i = 0; i < R / W; i++) {
+        const int r = r0 + warp + i * W;
+#pragma unroll
+        for (int c = 0; c < E; c++) qx[i][c] = 0.f;
+        if (r < rows) {
+            const float *src = a.q + (long long)(e.start + r / a.group) * a.q_stride + (h * a.group + r % a.group) * DIM;
             if constexpr (E == 4) {
                 const float4 f = reinterpret_cast<const float4 *>(src)[lane];
-                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+                qx[i][0] = f.x, qx[i][1] = f.y, qx[i][2] = f.z, qx[i][3] = f.w;
             } else {
                 const float2 f = reinterpret_cast<const float2 *>(src)[lane];
-                x[0] = f.x, x[1] = f.y;
+                qx[i][0] = f.x, qx[i][1] = f.y;
             }
         }
+    }
+    unsigned there = fetch(k, id0, 0), there1 = fetch(k + W, id1, 1);
+
+    // ---- the queries as fragments
+#pragma unroll
+    for (int i = 0; i < R / W; i++) {
+        const int r = warp + i * W;
+        float(&x)[E] = qx[i];
         // R = 8: part p is rows 8 (p % 2) + r of operand p / 2; else row r % 16 of operand 3 (r / 16) + p.
         auto place = [&](int p, int ks, int ft, int fh) {
             const int tile = R == 8 ? p / 2 : r / 16 * 3 + p, row = R == 8 ? (p % 2) * 8 + r : r % 16;
@@ -679,7 +702,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __syncthreads();
     {
     const volatile PdSegment &z = seg;
-    const int from = z.from, to = z.to, r0 = z.r0, rows = z.e.count * a.group, start = z.e.start, h = z.h;
+    const int from = z.from, n = z.n, r0 = z.rt * R, rows = z.e.count * a.group, start = z.e.start, h = z.h;
     auto store_out = [&](int r, int d4, float4 y, float sum) {
         const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);  // nothing seen: zeros
         *reinterpret_cast<float4 *>(a.out + (long long)(start + (r0 + r) / a.group) * a.out_stride +
@@ -687,8 +710,8 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
     };
     const int live = min(R, rows - r0);
-    const bool alone = from >= begin && to <= end;
-    const int slot = 2 * blockIdx.x + (pos == begin ? 0 : 1);
+    const bool alone = from >= begin && from + n <= end;
+    const int slot = 2 * blockIdx.x + (from >= begin ? 1 : 0);
     for (int i = tid; i < live * (DIM / 4); i += T) {
         const int r = i / (DIM / 4), d4 = i % (DIM / 4);
         float top = -INFINITY, sum = 0.f;
@@ -713,11 +736,10 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             if (d4 == 0) a.ml[slot * R + r] = make_float2(top, sum);
         }
     }
-    pos += to <= end ? to - pos : end - pos;
     if (!alone) {
         // ---- the last CTA of the row tile to arrive adds all their partials, in order
-        const int c0 = (int)(from / share), pieces = (int)((to - 1) / share) - c0 + 1;
-        auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 && from != c0 * share ? 1 : 0); };
+        const int c0 = from / share, pieces = (from + n - 1) / share - c0 + 1;
+        auto slot_of = [&](int i) { return 2 * (c0 + i) + (i == 0 ? 1 : 0); };
         __threadfence();
         __syncthreads();
         if (tid == 0) last_s = atomicAdd(&a.counters[c0], 1u) == (unsigned)(pieces - 1);
@@ -725,6 +747,30 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
         if (last_s) {
             __threadfence();
             if (tid == 0) a.counters[c0] = 0u;
+            if (pieces <= 8) {  // a thread's share of the row from each at once
+                for (int i = tid; i < live * (DIM / 4); i += T) {
+                    const int r = i / (DIM / 4), d4 = i % (DIM / 4);
+                    float2 ml[8];
+                    float4 x[8], y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 8; w++) {
+                        const int64_t at = (int64_t)slot_of(min(w, pieces - 1)) * R + r;
+                        ml[w] = __ldcg(&a.ml[at]);
+                        x[w] = __ldcg(reinterpret_cast<const float4 *>(a.part) + at * (DIM / 4) + d4);
+                    }
+#pragma unroll
+                    for (int w = 0; w < 8; w++) top = fmaxf(top, ml[w].x);
+#pragma unroll
+                    for (int w = 0; w < 8; w++)
+                        if (w < pieces) {
+                            const float f = pd_factor(ml[w], top);
+                            sum = fmaf(ml[w].y, f, sum);
+                            y = make_float4(fmaf(x[w].x, f, y.x), fmaf(x[w].y, f, y.y), fmaf(x[w].z, f, y.z), fmaf(x[w].w, f, y.w));
+                        }
+                    store_out(r, d4, y, sum);
+                }
+            } else {
             // Warp w sums pieces w, w + W, ..., eight rows' loads in flight; then the warps are added
             // as above.
             constexpr int L = DIM / 4, PR = 32 / L, B = 8;  // lanes a row, rows a load, loads in flight
@@ -781,10 +827,32 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                 }
                 store_out(r, d4, y, sum);
             }
+            }
         }
     }
     }
+    }
     __syncthreads();  // the merge buffer, the fragments and the segment are free for the next
+    if (tid == 0) {
+        PdSegment z = seg;
+        z.from += z.n;
+        if (++z.rt * R >= z.e.count * a.group) {
+            z.rt = 0;
+            if (++z.h == v.kvheads) {
+                z.h = 0;
+                do z.s++;
+                while (z.s < v.sequences && !units[z.s]);
+                if (z.s < v.sequences) z.e = extents[z.s];
+            }
+        }
+        z.from += kPdSegmentCost;
+        z.tiles = tiles_of(z.e, z.rt);
+        z.n = max(1, z.tiles.count);
+        if (z.s >= v.sequences) z.from = end;
+        seg = z;
+    }
+    __syncthreads();
+    if (seg.from >= end) break;
     }
     if (bad) paged_report(a.status, bad);
 }
