@@ -378,7 +378,12 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             }
         }
     }
-    unsigned there = fetch(k, id0, 0), there1 = fetch(k + W, id1, 1);
+    unsigned there = 0, there1 = 0;
+#pragma unroll 1  // one copy of the code: a cold instruction cache shows in short calls
+    for (int i = 0; i < 2; i++) {
+        there = there1;
+        there1 = fetch(k + i * W, i ? id1 : id0, i);
+    }
 
     // ---- the queries as fragments
 #pragma unroll
