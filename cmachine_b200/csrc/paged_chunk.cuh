@@ -38,6 +38,8 @@ constexpr int kPcSplitsMax = 32;
 // SM's four register files holds one warp of each group: 200 + 200 + 64 + 48 = 4 x 128.
 constexpr int kPcRegs = 128, kPcSoftmaxRegs = 200, kPcConvertRegs = 64, kPcIssueRegs = 48;
 static_assert(2 * kPcSoftmaxRegs + kPcConvertRegs + kPcIssueRegs <= 4 * kPcRegs, "register split");
+constexpr float kPcSlack = 3.f;   // log2 of how far a row's weights may pass 1 before its reference moves
+constexpr int kPcWeightTop = 12;  // log2 of the largest weight times V scale at 1: 2^15 with the slack, inside FP16
 constexpr unsigned kPagedWaitRanOut = 8u;     // status bit
 
 struct PagedChunkArgs {
@@ -62,19 +64,19 @@ template <int DIM> struct PcGeo {
     static constexpr uint32_t kQ = 4 * kOperand;                  // [row half][part]
     static constexpr uint32_t kScales = kQ + kPcSlots * kOperand; // float [2 K|V][2][128]
     static constexpr uint32_t kMisc = kScales + 2 * 2 * 128 * 4;
-    static constexpr size_t kSmem = kMisc + 256;
+    static constexpr size_t kSmem = kMisc + 320;
     static constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | (8u << 24);                     // FP16, K-major
     static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(DIM >> 3) << 17) | (8u << 24);  // B MN-major
 };
 struct PcMisc {  // in shared memory behind the scales
-    uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
+    uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_first[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
     uint32_t tmem;
     int last;
     uint32_t there[2][4];
     float v_scale[2];
     float vmax[2][4];
 };
-static_assert(sizeof(PcMisc) <= 256, "misc area");
+static_assert(sizeof(PcMisc) <= 320, "misc area");
 
 // Shared-memory operand descriptors, in halves: bits 0-13 the address / 16 with the stride of
 // 64-dim halves above it, and for both operands 8-row groups 1024 bytes apart in the 128-byte
@@ -208,21 +210,20 @@ template <bool MASKED> __device__ __forceinline__ float pc_row_max(uint32_t ts, 
     }
     return fmaxf(a, b);
 }
-// The row's weights over the scores they come from, and their sum before the V scales: the 16
-// columns of an MMA k-step become eight of first parts and eight of second parts.
+// The weights of 64 of a row's scores, over the scores they come from, and their sum before the
+// V scales: the 16 columns of an MMA k-step become eight of first parts and eight of second parts.
 template <bool MASKED>
 __device__ __forceinline__ float pc_row_weights(uint32_t ts, const float *ks, const float *vs, float qs, float m,
-                                                const uint32_t (&vis)[4]) {
+                                                uint32_t vis0, uint32_t vis1) {
     uint32_t buf[2][16];
     float2 sum = make_float2(0.f, 0.f);
-    const float2 qs2 = make_float2(qs, qs), m2 = make_float2(-m, -m);
     tc_ld16_async(ts, buf[0]);
 #pragma unroll
-    for (int c = 0; c < 8; c++) {
+    for (int c = 0; c < 4; c++) {
         uint32_t(&f)[16] = buf[c & 1];
         uint32_t hi[8], lo[8];
         tc_wait_ld(f);
-        if (c < 7) tc_ld16_async(ts + 16 * (c + 1), buf[(c + 1) & 1]);
+        if (c < 3) tc_ld16_async(ts + 16 * (c + 1), buf[(c + 1) & 1]);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             const float4 k4 = *reinterpret_cast<const float4 *>(ks + 16 * c + j);
@@ -230,17 +231,15 @@ __device__ __forceinline__ float pc_row_weights(uint32_t ts, const float *ks, co
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int b = j + 2 * u;
-                const float2 kk = u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y);
-                const float2 vv = u ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
-                const float2 y = __ffma2_rn(__fmul2_rn(as_pair(f[b], f[b + 1]), kk), qs2, m2);
-                float2 p = make_float2(ex2(y.x), ex2(y.y)), w;
-                const uint32_t seen = vis[c / 2] >> (16 * (c & 1) + b);
+                const float2 y = __fmul2_rn(as_pair(f[b], f[b + 1]), u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y));
+                float2 p = make_float2(ex2(fmaf(y.x, qs, -m)), ex2(fmaf(y.y, qs, -m)));
+                const uint32_t seen = (c < 2 ? vis0 : vis1) >> (16 * (c & 1) + b);
                 if (MASKED) {
                     p.x = seen & 1 ? p.x : 0.f;
                     p.y = seen & 2 ? p.y : 0.f;
                 }
                 sum = __fadd2_rn(sum, p);
-                w = __fmul2_rn(p, vv);
+                float2 w = __fmul2_rn(p, u ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
                 if (MASKED) {  // the scale of a row not seen may be anything
                     w.x = seen & 1 ? w.x : 0.f;
                     w.y = seen & 2 ? w.y : 0.f;
@@ -297,6 +296,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&x.s_full[i], 1);
+            mbar_init(&x.p_first[i], 128);
             mbar_init(&x.p_full[i], 128);
             mbar_init(&x.o_full[i], 1);
             mbar_init(&x.ks_full[i], 128);
@@ -404,21 +404,35 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                         vis[w] &= bits_below(hi - 32 * w) & (~bits_below(lo - 32 * w) | bits_below(sk - 32 * w));
                 }
                 const float top = full ? pc_row_max<false>(ts, ks, vis) : pc_row_max<true>(ts, ks, vis);
-                const float m_new = fmaxf(m, top * qs);
-                const float mr = m_new == -INFINITY ? 0.f : m_new;
-                const float keep = m == -INFINITY ? 0.f : ex2(m - mr);
-                m = m_new;
+                // The reference moves only when the maximum has passed it by 2^3: weights have that much
+                // room, and output rows whose reference stays need no rescaling.
+                float keep = 1.f;
+                if (top * qs > m + kPcSlack) {
+                    keep = m == -INFINITY ? 0.f : ex2(m - top * qs);
+                    m = top * qs;
+                }
+                const float mr = m == -INFINITY ? 0.f : m;
+                const bool moved = __any_sync(0xffffffffu, keep != 1.f);
                 if (!warp_wait(&x.vs_full[par], (t >> 1) & 1, a.err)) break;
                 const float v_scale = x.v_scale[par];
-                const float sum = full ? pc_row_weights<false>(ts, ks, vs, qs, mr, vis) : pc_row_weights<true>(ts, ks, vs, qs, mr, vis);
-                l = fmaf(l, keep, sum);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                mbar_arrive(&x.p_full[i]);
+                // In two halves of the columns: the first half's products start while the second is computed.
+                l *= keep;
+#pragma unroll 1
+                for (int c = 0; c < 128; c += 64) {
+                    const uint32_t v0 = c ? vis[2] : vis[0], v1 = c ? vis[3] : vis[1];
+                    l += full ? pc_row_weights<false>(ts + c, ks + c, vs + c, qs, mr, 0, 0)
+                              : pc_row_weights<true>(ts + c, ks + c, vs + c, qs, mr, v0, v1);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    mbar_arrive(c ? &x.p_full[i] : &x.p_first[i]);
+                }
                 // ---- this tile's output
                 if (!warp_wait(&x.o_full[i], t & 1, a.err)) break;
                 tc_fence_after();
-                const float2 keep2 = make_float2(keep, keep), vsc2 = make_float2(v_scale, v_scale);
+                if (moved) {
+#pragma unroll
+                    for (int c = 0; c < DIM; c++) o[c] *= keep;
+                }
                 uint32_t buf[2][16];
                 tc_ld16_async(to, buf[0]);
 #pragma unroll
@@ -427,12 +441,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     tc_wait_ld(f);
                     if (c + 1 < DIM / 16) tc_ld16_async(to + 16 * (c + 1), buf[(c + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float2 y = __ffma2_rn(as_pair(f[j], f[j + 1]), vsc2,
-                                                    __fmul2_rn(make_float2(o[16 * c + j], o[16 * c + j + 1]), keep2));
-                        o[16 * c + j] = y.x;
-                        o[16 * c + j + 1] = y.y;
-                    }
+                    for (int j = 0; j < 16; j++) o[16 * c + j] = fmaf(__uint_as_float(f[j]), v_scale, o[16 * c + j]);
                 }
                 tc_fence_before();
             }
@@ -548,7 +557,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     if (lane == 0) x.there[par][w] = there;
                     mbar_arrive(&x.ks_full[par]);
                 } else {
-                    // Weights are scaled by the tile's largest V scale: p s 2^14 / R < 2^14.
+                    // Weights are scaled by the tile's largest V scale: s 2^12 / R < 2^12.
                     if (mine < 0) scale = 0.f;
                     const float top = warp_max(isfinite(scale) ? scale : 0.f);
                     if (lane == 0) {
@@ -558,7 +567,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     ok = warp_wait(&x.vm_full[par], (t >> 1) & 1, a.err);
                     if (!ok) break;
                     const float vmax = fmaxf(fmaxf(x.vmax[par][0], x.vmax[par][1]), fmaxf(x.vmax[par][2], x.vmax[par][3]));
-                    const int er = max(-100, exponent_of(vmax) + 1) - 14;
+                    const int er = max(-100, exponent_of(vmax) + 1) - kPcWeightTop;
                     scales[256 + par * 128 + 32 * w + lane] = scale * power_of_two(-er);
                     if (w == 0 && lane == 0) x.v_scale[par] = power_of_two(er);
                     mbar_arrive(&x.vs_full[par]);
@@ -601,26 +610,31 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         for (int t = 0; t < n && ok; t++)
             for (int i = 0; i < halves && ok; i++) {
                 const int use = 2 * t + 1, slot = use % kPcSlots;
-                if (!warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err) || !warp_wait(&x.p_full[i], t & 1, a.err)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                if (pc_elect()) {
-                    const uint32_t d = tmem + 256u + (uint32_t)(128 * i), p = tmem + (uint32_t)(128 * i),
-                                   vd = pc_desc_v(ring + (uint32_t)slot * G::kOperand);
+                ok = warp_wait(&x.full[slot], (use / kPcSlots) & 1, a.err);
 #pragma unroll
-                    for (int part = 1; part >= 0; part--)
+                for (int first = 0; first < 2 && ok; first++) {
+                    ok = warp_wait(first ? &x.p_full[i] : &x.p_first[i], t & 1, a.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (pc_elect()) {
+                        const uint32_t d = tmem + 256u + (uint32_t)(128 * i), p = tmem + (uint32_t)(128 * i),
+                                       vd = pc_desc_v(ring + (uint32_t)slot * G::kOperand);
 #pragma unroll
-                        for (int ks = 0; ks < kPcTile / 16; ks++) {  // 16 keys: 2048 bytes on in V, 16 columns on in P
-                            const uint32_t pa = p + 16 * ks + 8 * part, vb = vd + (uint32_t)(128 * ks);
-                            if (part == 1 && ks == 0) pc_mma_ts<false>(d, pa, vb, G::kIdescO);
-                            else pc_mma_ts<true>(d, pa, vb, G::kIdescO);
+                        for (int part = 1; part >= 0; part--)
+#pragma unroll
+                            for (int ks = 4 * first; ks < 4 * first + 4; ks++) {  // 16 keys: 2048 bytes on in V, 16 columns on in P
+                                const uint32_t pa = p + 16 * ks + 8 * part, vb = vd + (uint32_t)(128 * ks);
+                                if (part == 1 && ks == 0) pc_mma_ts<false>(d, pa, vb, G::kIdescO);
+                                else pc_mma_ts<true>(d, pa, vb, G::kIdescO);
+                            }
+                        if (first) {
+                            tc_commit(&x.o_full[i]);
+                            if (i == halves - 1) tc_commit(&x.empty[slot]);
                         }
-                    tc_commit(&x.o_full[i]);
-                    if (i == halves - 1) tc_commit(&x.empty[slot]);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (!ok) break;
                 if (t + 1 < n) ok = scores(t + 1, i);
             }
         // Every product and arrival is over before tensor memory and the barriers are given back.
