@@ -446,7 +446,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                 tc_fence_before();
             }
             // ---- rows out, through this half's part of the Q area (its products are over) so that a
-            // warp writes whole rows
+            // warp writes whole rows. Every warp has written its queries there (with no tile at all nothing
+            // else has made sure of that).
+            warp_wait(&x.q_full, 0, a.err);
             const float f = splits > 1 ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
             const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits + sp;
             if (splits > 1 && r < rows) a.ml[item * kPcRows + (r - r0)] = make_float2(m, l);

@@ -344,10 +344,11 @@ def test_a_non_finite_query_touches_only_its_own_row(kind):
 def test_queries_that_see_nothing_get_zeros(kind, news, lengths):
     p = Pool(kind, QWEN, 16, news, lengths, seed=11)
     q = p.queries()
-    got = p.attend(q)
-    for s, (n, length) in enumerate(zip(news, lengths)):
-        a = p.starts[s]
-        assert np.all(got[a:a + max(0, n - length)] == 0)
+    for _ in range(20):  # nothing of the queries' own staging may show, whichever warp is first
+        got = p.attend(q)
+        for s, (n, length) in enumerate(zip(news, lengths)):
+            a = p.starts[s]
+            assert np.all(got[a:a + max(0, n - length)] == 0)
     p.check(got, q)
     assert p.flags() == 0
     p.free()
