@@ -18,96 +18,146 @@ namespace {
 constexpr int kRowThreads = 256;
 
 // ---------------------------------------------------------------- append, read back
-// One warp per (new row, KV head), K and V together: DIM / 32 elements a lane.
-// Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x /
-// scale), +-127), the divisions IEEE as in byte_cache.cu, so codes and scales are
-// the ring's bit for bit.
+// Memory bound, and launch bound for single tokens. A warp takes kRowBatch items of (new row,
+// KV head) at a time, K and V of each, so that 2 kRowBatch loads a lane are in flight.
+constexpr int kRowBatch = 4;
+
+// Item `item` of a sequence: its new row, KV head and place, and where the place lies in the pool.
+struct PagedItem {
+    long long at;  // offset of the head's first float in the callers' rows
+    int64_t row;   // in the pool's rows; -1 where there is none
+    bool on;       // an item at all
+};
+__device__ __forceinline__ PagedItem paged_item(const PagedView &v, const PagedExtent &e, int s, int item, long long stride,
+                                                int &bad) {
+    PagedItem x = {0, -1, item < e.count * v.kvheads};
+    if (x.on) {
+        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
+        x.at = (long long)(e.start + i) * stride + h * v.dim;
+        if (j >= 0 && (x.row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
+    }
+    return x;
+}
+
+// Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x / scale), +-127),
+// the divisions IEEE as in byte_cache.cu, so codes and scales are the ring's bit for bit. The row's
+// values are asked for before its page id, which they do not need.
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, const float *k, const float *vals,
                                                                    long long stride, int *status) {
     constexpr int E = DIM / 32;
+    pdl_trigger();  // the attention that follows may start to look at the batch
     const int lane = threadIdx.x & 31, s = blockIdx.y;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
     const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
-    for (int item = (blockIdx.x * kRowThreads + threadIdx.x) >> 5; item < items; item += warps) {
-        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
-        if (j < 0) continue;
-        const int64_t row = paged_slot(&v, s, j, h);
-        if (row < 0) {
-            bad |= kPagedBadPage;
-            continue;
+    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * kRowBatch; first < items; first += warps * kRowBatch) {
+        float x[kRowBatch][2][E];
+#pragma unroll
+        for (int u = 0; u < kRowBatch; u++) {
+            const int item = min(first + u, items - 1), i = item / v.kvheads;
+            const long long at = (long long)(e.start + i) * stride + (item - i * v.kvheads) * DIM + lane * E;
+#pragma unroll
+            for (int kind = 0; kind < 2; kind++) {
+                const float *src = (kind ? vals : k) + at;
+                if constexpr (E == 4) {
+                    const float4 t = *reinterpret_cast<const float4 *>(src);
+                    x[u][kind][0] = t.x, x[u][kind][1] = t.y, x[u][kind][2] = t.z, x[u][kind][3] = t.w;
+                } else {
+                    const float2 t = *reinterpret_cast<const float2 *>(src);
+                    x[u][kind][0] = t.x, x[u][kind][1] = t.y;
+                }
+            }
         }
+        PagedItem it[kRowBatch];
 #pragma unroll
-        for (int kind = 0; kind < 2; kind++) {
-            const float *src = (kind ? vals : k) + (long long)(e.start + i) * stride + h * DIM + lane * E;
-            float x[E], m = 0.f;
-            bool finite = true;
+        for (int u = 0; u < kRowBatch; u++) it[u] = paged_item(v, e, s, first + u, stride, bad);
 #pragma unroll
-            for (int c = 0; c < E; c++) {
-                x[c] = src[c];
-                finite &= isfinite(x[c]);
-                m = fmaxf(m, fabsf(x[c]));
-            }
-            if (!__all_sync(0xffffffffu, finite)) {
-                bad |= kPagedNonFinite;
-                m = 0.f;
+        for (int u = 0; u < kRowBatch; u++) {
+            if (it[u].row < 0) continue;
 #pragma unroll
-                for (int c = 0; c < E; c++) x[c] = 0.f;
-            }
-            void *dst = kind ? v.values : v.keys;
-            if constexpr (KIND == kPagedBytes) {
-                m = warp_max(m);
-                const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
-                // A row so small that m / 127 underflows stands for zeros (scale 0, codes 0).
-                int8_t q[E];
+            for (int kind = 0; kind < 2; kind++) {
+                float(&y)[E] = x[u][kind];
+                float m = 0.f;
+                bool finite = true;
 #pragma unroll
-                for (int c = 0; c < E; c++)
-                    q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(x[c], scale)))) : (int8_t)0;
-                if constexpr (E == 4)
-                    *reinterpret_cast<char4 *>(static_cast<int8_t *>(dst) + row * DIM + lane * E) = make_char4(q[0], q[1], q[2], q[3]);
-                else
-                    *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + row * DIM + lane * E) = make_char2(q[0], q[1]);
-                if (lane == 0) v.scales[(int64_t)kind * v.pages * v.kvheads * v.page + row] = scale;
-            } else {
-                uint16_t *d = static_cast<uint16_t *>(dst) + row * DIM + lane * E;
-                uint32_t w[E / 2];
+                for (int c = 0; c < E; c++) {
+                    finite &= isfinite(y[c]);
+                    m = fmaxf(m, fabsf(y[c]));
+                }
+                if (!__all_sync(0xffffffffu, finite)) {
+                    bad |= kPagedNonFinite;
+                    m = 0.f;
 #pragma unroll
-                for (int c = 0; c < E; c += 2) w[c / 2] = (uint32_t)tcm_bf16_rne(x[c]) | ((uint32_t)tcm_bf16_rne(x[c + 1]) << 16);
-                if constexpr (E == 4) *reinterpret_cast<uint2 *>(d) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t *>(d) = w[0];
+                    for (int c = 0; c < E; c++) y[c] = 0.f;
+                }
+                void *dst = kind ? v.values : v.keys;
+                const int64_t to = it[u].row * DIM + lane * E;
+                if constexpr (KIND == kPagedBytes) {
+                    m = warp_max(m);
+                    const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
+                    // A row so small that m / 127 underflows stands for zeros (scale 0, codes 0).
+                    int8_t q[E];
+#pragma unroll
+                    for (int c = 0; c < E; c++)
+                        q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(y[c], scale)))) : (int8_t)0;
+                    if constexpr (E == 4)
+                        *reinterpret_cast<char4 *>(static_cast<int8_t *>(dst) + to) = make_char4(q[0], q[1], q[2], q[3]);
+                    else
+                        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to) = make_char2(q[0], q[1]);
+                    if (lane == 0) v.scales[(int64_t)kind * v.pages * v.kvheads * v.page + it[u].row] = scale;
+                } else {
+                    uint32_t w[E / 2];
+#pragma unroll
+                    for (int c = 0; c < E; c += 2)
+                        w[c / 2] = (uint32_t)tcm_bf16_rne(y[c]) | ((uint32_t)tcm_bf16_rne(y[c + 1]) << 16);
+                    uint16_t *d = static_cast<uint16_t *>(dst) + to;
+                    if constexpr (E == 4) *reinterpret_cast<uint2 *>(d) = make_uint2(w[0], w[1]);
+                    else *reinterpret_cast<uint32_t *>(d) = w[0];
+                }
             }
         }
     }
     if (lane == 0) paged_report(status, bad);
 }
 
+// DIM / 4 lanes a row.
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, float *k, float *vals, long long stride,
                                                                  int *status) {
-    constexpr int L = DIM / 4, R = 32 / L;  // lanes a row, rows a warp
+    constexpr int L = DIM / 4, R = 32 / L;  // lanes a row, rows a warp at a time
+    pdl_wait();
     const int lane = threadIdx.x & 31, s = blockIdx.y, c = (lane % L) * 4;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
     const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
-    for (int item = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R + lane / L; item < items; item += warps * R) {
-        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
-        int64_t row = -1;
-        if (j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
-        const long long at = (long long)(e.start + i) * stride + h * DIM + c;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (row >= 0) {
-            a = paged_load4<KIND>(v.keys, row * DIM + c);
-            b = paged_load4<KIND>(v.values, row * DIM + c);
-            if constexpr (KIND == kPagedBytes) {
-                const float sk = v.scales[row], sv = v.scales[half + row];
-                a = make_float4(a.x * sk, a.y * sk, a.z * sk, a.w * sk);
-                b = make_float4(b.x * sv, b.y * sv, b.z * sv, b.w * sv);
+    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R * kRowBatch; first < items; first += warps * R * kRowBatch) {
+        PagedItem it[kRowBatch];
+        float4 a[kRowBatch], b[kRowBatch];
+        float sk[kRowBatch], sv[kRowBatch];
+#pragma unroll
+        for (int u = 0; u < kRowBatch; u++) it[u] = paged_item(v, e, s, first + u * R + lane / L, stride, bad);
+#pragma unroll
+        for (int u = 0; u < kRowBatch; u++) {
+            a[u] = b[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            sk[u] = sv[u] = 1.f;
+            if (it[u].row >= 0) {
+                a[u] = paged_load4<KIND>(v.keys, it[u].row * DIM + c);
+                b[u] = paged_load4<KIND>(v.values, it[u].row * DIM + c);
+                if constexpr (KIND == kPagedBytes) sk[u] = v.scales[it[u].row], sv[u] = v.scales[half + it[u].row];
             }
         }
-        *reinterpret_cast<float4 *>(k + at) = a;
-        *reinterpret_cast<float4 *>(vals + at) = b;
+#pragma unroll
+        for (int u = 0; u < kRowBatch; u++) {
+            if (!it[u].on) continue;
+            if constexpr (KIND == kPagedBytes) {
+                a[u] = make_float4(a[u].x * sk[u], a[u].y * sk[u], a[u].z * sk[u], a[u].w * sk[u]);
+                b[u] = make_float4(b[u].x * sv[u], b[u].y * sv[u], b[u].z * sv[u], b[u].w * sv[u]);
+            }
+            *reinterpret_cast<float4 *>(k + it[u].at + c) = a[u];
+            *reinterpret_cast<float4 *>(vals + it[u].at + c) = b[u];
+        }
     }
     paged_report(status, bad);
 }
@@ -195,6 +245,7 @@ template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) 
 }
 
 template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
+    // One kernel of the chunk's tiles; if those are split, a second that joins the parts.
     const PagedView &v = a.v;
     static PerDeviceOnce once;
     once.run([] {
@@ -219,11 +270,13 @@ template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
         }
     }
     unsigned *count;
-    paged_scratch(gpu, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, items + 1, &a.part, &a.ml, &count);
-    a.counters = count + 1;
+    paged_scratch(gpu, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, 1, &a.part, &a.ml, &count);
     a.err = a.status ? reinterpret_cast<unsigned *>(a.status) : count;
     const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
     launch(paged_chunk_kernel<KIND, DIM>, grid, dim3(kPcThreads), PcGeo<DIM>::kSmem, stream(), true, a);
+    if (a.splits > 1)
+        launch(paged_chunk_join_kernel<DIM>, dim3((unsigned)(a.row_tiles * (kPcRows / (kPcJoinThreads / 32))), v.kvheads, v.sequences),
+               dim3(kPcJoinThreads), 0, stream(), true, a);
 }
 
 unsigned blocks_of(long long items, int a_block) {
@@ -257,7 +310,7 @@ int gpu_paged_append(const TcmPagedCache *cache, const TcmPagedBatch *batch, con
     if (check_rows("gpu_paged_append", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_append", v, stride, view.kvheads, view.dim))
         return -1;
-    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32), view.sequences);
+    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32 * kRowBatch), view.sequences);
 #define CALL(K, D) paged_append_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, k, v, stride, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
@@ -273,11 +326,10 @@ int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float
     if (check_rows("gpu_paged_read", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_read", v, stride, view.kvheads, view.dim))
         return -1;
-    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32), view.sequences);
-#define CALL(K, D) paged_read_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, k, v, stride, status)
+    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32 * (128 / view.dim) * kRowBatch), view.sequences);
+#define CALL(K, D) launch(paged_read_kernel<K, D>, grid, dim3(kRowThreads), 0, stream(), true, view, k, v, stride, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
-    TCM_CUDA(cudaGetLastError());
     return 0;
 }
 
@@ -296,14 +348,19 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     const int group = qheads / view.kvheads, few = kFewRows / group;
     if (decode_steps(view, few, group) > 0x7fffffff) return refuse(name, "max_length times kvheads is too large");
     const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
-    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
-                         status};
+    // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever
+    // it has: an empty launch of the other costs 3 us, the chunk kernel with few rows about as much more.
+    const bool lone = view.sequences == 1 && view.max_new > few;
+    if (!lone) {
+        PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
+                             status};
 #define CALL(K, D) decode_launch<K, D>(gpu, d)
-    PAGED_DISPATCH(view, CALL);
+        PAGED_DISPATCH(view, CALL);
 #undef CALL
+    }
     if (view.max_new <= few) return 0;
-    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, few, 1, 1, scale2, nullptr, nullptr,
-                        nullptr, status, nullptr};
+    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 1, 1, scale2, nullptr, nullptr,
+                        status, nullptr};
 #define CALL(K, D) chunk_launch<K, D>(gpu, c)
     PAGED_DISPATCH(view, CALL);
 #undef CALL

@@ -52,7 +52,6 @@ struct PagedChunkArgs {
     float scale2;
     float *part;             // [item][256][DIM]
     float2 *ml;              // [item][256]
-    unsigned *counters;      // [sequence][KV head][row tile]
     int *status;
     unsigned *err;           // where waits that run out are recorded (status, or scratch)
 };
@@ -71,7 +70,6 @@ template <int DIM> struct PcGeo {
 struct PcMisc {  // in shared memory behind the scales
     uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_first[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
     uint32_t tmem;
-    int last;
     uint32_t there[2][4];
     float v_scale[2];
     float vmax[2][4];
@@ -256,6 +254,14 @@ __device__ __forceinline__ float pc_row_weights(uint32_t ts, const float *ks, co
     return sum.x + sum.y;
 }
 
+// The tiles that the queries of row tile rt see, and how many splits share them.
+__device__ __forceinline__ PagedTiles pc_tiles(const PagedChunkArgs &a, const PagedExtent &e, int rt, int &splits) {
+    const int origin = e.length - e.count, r0 = rt * kPcRows, live = min(kPcRows, e.count * a.group - r0);
+    const PagedTiles tiles = paged_tiles(origin + r0 / a.group, origin + (r0 + live - 1) / a.group, a.window, a.sinks, 7);
+    splits = max(1, min(a.splits, tiles.count));
+    return tiles;
+}
+
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedChunkArgs a) {
     using G = PcGeo<DIM>;
@@ -279,8 +285,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     const int origin = e.length - e.count;  // place of the first new row
     const int live = min(kPcRows, rows - r0), halves = live > 128 ? 2 : 1;
     const int first = origin + r0 / a.group, last = origin + (r0 + live - 1) / a.group;
-    const PagedTiles tiles = paged_tiles(first, last, a.window, a.sinks, 7);
-    const int splits = max(1, min(a.splits, tiles.count));
+    int splits;
+    const PagedTiles tiles = pc_tiles(a, e, rt, splits);
     if (sp >= splits) return;
     const int k0 = (int)((int64_t)tiles.count * sp / splits), n = (int)((int64_t)tiles.count * (sp + 1) / splits) - k0;
 
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         if (i < halves) {
             // ---- Q: this warp's 32 rows as two FP16 parts, scaled by the row's power of two
             float mine = 0.f;
-            constexpr int E = DIM / 32, QB = 16;  // rows whose loads are in flight together
+            constexpr int E = DIM / 32, QB = 32;  // rows whose loads are in flight together
             const long long q_at = r < rows ? (long long)(e.start + r / a.group) * a.q_stride + (h * a.group + r % a.group) * DIM : -1;
 #pragma unroll 1
             for (int first_k = 0; first_k < 32; first_k += QB) {
@@ -651,56 +657,58 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
-    if (splits == 1) return;
+}
 
-    // ---- the last split of the row tile to arrive adds all of them, in order
-    __threadfence();
-    __syncthreads();
-    unsigned *counter = &a.counters[((int64_t)s * v.kvheads + h) * a.row_tiles + rt];
-    if (tid == 0) x.last = atomicAdd(counter, 1u) == (unsigned)(splits - 1);
-    __syncthreads();
-    if (!x.last) return;
-    __threadfence();
-    if (tid == 0) *counter = 0u;
+// The parts of split row tiles, joined in order: a warp a query row. A kernel of its own, because
+// the last of a row tile's CTAs alone took 10 us over its 256 rows.
+constexpr int kPcJoinThreads = 256;
+template <int DIM>
+__global__ void __launch_bounds__(kPcJoinThreads) paged_chunk_join_kernel(const PagedChunkArgs a) {
+    constexpr int E = DIM / 32;
+    const PagedView &v = a.v;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = blockIdx.z, h = blockIdx.y;
+    pdl_wait();
+    PagedExtent e;
+    paged_extent(&v, s, &e);
+    const int rows = e.count * a.group, r = blockIdx.x * (kPcJoinThreads / 32) + warp, rt = r / kPcRows;
+    if (e.count <= a.few || r >= rows) return;
+    int splits;
+    pc_tiles(a, e, rt, splits);
+    if (splits == 1) return;
     const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits;
+    const int rr = r - rt * kPcRows;
     static_assert(kPcSplitsMax <= 32, "a lane for each split");
-    for (int rr = warp; rr < live; rr += kPcThreads / 32) {
-        constexpr int E = DIM / 32;
-        // Lane w holds split w's maximum and sum; every lane a piece of the row of each split.
-        const float2 ml = lane < splits ? __ldcg(&a.ml[(item + lane) * kPcRows + rr]) : make_float2(-INFINITY, 0.f);
-        const float top = warp_max(ml.x);
-        const float mine = pd_factor(ml, top);
-        const float sum = warp_sum(ml.y * mine);
-        float y[E];
+    // Lane w holds split w's maximum and sum; every lane a piece of the row of each split.
+    const float2 ml = lane < splits ? __ldcg(&a.ml[(item + lane) * kPcRows + rr]) : make_float2(-INFINITY, 0.f);
+    const float top = warp_max(ml.x), mine = pd_factor(ml, top), sum = warp_sum(ml.y * mine);
+    float y[E];
 #pragma unroll
-        for (int c = 0; c < E; c++) y[c] = 0.f;
-        for (int w0 = 0; w0 < splits; w0 += 8) {
-            float z[8][E];
+    for (int c = 0; c < E; c++) y[c] = 0.f;
+    for (int w0 = 0; w0 < splits; w0 += 8) {
+        float z[8][E];
 #pragma unroll
-            for (int w = 0; w < 8; w++) {
-                const float *src = a.part + ((item + min(w0 + w, splits - 1)) * kPcRows + rr) * DIM + lane * E;
-                if constexpr (E == 4) {
-                    const float4 t = __ldcg(reinterpret_cast<const float4 *>(src));
-                    z[w][0] = t.x, z[w][1] = t.y, z[w][2] = t.z, z[w][3] = t.w;
-                } else {
-                    const float2 t = __ldcg(reinterpret_cast<const float2 *>(src));
-                    z[w][0] = t.x, z[w][1] = t.y;
-                }
-            }
-#pragma unroll
-            for (int w = 0; w < 8; w++) {
-                const float f = __shfl_sync(0xffffffffu, mine, (w0 + w) & 31);
-                if (w0 + w < splits)
-#pragma unroll
-                    for (int c = 0; c < E; c++) y[c] = fmaf(z[w][c], f, y[c]);
+        for (int w = 0; w < 8; w++) {
+            const float *src = a.part + ((item + min(w0 + w, splits - 1)) * kPcRows + rr) * DIM + lane * E;
+            if constexpr (E == 4) {
+                const float4 t = __ldcg(reinterpret_cast<const float4 *>(src));
+                z[w][0] = t.x, z[w][1] = t.y, z[w][2] = t.z, z[w][3] = t.w;
+            } else {
+                const float2 t = __ldcg(reinterpret_cast<const float2 *>(src));
+                z[w][0] = t.x, z[w][1] = t.y;
             }
         }
-        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-        const int r = r0 + rr;
-        float *dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
-        if constexpr (E == 4) *reinterpret_cast<float4 *>(dst) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-        else *reinterpret_cast<float2 *>(dst) = make_float2(y[0] * inv, y[1] * inv);
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            const float f = __shfl_sync(0xffffffffu, mine, (w0 + w) & 31);
+            if (w0 + w < splits)
+#pragma unroll
+                for (int c = 0; c < E; c++) y[c] = fmaf(z[w][c], f, y[c]);
+        }
     }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+    float *dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
+    if constexpr (E == 4) *reinterpret_cast<float4 *>(dst) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+    else *reinterpret_cast<float2 *>(dst) = make_float2(y[0] * inv, y[1] * inv);
 }
 
 }  // namespace tcm

@@ -214,9 +214,10 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __shared__ PdSegment seg;
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    pdl_wait();
 
-    // ---- this CTA's stretch of the line of steps
+    // ---- this CTA's stretch of the line of steps. The extents are read before the dependency
+    // wait, while an append is still at work: a kernel that lets its successor start early
+    // (the append, the decoder's) writes none, and what came before it is over.
     auto tiles_of = [&](const PagedExtent &e, int rt) {
         const int origin = e.length - e.count, r0 = rt * R, r1 = min(e.count * a.group, r0 + R) - 1;
         return paged_tiles(origin + r0 / a.group, origin + r1 / a.group, a.window, a.sinks, 4);
@@ -258,7 +259,10 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     int share = max((int)(((unsigned)steps + gridDim.x - 1) / gridDim.x), (int)sqrtf(0.4f * (float)longest));
     share = (share + W - 1) / W * W;
     const int begin = (int)min((long long)steps, (long long)share * blockIdx.x), end = (int)min((long long)steps, begin + (long long)share);
-    if (begin >= end) return;
+    if (begin >= end) {
+        pdl_wait();  // a CTA that exits without it would let this kernel end before its predecessor
+        return;
+    }
     // The sequence, and by thread 0 the segment, that `begin` lies in.
     {
         const int holder = __ffs(__ballot_sync(0xffffffffu, upto > begin)) - 1;
@@ -285,6 +289,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __syncthreads();
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     int bad = 0;
+    pdl_wait();
     for (;;) {
     const int s = seg.s, h = seg.h;
     const PagedExtent e = seg.e;
