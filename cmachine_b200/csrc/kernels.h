@@ -21,9 +21,11 @@ void attention_split(const float *q, const AttnSource &source, bool bytes, int c
                      float *out, cudaStream_t s, bool pdl);
 // Split-K scratch of a primitive handle (grown on demand, kAttnSplits slices).
 void attention_scratch(TcmGpu *g, int kvheads, float **part, unsigned **counters);
-// Split scratch of the paged attention (grown on demand): `rows` partial rows of `dim`
-// floats with their maxima and sums, and `counters` arrival counters, zero between calls.
-void paged_scratch(TcmGpu *g, long long rows, int dim, long long counters, float **part, float2 **ml, unsigned **count);
+// Split scratch of the paged attention's decode (which 0) and chunk kernels (1), which may run side
+// by side; grown on demand: `rows` partial rows of `dim` floats with their maxima and sums, and
+// `counters` words that are zero between calls.
+void paged_scratch(TcmGpu *g, int which, long long rows, int dim, long long counters, float **part, float2 **ml,
+                   unsigned **count);
 // Generic attention for any head size (reference semantics, scores written).
 void attention_generic(float *out, const float *q, const float *keys, const float *values, float *scores,
                        int qheads, int kvheads, int dim, int capacity, int length, cudaStream_t s);

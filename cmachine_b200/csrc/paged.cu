@@ -15,29 +15,13 @@
 namespace tcm {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 
 // ---------------------------------------------------------------- append, read back
-// Memory bound, and launch bound for single tokens. A warp takes kRowBatch items of (new row,
-// KV head) at a time, K and V of each, so that 2 kRowBatch loads a lane are in flight.
+// Memory bound, and launch bound for single tokens. A warp takes kRowBatch new rows of one KV head
+// (a grid row each: no division per row) at a time, K and V of each, so that its loads are in
+// flight together.
 constexpr int kRowBatch = 4;
-
-// Item `item` of a sequence: its new row, KV head and place, and where the place lies in the pool.
-struct PagedItem {
-    long long at;  // offset of the head's first float in the callers' rows
-    int64_t row;   // in the pool's rows; -1 where there is none
-    bool on;       // an item at all
-};
-__device__ __forceinline__ PagedItem paged_item(const PagedView &v, const PagedExtent &e, int s, int item, long long stride,
-                                                int &bad) {
-    PagedItem x = {0, -1, item < e.count * v.kvheads};
-    if (x.on) {
-        const int i = item / v.kvheads, h = item - i * v.kvheads, j = e.length - e.count + i;
-        x.at = (long long)(e.start + i) * stride + h * v.dim;
-        if (j >= 0 && (x.row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
-    }
-    return x;
-}
 
 // Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x / scale), +-127),
 // the divisions IEEE as in byte_cache.cu, so codes and scales are the ring's bit for bit. The row's
@@ -47,16 +31,15 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, 
                                                                    long long stride, int *status) {
     constexpr int E = DIM / 32;
     pdl_trigger();  // the attention that follows may start to look at the batch
-    const int lane = threadIdx.x & 31, s = blockIdx.y;
+    const int lane = threadIdx.x & 31, h = blockIdx.y, s = blockIdx.z;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
-    const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
-    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * kRowBatch; first < items; first += warps * kRowBatch) {
+    const int step = gridDim.x * (kRowThreads / 32) * kRowBatch;
+    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * kRowBatch; first < e.count; first += step) {
         float x[kRowBatch][2][E];
 #pragma unroll
         for (int u = 0; u < kRowBatch; u++) {
-            const int item = min(first + u, items - 1), i = item / v.kvheads;
-            const long long at = (long long)(e.start + i) * stride + (item - i * v.kvheads) * DIM + lane * E;
+            const long long at = (long long)(e.start + min(first + u, e.count - 1)) * stride + h * DIM + lane * E;
 #pragma unroll
             for (int kind = 0; kind < 2; kind++) {
                 const float *src = (kind ? vals : k) + at;
@@ -69,43 +52,58 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, 
                 }
             }
         }
-        PagedItem it[kRowBatch];
-#pragma unroll
-        for (int u = 0; u < kRowBatch; u++) it[u] = paged_item(v, e, s, first + u, stride, bad);
+        int64_t row[kRowBatch];
 #pragma unroll
         for (int u = 0; u < kRowBatch; u++) {
-            if (it[u].row < 0) continue;
+            const int j = e.length - e.count + first + u;
+            row[u] = -1;
+            if (first + u < e.count && j >= 0 && (row[u] = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
+        }
+#pragma unroll
+        for (int u = 0; u < kRowBatch; u++) {
+            if (row[u] < 0) continue;
 #pragma unroll
             for (int kind = 0; kind < 2; kind++) {
                 float(&y)[E] = x[u][kind];
-                float m = 0.f;
-                bool finite = true;
+                float m = 0.f, zero = 0.f;
 #pragma unroll
                 for (int c = 0; c < E; c++) {
-                    finite &= isfinite(y[c]);
+                    zero = fmaf(y[c], 0.f, zero);  // NaN once a value is not finite
                     m = fmaxf(m, fabsf(y[c]));
                 }
-                if (!__all_sync(0xffffffffu, finite)) {
+                if (!__all_sync(0xffffffffu, zero == 0.f)) {
                     bad |= kPagedNonFinite;
                     m = 0.f;
 #pragma unroll
                     for (int c = 0; c < E; c++) y[c] = 0.f;
                 }
                 void *dst = kind ? v.values : v.keys;
-                const int64_t to = it[u].row * DIM + lane * E;
+                const int64_t to = row[u] * DIM + lane * E;
                 if constexpr (KIND == kPagedBytes) {
                     m = warp_max(m);
                     const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
                     // A row so small that m / 127 underflows stands for zeros (scale 0, codes 0).
+                    // The quotient by a reciprocal is within 5e-5 of the divided one; only where it comes near a
+                    // half does the division decide (all of them by division: 26 us instead of 20 for 42,000 rows).
+                    // The largest scale, 2^128 / 127, still has a reciprocal.
                     int8_t q[E];
+                    const float up = __fdividef(1.f, scale);
+                    bool near_half = false;
 #pragma unroll
-                    for (int c = 0; c < E; c++)
-                        q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(y[c], scale)))) : (int8_t)0;
+                    for (int c = 0; c < E; c++) {
+                        const float quotient = y[c] * up, code = rintf(quotient);
+                        near_half |= !(fabsf(quotient - code) <= 0.4999f);
+                        q[c] = (int8_t)fminf(127.f, fmaxf(-127.f, code));
+                    }
+                    if (near_half)
+#pragma unroll
+                        for (int c = 0; c < E; c++)
+                            q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(y[c], scale)))) : (int8_t)0;
                     if constexpr (E == 4)
                         *reinterpret_cast<char4 *>(static_cast<int8_t *>(dst) + to) = make_char4(q[0], q[1], q[2], q[3]);
                     else
                         *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to) = make_char2(q[0], q[1]);
-                    if (lane == 0) v.scales[(int64_t)kind * v.pages * v.kvheads * v.page + it[u].row] = scale;
+                    if (lane == 0) v.scales[(int64_t)kind * v.pages * v.kvheads * v.page + row[u]] = scale;
                 } else {
                     uint32_t w[E / 2];
 #pragma unroll
@@ -127,36 +125,38 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
                                                                  int *status) {
     constexpr int L = DIM / 4, R = 32 / L;  // lanes a row, rows a warp at a time
     pdl_wait();
-    const int lane = threadIdx.x & 31, s = blockIdx.y, c = (lane % L) * 4;
+    const int lane = threadIdx.x & 31, h = blockIdx.y, s = blockIdx.z, c = (lane % L) * 4;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
-    const int items = e.count * v.kvheads, warps = gridDim.x * (kRowThreads / 32);
+    const int step = gridDim.x * (kRowThreads / 32) * R * kRowBatch;
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
-    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R * kRowBatch; first < items; first += warps * R * kRowBatch) {
-        PagedItem it[kRowBatch];
+    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R * kRowBatch + lane / L; first < e.count; first += step) {
         float4 a[kRowBatch], b[kRowBatch];
         float sk[kRowBatch], sv[kRowBatch];
 #pragma unroll
-        for (int u = 0; u < kRowBatch; u++) it[u] = paged_item(v, e, s, first + u * R + lane / L, stride, bad);
-#pragma unroll
         for (int u = 0; u < kRowBatch; u++) {
+            const int i = first + u * R, j = e.length - e.count + i;
+            int64_t row = -1;
+            if (i < e.count && j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
             a[u] = b[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             sk[u] = sv[u] = 1.f;
-            if (it[u].row >= 0) {
-                a[u] = paged_load4<KIND>(v.keys, it[u].row * DIM + c);
-                b[u] = paged_load4<KIND>(v.values, it[u].row * DIM + c);
-                if constexpr (KIND == kPagedBytes) sk[u] = v.scales[it[u].row], sv[u] = v.scales[half + it[u].row];
+            if (row >= 0) {
+                a[u] = paged_load4<KIND>(v.keys, row * DIM + c);
+                b[u] = paged_load4<KIND>(v.values, row * DIM + c);
+                if constexpr (KIND == kPagedBytes) sk[u] = v.scales[row], sv[u] = v.scales[half + row];
             }
         }
 #pragma unroll
         for (int u = 0; u < kRowBatch; u++) {
-            if (!it[u].on) continue;
+            const int i = first + u * R;
+            if (i >= e.count) break;
             if constexpr (KIND == kPagedBytes) {
                 a[u] = make_float4(a[u].x * sk[u], a[u].y * sk[u], a[u].z * sk[u], a[u].w * sk[u]);
                 b[u] = make_float4(b[u].x * sv[u], b[u].y * sv[u], b[u].z * sv[u], b[u].w * sv[u]);
             }
-            *reinterpret_cast<float4 *>(k + it[u].at + c) = a[u];
-            *reinterpret_cast<float4 *>(vals + it[u].at + c) = b[u];
+            const long long at = (long long)(e.start + i) * stride + h * DIM + c;
+            __stcs(reinterpret_cast<float4 *>(k + at), a[u]);
+            __stcs(reinterpret_cast<float4 *>(vals + at), b[u]);
         }
     }
     paged_report(status, bad);
@@ -221,9 +221,7 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
         TCM_CUDA(cudaFuncSetAttribute(paged_decode_kernel<KIND, DIM, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     });
     const int ctas = sm_count() * kPdCtas<KIND, DIM, R>;
-    unsigned *count;
-    paged_scratch(gpu, 2ll * ctas * R, DIM, ctas + 1, &a.part, &a.ml, &count);
-    a.counters = count + 1;  // [0] takes the chunk kernel's wait errors when there is no status word
+    paged_scratch(gpu, 0, 2ll * ctas * R, DIM, ctas, &a.part, &a.ml, &a.counters);
     // As many sequences a launch as it counts, and steps below 2^31 (paged_attention refuses a
     // sequence that alone has more).
     const PagedView all = a.v;
@@ -244,8 +242,9 @@ template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) 
     else decode_launch_rows<KIND, DIM, 32>(gpu, a);
 }
 
-template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
-    // One kernel of the chunk's tiles; if those are split, a second that joins the parts.
+// One kernel of the chunks' tiles, then (`few`, unless null) the decode kernel beside its last
+// CTAs, and if tiles are split one that joins the parts.
+template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a, PagedDecodeArgs *few) {
     const PagedView &v = a.v;
     static PerDeviceOnce once;
     once.run([] {
@@ -270,10 +269,14 @@ template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a) {
         }
     }
     unsigned *count;
-    paged_scratch(gpu, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, 1, &a.part, &a.ml, &count);
+    paged_scratch(gpu, 1, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, 1, &a.part, &a.ml, &count);
     a.err = a.status ? reinterpret_cast<unsigned *>(a.status) : count;
     const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
     launch(paged_chunk_kernel<KIND, DIM>, grid, dim3(kPcThreads), PcGeo<DIM>::kSmem, stream(), true, a);
+    if (few) {
+        few->beside = 1;
+        decode_launch<KIND, DIM>(gpu, *few);
+    }
     if (a.splits > 1)
         launch(paged_chunk_join_kernel<DIM>, dim3((unsigned)(a.row_tiles * (kPcRows / (kPcJoinThreads / 32))), v.kvheads, v.sequences),
                dim3(kPcJoinThreads), 0, stream(), true, a);
@@ -310,7 +313,7 @@ int gpu_paged_append(const TcmPagedCache *cache, const TcmPagedBatch *batch, con
     if (check_rows("gpu_paged_append", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_append", v, stride, view.kvheads, view.dim))
         return -1;
-    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32 * kRowBatch), view.sequences);
+    const dim3 grid(blocks_of(view.max_new, kRowThreads / 32 * kRowBatch), view.kvheads, view.sequences);
 #define CALL(K, D) paged_append_kernel<K, D><<<grid, kRowThreads, 0, stream()>>>(view, k, v, stride, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
@@ -326,7 +329,7 @@ int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float
     if (check_rows("gpu_paged_read", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_read", v, stride, view.kvheads, view.dim))
         return -1;
-    const dim3 grid(blocks_of((long long)view.max_new * view.kvheads, kRowThreads / 32 * (128 / view.dim) * kRowBatch), view.sequences);
+    const dim3 grid(blocks_of(view.max_new, kRowThreads / 32 * (128 / view.dim) * kRowBatch), view.kvheads, view.sequences);
 #define CALL(K, D) launch(paged_read_kernel<K, D>, grid, dim3(kRowThreads), 0, stream(), true, view, k, v, stride, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
@@ -351,17 +354,13 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever
     // it has: an empty launch of the other costs 3 us, the chunk kernel with few rows about as much more.
     const bool lone = view.sequences == 1 && view.max_new > few;
-    if (!lone) {
-        PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
-                             status};
-#define CALL(K, D) decode_launch<K, D>(gpu, d)
-        PAGED_DISPATCH(view, CALL);
-#undef CALL
-    }
-    if (view.max_new <= few) return 0;
+    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
+                         status, 0};
     PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 1, 1, scale2, nullptr, nullptr,
                         status, nullptr};
-#define CALL(K, D) chunk_launch<K, D>(gpu, c)
+#define CALL(K, D)                                                  \
+    if (view.max_new <= few) decode_launch<K, D>(gpu, d);           \
+    else chunk_launch<K, D>(gpu, c, lone ? nullptr : &d)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
     return 0;

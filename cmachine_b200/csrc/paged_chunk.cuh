@@ -276,6 +276,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     // The longest row tiles (the last ones) start first.
     const int rt = a.row_tiles - 1 - (int)blockIdx.x / a.splits, sp = (int)blockIdx.x % a.splits;
     pdl_wait();
+    pdl_trigger();  // the decode kernel of the same call starts beside the last CTAs
     PagedExtent e;
     const int bad_extent = paged_extent(&v, s, &e);
     if (bad_extent && !blockIdx.x && !h && !tid) paged_report(a.status, bad_extent);

@@ -53,6 +53,7 @@ struct PagedDecodeArgs {
     float2 *ml;           // [CTA][2][R]: running maximum and sum
     unsigned *counters;   // [CTA], of the segment that begins there and goes on; zero between calls
     int *status;
+    int beside;           // launched beside the chunk kernel of the same call, which has waited for what came before
 };
 
 // Eight warps a CTA; two CTAs an SM where their rings fit.
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     share = (share + W - 1) / W * W;
     const int begin = (int)min((long long)steps, (long long)share * blockIdx.x), end = (int)min((long long)steps, begin + (long long)share);
     if (begin >= end) {
-        pdl_wait();  // a CTA that exits without it would let this kernel end before its predecessor
+        pdl_wait();  // every CTA waits: this kernel must not be over before its predecessor is
         return;
     }
     // The sequence, and by thread 0 the segment, that `begin` lies in.
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __syncthreads();
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     int bad = 0;
-    pdl_wait();
+    if (!a.beside) pdl_wait();
     for (;;) {
     const int s = seg.s, h = seg.h;
     const PagedExtent e = seg.e;
@@ -864,6 +865,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __syncthreads();
     if (seg.from >= end) break;
     }
+    if (a.beside) pdl_wait();
     if (bad) paged_report(a.status, bad);
 }
 

@@ -8,6 +8,11 @@
 #include <math.h>
 #include <mutex>
 
+struct PagedScratch {
+    float *part;  // split partials
+    unsigned *counters;
+    size_t floats, count;
+};
 struct TcmGpu {
     float *part_values;  // top-2 partials [2 * kTopBlocks]
     int *part_ids;
@@ -17,9 +22,7 @@ struct TcmGpu {
     unsigned *attn_counters;
     size_t attn_part_floats;
     int attn_kv;
-    float *paged_part;   // the paged attention's split partials and arrival counters (grown on demand)
-    unsigned *paged_counters;
-    size_t paged_floats, paged_count;
+    PagedScratch paged[2];  // of the paged attention's decode and chunk kernels (grown on demand)
 };
 
 namespace tcm {
@@ -374,22 +377,24 @@ void attention_scratch(TcmGpu *g, int kvheads, float **part, unsigned **counters
     *counters = g->attn_counters;
 }
 
-void paged_scratch(TcmGpu *g, long long rows, int dim, long long counters, float **part, float2 **ml, unsigned **count) {
+void paged_scratch(TcmGpu *g, int which, long long rows, int dim, long long counters, float **part, float2 **ml,
+                   unsigned **count) {
+    PagedScratch &x = g->paged[which];
     const size_t floats = (size_t)rows * (dim + 2);
-    if (g->paged_floats < floats) {
-        gpu_free(g->paged_part);
-        g->paged_part = (float *)gpu_alloc(floats * sizeof(float));
-        g->paged_floats = floats;
+    if (x.floats < floats) {
+        gpu_free(x.part);
+        x.part = (float *)gpu_alloc(floats * sizeof(float));
+        x.floats = floats;
     }
-    if (g->paged_count < (size_t)counters) {
-        gpu_free(g->paged_counters);
-        g->paged_counters = (unsigned *)gpu_alloc((size_t)counters * sizeof(unsigned));
-        gpu_zero(g->paged_counters, (size_t)counters * sizeof(unsigned));
-        g->paged_count = (size_t)counters;
+    if (x.count < (size_t)counters) {
+        gpu_free(x.counters);
+        x.counters = (unsigned *)gpu_alloc((size_t)counters * sizeof(unsigned));
+        gpu_zero(x.counters, (size_t)counters * sizeof(unsigned));
+        x.count = (size_t)counters;
     }
-    *part = g->paged_part;
-    *ml = reinterpret_cast<float2 *>(g->paged_part + (size_t)rows * dim);
-    *count = g->paged_counters;
+    *part = x.part;
+    *ml = reinterpret_cast<float2 *>(x.part + (size_t)rows * dim);
+    *count = x.counters;
 }
 }  // namespace tcm
 
@@ -414,8 +419,10 @@ void gpu_close(TcmGpu *g) {
     gpu_free(g->result);
     gpu_free(g->attn_part);
     gpu_free(g->attn_counters);
-    gpu_free(g->paged_part);
-    gpu_free(g->paged_counters);
+    for (PagedScratch &x : g->paged) {
+        gpu_free(x.part);
+        gpu_free(x.counters);
+    }
     free(g);
 }
 
