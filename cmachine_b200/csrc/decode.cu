@@ -1598,6 +1598,7 @@ int qwen_b200_wait_limit(unsigned long long ns) {
     set_module_wait_limit(ns);  // this file's kernels
     set_wait_limit_persistent(ns);
     set_wait_limit_batch(ns);
+    set_wait_limit_paged(ns);
     return 0;
 }
 

@@ -46,5 +46,6 @@ int decoder_view(const QwenB200Decoder *d, QwenB200Shape *shape, const QwenB200L
 void set_wait_limit_decode(unsigned long long ns);
 void set_wait_limit_persistent(unsigned long long ns);
 void set_wait_limit_batch(unsigned long long ns);
+void set_wait_limit_paged(unsigned long long ns);
 
 }  // namespace tcm

@@ -262,6 +262,7 @@ template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a, Pa
     a.splits = 1;
     double best = 0;
     for (int k = 1; k <= kPcSplitsMax && k * 2 <= tiles; k++) {
+        if (k > 1 && items * k > 8ll * sm_count()) break;  // at most 160 MB of parts
         const double cost = (double)((items * k + sm_count() - 1) / sm_count()) * ((double)tiles / k + 3);
         if (k == 1 || cost < 0.97 * best) {
             best = cost;
@@ -288,6 +289,9 @@ unsigned blocks_of(long long items, int a_block) {
 }
 
 }  // namespace
+
+void set_wait_limit_paged(unsigned long long ns) { set_module_wait_limit(ns); }
+
 }  // namespace tcm
 
 using namespace tcm;

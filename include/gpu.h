@@ -156,7 +156,8 @@ typedef struct {
  * the device. What only the device can see is reported in *status (a device word
  * the kernels OR into and never clear; may be NULL): 1 a non-finite row was
  * appended, 2 a page id outside the pool for a row that was needed, 4 extents that
- * do not fit rows, max_new, max_length or the table. A row without a page is not
+ * do not fit rows, max_new, max_length or the table, 8 a wait inside the attention
+ * ran out (qwen_b200_wait_limit): its outputs are not to be used. A row without a page is not
  * written, reads as zeros and is visible to no query; a sequence with bad extents
  * is left out, its rows of the outputs untouched. Row buffers are FP32, strides
  * count floats from one row to the next (multiples of 4), buffers are 16-byte

@@ -193,6 +193,7 @@ class Pool:
 
 
 QWEN, GROUP4, MHA64, MQA, ONE, ODD64 = (12, 2, 128), (8, 2, 128), (4, 4, 64), (8, 1, 128), (1, 1, 128), (14, 2, 64)
+GROUP5, GROUP3 = (15, 3, 128), (6, 2, 64)
 KINDS = pytest.mark.parametrize("kind", [BF16, BYTES])
 
 # (heads, page, new rows of each sequence, lengths)
@@ -204,6 +205,8 @@ SHAPES = [
     (QWEN, 64, [43], [43]), (QWEN, 64, [42, 43, 44], [128, 129, 130]), (GROUP4, 24, [31, 32, 33, 64], [31, 128, 333, 64]),
     (MQA, 128, [100], [1500]), (ODD64, 48, [150, 1, 40], [150, 900, 1024]), (ONE, 256, [130, 257], [130, 600]),
     (QWEN, 50, [0, 4, 0, 60, 0], [9, 40, 0, 61, 200]),
+    (GROUP5, 16, [1, 2, 3, 6, 7], [19, 300, 64, 6, 1025]), (GROUP5, 33, [51, 52, 1], [51, 90, 33]),
+    (GROUP3, 64, [5, 6, 10, 11], [640, 129, 10, 65]), (GROUP3, 10, [85, 86, 171], [85, 400, 1111]),
 ]
 
 
@@ -228,6 +231,39 @@ def test_window_and_first_rows(kind, window, sinks, shape):
     p.check(p.attend(q, window, sinks), q, window, sinks)
     assert p.flags() == 0
     p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("heads,most", [(QWEN, 1), (MHA64, 3), (GROUP5, 40)])
+def test_many_sequences(kind, heads, most):
+    """More sequences than one launch of the decode kernel counts, empty ones among them, and (40) both
+    kernels of a call at once."""
+    rng, count = np.random.default_rng(most), 300 if most < 40 else 140
+    news = rng.integers(0, most + 1, count)
+    lengths = np.maximum(news, rng.integers(0, 90, count))
+    p = Pool(kind, heads, 16, news, lengths, seed=most)
+    q = p.queries()
+    p.check(p.attend(q), q)
+    p.check(p.attend(q, 20, 3), q, 20, 3)
+    assert p.flags() == 0
+    p.free()
+
+
+@KINDS
+def test_no_status_word(kind):
+    L = cm.lib()
+    for news, lengths in (([2], [40]), ([60], [90])):
+        p = Pool(kind, QWEN, 16, news, lengths, seed=6)
+        p.table[0, 1] = p.pages
+        p.put()
+        q, g = p.queries(), L.gpu_open()
+        dq, out = upload(q), upload(np.full_like(q, SENTINEL))
+        assert L.gpu_paged_attention(g, out, q.shape[1], dq, q.shape[1], p.cache, p.batch, 12, 0, 0, None) == 0
+        p.check(download(out, q.shape), q)
+        for x in (dq, out):
+            L.gpu_free(x)
+        L.gpu_close(g)
+        p.free()
 
 
 @KINDS
@@ -509,6 +545,31 @@ def test_append_and_read_back(kind, heads, page, news, lengths):
             v, _ = p.held(s, kk)
             new = v[:, lengths[s] - news[s]:].transpose(1, 0, 2).reshape(news[s], p.kvheads * p.dim)
             assert np.array_equal(got[kk][p.starts[s]:p.starts[s + 1]], new.astype(np.float32))
+    p.free()
+
+
+def test_codes_near_halves():
+    """Quotients at, just below and just above halves are rounded as the division says: every element of
+    4096 rows against single-precision NumPy."""
+    p = Pool(BYTES, (1, 1, 128), 64, [4096], [4096], seed=35)
+    rng = p.rng
+    m = np.exp(rng.standard_normal((4096, 1)) * 4).astype(np.float32)
+    scale = (m / np.float32(127)).astype(np.float32)
+    half = (rng.integers(-127, 127, (4096, 128)) + 0.5).astype(np.float32)
+    x = (half * scale).astype(np.float32)
+    side = rng.integers(0, 3, x.shape)  # the product itself, or its neighbour on either side
+    x = np.nextafter(x, np.where(side == 0, x, np.where(side == 1, np.float32(np.inf), np.float32(-np.inf))))
+    assert np.all(np.isfinite(x))
+    x = np.clip(x, -m, m).astype(np.float32)
+    x[:, 0] = m[:, 0]
+    x = x.reshape(4096, 1, 128)
+    store(p, x, -x)
+    (codes, vcodes), scales = p.get()
+    want, ws = encode(x)
+    at = p.table[0][np.arange(4096) // 64]
+    assert np.array_equal(codes[at, :, np.arange(4096) % 64], want)
+    assert np.array_equal(vcodes[at, :, np.arange(4096) % 64], -want)
+    assert np.array_equal(scales[0][at, :, np.arange(4096) % 64], ws)
     p.free()
 
 
