@@ -396,9 +396,10 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     for (int i = 0; i < R / W; i++) {
         const int r = warp + i * W;
         float(&x)[E] = qx[i];
-        // R = 8: part p is rows 8 (p % 2) + r of operand p / 2; else row r % 16 of operand 3 (r / 16) + p.
+        // R = 8: part p is rows 8 (p % 2) + r of operand p / 2; else row r % 16 of operand 3 (r / 16) + p. BF16's
+        // third part goes below the second: only first parts meet in the sums that truncate noticeably.
         auto place = [&](int p, int ks, int ft, int fh) {
-            const int tile = R == 8 ? p / 2 : r / 16 * 3 + p, row = R == 8 ? (p % 2) * 8 + r : r % 16;
+            const int tile = R == 8 ? p / 2 : r / 16 * 3 + p, row = R == 8 ? (p % 2 ^ (!kBytes && p > 1)) * 8 + r : r % 16;
             return &reinterpret_cast<uint32_t *>(&qf[tile][ks][(row % 8) * 4 + ft])[2 * fh + row / 8];
         };
         const int d = lane * E;
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
 #pragma unroll
                         for (int p = 1; p >= 0; p--) mma_f16(acc, w[0][0][p], w[RL - 1][0][p], w[0][1][p], w[RL - 1][1][p], b0, b1);
                 } else if constexpr (R == 8) {
-                    mma_bf16(acc, w[0][0][P - 1], 0u, w[0][1][P - 1], 0u, b0, b1);
+                    mma_bf16(acc, 0u, w[0][0][P - 1], 0u, w[0][1][P - 1], b0, b1);
                     mma_bf16(acc, w[0][0][0], w[0][0][1], w[0][1][0], w[0][1][1], b0, b1);
                 } else {
 #pragma unroll
