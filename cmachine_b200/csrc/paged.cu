@@ -21,7 +21,7 @@ constexpr int kRowThreads = 128;
 // Memory bound, and launch bound for single tokens. A warp takes kRowBatch new rows of one KV head
 // (a grid row each: no division per row) at a time, K and V of each, so that its loads are in
 // flight together.
-constexpr int kRowBatch = 4;
+constexpr int kRowBatch = 4, kReadBatch = 1;
 
 // Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x / scale), +-127),
 // the divisions IEEE as in byte_cache.cu, so codes and scales are the ring's bit for bit. The row's
@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
     const int lane = threadIdx.x & 31, h = blockIdx.y, s = blockIdx.z, c = (lane % L) * 4;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
-    const int step = gridDim.x * (kRowThreads / 32) * R * kRowBatch;
+    const int step = gridDim.x * (kRowThreads / 32) * R * kReadBatch;
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
-    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R * kRowBatch + lane / L; first < e.count; first += step) {
-        float4 a[kRowBatch], b[kRowBatch];
-        float sk[kRowBatch], sv[kRowBatch];
+    for (int first = ((blockIdx.x * kRowThreads + threadIdx.x) >> 5) * R * kReadBatch + lane / L; first < e.count; first += step) {
+        float4 a[kReadBatch], b[kReadBatch];
+        float sk[kReadBatch], sv[kReadBatch];
 #pragma unroll
-        for (int u = 0; u < kRowBatch; u++) {
+        for (int u = 0; u < kReadBatch; u++) {
             const int i = first + u * R, j = e.length - e.count + i;
             int64_t row = -1;
             if (i < e.count && j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
             }
         }
 #pragma unroll
-        for (int u = 0; u < kRowBatch; u++) {
+        for (int u = 0; u < kReadBatch; u++) {
             const int i = first + u * R;
             if (i >= e.count) break;
             if constexpr (KIND == kPagedBytes) {
@@ -155,8 +155,8 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
                 b[u] = make_float4(b[u].x * sv[u], b[u].y * sv[u], b[u].z * sv[u], b[u].w * sv[u]);
             }
             const long long at = (long long)(e.start + i) * stride + h * DIM + c;
-            __stcs(reinterpret_cast<float4 *>(k + at), a[u]);
-            __stcs(reinterpret_cast<float4 *>(vals + at), b[u]);
+            *reinterpret_cast<float4 *>(k + at) = a[u];
+            *reinterpret_cast<float4 *>(vals + at) = b[u];
         }
     }
     paged_report(status, bad);
@@ -333,7 +333,7 @@ int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float
     if (check_rows("gpu_paged_read", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_read", v, stride, view.kvheads, view.dim))
         return -1;
-    const dim3 grid(blocks_of(view.max_new, kRowThreads / 32 * (128 / view.dim) * kRowBatch), view.kvheads, view.sequences);
+    const dim3 grid(blocks_of(view.max_new, kRowThreads / 32 * (128 / view.dim) * kReadBatch), view.kvheads, view.sequences);
 #define CALL(K, D) launch(paged_read_kernel<K, D>, grid, dim3(kRowThreads), 0, stream(), true, view, k, v, stride, status)
     PAGED_DISPATCH(view, CALL);
 #undef CALL
