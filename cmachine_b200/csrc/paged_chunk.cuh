@@ -13,6 +13,14 @@
 // the tensor cores run the other's products. A ring of three operand tiles holds
 // K(t + 1), V(t) and the next.
 //
+// Measured: 4096 new rows over 32,768 byte rows (12 query heads, 2 KV heads) in 1.52 ms, 508 TFLOP/s
+// of result and 1.02 PFLOP/s of products; 512 over 4,609 in 46 us. A tile takes 7,400 cycles, of
+// which the MMAs are 4,100: the chain of one half (its maximum 700, its weights 3,700, the rest of
+// P V 900, Q K^T 1,450) bounds it. The weights' 128 exponentials alone are 1,024 cycles of the
+// special-function unit, and their broadcast reads of the row scales from shared memory wait behind
+// the MMAs' operands. Tried and slower: two threads a row (1.78 ms), scales through L1 (2.03 ms), the
+// exponentials of 16 columns beside the splitting of the 16 before (1.67 ms).
+//
 // Precision. Results are FP32, so a 16-bit rounding of Q or P would be visible:
 // both enter as two FP16 parts (22 bits) after scaling into FP16's range by powers
 // of two, against operands that are exact: a byte row is its codes, with the row's

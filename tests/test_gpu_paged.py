@@ -205,7 +205,7 @@ SHAPES = [
     (QWEN, 64, [43], [43]), (QWEN, 64, [42, 43, 44], [128, 129, 130]), (GROUP4, 24, [31, 32, 33, 64], [31, 128, 333, 64]),
     (MQA, 128, [100], [1500]), (ODD64, 48, [150, 1, 40], [150, 900, 1024]), (ONE, 256, [130, 257], [130, 600]),
     (QWEN, 50, [0, 4, 0, 60, 0], [9, 40, 0, 61, 200]),
-    (GROUP5, 16, [1, 2, 3, 6, 7], [19, 300, 64, 6, 1025]), (GROUP5, 33, [51, 52, 1], [51, 90, 33]),
+    (QWEN, 16, [5, 6, 10, 11], [400, 36, 129, 65]), (GROUP5, 16, [1, 2, 3, 6, 7], [19, 300, 64, 6, 1025]), (GROUP5, 33, [51, 52, 1], [51, 90, 33]),
     (GROUP3, 64, [5, 6, 10, 11], [640, 129, 10, 65]), (GROUP3, 10, [85, 86, 171], [85, 400, 1111]),
 ]
 
