@@ -501,11 +501,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
             // This lane's row: place base + 32 w + lane.
             const int j = base + 32 * w + lane;
             int64_t mine = -1;
-            if (j <= last) {
+            // Rows that no query of the tile sees are left out: they may hold anything, a scale that would
+            // drown the others' too, and their page may be missing.
+            if (j <= last && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) {
                 const int pg = paged_div(&v, j);
                 mine = paged_row(&v, v.table[(int64_t)s * v.table_stride + pg], j, pg, h);
-                // A page that no query of the sequence needs may be missing; one that holds a visible row may not.
-                if (mine < 0 && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) bad |= kPagedBadPage;
+                if (mine < 0) bad |= kPagedBadPage;
             }
             const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0);
 #pragma unroll 1

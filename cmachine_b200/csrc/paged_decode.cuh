@@ -571,10 +571,14 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
         float v_most = 0.f;
         if constexpr (kBytes) {
             v_most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            if (!full) {  // the scale of a row that some query does not see may be anything
+            if (!full) {  // a row that no query of the tile sees may have any scale
                 v_most = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) v_most = fmaxf(v_most, vs[i] < INFINITY ? vs[i] : 0.f);
+                for (int i = 0; i < 4; i++) {
+                    const int c = (i >> 1) * 8 + 2 * t + (i & 1);
+                    const bool seen = a.window == 0 || base + c < a.sinks || (int64_t)base + c > (int64_t)first - a.window;
+                    v_most = fmaxf(v_most, seen && vs[i] < INFINITY ? vs[i] : 0.f);
+                }
             }
             v_most = quad_max(v_most);
             moves |= v_most > v_top;

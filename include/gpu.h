@@ -143,7 +143,8 @@ typedef struct {
  * the cache counting them, so new row i stands at place lengths[s] - count + i.
  * table[s * table_stride + p] is the page of places p * page .. p * page + page - 1;
  * entries of places that nothing reads or writes may hold anything. max_new and
- * max_length are upper bounds of the new rows and the length of any sequence. */
+ * max_length (at most 2^30) are upper bounds of the new rows and the length of any
+ * sequence. */
 typedef struct {
     int sequences, rows, max_new, max_length; /* sequences <= 65535 */
     const int *starts;  /* [sequences + 1] */
@@ -165,8 +166,8 @@ typedef struct {
  *
  * Write the new rows: k and v hold [kvheads][dim] a row, `stride` apart (both). A
  * row of one KV head with a non-finite value is stored as zeros. New rows at
- * negative places (count > length) are skipped. Two sequences that write the same
- * row of a shared page leave either's. */
+ * negative places (count > length) are skipped. What two sequences of one call that
+ * write the same row of a shared page leave there is unspecified. */
 int gpu_paged_append(const TcmPagedCache *, const TcmPagedBatch *, const float *k, const float *v, long long stride,
                      int *status);
 /* Read the same rows back as the FP32 values they stand for. */

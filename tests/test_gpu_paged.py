@@ -303,27 +303,33 @@ def test_rows_of_unlike_size(kind):
 
 
 @KINDS
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("what", ["non-finite", "huge"])
 @pytest.mark.parametrize("news,lengths", [([1, 1], [37, 80]), ([4, 3], [50, 20]), ([90, 33], [130, 33])])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (11, 2)])
-def test_what_nothing_sees_may_hold_anything(kind, news, lengths, window, sinks):
-    """NaN and infinities in free pages, behind a sequence's last row and before every window, and freed pages there."""
-    p = Pool(kind, QWEN, 16, news, lengths, seed=9)
-    plain = Pool(kind, QWEN, 16, news, lengths, seed=9)
-    used = np.zeros((p.pages, 16), bool)
+def test_what_nothing_sees_may_hold_anything(kind, news, lengths, window, sinks, what, page):
+    """NaN and infinities, or numbers far larger than any other, in free pages, behind a sequence's last row and
+    before every window, and freed pages there (their entries may also name a page of such rows)."""
+    p = Pool(kind, QWEN, page, news, lengths, seed=9)
+    plain = Pool(kind, QWEN, page, news, lengths, seed=9)
+    used = np.zeros((p.pages, page), bool)
     for s, n in enumerate(lengths):
         low = max(0, n - news[s] - window + 1) if window else 0
         for j in range(n):
             if j >= low or j < sinks:
-                used[p.table[s, j // 16], j % 16] = True
+                used[p.table[s, j // page], j % page] = True
+    free = int(np.argwhere(~used.any(1))[0, 0])
+    for s, n in enumerate(lengths):
+        low = max(0, n - news[s] - window + 1) if window else 0
         if window:
-            for page in range(-(-sinks // 16), low // 16):
-                p.table[s, page] = [-1, 2**31 - 1, p.pages][page % 3]
+            for k in range(-(-sinks // page), low // page):
+                p.table[s, k] = [-1, 2**31 - 1, p.pages, free][(s + k) % 4]
     hide = ~used[:, None, :]
     if kind == BYTES:
-        for kk, bad in ((0, np.nan), (1, np.inf)):
+        for kk, bad in ((0, np.nan), (1, np.inf)) if what == "non-finite" else ((0, 1e30), (1, 1e30)):
             p.scales[kk][np.broadcast_to(hide, p.scales[kk].shape)] = bad
     else:
-        for kk, bad in ((0, 0x7FC0), (1, 0xFF80)):
+        for kk, bad in ((0, 0x7FC0), (1, 0xFF80)) if what == "non-finite" else ((0, 0x7149), (1, 0xF149)):
             p.host[kk][np.broadcast_to(hide, p.host[kk].shape[:3])] = bad
     p.put()
     q = p.queries()

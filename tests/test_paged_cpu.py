@@ -133,7 +133,7 @@ def test_bad_caches_are_refused(field, value, capfd):
 
 
 @pytest.mark.parametrize("field,value", [
-    ("sequences", -1), ("sequences", 65536), ("rows", -1), ("max_new", -1), ("max_length", -1), ("starts", None),
+    ("sequences", -1), ("sequences", 65536), ("rows", -1), ("max_new", -1), ("max_length", -1), ("max_length", (1 << 30) + 1), ("starts", None),
     ("lengths", None), ("table", None), ("table_stride", 0), ("starts", (1 << 20) + 2), ("table", (1 << 20) + 1)])
 def test_bad_batches_are_refused(field, value):
     cache, batch, a = good()
