@@ -240,6 +240,8 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
         a.v.lengths = all.lengths + s;
         a.v.table = all.table + (int64_t)s * all.table_stride;
         launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
+        // The next one follows this launch, whose counters and partials it uses again: it waits for them.
+        a.beside = 0;
     }
 }
 template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) {

@@ -61,7 +61,8 @@ struct PagedDecodeArgs {
     float2 *ml;           // [CTA][2][R]: running maximum and sum
     unsigned *counters;   // [CTA], of the segment that begins there and goes on; zero between calls
     int *status;
-    int beside;           // launched beside the chunk kernel of the same call, which has waited for what came before
+    int beside;           // the launch right behind the chunk kernel of the same call, which has waited for what came
+                          // before and shares no scratch with this one: no wait until the end
 };
 
 // Eight warps a CTA; two CTAs an SM where their rings fit.
