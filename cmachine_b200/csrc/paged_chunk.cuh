@@ -77,10 +77,13 @@ template <int DIM> struct PcGeo {
 };
 struct PcMisc {  // in shared memory behind the scales
     uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_first[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
-    uint32_t tmem;
     uint32_t there[2][4];
     float v_scale[2];
+    // Not zero: the tile's V scales are too far above one of the warp's rows, or of its rows in an earlier tile, to
+    // share one.
+    uint4 wide[2];
     float vmax[2][4];
+    uint32_t tmem;
 };
 static_assert(sizeof(PcMisc) <= 320, "misc area");
 
@@ -215,6 +218,23 @@ template <bool MASKED> __device__ __forceinline__ float pc_row_max(uint32_t ts, 
         }
     }
     return fmaxf(a, b);
+}
+// The largest weight times V scale among 64 of a row's columns that it sees.
+__device__ __forceinline__ float pc_row_most(uint32_t ts, const float *ks, const float *vs, float qs, float m, uint32_t vis0,
+                                             uint32_t vis1) {
+    float most = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        uint32_t f[16];
+        tc_ld16_async(ts + 16 * c, f);
+        tc_wait_ld(f);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float w = ex2(fmaf(__uint_as_float(f[j]) * ks[16 * c + j], qs, -m)) * vs[16 * c + j];
+            if (((c < 2 ? vis0 : vis1) >> (16 * (c & 1) + j)) & 1) most = fmaxf(most, w);
+        }
+    }
+    return most;
 }
 // The weights of 64 of a row's scores, over the scores they come from, and their sum before the
 // V scales: the 16 columns of an MMA k-step become eight of first parts and eight of second parts.
@@ -429,17 +449,41 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                 const float mr = m == -INFINITY ? 0.f : m;
                 const bool moved = __any_sync(0xffffffffu, keep != 1.f);
                 if (!warp_wait(&x.vs_full[par], (t >> 1) & 1, a.err)) break;
-                const float v_scale = x.v_scale[par];
-                // In two halves of the columns: the first half's products start while the second is computed.
+                float v_scale = x.v_scale[par];
+                const uint4 far = x.wide[par];
                 l *= keep;
-#pragma unroll 1
-                for (int c = 0; c < 128; c += 64) {
-                    const uint32_t v0 = c ? vis[2] : vis[0], v1 = c ? vis[3] : vis[1];
-                    l += full ? pc_row_weights<false>(ts + c, ks + c, vs + c, qs, mr, 0, 0)
-                              : pc_row_weights<true>(ts + c, ks + c, vs + c, qs, mr, v0, v1);
+                // In two halves of the columns: the first half's products start while the second is computed.
+                auto half_done = [&](int c) {
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     mbar_arrive(c ? &x.p_full[i] : &x.p_first[i]);
+                };
+                if (!(far.x | far.y | far.z | far.w)) {
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 64) {
+                        const uint32_t v0 = c ? vis[2] : vis[0], v1 = c ? vis[3] : vis[1];
+                        l += full ? pc_row_weights<false>(ts + c, ks + c, vs + c, qs, mr, 0, 0)
+                                  : pc_row_weights<true>(ts + c, ks + c, vs + c, qs, mr, v0, v1);
+                        half_done(c);
+                    }
+                } else {
+                    // V scales far apart meet: the largest weight of the columns that a row sees sets its scale, so
+                    // that none that it does not see or that hardly counts can push its weights below FP16. The
+                    // factor 2^up goes into the exponent, and what the subtraction rounds off comes back with it.
+                    float most = 0.f, sum = 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 64)
+                        most = fmaxf(most, pc_row_most(ts + c, ks + c, vs + c, qs, mr, c ? vis[2] : vis[0], c ? vis[3] : vis[1]));
+                    const float up = (float)min(100, kPcWeightTop - exponent_of(most)), mw = __fsub_rn(mr, up);
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 64) {
+                        sum += pc_row_weights<true>(ts + c, ks + c, vs + c, qs, mw, c ? vis[2] : vis[0], c ? vis[3] : vis[1]);
+                        half_done(c);
+                    }
+                    const float by = __fsub_rn(mw, mr), off = __fadd_rn(__fsub_rn(mr, __fsub_rn(mw, by)), __fsub_rn(-up, by));
+                    const float back = power_of_two(-(int)up) * ex2(-off);
+                    l = fmaf(sum, back, l);
+                    v_scale *= back;
                 }
                 // ---- this tile's output
                 if (!warp_wait(&x.o_full[i], t & 1, a.err)) break;
@@ -496,6 +540,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
         int bad = 0;
         bool ok = true;
+        float v_low = INFINITY;  // the smallest V scale of this lane's rows so far
         for (int t = 0; t < n && ok; t++) {
             const int base = paged_tile(tiles, k0 + t) * kPcTile, par = t & 1;
             // This lane's row: place base + 32 w + lane.
@@ -552,8 +597,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
 #pragma unroll
                             for (int off = C::LPR / 2; off; off >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, off));
                             const int ef = (int)(mb >> 7);
-                            int ex = (ef == 0 || ef == 255 ? 0 : ef - 127) - 14;
-                            ex = max(-126, min(126, ex));
+                            const int ex = ef == 255 ? 0 : max(-126, ef - 127 - 14);
                             const float up = power_of_two(-ex);
                             // A non-finite V row enters as zeros with a NaN weight: only who sees it is touched.
                             if (ef == 255 && which) y = make_uint4(0, 0, 0, 0);
@@ -575,9 +619,11 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     if (lane == 0) x.there[par][w] = there;
                     mbar_arrive(&x.ks_full[par]);
                 } else {
-                    // Weights are scaled by the tile's largest V scale: s 2^12 / R < 2^12.
+                    // Weights are scaled by the tile's largest V scale: s 2^12 / R < 2^12. Rows of zeros (and those
+                    // below about 2^-105) say nothing about how far scales lie apart.
                     if (mine < 0) scale = 0.f;
                     const float top = warp_max(isfinite(scale) ? scale : 0.f);
+                    if (scale > 0x1p-120f) v_low = fminf(v_low, scale);
                     if (lane == 0) {
                         x.vmax[par][w] = top;
                         mbar_arrive(&x.vm_full[par]);
@@ -587,6 +633,8 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     const float vmax = fmaxf(fmaxf(x.vmax[par][0], x.vmax[par][1]), fmaxf(x.vmax[par][2], x.vmax[par][3]));
                     const int er = max(-100, exponent_of(vmax) + 1) - kPcWeightTop;
                     scales[256 + par * 128 + 32 * w + lane] = scale * power_of_two(-er);
+                    const bool far = __any_sync(0xffffffffu, v_low < power_of_two(er + kPcWeightTop - kPagedSpread));
+                    if (lane == 0) reinterpret_cast<uint32_t *>(&x.wide[par])[w] = far;
                     if (w == 0 && lane == 0) x.v_scale[par] = power_of_two(er);
                     mbar_arrive(&x.vs_full[par]);
                 }

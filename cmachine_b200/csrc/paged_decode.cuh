@@ -153,10 +153,10 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t select) {
     return r;
 }
 
-// floor(log2 |x|) of a normal number; 0 for 0, subnormals, infinities and NaN.
+// floor(log2 |x|) of a normal number; -127 for 0 and subnormals, 0 for infinities and NaN.
 __device__ __forceinline__ int exponent_of(float x) {
     const int e = (int)((__float_as_uint(x) >> 23) & 0xff);
-    return e == 0 || e == 0xff ? 0 : e - 127;
+    return e == 0xff ? 0 : e - 127;
 }
 __device__ __forceinline__ float power_of_two(int e) {
     e = e < -126 ? -126 : (e > 127 ? 127 : e);
@@ -187,6 +187,10 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 constexpr float kPdSlack = 3.f;   // log2 of how far a row's weights may pass 1 before its reference moves
+// log2 of how far the V scales of the rows at hand may lie apart while their weights share one: 2^-28 of a
+// row's size is left as the weights' step. Real caches stay inside; beyond it every query row scales its weights
+// for itself, at the cost of another pass over them (a chunk's tile) or some 40 instructions a step.
+constexpr int kPagedSpread = 8;
 constexpr int kPdWeightTop = 12;  // log2 of the largest byte row's weight at 1: 2^15 with the slack, inside FP16
 
 // A CTA's present segment, kept by thread 0; read again after the loop, so that the loop
@@ -217,6 +221,9 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __shared__ __align__(16) uint4 qf[M * NA][KS][32];  // Q's fragments
     __shared__ float qs[R];                             // scale2 times what the row was multiplied down by
     __shared__ float2 wml[W][R];
+    // Of a warp's row whose weights have a scale of their own (`wide` below): its log2, and log2 of the largest
+    // weight times V scale so far, times the running maximum's power.
+    __shared__ float2 own_scale[kBytes ? W : 1][R];
     __shared__ __align__(16) int units[kPdSequences];  // each sequence's stretch of the line
     __shared__ int longest;
     __shared__ PagedExtent extents[kPdSequences];
@@ -473,8 +480,12 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             }
             // Byte rows: weights carry the rows' scales, times 2^12 over a power of two above the largest
             // scale so far (v_top, exponent v_exp).
-            float v_top = 0.f, v_factor = 0.f;
+            // Rows share it until scales far apart meet (v_low is the smallest so far): then a row that it does
+            // not see, or that hardly counts for it, must not push a query's weights below FP16.
+            float v_top = 0.f, v_factor = 0.f, v_low = INFINITY;
             int v_exp = 0;
+            bool wide = false;
+            constexpr float kNear = 1.f / (1 << kPagedSpread);
             const int see_all = a.window == 0 || a.window > last ? 0 : last - a.window + 1;  // every query sees from here to `first`
             for (int stage = 0; k < k1; k += W, stage = stage == kPdStages - 1 ? 0 : stage + 1) {
                 const int ahead = stage == 0 ? kPdStages - 1 : stage - 1;  // the stage read in the step before
@@ -575,29 +586,43 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                 float v_most = 0.f;
                 if constexpr (kBytes) {
                     v_most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+                    float least = fminf(fminf(vs[0], vs[1]), fminf(vs[2], vs[3]));
                     if (!full) {  // a row that no query of the tile sees may have any scale
-                        v_most = 0.f;
+                        v_most = 0.f, least = INFINITY;
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int c = (i >> 1) * 8 + 2 * t + (i & 1);
                             const bool seen = a.window == 0 || base + c < a.sinks || (int64_t)base + c > (int64_t)first - a.window;
                             v_most = fmaxf(v_most, seen && vs[i] < INFINITY ? vs[i] : 0.f);
+                            least = fminf(least, seen && vs[i] > 0.f ? vs[i] : INFINITY);
                         }
                     }
+                    v_low = fminf(v_low, least);
                     v_most = quad_max(v_most);
-                    moves |= v_most > v_top;
+                    moves |= !wide && (v_most > v_top || v_low < kNear * v_top);
                 }
                 // References move rarely: a row's when its maximum has passed it by 2^3 (weights have that
                 // much room), the scale's when a larger one turns up.
                 if (__any_sync(0xffffffffu, moves)) {
                     float shrink = 1.f;
                     if constexpr (kBytes) {
-                        if (v_most > v_top) {  // the same in every lane
+                        if (!wide && v_most > v_top) {  // the same in every lane
                             const int was = v_exp;
                             v_exp = max(-100, exponent_of(v_most) + 1);
                             shrink = v_top == 0.f ? 0.f : power_of_two(was - v_exp);
                             v_top = power_of_two(v_exp);
                             v_factor = power_of_two(kPdWeightTop - v_exp);
+                        }
+                        if (!wide && __any_sync(0xffffffffu, v_low < kNear * v_top)) {
+                            wide = true;
+                            v_factor = 1.f;
+                            if (t == 0)
+#pragma unroll
+                                for (int mt = 0; mt < M; mt++)
+#pragma unroll
+                                    for (int r = 0; r < RL; r++)
+                                        own_scale[warp][16 * mt + 8 * r + g] = make_float2((float)v_exp, m[mt][r] + ((float)v_exp + kPdSlack));
+                            __syncwarp();
                         }
                     }
 #pragma unroll
@@ -639,6 +664,26 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                             l[mt][r] += w[i];
                             if constexpr (kBytes) w[i] *= vs[i];
                             if (kBytes && !full && x[mt][r][i] == -INFINITY) w[i] = 0.f;
+                        }
+                        if (kBytes && wide) {
+                            const int row = 16 * mt + 8 * r + g;
+                            const float2 own = own_scale[warp][row];
+                            const float most = quad_max(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+                            const float bound = most > 0.f ? fmaxf(own.y, m[mt][r] + (float)(exponent_of(most) + 1)) : own.y;
+                            const int was = (int)own.x;  // falls by at most 2^120 at a time, which FP32 can scale by
+                            const int now = bound == -INFINITY ? was : max(max(-100, was - 120), (int)ceilf(fminf(bound - m[mt][r], 127.f)));
+                            if (t == 0) own_scale[warp][row] = make_float2((float)now, bound);
+                            if (now != was) {
+                                const float keep = power_of_two(was - now);
+#pragma unroll
+                                for (int j = 0; j < DV; j++)
+#pragma unroll
+                                    for (int c = 0; c < 4; c++)
+                                        if (RL == 1 || c / 2 == r) o[mt][j][c] *= keep;
+                            }
+                            const float up = power_of_two(kPdWeightTop - now);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) w[i] *= up;
                         }
                         split_pair<KIND>(w[0], w[1], pa[mt][r][0]);
                         split_pair<KIND>(w[2], w[3], pa[mt][r][1]);
@@ -703,7 +748,6 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             __syncthreads();  // no copy is left in flight, and the rings' memory is free for the outputs
 
             // ---- the warps' states: lane (g, t) holds dims [2 t DV, (2 t + 2) DV) of row g (+ 8)
-            const float unscale = kBytes ? power_of_two(v_exp - kPdWeightTop) : 1.f;
 #pragma unroll
             for (int mt = 0; mt < M; mt++)
 #pragma unroll
@@ -713,6 +757,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                     const int row = 16 * mt + 8 * r + g;
                     if (t == 0) wml[warp][row] = make_float2(m[mt][r], sum);
+                    const float unscale = kBytes ? power_of_two((wide ? (int)own_scale[warp][row].x : v_exp) - kPdWeightTop) : 1.f;
 #pragma unroll
                     for (int c = 0; c < 2; c++)
 #pragma unroll

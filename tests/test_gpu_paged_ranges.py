@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import cmachine_b200 as cm
-from test_gpu_paged import KINDS, MHA64, Pool
+from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool
 
 pytestmark = pytest.mark.gpu
 
@@ -25,4 +25,90 @@ def test_many_launches_beside_chunks_give_the_same_bits(kind):
         assert np.array_equal(p.attend(q, gpu=g), first)
     assert p.flags() == 0
     cm.lib().gpu_close(g)
+    p.free()
+
+
+def check_by_query(p, got, q, window=0, sinks=0):
+    """Every element against float64, by a bound that takes nothing from rows the query does not see and little from
+    rows that hardly count for it. With e_j = exp(t_j) off by a factor 1 + d_j, the result sum e v / sum e is off
+    by at most
+
+        sum_j p_j |d_j| |v_j| + (sum_j p_j |d_j|) (sum_j p_j |v_j|),   |d_j| <= 2^-23 (32 S_j + 4 S_a + 64 + n / 16),
+
+    S_j = sum_c max(|q_c|, |q|max / 16) |k_jc| / sqrt(dim) and a the row of the largest score: a score is off by 24 S_j
+    and the subtraction of a reference near t_a by S_j + S_a (both roundings), the rest is exp2, a 22-bit weight, its
+    scale and the sums' (as in the bound of tests/test_gpu_paged.py). Weights carried as FP16 halves are multiples of
+    2^-24, off by 2^-25 at most, where rows whose sizes differ by no more than 2^8 share a scale that brings the largest
+    weight times size to 2^11 or more: 2^-25 / 2^(11 - 8) = 2^-28 of the size of the row that counts most, twice that
+    for the part of a size above its power of two."""
+    d, group = p.dim, p.qheads // p.kvheads
+    for s in range(len(p.news)):
+        a, b = int(p.starts[s]), int(p.starts[s + 1])
+        if a == b:
+            continue
+        (k, there), (v, _) = p.held(s, 0), p.held(s, 1)
+        n = int(p.lengths[s])
+        at, j = (n - (b - a) + np.arange(b - a))[:, None], np.arange(n)[None]
+        seen = (j <= at) & there[None]
+        if window:
+            seen &= (j > at - window) | (j < sinks)
+        for h in range(p.qheads):
+            x = q[a:b, h * d:(h + 1) * d].astype(np.float64)
+            kk, vv = k[h // group], v[h // group]
+            t = np.where(seen, x @ kk.T / np.sqrt(d), -np.inf)
+            size = np.maximum(np.abs(x), np.abs(x).max(1, keepdims=True) / 16) @ np.abs(kk).T / np.sqrt(d)
+            w = np.exp(t - t.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            top = np.take_along_axis(size, t.argmax(1)[:, None], 1)
+            count = seen.sum(1, keepdims=True)
+            wd = w * 2.0**-23 * (32 * size + 4 * top + 64 + count / 16)
+            tol = wd @ np.abs(vv) + wd.sum(1, keepdims=True) * (w @ np.abs(vv))
+            tol = tol + count * 2.0**-27 * (w * np.abs(vv).max(1)[None]).max(1, keepdims=True)
+            off = np.abs(got[a:b, h * d:(h + 1) * d] - w @ vv)
+            assert np.all(off <= tol), (s, h, float((off / tol).max()), np.argwhere(off > tol)[:4].tolist())
+
+
+@KINDS
+@pytest.mark.parametrize("power", [10, 30, 60])
+@pytest.mark.parametrize("news,lengths,place,window,sinks", [
+    ([64], [64], 40, 0, 0), ([64], [64], 40, 9, 2), ([3, 200], [3, 700], 650, 0, 0), ([200], [300], 3, 0, 0),
+    ([5], [43], 41, 0, 0), ([5], [43], 41, 2, 0), ([2, 5], [40, 2000], 1997, 0, 0), ([5], [300], 2, 0, 0), ([5], [300], 297, 0, 4)])
+def test_a_huge_row_counts_only_where_it_is_seen(kind, power, news, lengths, place, window, sinks):
+    """A row whose V is 2^power times the others', in the middle of a chunk and of a short run: the queries before it
+    and those whose window has left it are as right as without it."""
+    p = Pool(kind, QWEN, 16, news, lengths, seed=power + place)
+    s = len(news) - 1
+    at = (p.table[s, place // 16], slice(None), place % 16)
+    if kind == BYTES:
+        p.scales[1][at] *= np.float32(2.0**power)
+    else:
+        p.host[1][at] = np.where(p.host[1][at] & 0x7F80, p.host[1][at] + (power << 7), 0)
+    p.put()
+    q = p.queries()
+    check_by_query(p, p.attend(q, window, sinks), q, window, sinks)
+    assert p.flags() == 0
+    p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("power", [30, 60])
+@pytest.mark.parametrize("small", [False, True])
+@pytest.mark.parametrize("news,lengths,places", [([64], [64], [0]), ([64], [200], [150]), ([200], [900], [5, 300, 640]),
+                                                 ([5], [43], [0]), ([5], [300], [17, 150]), ([1], [3000], [0, 1600])])
+def test_a_huge_row_with_no_weight(kind, power, small, news, lengths, places):
+    """Rows whose V is 2^power times the others' and whose weight vanishes for every query that sees them (small: the
+    other way round, rows of 2^-power that take all the weight of a query)."""
+    p = Pool(kind, QWEN, 16, news, lengths, seed=power + places[0])
+    q = (p.queries() * 0.1 + np.float32(0.5 if not small else 0.1)).astype(np.float32)
+    for place in places:
+        at = (p.table[0, place // 16], slice(None), place % 16)
+        if kind == BYTES:
+            p.host[0][at] = 127 if small else -127
+            p.scales[0][at] = np.float32((60 if small else 40) / 127)
+            p.scales[1][at] *= np.float32(2.0**(-power if small else power))
+        else:
+            p.host[0][at] = 0x4270 if small else 0xC220  # 60, -40
+            p.host[1][at] = np.where(p.host[1][at] & 0x7F80, (p.host[1][at].astype(int) + ((-power if small else power) << 7)).astype(np.uint16), 0)
+    p.put()
+    check_by_query(p, p.attend(q), q)
     p.free()
