@@ -35,18 +35,23 @@
 // conversion (as FP16 they took 84 of a step's 600 instructions); weights meet them in
 // FP16, two parts of 22 bits together. BF16 rows take three BF16 parts (24 bits) both times.
 // With R = 8 a tile of 16 rows is [first parts; second parts], so one MMA forms both.
-// Floating-point sums in the tensor core truncate (about 4e-8 of the sum a step): chains
-// stay as short as one warp's share of a segment.
+// Floating-point sums in the tensor cores truncate: long ones are taken apart (kPdChain).
 #pragma once
 #include "paged.cuh"
 #include "stream.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace tcm {
 
 // Empty steps a segment counts for. Measured with 16, 32 and 56: 64 ragged sessions of BF16 rows 34.6,
 // 32.8 and 35.1 us, of byte rows 26.0, 25.6 and 27.1; 64 of 20 to 600 rows 11.9, 13.4 and 13.8.
 constexpr int kPdSegmentCost = 32;
+// Steps that a warp may sum inside the tensor cores. They truncate: about 2e-8 of a sum a step, 1e-7 where all values
+// have one sign, so 3e-6 at most after these, what FP32 products summed in FP32 may err too. In a longer segment every
+// step is summed from zero and added in FP32. Measured of doing so always: 16 BF16 sessions of 46 steps a warp 75.2 ->
+// 78.2 us, 5 tokens of 4 heads over 900 to 4100 BF16 rows 105 -> 113, 64 sessions of up to 8192 byte rows 29.9 -> 30.8.
+constexpr int kPdChain = 32;
 constexpr int kPdSequences = 128;  // sequences a launch counts in shared memory (two CTAs an SM still fit)
 
 struct PagedDecodeArgs {
@@ -486,6 +491,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             int v_exp = 0;
             bool wide = false;
             constexpr float kNear = 1.f / (1 << kPagedSpread);
+            const bool long_sum = k1 - k0 > kPdChain * W;
             const int see_all = a.window == 0 || a.window > last ? 0 : last - a.window + 1;  // every query sees from here to `first`
             for (int stage = 0; k < k1; k += W, stage = stage == kPdStages - 1 ? 0 : stage + 1) {
                 const int ahead = stage == 0 ? kPdStages - 1 : stage - 1;  // the stage read in the step before
@@ -688,10 +694,11 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                         split_pair<KIND>(w[0], w[1], pa[mt][r][0]);
                         split_pair<KIND>(w[2], w[3], pa[mt][r][1]);
                     }
-                auto pv = [&](int j, uint32_t b0, uint32_t b1) {
+                auto pv = [&](int j, uint32_t b0, uint32_t b1, auto apart) {
 #pragma unroll
                     for (int mt = 0; mt < M; mt++) {
-                        float(&acc)[4] = o[mt][j];
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                        float(&acc)[4] = decltype(apart)::value ? sum : o[mt][j];
                         const auto &w = pa[mt];
                         if constexpr (kBytes) {
                             if constexpr (R == 8) mma_f16(acc, w[0][0][0], w[0][0][1], w[0][1][0], w[0][1][1], b0, b1);
@@ -705,41 +712,48 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
 #pragma unroll
                             for (int p = P - 1; p >= 0; p--) mma_bf16(acc, w[0][0][p], w[RL - 1][0][p], w[0][1][p], w[RL - 1][1][p], b0, b1);
                         }
+                        if constexpr (decltype(apart)::value)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[mt][j][i] += sum[i];
                     }
                 };
-                uint4 vr[4];
+                auto add_values = [&](auto apart) {
+                    uint4 vr[4];
 #pragma unroll
-                for (int c = 0; c < VW; c++) {
-                    if (c % 4 == 0)
+                    for (int c = 0; c < VW; c++) {
+                        if (c % 4 == 0)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int key = (i >> 1) * 8 + 2 * t + (i & 1), byte = g * (DV * ES) + c * 4;
-                            const unsigned char *p = st + (16 + key) * G::kRow + pd_swizzle<G::kRow>(key, byte / 16) * 16;
-                            if constexpr (VW == 2) {
-                                const uint2 w = *reinterpret_cast<const uint2 *>(p + byte % 16);
-                                vr[i] = make_uint4(w.x, w.y, 0, 0);
-                            } else {
-                                vr[i] = *reinterpret_cast<const uint4 *>(p);
+                            for (int i = 0; i < 4; i++) {
+                                const int key = (i >> 1) * 8 + 2 * t + (i & 1), byte = g * (DV * ES) + c * 4;
+                                const unsigned char *p = st + (16 + key) * G::kRow + pd_swizzle<G::kRow>(key, byte / 16) * 16;
+                                if constexpr (VW == 2) {
+                                    const uint2 w = *reinterpret_cast<const uint2 *>(p + byte % 16);
+                                    vr[i] = make_uint4(w.x, w.y, 0, 0);
+                                } else {
+                                    vr[i] = *reinterpret_cast<const uint4 *>(p);
+                                }
+                                // A weight of 0 times a non-finite value would spoil queries that do not see it.
+                                if (!kBytes && !full)
+                                    vr[i] = make_uint4(finite_pair(vr[i].x), finite_pair(vr[i].y), finite_pair(vr[i].z), finite_pair(vr[i].w));
                             }
-                            // A weight of 0 times a non-finite value would spoil queries that do not see it.
-                            if (!kBytes && !full)
-                                vr[i] = make_uint4(finite_pair(vr[i].x), finite_pair(vr[i].y), finite_pair(vr[i].z), finite_pair(vr[i].w));
-                        }
-                    uint32_t y[4];
+                        uint32_t y[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] = word(vr[i], c % 4);
-                    if constexpr (kBytes) {
-                        const uint32_t lo0 = __byte_perm(y[0], y[1], 0x5140) ^ 0x80808080u, hi0 = __byte_perm(y[0], y[1], 0x7362) ^ 0x80808080u;
-                        const uint32_t lo1 = __byte_perm(y[2], y[3], 0x5140) ^ 0x80808080u, hi1 = __byte_perm(y[2], y[3], 0x7362) ^ 0x80808080u;
-                        pv(4 * c, codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140));
-                        pv(4 * c + 1, codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342));
-                        pv(4 * c + 2, codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140));
-                        pv(4 * c + 3, codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342));
-                    } else {
-                        pv(2 * c, __byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410));
-                        pv(2 * c + 1, __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
+                        for (int i = 0; i < 4; i++) y[i] = word(vr[i], c % 4);
+                        if constexpr (kBytes) {
+                            const uint32_t lo0 = __byte_perm(y[0], y[1], 0x5140) ^ 0x80808080u, hi0 = __byte_perm(y[0], y[1], 0x7362) ^ 0x80808080u;
+                            const uint32_t lo1 = __byte_perm(y[2], y[3], 0x5140) ^ 0x80808080u, hi1 = __byte_perm(y[2], y[3], 0x7362) ^ 0x80808080u;
+                            pv(4 * c, codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140), apart);
+                            pv(4 * c + 1, codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342), apart);
+                            pv(4 * c + 2, codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140), apart);
+                            pv(4 * c + 3, codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342), apart);
+                        } else {
+                            pv(2 * c, __byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), apart);
+                            pv(2 * c + 1, __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632), apart);
+                        }
                     }
-                }
+                };
+                if (long_sum) add_values(std::true_type{});
+                else add_values(std::false_type{});
                 there = there1;
                 there1 = there2;
                 __syncwarp();  // every lane has read the stage before it is copied into again

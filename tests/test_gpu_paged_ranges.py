@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import cmachine_b200 as cm
-from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool
+from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool, bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,41 @@ def test_a_huge_row_with_no_weight(kind, power, small, news, lengths, places):
     p.put()
     check_by_query(p, p.attend(q), q)
     p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("heads,new", [((4, 4, 64), 1), ((8, 4, 64), 5), ((8, 4, 64), 10)], ids=["8", "16", "32"])
+def test_long_sums(kind, heads, new):
+    """262,144 rows of positive values, in so many sequences (all on the same pages) that most are not split: a warp
+    sums up to K = 2048 steps of 16 rows. Added in FP32 to nearest, K sums err by about sqrt(K) / 4 units of 2^-24
+    (each by up to half a unit of a partial sum, with either sign): 2 sqrt(K) is eight times that, and 32 covers a
+    step's products, the warps' merge and the division. Weights are off by 2^-23 (32 S + 8), S as in check_by_query, in
+    numerator and denominator. An adder that truncates every step is off by 2e-4 here, all to one side."""
+    length, page, seqs = 262144, 256, 80
+    p = Pool(kind, heads, page, [new], [length], seed=3, extra=0)
+    size = np.exp(p.rng.standard_normal((p.pages, p.kvheads, page)) * 0.3).astype(np.float32)
+    value = p.rng.integers(64, 128, p.host[1].shape)
+    if kind == BYTES:
+        p.host[1], p.scales[1] = value.astype(np.int8), size / 64
+    else:
+        p.host[1] = bf16((value / 64).astype(np.float32) * size[..., None])
+    q = np.tile(p.queries(0.02)[None], (seqs, 1, 1)).reshape(seqs * new, -1)
+    p.news, p.lengths = np.full(seqs, new), np.full(seqs, length)
+    p.table = np.tile(p.table, (seqs, 1))
+    p.starts = (np.arange(seqs + 1) * new).astype(np.int32)
+    p.rows = seqs * new
+    p.put()
+    got = p.attend(q).reshape(seqs, new, p.qheads, p.dim)
+    assert p.flags() == 0
+    p.free()
+    pages, group = p.table[0, :p.pages], p.qheads // p.kvheads
+    k, v = (p.values(kk)[pages].transpose(1, 0, 2, 3).reshape(p.kvheads, length, p.dim) for kk in (0, 1))
+    for i in range(new):
+        n = length - (new - 1 - i)
+        for h in range(p.qheads):
+            x = q[i, h * p.dim:(h + 1) * p.dim].astype(np.float64)
+            w = np.exp(k[h // group, :n] @ x / 8)
+            exact = (w @ v[h // group, :n]) / w.sum()
+            s = float((np.abs(k[h // group]) @ np.maximum(np.abs(x), np.abs(x).max() / 16)).max() / 8)
+            off = np.abs(got[:, i, h] / exact - 1).max()
+            assert off <= (2 * np.sqrt(n / 128) + 32) * 2.0**-24 + 2 * 2.0**-23 * (32 * s + 8), (i, h, float(off))
