@@ -434,13 +434,16 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                     for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(x[c])), finite &= isfinite(x[c]);
                     finite = __all_sync(0xffffffffu, finite);
                     m = warp_max(m);
-                    const bool any = finite && m >= 1e-30f;  // smaller queries see every row alike
-                    const float up = any ? kMost / m : 0.f;
-                    if (lane == 0) qs[r] = finite ? a.scale2 * (m * (1.f / kMost)) : __uint_as_float(0x7fc00000u);
+                    const bool any = finite && m > 0.f;
+                    const float lift = m < 0x1p-60f ? 0x1p100f : 1.f;  // exact, and up stays finite
+                    const float up = any ? kMost / (m * lift) : 0.f;
+                    // The integers enter the scores times 2^-24, so that neither they times a row's scale nor this
+                    // leaves FP32's range before the two meet.
+                    if (lane == 0) qs[r] = finite ? (a.scale2 * m) * (0x1p24f / kMost) : __uint_as_float(0x7fc00000u);
                     uint32_t w[3] = {0, 0, 0};
 #pragma unroll
                     for (int c = 0; c < E; c++) {
-                        int n = any ? __float2int_rn(x[c] * up) : 0;
+                        int n = any ? __float2int_rn(x[c] * lift * up) : 0;
                         const int lo = (int)(signed char)n;
                         n = (n - lo) >> 8;
                         const int mid = (int)(signed char)n;
@@ -551,7 +554,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                                     const int top = R == 8 ? ci[0][gr][c] : ci[mt * NA][gr][2 * r + c];
                                     const int mid = R == 8 ? ci[0][gr][2 + c] : ci[mt * NA + 1][gr][2 * r + c];
                                     const int low = R == 8 ? ci[1][gr][c] : ci[mt * NA + NA - 1][gr][2 * r + c];
-                                    x[mt][r][i] = fmaf((float)top, 65536.f, (float)(mid * 256 + low));
+                                    x[mt][r][i] = fmaf((float)top, 0x1p-8f, (float)(mid * 256 + low) * 0x1p-24f);
                                 } else {
                                     x[mt][r][i] = R == 8 ? cf[0][gr][c] + cf[0][gr][2 + c] : cf[mt][gr][2 * r + c];
                                 }

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import cmachine_b200 as cm
-from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool, bf16
+from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool, bf16, widen
 
 pytestmark = pytest.mark.gpu
 
@@ -150,3 +150,19 @@ def test_long_sums(kind, heads, new):
             s = float((np.abs(k[h // group]) @ np.maximum(np.abs(x), np.abs(x).max() / 16)).max() / 8)
             off = np.abs(got[:, i, h] / exact - 1).max()
             assert off <= (2 * np.sqrt(n / 128) + 32) * 2.0**-24 + 2 * 2.0**-23 * (32 * s + 8), (i, h, float(off))
+
+
+@KINDS
+@pytest.mark.parametrize("news,lengths", [([1, 3], [60, 33]), ([90], [100])])
+@pytest.mark.parametrize("q_size,k_size", [(1e-31, 1e30), (1.5e-34, 1e32), (1e-42, 1e30), (1e29, 1e-31)])
+def test_small_queries_against_large_rows(kind, news, lengths, q_size, k_size):
+    """Queries and cached rows at opposite ends of FP32, whose products are ordinary numbers."""
+    p = Pool(kind, QWEN, 16, news, lengths, seed=2)
+    if kind == BYTES:
+        p.scales[0] *= np.float32(k_size)
+    else:
+        p.host[0] = bf16(widen(p.host[0]) * np.float32(k_size))
+    p.put()
+    q = p.queries(q_size)
+    check_by_query(p, p.attend(q), q)
+    p.free()
