@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                     float m = 0.f;
 #pragma unroll
                     for (int c = 0; c < E; c++) m = fmaxf(m, fabsf(f[k][c]));
-                    const int ex = exponent_of(warp_max(m)) - 14;
+                    const int ex = max(-126, exponent_of(warp_max(m)) - 14);  // up and its inverse are both normal
                     const float up = power_of_two(-ex);
                     if (lane == first_k + k) mine = a.scale2 * power_of_two(ex);
                     uint32_t hi[E / 2], lo[E / 2];

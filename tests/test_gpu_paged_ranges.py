@@ -154,7 +154,7 @@ def test_long_sums(kind, heads, new):
 
 @KINDS
 @pytest.mark.parametrize("news,lengths", [([1, 3], [60, 33]), ([90], [100])])
-@pytest.mark.parametrize("q_size,k_size", [(1e-31, 1e30), (1.5e-34, 1e32), (1e-42, 1e30), (1e29, 1e-31)])
+@pytest.mark.parametrize("q_size,k_size", [(1e-31, 1e30), (1.5e-34, 1e32), (2e-35, 1e32), (1e-42, 1e30), (1e29, 1e-31)])
 def test_small_queries_against_large_rows(kind, news, lengths, q_size, k_size):
     """Queries and cached rows at opposite ends of FP32, whose products are ordinary numbers."""
     p = Pool(kind, QWEN, 16, news, lengths, seed=2)
