@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, 
                     zero = fmaf(y[c], 0.f, zero);  // NaN once a value is not finite
                     m = fmaxf(m, fabsf(y[c]));
                 }
-                if (!__all_sync(0xffffffffu, zero == 0.f)) {
+                // BF16 rounds from 2^128 - 2^119 on to infinity; 127 times FP32's largest number over 127 is one too.
+                if (!__all_sync(0xffffffffu, zero == 0.f && m < (KIND == kPagedBytes ? 0x1.fffffep127f : 0x1.ffp127f))) {
                     bad |= kPagedNonFinite;
                     m = 0.f;
 #pragma unroll

@@ -155,8 +155,8 @@ typedef struct {
 /* All three return 0 when launched, or -1 with a message on stderr for sizes,
  * strides or alignment they do not take, and launch nothing; they never wait for
  * the device. What only the device can see is reported in *status (a device word
- * the kernels OR into and never clear; may be NULL): 1 a non-finite row was
- * appended, 2 a page id outside the pool for a row that was needed, 4 extents that
+ * the kernels OR into and never clear; may be NULL): 1 a row was appended that
+ * the pool cannot hold, 2 a page id outside the pool for a row that was needed, 4 extents that
  * do not fit rows, max_new, max_length or the table, 8 a wait inside the attention
  * ran out (qwen_b200_wait_limit): its outputs are not to be used. A row without a page is not
  * written, reads as zeros and is visible to no query; a sequence with bad extents
@@ -165,8 +165,9 @@ typedef struct {
  * aligned; rows of no sequence are neither read nor written.
  *
  * Write the new rows: k and v hold [kvheads][dim] a row, `stride` apart (both). A
- * row of one KV head with a non-finite value is stored as zeros. New rows at
- * negative places (count > length) are skipped. What two sequences of one call that
+ * row of one KV head with a non-finite value, or one whose stored form would be
+ * infinite (BF16 from 2^128 - 2^119 on, bytes FP32's largest number), is stored as
+ * zeros and reported. New rows at negative places (count > length) are skipped. What two sequences of one call that
  * write the same row of a shared page leave there is unspecified. */
 int gpu_paged_append(const TcmPagedCache *, const TcmPagedBatch *, const float *k, const float *v, long long stride,
                      int *status);

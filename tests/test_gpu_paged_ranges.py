@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import cmachine_b200 as cm
-from test_gpu_paged import BYTES, KINDS, MHA64, QWEN, Pool, bf16, widen
+from test_gpu_paged import BF16, BYTES, KINDS, MHA64, QWEN, Pool, bf16, encode, read_back, store, widen
 
 pytestmark = pytest.mark.gpu
 
@@ -165,4 +165,29 @@ def test_small_queries_against_large_rows(kind, news, lengths, q_size, k_size):
     p.put()
     q = p.queries(q_size)
     check_by_query(p, p.attend(q), q)
+    p.free()
+
+
+@KINDS
+def test_rows_at_the_top_of_fp32(kind):
+    """In BF16 values from 2^128 - 2^119 on round to infinity, and FP32's largest number over 127 times 127 does: such a
+    row is stored as zeros and reported, as one of infinities is; any other finite one is an ordinary one."""
+    p = Pool(kind, QWEN, 16, [4], [20], seed=33)
+    x = [p.rng.standard_normal((4, 2, 128)).astype(np.float32) for _ in range(2)]
+    edge = np.float32(2.0**128 - 2.0**119)
+    x[0][1, 0, 5], x[1][0, 1, 127] = edge, -np.finfo(np.float32).max
+    x[1][2, 1, 5] = np.nextafter(edge, np.float32(0))
+    store(p, *x)
+    assert p.flags() == 1
+    x[1][0, 1] = 0
+    if kind == BF16:
+        x[0][1, 0] = 0
+    got = read_back(p)
+    for kk in (0, 1):
+        if kind == BYTES:
+            codes, scale = encode(x[kk])
+            want = codes.astype(np.float32) * scale[..., None]
+        else:
+            want = widen(bf16(x[kk]))
+        assert np.all(np.isfinite(want)) and np.array_equal(got[kk].reshape(4, 2, 128), want)
     p.free()
