@@ -190,9 +190,12 @@ int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, 
     if (((uintptr_t)b->starts | (uintptr_t)b->lengths | (uintptr_t)b->table) & 3)
         return refuse(call, "starts, lengths and table are 4-byte aligned");
     const int max_new = b->max_new < b->rows ? b->max_new : b->rows;
+    // No sequence is longer than its table either.
+    const long long held = (long long)b->table_stride * c->page;
+    const int max_length = b->max_length < held ? b->max_length : (int)held;
     if ((long long)max_new * c->kvheads > 0x7fffffff / 8) return refuse(call, "too many new rows for one call");
     *v = PagedView{c->kind, c->pages, c->page, c->kvheads, c->dim, c->keys, c->values, c->scales, b->sequences, b->rows,
-                   max_new, b->max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0};
+                   max_new, max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0};
     paged_divider(v);
     return 0;
 }
@@ -216,11 +219,11 @@ long long visible_rows(const PagedView &v, int window, int sinks) {
     return most < v.max_length ? most : v.max_length;
 }
 
-// Most steps one sequence of the decode kernel can have: rows below the length, and for each KV
-// head and row tile.
+// Most steps one KV head of one sequence of the decode kernel can have: rows below the length, for each
+// of up to 8 row tiles. Below 2^30.
 long long decode_steps(const PagedView &v, int few, int group) {
     const long long rows = (long long)(v.max_new < few ? v.max_new : few) * group;
-    return ((long long)v.max_length / 16 + 2 + kPdSegmentCost) * v.kvheads * ((rows + 7) / 8);
+    return ((long long)v.max_length / 16 + 2 + kPdSegmentCost) * ((rows + 7) / 8);
 }
 template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDecodeArgs a) {
     constexpr size_t smem = kPdSmem<KIND, DIM, R>;
@@ -230,20 +233,23 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
     });
     const int ctas = sm_count() * kPdCtas<KIND, DIM, R>;
     paged_scratch(gpu, 0, 2ll * ctas * R, DIM, ctas, &a.part, &a.ml, &a.counters);
-    // As many sequences a launch as it counts, and steps below 2^31 (paged_attention refuses a
-    // sequence that alone has more).
+    // As many sequences a launch as it counts, and KV heads and sequences with fewer than 2^31 steps in all.
     const PagedView all = a.v;
-    long long most = 0x7fffffff / decode_steps(all, a.few, a.group);
-    if (most > kPdSequences) most = kPdSequences;
-    for (int s = 0; s < all.sequences; s += (int)most) {
-        a.v.sequences = all.sequences - s < most ? all.sequences - s : (int)most;
-        a.v.starts = all.starts + s;
-        a.v.lengths = all.lengths + s;
-        a.v.table = all.table + (int64_t)s * all.table_stride;
-        launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
-        // The next one follows this launch, whose counters and partials it uses again: it waits for them.
-        a.beside = 0;
-    }
+    const long long steps = decode_steps(all, a.few, a.group);
+    const int heads = 0x7fffffff / steps < all.kvheads ? (int)(0x7fffffff / steps) : all.kvheads;
+    const long long fit = 0x7fffffff / (steps * heads);
+    const int most = fit < kPdSequences ? (int)fit : kPdSequences;
+    for (int s = 0; s < all.sequences; s += most)
+        for (a.head0 = 0; a.head0 < all.kvheads; a.head0 += heads) {
+            a.heads = all.kvheads - a.head0 < heads ? all.kvheads - a.head0 : heads;
+            a.v.sequences = all.sequences - s < most ? all.sequences - s : most;
+            a.v.starts = all.starts + s;
+            a.v.lengths = all.lengths + s;
+            a.v.table = all.table + (int64_t)s * all.table_stride;
+            launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
+            // The next one follows this launch, whose counters and partials it uses again: it waits for them.
+            a.beside = 0;
+        }
 }
 template <int KIND, int DIM> void decode_launch(TcmGpu *gpu, PagedDecodeArgs a) {
     const int rows = (a.v.max_new < a.few ? a.v.max_new : a.few) * a.group;
@@ -363,13 +369,12 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     if (nothing(view)) return 0;
     if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
     const int group = qheads / view.kvheads, few = few_rows(view.kind) / group;
-    if (decode_steps(view, few, group) > 0x7fffffff) return refuse(name, "max_length times kvheads is too large");
     const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
     // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever it
     // has: it nearly always has them, and an empty launch of the other takes 2.6 us of the device.
     const bool lone = view.sequences == 1 && view.max_new > few;
-    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, few, scale2, nullptr, nullptr, nullptr,
-                         status, 0};
+    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, 0, 0, few, scale2, nullptr, nullptr,
+                         nullptr, status, 0};
     PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 1, 1, scale2, nullptr, nullptr,
                         status, nullptr};
 #define CALL(K, D)                                                  \

@@ -60,6 +60,7 @@ struct PagedDecodeArgs {
     const float *q;
     long long out_stride, q_stride;
     int group, window, sinks;
+    int head0, heads;     // the KV heads of this launch
     int few;              // sequences of at most this many new rows are this kernel's
     float scale2;         // log2(e) / sqrt(dim): base-2 scores
     float *part;          // [CTA][2][R][DIM]: the first and the last segment of a CTA's stretch
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                 }
         }
         extents[tid] = e;
-        units[tid] = steps * v.kvheads;
+        units[tid] = steps * a.heads;
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) atomicMax(&longest, most);
     }
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             PdSegment z;
             z.s = s;
             z.e = extents[s];
-            const int a_head = units[s] / v.kvheads;
+            const int a_head = units[s] / a.heads;
             z.h = (begin - before) / a_head;
             z.rt = 0;
             z.tiles = tiles_of(z.e, 0);
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     int bad = 0;
     if (!a.beside) pdl_wait();
     for (;;) {
-        const int s = seg.s, h = seg.h;
+        const int s = seg.s, h = a.head0 + seg.h;
         const PagedExtent e = seg.e;
         const PagedTiles tiles = seg.tiles;
         const int r0 = seg.rt * R, rows = e.count * a.group;  // row r of the KV head: new row r / group, head r % group
@@ -789,7 +790,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             __syncthreads();
             {
                 const volatile PdSegment &z = seg;
-                const int from = z.from, n = z.n, r0 = z.rt * R, rows = z.e.count * a.group, start = z.e.start, h = z.h;
+                const int from = z.from, n = z.n, r0 = z.rt * R, rows = z.e.count * a.group, start = z.e.start, h = a.head0 + z.h;
                 auto store_out = [&](int r, int d4, float4 y, float sum) {
                     const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);  // nothing seen: zeros
                     *reinterpret_cast<float4 *>(a.out + (long long)(start + (r0 + r) / a.group) * a.out_stride +
@@ -925,7 +926,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             z.from += z.n;
             if (++z.rt * R >= z.e.count * a.group) {
                 z.rt = 0;
-                if (++z.h == v.kvheads) {
+                if (++z.h == a.heads) {
                     z.h = 0;
                     do z.s++;
                     while (z.s < v.sequences && !units[z.s]);

@@ -132,7 +132,8 @@ void gpu_ring_attention(TcmGpu *, float *out, const float *q, const signed char 
  * keys and values are [pages][kvheads][page][dim]: BF16 (kind 2, round to nearest
  * even), or the byte codec above (kind 3: int8 codes, with scales [2][pages]
  * [kvheads][page], K's then V's). Limits: dim 64 or 128; 1 <= page <= 65536;
- * keys and values 16-byte aligned; kvheads <= 1024. */
+ * keys and values 16-byte aligned; kvheads <= 1024; at most (2^28 - 1) / kvheads
+ * new rows a sequence. */
 typedef struct {
     int kind, pages, page, kvheads, dim;
     void *keys, *values;

@@ -191,3 +191,19 @@ def test_rows_at_the_top_of_fp32(kind):
             want = widen(bf16(x[kk]))
         assert np.all(np.isfinite(want)) and np.array_equal(got[kk].reshape(4, 2, 128), want)
     p.free()
+
+
+@pytest.mark.parametrize("news,lengths", [([32, 20, 1, 0, 7], [300, 20, 65, 9, 1000]), ([300], [900]), ([1, 200], [400, 333])])
+def test_a_table_for_very_long_sequences(news, lengths):
+    """max_length is an upper bound: tables of 2^30 places for short sequences, whose steps would pass 2^31, are
+    taken in launches of some KV heads each."""
+    p = Pool(BYTES, (16, 16, 64), 4096, news, lengths, seed=6, extra=0)
+    table = np.full((len(news), 2**18), -1, np.int32)
+    table[:, :p.stride] = p.table
+    p.table, p.stride = table, table.shape[1]
+    p.put()
+    p.batch.max_length = 2**30
+    q = p.queries()
+    p.check(p.attend(q), q)
+    assert p.flags() == 0
+    p.free()
