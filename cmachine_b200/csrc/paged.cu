@@ -32,7 +32,7 @@ template <int KIND, int DIM>
 __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, const float *k, const float *vals,
                                                                    long long stride, int *status) {
     constexpr int E = DIM / 32;
-    pdl_trigger();  // the attention that follows may start to look at the batch
+    pdl_trigger();  // the kernel that follows may be set up meanwhile; it waits before it reads anything
     const int lane = threadIdx.x & 31, h = blockIdx.y, s = blockIdx.z;
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);

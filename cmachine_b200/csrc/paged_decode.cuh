@@ -238,9 +238,11 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    // ---- this CTA's stretch of the line of steps. The extents are read before the dependency
-    // wait, while an append is still at work: a kernel that lets its successor start early
-    // (the append, the decoder's) writes none, and what came before it is over.
+    // ---- this CTA's stretch of the line of steps. Nothing is read before the dependency wait: whatever runs before
+    // may have written the extents. (Reading them during an append saved 0.25 us.) Beside the chunk kernel, which
+    // has waited itself before it lets this one start, every CTA waits at its end: this kernel must not be over
+    // before its predecessor is.
+    if (!a.beside) pdl_wait();
     auto tiles_of = [&](const PagedExtent &e, int rt) {
         const int origin = e.length - e.count, r0 = rt * R, r1 = min(e.count * a.group, r0 + R) - 1;
         return paged_tiles(origin + r0 / a.group, origin + r1 / a.group, a.window, a.sinks, 4);
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     share = (share + W - 1) / W * W;
     const int begin = (int)min((long long)steps, (long long)share * blockIdx.x), end = (int)min((long long)steps, begin + (long long)share);
     if (begin >= end) {
-        pdl_wait();  // every CTA waits: this kernel must not be over before its predecessor is
+        if (a.beside) pdl_wait();
         return;
     }
     // The sequence, and by thread 0 the segment, that `begin` lies in.
@@ -312,7 +314,6 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     __syncthreads();
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     int bad = 0;
-    if (!a.beside) pdl_wait();
     for (;;) {
         const int s = seg.s, h = a.head0 + seg.h;
         const PagedExtent e = seg.e;
