@@ -271,32 +271,27 @@ template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a, Pa
         TCM_CUDA(cudaFuncGetAttributes(&attr, paged_chunk_kernel<KIND, DIM>));
         if (attr.numRegs != kPcRegs) TCM_FATAL("paged attention: built with %d registers, not %d", attr.numRegs, kPcRegs);
     });
-    a.row_tiles = (int)(((long long)v.max_new * a.group + kPcRows - 1) / kPcRows);
-    // Splits: the fewest rounds of the SMs, counting an item's start and end as three tiles.
-    const long long items = (long long)v.sequences * v.kvheads * a.row_tiles;
-    const long long tiles = (visible_rows(v, a.window, a.sinks) + kPcTile - 1) / kPcTile + 2;
-    a.splits = 1;
-    double best = 0;
-    for (int k = 1; k <= kPcSplitsMax && k * 2 <= tiles; k++) {
-        if (k > 1 && items * k > 8ll * sm_count()) break;  // at most 160 MB of parts
-        const double cost = (double)((items * k + sm_count() - 1) / sm_count()) * ((double)tiles / k + 3);
-        if (k == 1 || cost < 0.97 * best) {
-            best = cost;
-            a.splits = k;
-        }
-    }
+    // CTAs for every item that there can be, and for those there probably are with their splits; the device
+    // counts them and takes the splits that fit.
+    const long long tiles = (visible_rows(v, a.window, a.sinks) + kPcTile - 1) / kPcTile + 1, room = 8ll * sm_count();
+    const long long guess = v.kvheads * paged_tile_guess(v.sequences, v.rows, v.max_new, a.group, a.few, kPcRows);
+    const long long split = guess * paged_splits(guess, (int)tiles, sm_count(), room, kPcSplitsMax);
+    const long long bound = paged_tile_bound(v.sequences, v.rows, v.max_new, a.group, a.few, kPcRows);
+    const long long grid = split > v.kvheads * bound ? split : v.kvheads * bound;
+    a.sms = sm_count();
+    a.slots = tiles < 4 ? 0 : (int)(grid < room ? grid : room);  // at most 160 MB of parts
     unsigned *count;
-    paged_scratch(gpu, 1, a.splits > 1 ? items * a.splits * kPcRows : 0, DIM, 1, &a.part, &a.ml, &count);
+    paged_scratch(gpu, 1, (long long)a.slots * kPcRows, DIM, 4 * (grid / v.kvheads + 3), &a.part, &a.ml, &count);
+    a.plan = reinterpret_cast<int4 *>(count) + 1;
     a.err = a.status ? reinterpret_cast<unsigned *>(a.status) : count;
-    const dim3 grid((unsigned)(a.splits * a.row_tiles), v.kvheads, v.sequences);
-    launch(paged_chunk_kernel<KIND, DIM>, grid, dim3(kPcThreads), PcGeo<DIM>::kSmem, stream(), true, a);
+    launch(paged_chunk_kernel<KIND, DIM>, dim3((unsigned)grid), dim3(kPcThreads), PcGeo<DIM>::kSmem, stream(), true, a);
     if (few) {
         few->beside = 1;
         decode_launch<KIND, DIM>(gpu, *few);
     }
-    if (a.splits > 1)
-        launch(paged_chunk_join_kernel<DIM>, dim3((unsigned)(a.row_tiles * (kPcRows / (kPcJoinThreads / 32))), v.kvheads, v.sequences),
-               dim3(kPcJoinThreads), 0, stream(), true, a);
+    const long long joins = v.kvheads * bound * (kPcRows / (kPcJoinThreads / 32));
+    if (a.slots)
+        launch(paged_chunk_join_kernel<DIM>, dim3((unsigned)(joins < room ? joins : room)), dim3(kPcJoinThreads), 0, stream(), true, a);
 }
 
 unsigned blocks_of(long long items, int a_block) {
@@ -369,14 +364,17 @@ int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const flo
     if (nothing(view)) return 0;
     if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
     const int group = qheads / view.kvheads, few = few_rows(view.kind) / group;
+    if (view.max_new > few &&
+        view.kvheads * paged_tile_bound(view.sequences, view.rows, view.max_new, group, 0, kPcRows) > 0x7fffffff)
+        return refuse(name, "too many rows and sequences for one call");
     const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
     // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever it
     // has: it nearly always has them, and an empty launch of the other takes 2.6 us of the device.
     const bool lone = view.sequences == 1 && view.max_new > few;
     PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, 0, 0, few, scale2, nullptr, nullptr,
                          nullptr, status, 0};
-    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 1, 1, scale2, nullptr, nullptr,
-                        status, nullptr};
+    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 0, 0, scale2, nullptr, nullptr,
+                        nullptr, status, nullptr};
 #define CALL(K, D)                                                  \
     if (view.max_new <= few) decode_launch<K, D>(gpu, d);           \
     else chunk_launch<K, D>(gpu, c, lone ? nullptr : &d)

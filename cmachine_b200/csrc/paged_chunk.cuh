@@ -56,10 +56,11 @@ struct PagedChunkArgs {
     const float *q;
     long long out_stride, q_stride;
     int group, window, sinks, few;
-    int row_tiles, splits;   // splits: of the tiles that a row tile sees
+    int sms, slots;          // CTAs that have a place for a part
     float scale2;
-    float *part;             // [item][256][DIM]
-    float2 *ml;              // [item][256]
+    float *part;             // [CTA][256][DIM], of items that are split
+    float2 *ml;              // [CTA][256]
+    int4 *plan;              // [0] the row tiles and their splits, then each tile's first row, query rows, number and splits
     int *status;
     unsigned *err;           // where waits that run out are recorded (status, or scratch)
 };
@@ -71,9 +72,21 @@ template <int DIM> struct PcGeo {
     static constexpr uint32_t kQ = 4 * kOperand;                  // [row half][part]
     static constexpr uint32_t kScales = kQ + kPcSlots * kOperand; // float [2 K|V][2][128]
     static constexpr uint32_t kMisc = kScales + 2 * 2 * 128 * 4;
-    static constexpr size_t kSmem = kMisc + 320;
+    static constexpr size_t kSmem = kMisc + 384;
     static constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | (8u << 24);                     // FP16, K-major
     static constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(DIM >> 3) << 17) | (8u << 24);  // B MN-major
+};
+// A CTA's work, in shared memory: what the roles need of it they read there, and their loops keep their registers.
+struct PcWork {
+    int s, h, start, rows, origin;  // sequence, KV head, first row in the callers' buffers, query rows, place of the first
+    int r0, live, splits;           // the row tile's first query row, how many it has, into how many parts it is split
+    int first, last;                // the places of its first and last
+    PagedTiles tiles;               // the tiles it sees, of which
+    int k0, n;                      // this CTA takes n from k0
+    __device__ __forceinline__ int base(int t) const volatile {
+        const int k = k0 + t;
+        return (k < tiles.a ? k : tiles.b + (k - tiles.a)) * kPcTile;
+    }
 };
 struct PcMisc {  // in shared memory behind the scales
     uint64_t full[kPcSlots], empty[kPcSlots], s_full[2], p_first[2], p_full[2], o_full[2], ks_full[2], vm_full[2], vs_full[2], q_full, done;
@@ -84,8 +97,9 @@ struct PcMisc {  // in shared memory behind the scales
     uint4 wide[2];
     float vmax[2][4];
     uint32_t tmem;
+    PcWork work;
 };
-static_assert(sizeof(PcMisc) <= 320, "misc area");
+static_assert(sizeof(PcMisc) <= 384, "misc area");
 
 // Shared-memory operand descriptors, in halves: bits 0-13 the address / 16 with the stride of
 // 64-dim halves above it, and for both operands 8-row groups 1024 bytes apart in the 128-byte
@@ -282,12 +296,101 @@ __device__ __forceinline__ float pc_row_weights(uint32_t ts, const float *ks, co
     return sum.x + sum.y;
 }
 
-// The tiles that the queries of row tile rt see, and how many splits share them.
-__device__ __forceinline__ PagedTiles pc_tiles(const PagedChunkArgs &a, const PagedExtent &e, int rt, int &splits) {
+// The tiles that the queries of row tile rt see.
+__device__ __forceinline__ PagedTiles pc_tiles(const PagedChunkArgs &a, const PagedExtent &e, int rt) {
     const int origin = e.length - e.count, r0 = rt * kPcRows, live = min(kPcRows, e.count * a.group - r0);
-    const PagedTiles tiles = paged_tiles(origin + r0 / a.group, origin + (r0 + live - 1) / a.group, a.window, a.sinks, 7);
-    splits = max(1, min(a.splits, tiles.count));
-    return tiles;
+    return paged_tiles(origin + r0 / a.group, origin + (r0 + live - 1) / a.group, a.window, a.sinks, 7);
+}
+
+// What a CTA works on: split sp of `splits` of row tile rt (the j-th of the batch) of sequence s, for KV head h.
+struct PcItem {
+    int s, rt, j, h, sp, splits;
+};
+// Finds it, the same in every thread, or returns false. Every CTA counts the row tiles of all sequences (their
+// extents are on the device) and takes the splits for what there is, not for the declared maxima: with one chunk of
+// 512 rows beside 63 single tokens that had left the chunk on 24 SMs (196 us; 46 alone), and an empty CTA takes
+// 3 us of an SM. `sh` is shared memory that the caller uses for nothing else before its next barrier.
+__device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem &it) {
+    const PagedView &v = a.v;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int W = kPcThreads / 32;
+    int bad = 0, longest = 0, sum = 0;  // of this thread's sequences: the tiles of the longest row tile, and of all
+    auto row_tiles = [&](int s) {
+        PagedExtent e = {0, 0, 0};
+        if (s < v.sequences) bad |= paged_extent(&v, s, &e);
+        if (e.count <= a.few) return 0;
+        const int n = (e.count * a.group + kPcRows - 1) / kPcRows, most = pc_tiles(a, e, n - 1).count;
+        longest = max(longest, most);
+        sum += n * ((pc_tiles(a, e, 0).count + most + 1) / 2);
+        return n;
+    };
+    // A sequence a thread: how many row tiles it has (n), and the sequences before it (low); then `total` counts
+    // those of this round too.
+    int n = 0, low = 0, total = 0;
+    auto round = [&](int s0) {
+        n = row_tiles(s0 + tid);
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const int far = __reduce_max_sync(0xffffffffu, longest), all = __reduce_add_sync(0xffffffffu, sum);
+        if (s0) __syncthreads();  // the last round's sums have been read
+        if (lane == 31) sh[4 + warp] = upto, sh[4 + W + warp] = far, sh[4 + 2 * W + warp] = all;
+        __syncthreads();
+        const int sums = lane < W ? sh[4 + lane] : 0;
+        low = total + __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0) + upto - n;
+        total += __reduce_add_sync(0xffffffffu, sums);
+    };
+    if (v.sequences == 1) {
+        total = n = row_tiles(0);  // of every thread
+    } else {
+        for (int s0 = 0; s0 < v.sequences; s0 += kPcThreads) round(s0);
+        longest = __reduce_max_sync(0xffffffffu, lane < W ? sh[4 + W + lane] : 0);
+        sum = __reduce_add_sync(0xffffffffu, lane < W ? sh[4 + 2 * W + lane] : 0);
+    }
+    // Splits: a number a lane (paged_splits).
+    static_assert(kPcSplitsMax == 32, "a lane for each number of splits");
+    const int64_t items = (int64_t)total * v.kvheads;
+    const int mean = (sum + total - 1) / max(total, 1);
+    const float cost = paged_may_split(items, lane + 1, longest, a.slots) ? paged_split_cost((unsigned)items, lane + 1, mean, longest, a.sms) : INFINITY;
+    const int splits = __ffs(__ballot_sync(0xffffffffu, cost <= -1.03f * warp_max(-cost)));
+    if (blockIdx.x == 0) {
+        if (items > gridDim.x) bad |= kPagedBadExtent;  // only where sequences share rows of the callers' buffers
+        paged_report(a.status, bad);
+        if (tid == 0) a.plan[0] = make_int4(total, splits, 0, 0);
+    }
+    const unsigned index = blockIdx.x / (unsigned)splits;
+    if (index >= items) return false;
+    it.splits = splits;
+    it.sp = (int)(blockIdx.x - index * (unsigned)splits);
+    it.j = (int)(index / (unsigned)v.kvheads);
+    it.h = (int)(index - (unsigned)it.j * (unsigned)v.kvheads);
+    if (v.sequences == 1) {
+        it.s = 0;
+        it.rt = n - 1 - it.j;
+        return true;
+    }
+    if (tid == 0) sh[0] = -1;
+    const int count = total;
+    if (v.sequences > kPcThreads) {
+        __syncthreads();  // every warp has read the sums
+        total = 0;
+    }
+    for (int s0 = 0; s0 < v.sequences; s0 += kPcThreads) {  // one round's n and low are still there
+        if (v.sequences > kPcThreads) round(s0);
+        else __syncthreads();
+        if (it.j >= low && it.j < low + n) {
+            sh[0] = s0 + tid;
+            sh[1] = n - 1 - (it.j - low);  // the longest row tiles (the last ones) start first
+        }
+        if (it.j < total || total >= count) break;
+    }
+    __syncthreads();
+    it.s = sh[0];
+    it.rt = sh[1];
+    return it.s >= 0;
 }
 
 template <int KIND, int DIM>
@@ -300,24 +403,28 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     float *scales = reinterpret_cast<float *>(smem + G::kScales);  // [K|V][tile parity][128]
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int s = blockIdx.z, h = blockIdx.y;
-    // The longest row tiles (the last ones) start first.
-    const int rt = a.row_tiles - 1 - (int)blockIdx.x / a.splits, sp = (int)blockIdx.x % a.splits;
     pdl_wait();
     pdl_trigger();  // the decode kernel of the same call starts beside the last CTAs
-    PagedExtent e;
-    const int bad_extent = paged_extent(&v, s, &e);
-    if (bad_extent && !blockIdx.x && !h && !tid) paged_report(a.status, bad_extent);
-    if (e.count <= a.few) return;
-    const int rows = e.count * a.group, r0 = rt * kPcRows;
-    if (r0 >= rows) return;
-    const int origin = e.length - e.count;  // place of the first new row
-    const int live = min(kPcRows, rows - r0), halves = live > 128 ? 2 : 1;
-    const int first = origin + r0 / a.group, last = origin + (r0 + live - 1) / a.group;
-    int splits;
-    const PagedTiles tiles = pc_tiles(a, e, rt, splits);
-    if (sp >= splits) return;
-    const int k0 = (int)((int64_t)tiles.count * sp / splits), n = (int)((int64_t)tiles.count * (sp + 1) / splits) - k0;
+    PcItem it;
+    if (!pc_item(a, reinterpret_cast<int *>(smem), it)) return;
+    PagedExtent extent;
+    paged_extent(&v, it.s, &extent);
+    const PagedTiles tiles = pc_tiles(a, extent, it.rt);
+    const int splits = max(1, min(it.splits, tiles.count));
+    if (tid == 0 && it.h == 0 && it.sp == 0) a.plan[1 + it.j] = make_int4(extent.start, extent.count * a.group, it.rt, splits);
+    if (it.sp >= splits) return;
+    const int k0 = (int)((int64_t)tiles.count * it.sp / splits), n = (int)((int64_t)tiles.count * (it.sp + 1) / splits) - k0;
+    const int halves = extent.count * a.group - it.rt * kPcRows > 128 ? 2 : 1;
+    if (tid == 0) {
+        PcWork z;
+        z.s = it.s, z.h = it.h, z.start = extent.start, z.rows = extent.count * a.group;
+        z.origin = extent.length - extent.count;
+        z.r0 = it.rt * kPcRows, z.live = min(kPcRows, z.rows - z.r0), z.splits = splits;
+        z.first = z.origin + z.r0 / a.group, z.last = z.origin + (z.r0 + z.live - 1) / a.group;
+        z.tiles = tiles, z.k0 = k0, z.n = n;
+        x.work = z;
+    }
+    const volatile PcWork &z = x.work;
 
     const uint32_t base_s = smem_addr(smem);
     if (base_s & 1023u) {  // the swizzled tiles need it; a launch without static shared memory starts there
@@ -354,12 +461,12 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     if (warp < 8) {
         // ================================================================ softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPcSoftmaxRegs));
-        const int i = warp >> 2, row = (warp & 3) * 32 + lane, r = r0 + i * 128 + row;
-        if (i < halves) {
+        const int i = warp >> 2, row = (warp & 3) * 32 + lane, r = z.r0 + i * 128 + row;
+        if (i == 0 || z.live > 128) {
             // ---- Q: this warp's 32 rows as two FP16 parts, scaled by the row's power of two
             float mine = 0.f;
             constexpr int E = DIM / 32, QB = 32;  // rows whose loads are in flight together
-            const long long q_at = r < rows ? (long long)(e.start + r / a.group) * a.q_stride + (h * a.group + r % a.group) * DIM : -1;
+            const long long q_at = r < z.rows ? (long long)(z.start + r / a.group) * a.q_stride + (z.h * a.group + r % a.group) * DIM : -1;
 #pragma unroll 1
             for (int first_k = 0; first_k < 32; first_k += QB) {
                 float f[QB][E];
@@ -411,16 +518,16 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
             mbar_arrive(&x.q_full);
 
             const float qs = mine;
-            const int at = r < rows ? origin + r / a.group : -1;  // a row behind the last sees nothing
-            const int top_row = min(live, (i + 1) * 128) - 1;
-            const int first_i = origin + (r0 + i * 128) / a.group, last_i = origin + (r0 + top_row) / a.group;
+            const int at = r < z.rows ? z.origin + r / a.group : -1;  // a row behind the last sees nothing
+            const int top_row = min(z.live, (i + 1) * 128) - 1;
+            const int first_i = z.origin + (z.r0 + i * 128) / a.group, last_i = z.origin + (z.r0 + top_row) / a.group;
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + lanes + (uint32_t)(128 * i), to = tmem + lanes + 256u + (uint32_t)(128 * i);
             float o[DIM], m = -INFINITY, l = 0.f;
 #pragma unroll
             for (int c = 0; c < DIM; c++) o[c] = 0.f;
-            for (int t = 0; t < n; t++) {
-                const int base = paged_tile(tiles, k0 + t) * kPcTile, par = t & 1;
+            for (int t = 0; t < z.n; t++) {
+                const int base = z.base(t), par = t & 1;
                 const float *ks = scales + par * 128, *vs = scales + 256 + par * 128;
                 if (!warp_wait(&x.ks_full[par], (t >> 1) & 1, a.err)) break;
                 if (!warp_wait(&x.s_full[i], t & 1, a.err)) break;
@@ -508,9 +615,10 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
             // warp writes whole rows. Every warp has written its queries there (with no tile at all nothing
             // else has made sure of that).
             warp_wait(&x.q_full, 0, a.err);
-            const float f = splits > 1 ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
-            const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits + sp;
-            if (splits > 1 && r < rows) a.ml[item * kPcRows + (r - r0)] = make_float2(m, l);
+            const int parts = z.splits, rows = z.rows;
+            const float f = parts > 1 ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // nothing seen: zeros
+            const int64_t slot = blockIdx.x;
+            if (parts > 1 && r < rows) a.ml[slot * kPcRows + (r - z.r0)] = make_float2(m, l);
             constexpr int PR = DIM / 4;  // 16-byte pieces a row
             const uint32_t area = base_s + (uint32_t)(2 * i) * G::kOperand + (uint32_t)((warp & 3) * 32 * DIM * 4);
 #pragma unroll
@@ -518,9 +626,9 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                 st_smem16(area + (uint32_t)(lane * PR + (c ^ (lane & (PR - 1)))) * 16, __float_as_uint(o[4 * c] * f),
                           __float_as_uint(o[4 * c + 1] * f), __float_as_uint(o[4 * c + 2] * f), __float_as_uint(o[4 * c + 3] * f));
             __syncwarp();
-            const long long mine_at = splits > 1 ? (item * kPcRows + (r - r0)) * DIM
-                                                 : (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM;
-            float *dst = splits > 1 ? a.part : a.out;
+            const long long mine_at = parts > 1 ? (slot * kPcRows + (r - z.r0)) * DIM
+                                                : (long long)(z.start + r / a.group) * a.out_stride + (z.h * a.group + r % a.group) * DIM;
+            float *dst = parts > 1 ? a.part : a.out;
 #pragma unroll 4
             for (int k = 0; k < 32; k += 32 / PR) {
                 const int rr = k + lane / PR, c = lane % PR;
@@ -541,16 +649,16 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         int bad = 0;
         bool ok = true;
         float v_low = INFINITY;  // the smallest V scale of this lane's rows so far
-        for (int t = 0; t < n && ok; t++) {
-            const int base = paged_tile(tiles, k0 + t) * kPcTile, par = t & 1;
+        for (int t = 0; t < z.n && ok; t++) {
+            const int base = z.base(t), par = t & 1;
             // This lane's row: place base + 32 w + lane.
             const int j = base + 32 * w + lane;
             int64_t mine = -1;
             // Rows that no query of the tile sees are left out: they may hold anything, a scale that would
             // drown the others' too, and their page may be missing.
-            if (j <= last && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)first - a.window)) {
+            if (j <= z.last && (a.window == 0 || j < a.sinks || (int64_t)j > (int64_t)z.first - a.window)) {
                 const int pg = paged_div(&v, j);
-                mine = paged_row(&v, v.table[(int64_t)s * v.table_stride + pg], j, pg, h);
+                mine = paged_row(&v, v.table[(int64_t)z.s * v.table_stride + pg], j, pg, z.h);
                 if (mine < 0) bad |= kPagedBadPage;
             }
             const uint32_t there = __ballot_sync(0xffffffffu, mine >= 0);
@@ -647,6 +755,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     }
     if (warp == 12) {
         const uint32_t ring = base_s + G::kQ;
+        const int n = z.n, halves = z.live > 128 ? 2 : 1;
         bool ok = warp_wait(&x.q_full, 0, a.err);
         auto scores = [&](int t, int i) {  // S_i = Q_i K(t)^T
             const int use = 2 * t, slot = use % kPcSlots;
@@ -720,23 +829,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
 // The parts of split row tiles, joined in order: a warp a query row. A kernel of its own, because
 // the last of a row tile's CTAs alone took 10 us over its 256 rows.
 constexpr int kPcJoinThreads = 256;
-template <int DIM>
-__global__ void __launch_bounds__(kPcJoinThreads) paged_chunk_join_kernel(const PagedChunkArgs a) {
+// Query row rr of a row tile (its entry of the plan) and KV head h, whose parts begin at slot `item`.
+template <int DIM> __device__ __forceinline__ void pc_join_row(const PagedChunkArgs &a, int4 tile, int h, int64_t item, int rr, int lane) {
     constexpr int E = DIM / 32;
-    const PagedView &v = a.v;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, s = blockIdx.z, h = blockIdx.y;
-    pdl_wait();
-    PagedExtent e;
-    paged_extent(&v, s, &e);
-    const int rows = e.count * a.group, r = blockIdx.x * (kPcJoinThreads / 32) + warp, rt = r / kPcRows;
-    if (e.count <= a.few || r >= rows) return;
-    int splits;
-    pc_tiles(a, e, rt, splits);
-    if (splits == 1) return;
-    const int64_t item = (((int64_t)s * v.kvheads + h) * a.row_tiles + rt) * a.splits;
-    const int rr = r - rt * kPcRows;
-    static_assert(kPcSplitsMax <= 32, "a lane for each split");
+    const int start = tile.x, splits = tile.w, r = tile.z * kPcRows + rr;
+    if (splits == 1 || r >= tile.y) return;
     // Lane w holds split w's maximum and sum; every lane a piece of the row of each split.
+    static_assert(kPcSplitsMax <= 32, "a lane for each split");
     const float2 ml = lane < splits ? __ldcg(&a.ml[(item + lane) * kPcRows + rr]) : make_float2(-INFINITY, 0.f);
     const float top = warp_max(ml.x), mine = pd_factor(ml, top), sum = warp_sum(ml.y * mine);
     float y[E];
@@ -764,9 +863,25 @@ __global__ void __launch_bounds__(kPcJoinThreads) paged_chunk_join_kernel(const 
         }
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-    float *dst = a.out + (long long)(e.start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
+    float *dst = a.out + (long long)(start + r / a.group) * a.out_stride + (h * a.group + r % a.group) * DIM + lane * E;
     if constexpr (E == 4) *reinterpret_cast<float4 *>(dst) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     else *reinterpret_cast<float2 *>(dst) = make_float2(y[0] * inv, y[1] * inv);
+}
+template <int DIM>
+__global__ void __launch_bounds__(kPcJoinThreads) paged_chunk_join_kernel(const PagedChunkArgs a) {
+    const int kvheads = a.v.kvheads, lane = threadIdx.x & 31, step = gridDim.x * (kPcJoinThreads / 32);
+    int at = (blockIdx.x * kPcJoinThreads + threadIdx.x) / 32;  // an item's query row
+    pdl_wait();
+    int4 tile = __ldcg(a.plan + 1 + at / kPcRows / kvheads);  // the launch is no larger than the plan
+    const int4 head = __ldcg(a.plan);
+    if (head.y == 1) return;
+    for (;;) {  // a batch that is split has no more items than there are places for parts
+        const int index = at / kPcRows;
+        if (index >= head.x * kvheads) return;
+        pc_join_row<DIM>(a, tile, index % kvheads, (int64_t)index * head.y, at % kPcRows, lane);
+        at += step;
+        if (at / kPcRows < head.x * kvheads) tile = __ldcg(a.plan + 1 + at / kPcRows / kvheads);
+    }
 }
 
 }  // namespace tcm

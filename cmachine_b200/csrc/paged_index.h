@@ -110,4 +110,42 @@ TCM_HD PagedTiles paged_tiles(int first, int last, int window, int sinks, int sh
 }
 TCM_HD int paged_tile(PagedTiles t, int k) { return k < t.a ? k : t.b + (k - t.a); }
 
+/* How chunks are shared out. A row tile is `tile` query rows of one KV head; an item is a row tile of one KV head,
+ * and may be split over the rows that it sees. The device counts the row tiles of a batch; the host, which knows
+ * only sums and maxima, launches for a bound of them and for a guess.
+ *
+ * The most row tiles that sequences of more than `few` rows can have: each has at most max_new rows, and
+ * ceil(n / tile) adds up to less than the sum over tile and one for each, of rows / (few + 1) sequences at most. */
+TCM_HD int64_t paged_tile_bound(int sequences, int rows, int max_new, int group, int few, int tile) {
+    const int64_t each = ((int64_t)max_new * group + tile - 1) / tile, live = rows / (few + 1);
+    const int64_t all = (int64_t)rows * group / tile + (live < sequences ? live : sequences);
+    return all < each * sequences ? all : each * sequences;
+}
+/* Their number when some sequences have max_new rows and the others one, as many as the rows are enough for. */
+TCM_HD int64_t paged_tile_guess(int sequences, int rows, int max_new, int group, int few, int tile) {
+    const int64_t bound = paged_tile_bound(sequences, rows, max_new, group, few, tile);
+    int64_t full = max_new > 1 ? ((int64_t)rows - sequences + max_new - 2) / (max_new - 1) : sequences;
+    if (full < 1) full = 1;
+    full *= ((int64_t)max_new * group + tile - 1) / tile;
+    return full < bound ? full : bound;
+}
+/* The time of `items` items of `mean` cached-row tiles and `longest` at most, each of them split in k: rounds of the
+ * SMs, or the longest split, whose start and end count as three tiles; joining the parts counts as two. The k taken
+ * is the least within 3 % of the best. (items * k is below 2^32: it passes paged_may_split, or k is 1.) */
+TCM_HD float paged_split_cost(int64_t items, int k, int mean, int longest, int sms) {
+    const float rounds = (float)(((uint32_t)items * (uint32_t)k + (uint32_t)sms - 1) / (uint32_t)sms);
+    const float all = rounds * ((float)mean / (float)k + 3.f), one = (float)longest / (float)k + 3.f;
+    return (all > one ? all : one) + (k > 1 ? 2.f : 0.f);
+}
+TCM_HD int paged_may_split(int64_t items, int k, int tiles, int64_t room) { return k == 1 || (2 * k <= tiles && items * k <= room); }
+static inline int paged_splits(int64_t items, int tiles, int sms, int64_t room, int most) {
+    float least = paged_split_cost(items, 1, tiles, tiles, sms);
+    for (int k = 2; k <= most; k++)
+        if (paged_may_split(items, k, tiles, room) && paged_split_cost(items, k, tiles, tiles, sms) < least)
+            least = paged_split_cost(items, k, tiles, tiles, sms);
+    for (int k = 1;; k++)
+        if (k == most || (paged_may_split(items, k, tiles, room) && paged_split_cost(items, k, tiles, tiles, sms) <= 1.03f * least))
+            return k;
+}
+
 #endif

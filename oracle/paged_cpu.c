@@ -39,3 +39,12 @@ int paged_cpu_tiles(int first, int last, int window, int sinks, int shift, int *
     for (int k = 0; k < t.count && k < most; k++) out[k] = paged_tile(t, k);
     return t.count;
 }
+int64_t paged_cpu_tile_bound(int sequences, int rows, int max_new, int group, int few, int tile) {
+    return paged_tile_bound(sequences, rows, max_new, group, few, tile);
+}
+int64_t paged_cpu_tile_guess(int sequences, int rows, int max_new, int group, int few, int tile) {
+    return paged_tile_guess(sequences, rows, max_new, group, few, tile);
+}
+int paged_cpu_splits(int64_t items, int tiles, int sms, int64_t room, int most) {
+    return paged_splits(items, tiles, sms, room, most);
+}

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 import cmachine_b200 as cm
-from test_gpu_paged import BF16, BYTES, KINDS, MHA64, QWEN, Pool, bf16, encode, read_back, store, widen
+from test_gpu_paged import (BF16, BYTES, KINDS, MHA64, QWEN, SENTINEL, Pool, bf16, encode, read_back, store,
+                            widen)
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +19,7 @@ def test_many_launches_beside_chunks_give_the_same_bits(kind):
     news = np.where(np.arange(400) % 50 == 7, 70, rng.integers(0, 3, 400))
     lengths = np.maximum(news, np.where(np.arange(400) % 9 == 0, 900, rng.integers(0, 60, 400)))
     p = Pool(kind, MHA64, 16, news, lengths, seed=8)
+    p.values = [p.values(0), p.values(1)].__getitem__  # once, not for each sequence
     q, g = p.queries(), cm.lib().gpu_open()
     first = p.attend(q, gpu=g)
     p.check(first, q)
@@ -206,4 +208,34 @@ def test_a_table_for_very_long_sequences(news, lengths):
     q = p.queries()
     p.check(p.attend(q), q)
     assert p.flags() == 0
+    p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("count", [7, 512, 1300])
+def test_chunks_among_many_sequences(kind, count):
+    """Chunks at the first, last and other places among single tokens and sequences without rows, more of them than
+    a CTA's threads; one chunk's extents do not fit. Loose maxima and buffers change no result beyond the bound."""
+    rng = np.random.default_rng(count)
+    news, lengths = rng.integers(0, 2, count), rng.integers(1, 40, count)
+    chunks = sorted({0, 3, count // 2, min(511, count - 1), min(512, count - 1), count - 1})
+    for i, s in enumerate(chunks):
+        news[s], lengths[s] = 60 + 41 * i, 70 + 300 * i
+    p = Pool(kind, MHA64, 16, news, lengths, seed=count)
+    p.values = [p.values(0), p.values(1)].__getitem__  # once, not for each sequence
+    q = p.queries()
+    p.check(p.attend(q), q)
+    assert p.flags() == 0
+    p.batch.max_new, p.batch.rows = 5000, p.rows + 4000
+    more = np.zeros((p.rows + 4000, q.shape[1]), np.float32)
+    more[:p.rows] = q
+    got = p.attend(more, rows=p.rows + 4000)
+    p.check(got, q)
+    assert np.all(got[p.rows:] == SENTINEL) and p.flags() == 0
+    bad = p.lengths.astype(np.int32)
+    bad[chunks[2]] = p.stride * 16 + 1
+    cm.lib().gpu_write(p.live[4], cm.ptr(bad), bad.nbytes)
+    got = p.attend(q)
+    assert p.flags() == 4 and np.all(got[p.starts[chunks[2]]:p.starts[chunks[2] + 1]] == SENTINEL)
+    p.check(got, q, skip=[chunks[2]])
     p.free()
