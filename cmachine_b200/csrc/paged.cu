@@ -8,7 +8,7 @@
 #include "paged_decode.cuh"
 #include "paged_chunk.cuh"
 #include "kernels.h"
-#include "../../include/gpu.h"
+#include "../../include/qwen_b200.h"
 #include "../../include/tcm_seeded.h"
 #include <math.h>
 
@@ -299,14 +299,6 @@ unsigned blocks_of(long long items, int a_block) {
     return (unsigned)(blocks < 4096 ? blocks : 4096);
 }
 
-}  // namespace
-
-void set_wait_limit_paged(unsigned long long ns) { set_module_wait_limit(ns); }
-
-}  // namespace tcm
-
-using namespace tcm;
-
 #define PAGED_DISPATCH(view, call)                                      \
     do {                                                                \
         if ((view).kind == kPagedBf16) {                                \
@@ -317,6 +309,46 @@ using namespace tcm;
             else { call(kPagedBytes, 128); }                            \
         }                                                               \
     } while (0)
+
+// gpu_paged_attention, and its self-check.
+int attention(const char *name, TcmGpu *gpu, float *out, long long out_stride, const float *q, long long q_stride,
+              const TcmPagedCache *cache, const TcmPagedBatch *batch, int qheads, int window, int sinks, int *status,
+              int starve) {
+    PagedView view;
+    if (!gpu) return refuse(name, "no handle");
+    if (open_view(name, cache, batch, &view)) return -1;
+    if (qheads < 1 || qheads % view.kvheads || qheads / view.kvheads > 8)
+        return refuse(name, "qheads is 1 to 8 times kvheads");
+    if (window < 0 || sinks < 0) return refuse(name, "window and sinks are not negative");
+    if (nothing(view)) return 0;
+    if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
+    const int group = qheads / view.kvheads, few = few_rows(view.kind) / group;
+    if (view.max_new > few &&
+        view.kvheads * paged_tile_bound(view.sequences, view.rows, view.max_new, group, 0, kPcRows) > 0x7fffffff)
+        return refuse(name, "too many rows and sequences for one call");
+    const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
+    // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever it
+    // has: it nearly always has them, and an empty launch of the other takes 2.6 us of the device.
+    const bool lone = view.sequences == 1 && view.max_new > few;
+    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, 0, 0, few, scale2, nullptr, nullptr,
+                         nullptr, status, 0};
+    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 0, 0, scale2, nullptr, nullptr,
+                        nullptr, status, nullptr, starve};
+#define CALL(K, D)                                            \
+    if (view.max_new <= few) decode_launch<K, D>(gpu, d);     \
+    else chunk_launch<K, D>(gpu, c, lone ? nullptr : &d)
+    PAGED_DISPATCH(view, CALL);
+#undef CALL
+    return 0;
+}
+
+}  // namespace
+
+void set_wait_limit_paged(unsigned long long ns) { set_module_wait_limit(ns); }
+
+}  // namespace tcm
+
+using namespace tcm;
 
 extern "C" {
 
@@ -354,33 +386,14 @@ int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float
 int gpu_paged_attention(TcmGpu *gpu, float *out, long long out_stride, const float *q, long long q_stride,
                         const TcmPagedCache *cache, const TcmPagedBatch *batch, int qheads, int window, int sinks,
                         int *status) {
-    const char *name = "gpu_paged_attention";
-    PagedView view;
-    if (!gpu) return refuse(name, "no handle");
-    if (open_view(name, cache, batch, &view)) return -1;
-    if (qheads < 1 || qheads % view.kvheads || qheads / view.kvheads > 8)
-        return refuse(name, "qheads is 1 to 8 times kvheads");
-    if (window < 0 || sinks < 0) return refuse(name, "window and sinks are not negative");
-    if (nothing(view)) return 0;
-    if (check_rows(name, q, q_stride, qheads, view.dim) || check_rows(name, out, out_stride, qheads, view.dim)) return -1;
-    const int group = qheads / view.kvheads, few = few_rows(view.kind) / group;
-    if (view.max_new > few &&
-        view.kvheads * paged_tile_bound(view.sequences, view.rows, view.max_new, group, 0, kPcRows) > 0x7fffffff)
-        return refuse(name, "too many rows and sequences for one call");
-    const float scale2 = 1.44269504088896340736f / sqrtf((float)view.dim);  // log2(e) / sqrt(dim): base-2 scores
-    // A lone sequence that may have more rows than the decode kernel's is the chunk kernel's whatever it
-    // has: it nearly always has them, and an empty launch of the other takes 2.6 us of the device.
-    const bool lone = view.sequences == 1 && view.max_new > few;
-    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, window, sinks, 0, 0, few, scale2, nullptr, nullptr,
-                         nullptr, status, 0};
-    PagedChunkArgs c = {view, out, q, out_stride, q_stride, group, window, sinks, lone ? 0 : few, 0, 0, scale2, nullptr, nullptr,
-                        nullptr, status, nullptr};
-#define CALL(K, D)                                                  \
-    if (view.max_new <= few) decode_launch<K, D>(gpu, d);           \
-    else chunk_launch<K, D>(gpu, c, lone ? nullptr : &d)
-    PAGED_DISPATCH(view, CALL);
-#undef CALL
-    return 0;
+    return attention("gpu_paged_attention", gpu, out, out_stride, q, q_stride, cache, batch, qheads, window, sinks, status, 0);
+}
+
+int qwen_b200_paged_check(TcmGpu *gpu, float *out, long long out_stride, const float *q, long long q_stride,
+                          const TcmPagedCache *cache, const TcmPagedBatch *batch, int qheads, int window, int sinks,
+                          int *status, int starve) {
+    if (starve < 0 || starve > 2) return refuse("qwen_b200_paged_check", "starve is 0, 1 or 2");
+    return attention("qwen_b200_paged_check", gpu, out, out_stride, q, q_stride, cache, batch, qheads, window, sinks, status, starve);
 }
 
 }  // extern "C"

@@ -63,6 +63,7 @@ struct PagedChunkArgs {
     int4 *plan;              // [0] the row tiles and their splits, then each tile's first row, query rows, number and splits
     int *status;
     unsigned *err;           // where waits that run out are recorded (status, or scratch)
+    int starve;              // self-check: 1 or 2 keeps the first K or V tile from ever being ready
 };
 
 template <int DIM> struct PcGeo {
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
                 }
                 if (!ok) break;
                 fence_async_smem();
-                mbar_arrive(&x.full[slot]);
+                if (t || a.starve != 1 + which) mbar_arrive(&x.full[slot]);
                 if (!which) {
                     scales[par * 128 + 32 * w + lane] = mine >= 0 ? scale : 0.f;
                     if (lane == 0) x.there[par][w] = there;

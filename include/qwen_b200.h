@@ -251,9 +251,15 @@ int qwen_b200_tp_world(const QwenB200Runner *);
  * on one CTA: y[rows] = W[rows][1536] x (FP32 device pointers, rows <= 4096)
  * and returns the fault bits (0 when every wait completed; with starve != 0
  * the producer issues nothing, so the consumers' waits run out: bit 1), or -1
- * for invalid arguments. */
+ * for invalid arguments. qwen_b200_paged_check is gpu_paged_attention (gpu.h)
+ * whose chunk kernel, which sequences of many new rows take, is told never to
+ * have its first tile of K (starve 1) or V (2) ready: its waits run out, and
+ * *status gets bit 8. */
 int qwen_b200_wait_limit(unsigned long long ns);
 int qwen_b200_pipeline_check(const float *w, int rows, const float *x, float *y, int starve);
+int qwen_b200_paged_check(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
+                          const TcmPagedCache *, const TcmPagedBatch *, int qheads, int window, int sinks, int *status,
+                          int starve);
 
 /* Kernel launches one token issues (for launch accounting). */
 int qwen_b200_launches_per_token(const QwenB200Runner *);

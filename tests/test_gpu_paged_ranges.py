@@ -1,12 +1,14 @@
 """GPU tests of the paged K/V cache at the ends of its ranges: batches of several launches, values of unlike
 size, long sums, small queries, loose maxima. The pool, its float64 oracle and its bound are
 tests/test_gpu_paged.py's unless a test states its own."""
+import time
+
 import numpy as np
 import pytest
 
 import cmachine_b200 as cm
 from test_gpu_paged import (BF16, BYTES, KINDS, MHA64, QWEN, SENTINEL, Pool, bf16, encode, read_back, store,
-                            widen)
+                            upload, widen)
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +241,30 @@ def test_chunks_among_many_sequences(kind, count):
     assert p.flags() == 4 and np.all(got[p.starts[chunks[2]]:p.starts[chunks[2] + 1]] == SENTINEL)
     p.check(got, q, skip=[chunks[2]])
     p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("starve", [1, 2])
+@pytest.mark.parametrize("news,lengths", [([60], [90]), ([200], [2000]), ([300, 1, 40], [1000, 700, 40])])
+def test_waits_that_run_out_are_reported(kind, starve, news, lengths):
+    """A first tile that is never ready: every wait behind it runs out after 20 ms, the call comes to its end with
+    status 8, and the next one is right."""
+    L = cm.lib()
+    p = Pool(kind, QWEN, 16, news, lengths, seed=51)
+    q, g = p.queries(), L.gpu_open()
+    dq, out = upload(q), upload(q)
+    try:
+        assert L.qwen_b200_wait_limit(20_000_000) == 0
+        begin = time.perf_counter()
+        assert L.qwen_b200_paged_check(g, out, q.shape[1], dq, q.shape[1], p.cache, p.batch, 12, 0, 0, p.status, starve) == 0
+        assert p.flags() == 8
+        assert 0.015 <= time.perf_counter() - begin <= 1
+        L.gpu_zero(p.status, 4)
+        p.check(p.attend(q, gpu=g), q)
+        assert p.flags() == 0
+    finally:
+        assert L.qwen_b200_wait_limit(0) == 0
+        for x in (dq, out):
+            L.gpu_free(x)
+        L.gpu_close(g)
+        p.free()
