@@ -306,6 +306,7 @@ __device__ __forceinline__ PagedTiles pc_tiles(const PagedChunkArgs &a, const Pa
 // What a CTA works on: split sp of `splits` of row tile rt (the j-th of the batch) of sequence s, for KV head h.
 struct PcItem {
     int s, rt, j, h, sp, splits;
+    PagedExtent e;  // the sequence's
 };
 // Finds it, the same in every thread, or returns false. Every CTA counts the row tiles of all sequences (their
 // extents are on the device) and takes the splits for what there is, not for the declared maxima: with one chunk of
@@ -316,13 +317,14 @@ __device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int W = kPcThreads / 32;
     int bad = 0, longest = 0, sum = 0;  // of this thread's sequences: the tiles of the longest row tile, and of all
+    PagedExtent e;                      // of its last one
     auto row_tiles = [&](int s) {
-        PagedExtent e = {0, 0, 0};
+        e.start = e.count = e.length = 0;
         if (s < v.sequences) bad |= paged_extent(&v, s, &e);
         if (e.count <= a.few) return 0;
         const int n = (e.count * a.group + kPcRows - 1) / kPcRows, most = pc_tiles(a, e, n - 1).count;
         longest = max(longest, most);
-        sum += n * ((pc_tiles(a, e, 0).count + most + 1) / 2);
+        sum += n * (v.sequences == 1 ? most : (pc_tiles(a, e, 0).count + most + 1) / 2);
         return n;
     };
     // A sequence a thread: how many row tiles it has (n), and the sequences before it (low); then `total` counts
@@ -354,7 +356,7 @@ __device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem
     // Splits: a number a lane (paged_splits).
     static_assert(kPcSplitsMax == 32, "a lane for each number of splits");
     const int64_t items = (int64_t)total * v.kvheads;
-    const int mean = (sum + total - 1) / max(total, 1);
+    const int mean = v.sequences == 1 ? longest : (sum + total - 1) / max(total, 1);
     const float cost = paged_may_split(items, lane + 1, longest, a.slots) ? paged_split_cost((unsigned)items, lane + 1, mean, longest, a.sms) : INFINITY;
     const int splits = __ffs(__ballot_sync(0xffffffffu, cost <= -1.03f * warp_max(-cost)));
     if (blockIdx.x == 0) {
@@ -371,6 +373,7 @@ __device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem
     if (v.sequences == 1) {
         it.s = 0;
         it.rt = n - 1 - it.j;
+        it.e = e;
         return true;
     }
     if (tid == 0) sh[0] = -1;
@@ -385,12 +388,14 @@ __device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem
         if (it.j >= low && it.j < low + n) {
             sh[0] = s0 + tid;
             sh[1] = n - 1 - (it.j - low);  // the longest row tiles (the last ones) start first
+            sh[2] = e.start, sh[3] = e.count, sh[4 + 3 * W] = e.length;
         }
         if (it.j < total || total >= count) break;
     }
     __syncthreads();
     it.s = sh[0];
     it.rt = sh[1];
+    it.e.start = sh[2], it.e.count = sh[3], it.e.length = sh[4 + 3 * W];
     return it.s >= 0;
 }
 
@@ -408,13 +413,13 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
     pdl_trigger();  // the decode kernel of the same call starts beside the last CTAs
     PcItem it;
     if (!pc_item(a, reinterpret_cast<int *>(smem), it)) return;
-    PagedExtent extent;
-    paged_extent(&v, it.s, &extent);
+    const PagedExtent &extent = it.e;
     const PagedTiles tiles = pc_tiles(a, extent, it.rt);
     const int splits = max(1, min(it.splits, tiles.count));
     if (tid == 0 && it.h == 0 && it.sp == 0) a.plan[1 + it.j] = make_int4(extent.start, extent.count * a.group, it.rt, splits);
     if (it.sp >= splits) return;
-    const int k0 = (int)((int64_t)tiles.count * it.sp / splits), n = (int)((int64_t)tiles.count * (it.sp + 1) / splits) - k0;
+    // Below 2^23 tiles, at most 32 splits.
+    const int k0 = (int)((unsigned)(tiles.count * it.sp) / (unsigned)splits), n = (int)((unsigned)(tiles.count * (it.sp + 1)) / (unsigned)splits) - k0;
     const int halves = extent.count * a.group - it.rt * kPcRows > 128 ? 2 : 1;
     if (tid == 0) {
         PcWork z;
@@ -873,15 +878,16 @@ __global__ void __launch_bounds__(kPcJoinThreads) paged_chunk_join_kernel(const 
     const int kvheads = a.v.kvheads, lane = threadIdx.x & 31, step = gridDim.x * (kPcJoinThreads / 32);
     int at = (blockIdx.x * kPcJoinThreads + threadIdx.x) / 32;  // an item's query row
     pdl_wait();
-    int4 tile = __ldcg(a.plan + 1 + at / kPcRows / kvheads);  // the launch is no larger than the plan
-    const int4 head = __ldcg(a.plan);
+    // Every warp reads these: through L1 (past it, 6144 warps met in a few lines of L2, 1 us longer).
+    int4 tile = a.plan[1 + at / kPcRows / kvheads];  // the launch is no larger than the plan
+    const int4 head = a.plan[0];
     if (head.y == 1) return;
     for (;;) {  // a batch that is split has no more items than there are places for parts
         const int index = at / kPcRows;
         if (index >= head.x * kvheads) return;
         pc_join_row<DIM>(a, tile, index % kvheads, (int64_t)index * head.y, at % kPcRows, lane);
         at += step;
-        if (at / kPcRows < head.x * kvheads) tile = __ldcg(a.plan + 1 + at / kPcRows / kvheads);
+        if (at / kPcRows < head.x * kvheads) tile = a.plan[1 + at / kPcRows / kvheads];
     }
 }
 
