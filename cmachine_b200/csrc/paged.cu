@@ -173,7 +173,7 @@ int refuse(const char *call, const char *why) {
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // The call's descriptors as a view; 0, or -1 with a message.
-int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, PagedView *v) {
+int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, const int *status, PagedView *v) {
     if (!c || !b) return refuse(call, "no cache or no batch");
     if (c->kind != kPagedBf16 && c->kind != kPagedBytes) return refuse(call, "kind is 2 (BF16) or 3 (bytes)");
     if (c->dim != 64 && c->dim != 128) return refuse(call, "dim is 64 or 128");
@@ -189,6 +189,7 @@ int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, 
         return refuse(call, "a batch has starts, lengths and a table");
     if (((uintptr_t)b->starts | (uintptr_t)b->lengths | (uintptr_t)b->table) & 3)
         return refuse(call, "starts, lengths and table are 4-byte aligned");
+    if ((uintptr_t)status & 3) return refuse(call, "status is 4-byte aligned");
     const int max_new = b->max_new < b->rows ? b->max_new : b->rows;
     // No sequence is longer than its table either.
     const long long held = (long long)b->table_stride * c->page;
@@ -316,7 +317,7 @@ int attention(const char *name, TcmGpu *gpu, float *out, long long out_stride, c
               int starve) {
     PagedView view;
     if (!gpu) return refuse(name, "no handle");
-    if (open_view(name, cache, batch, &view)) return -1;
+    if (open_view(name, cache, batch, status, &view)) return -1;
     if (qheads < 1 || qheads % view.kvheads || qheads / view.kvheads > 8)
         return refuse(name, "qheads is 1 to 8 times kvheads");
     if (window < 0 || sinks < 0) return refuse(name, "window and sinks are not negative");
@@ -355,7 +356,7 @@ extern "C" {
 int gpu_paged_append(const TcmPagedCache *cache, const TcmPagedBatch *batch, const float *k, const float *v,
                      long long stride, int *status) {
     PagedView view;
-    if (open_view("gpu_paged_append", cache, batch, &view)) return -1;
+    if (open_view("gpu_paged_append", cache, batch, status, &view)) return -1;
     if (nothing(view)) return 0;
     if (check_rows("gpu_paged_append", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_append", v, stride, view.kvheads, view.dim))
@@ -371,7 +372,7 @@ int gpu_paged_append(const TcmPagedCache *cache, const TcmPagedBatch *batch, con
 int gpu_paged_read(const TcmPagedCache *cache, const TcmPagedBatch *batch, float *k, float *v, long long stride,
                    int *status) {
     PagedView view;
-    if (open_view("gpu_paged_read", cache, batch, &view)) return -1;
+    if (open_view("gpu_paged_read", cache, batch, status, &view)) return -1;
     if (nothing(view)) return 0;
     if (check_rows("gpu_paged_read", k, stride, view.kvheads, view.dim) ||
         check_rows("gpu_paged_read", v, stride, view.kvheads, view.dim))

@@ -1,11 +1,13 @@
 """How chunks of a paged batch are shared out (csrc/paged_index.h, built for the host): bounds of a batch's row
-tiles that the host launches for, and the splits taken for what there is."""
+tiles that the host launches for, the splits taken for what there is; and a call that is refused."""
 import ctypes
 from ctypes import c_int, c_int64
 from pathlib import Path
 
 import numpy as np
 import pytest
+
+import cmachine_b200 as cm
 
 ROOT = Path(__file__).resolve().parent.parent
 TILE, SMS = 256, 148
@@ -82,3 +84,16 @@ def test_splits_are_the_fewest_that_are_nearly_the_best():
         best = min(cost(items, x, tiles) for x in allowed)
         assert cost(items, k, tiles) <= 1.0301 * best
         assert all(cost(items, x, tiles) > 1.0299 * best for x in allowed if x < k)
+
+
+def test_a_status_word_out_of_step_is_refused(capfd):
+    """The kernels OR into it: an address that is no multiple of four would fault."""
+    L, a = cm.lib(), 1 << 20
+    cache, batch = cm.PagedCache(3, 8, 16, 2, 128, a, a, a), cm.PagedBatch(2, 4, 4, 64, a, a, a, 4)
+    for off in (1, 2, 3):
+        assert L.gpu_paged_append(cache, batch, a, a, 256, a + off) == -1
+        assert L.gpu_paged_read(cache, batch, a, a, 256, a + off) == -1
+        assert L.gpu_paged_attention(a, a, 1536, a, 1536, cache, batch, 12, 0, 0, a + off) == -1
+        assert L.qwen_b200_paged_check(a, a, 1536, a, 1536, cache, batch, 12, 0, 0, a + off, 0) == -1
+    assert L.qwen_b200_paged_check(a, a, 1536, a, 1536, cache, batch, 12, 0, 0, None, 3) == -1
+    assert capfd.readouterr().err.count("status is 4-byte aligned") == 12
