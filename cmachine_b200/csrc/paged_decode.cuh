@@ -525,25 +525,31 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                                 for (int mt = 0; mt < M; mt++) cf[mt][gr][c] = 0.f;
                         }
                     uint4 kr[2];
+                    // BF16 rows meet the queries' smaller parts first: the tensor cores truncate a sum as large as the
+                    // first parts' at every step that adds to it.
+                    constexpr int kPasses = kBytes || R == 8 ? 1 : 2;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        if (ks % 2 == 0)
+                    for (int pass = 0; pass < kPasses; pass++)
 #pragma unroll
-                            for (int gr = 0; gr < 2; gr++) {
-                                const int key = gr * 8 + g;
-                                kr[gr] = *reinterpret_cast<const uint4 *>(st + key * G::kRow + pd_swizzle<G::kRow>(key, (ks / 2) * 4 + t) * 16);
-                            }
+                        for (int ks = 0; ks < KS; ks++) {
+                            if (ks % 2 == 0)
 #pragma unroll
-                        for (int n = M * NA - 1; n >= 0; n--) {
-                            const uint4 f = qf[n][ks][lane];
+                                for (int gr = 0; gr < 2; gr++) {
+                                    const int key = gr * 8 + g;
+                                    kr[gr] = *reinterpret_cast<const uint4 *>(st + key * G::kRow + pd_swizzle<G::kRow>(key, (ks / 2) * 4 + t) * 16);
+                                }
 #pragma unroll
-                            for (int gr = 0; gr < 2; gr++) {
-                                const uint32_t b0 = ks % 2 ? kr[gr].z : kr[gr].x, b1 = ks % 2 ? kr[gr].w : kr[gr].y;
-                                if constexpr (kBytes) mma_s8(ci[n][gr], f, b0, b1);
-                                else mma_bf16(cf[n / NA][gr], f.x, f.y, f.z, f.w, b0, b1);
+                            for (int n = M * NA - 1; n >= 0; n--) {
+                                if (kPasses == 2 && (n % NA == 0) != (pass == 1)) continue;
+                                const uint4 f = qf[n][ks][lane];
+#pragma unroll
+                                for (int gr = 0; gr < 2; gr++) {
+                                    const uint32_t b0 = ks % 2 ? kr[gr].z : kr[gr].x, b1 = ks % 2 ? kr[gr].w : kr[gr].y;
+                                    if constexpr (kBytes) mma_s8(ci[n][gr], f, b0, b1);
+                                    else mma_bf16(cf[n / NA][gr], f.x, f.y, f.z, f.w, b0, b1);
+                                }
                             }
                         }
-                    }
 #pragma unroll
                     for (int mt = 0; mt < M; mt++)
 #pragma unroll

@@ -268,3 +268,34 @@ def test_waits_that_run_out_are_reported(kind, starve, news, lengths):
             L.gpu_free(x)
         L.gpu_close(g)
         p.free()
+
+
+@pytest.mark.parametrize("new", [1, 2, 5, 10])
+def test_scores_of_one_sign(new):
+    """BF16 rows, queries with full mantissas, all products of one score positive: row 0's score S is a sum of 128
+    products in three parts, row 1's one product near it, and no other row counts, so the output tanh((s0 - s1) / 2)
+    shows the score. Tensor cores truncate: at most 2^-23 of the sum so far a step, 8 steps of 16 dims, and the sum is
+    9/16 of S on average: 4.5. Smaller parts add 2^-8 of that; the factors and the difference round four times, by
+    half a unit each, some up and some down: below 6 units of 2^-23 S on average."""
+    p = Pool(BF16, QWEN, 16, [new], [new + 2], seed=new)
+    d, page = p.dim, p.table[0, 0]
+    k = bf16(p.rng.uniform(0.5, 1, (p.kvheads, d)) * 11.0)
+    p.host[0][:] = (k ^ 0x8000)[None, :, None]
+    p.host[0][page, :, 0] = k
+    one = np.zeros((p.kvheads, d), np.float32)
+    one[:, 0] = widen(k).sum(1)
+    p.host[0][page, :, 1] = bf16(one)
+    p.host[1][:] = 0
+    p.host[1][page, :, 0], p.host[1][page, :, 1] = 0x3F80, 0xBF80
+    p.put()
+    q = (1.5 + p.rng.uniform(0, 2.0**-8, (new, p.qheads * d))).astype(np.float32)
+    got = p.attend(q).reshape(new, p.qheads, d)
+    worst = []
+    for h in range(p.qheads):
+        kk = widen(p.host[0][page, h // (p.qheads // p.kvheads)]).astype(np.float64)
+        s = q.reshape(new, p.qheads, d)[:, h].astype(np.float64) @ kk[:2].T / np.sqrt(d)
+        out = np.tanh((s[:, 0] - s[:, 1]) / 2)
+        assert np.all(np.abs(s[:, 0] - s[:, 1]) < 3)
+        worst.append(np.abs(got[:, h, 0] - out) * 2 / (1 - out**2) / s[:, 0])
+    assert np.mean(worst) <= 6 * 2.0**-23, np.mean(worst) * 2**23
+    p.free()
