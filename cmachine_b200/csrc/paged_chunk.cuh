@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kPcThreads, 1) paged_chunk_kernel(const PagedC
         if (i == 0 || z.live > 128) {
             // ---- Q: this warp's 32 rows as two FP16 parts, scaled by the row's power of two
             float mine = 0.f;
-            constexpr int E = DIM / 32, QB = 32;  // rows whose loads are in flight together
+            constexpr int E = DIM / 32, QB = 16;  // rows whose loads are in flight together
             const long long q_at = r < z.rows ? (long long)(z.start + r / a.group) * a.q_stride + (z.h * a.group + r % a.group) * DIM : -1;
 #pragma unroll 1
             for (int first_k = 0; first_k < 32; first_k += QB) {

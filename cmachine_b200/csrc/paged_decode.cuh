@@ -298,11 +298,11 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             z.s = s;
             z.e = extents[s];
             const int a_head = units[s] / a.heads;
-            z.h = (begin - before) / a_head;
+            z.h = a.head0 + (begin - before) / a_head;
             z.rt = 0;
             z.tiles = tiles_of(z.e, 0);
             z.n = max(1, z.tiles.count);
-            z.from = before + z.h * a_head + kPdSegmentCost;
+            z.from = before + (z.h - a.head0) * a_head + kPdSegmentCost;
             while (z.from + z.n <= begin && (z.rt + 1) * R < z.e.count * a.group) {
                 z.tiles = tiles_of(z.e, ++z.rt);
                 z.from += z.n + kPdSegmentCost;
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     const int64_t half = (int64_t)v.pages * v.kvheads * v.page;
     int bad = 0;
     for (;;) {
-        const int s = seg.s, h = a.head0 + seg.h;
+        const int s = seg.s, h = seg.h;
         const PagedExtent e = seg.e;
         const PagedTiles tiles = seg.tiles;
         const int r0 = seg.rt * R, rows = e.count * a.group;  // row r of the KV head: new row r / group, head r % group
@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             __syncthreads();
             {
                 const volatile PdSegment &z = seg;
-                const int from = z.from, n = z.n, r0 = z.rt * R, rows = z.e.count * a.group, start = z.e.start, h = a.head0 + z.h;
+                const int from = z.from, n = z.n, r0 = z.rt * R, rows = z.e.count * a.group, start = z.e.start, h = z.h;
                 auto store_out = [&](int r, int d4, float4 y, float sum) {
                     const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);  // nothing seen: zeros
                     *reinterpret_cast<float4 *>(a.out + (long long)(start + (r0 + r) / a.group) * a.out_stride +
@@ -933,8 +933,8 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             z.from += z.n;
             if (++z.rt * R >= z.e.count * a.group) {
                 z.rt = 0;
-                if (++z.h == a.heads) {
-                    z.h = 0;
+                if (++z.h == a.head0 + a.heads) {
+                    z.h = a.head0;
                     do z.s++;
                     while (z.s < v.sequences && !units[z.s]);
                     if (z.s < v.sequences) z.e = extents[z.s];
