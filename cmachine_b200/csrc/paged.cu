@@ -21,12 +21,13 @@ constexpr int kRowThreads = 128;
 // Memory bound, and launch bound for single tokens. A warp takes kRowBatch new rows of one KV head
 // (a grid row each: no division per row) at a time, K and V of each, so that its loads are in
 // flight together. Measured: 42,298 rows of 128 as bytes written in 19 us (21 with one row at a
-// time, 21 with four; the codec's arithmetic bounds it), 204,656 BF16 rows read back in 52 us
-// (314 MB, 89 % of copy bandwidth; 61 with four).
+// time, 21 with four), 204,656 BF16 rows read back in 55 us (314 MB, 89 % of copy bandwidth; 65 with
+// four).
 constexpr int kRowBatch = 2, kReadBatch = 1;
 
 // Byte codec: scale = max|x| / 127 (1 for a zero row) and code = clamp(roundf(x / scale), +-127),
-// the divisions IEEE as in byte_cache.cu, so codes and scales are the ring's bit for bit. The row's
+// the divisions IEEE as in byte_cache.cu, so codes and scales are the ring's bit for bit (but for a row
+// whose max|x| / 127 underflows, which the ring refuses: zeros with scale 0 here). The row's
 // values are asked for before its page id, which they do not need.
 template <int KIND, int DIM>
 __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, const float *k, const float *vals,
@@ -210,8 +211,8 @@ bool nothing(const PagedView &v) { return !v.sequences || !v.rows || !v.max_new;
 
 // Sequences with at most this many query rows a KV head are the decode kernel's, in row tiles of 8, 16
 // or 32, those with more the chunk kernel's. Measured with 32 sequences of 4096 rows, 8 KV heads of 128
-// (decode kernel, chunk kernel): 32 rows of BF16 177 and 400 us, 64 rows 339 and 403; of bytes 145 and
-// 230 us, 64 rows 271 and 232.
+// (decode kernel, chunk kernel): 32 rows of BF16 183 and 425 us, 64 rows 353 and 428; of bytes 154 and
+// 253 us, 64 rows 307 and 254.
 int few_rows(int kind) { return kind == kPagedBf16 ? 64 : 32; }
 
 // Most rows of one sequence that the queries of one tile can see.

@@ -13,8 +13,8 @@
 // the tensor cores run the other's products. A ring of three operand tiles holds
 // K(t + 1), V(t) and the next.
 //
-// Measured: 4096 new rows over 32,768 byte rows (12 query heads, 2 KV heads) in 1.52 ms, 508 TFLOP/s
-// of result and 1.02 PFLOP/s of products; 512 over 4,609 in 46 us. A tile takes 7,400 cycles, of
+// Measured: 4096 new rows over 32,768 byte rows (12 query heads, 2 KV heads) in 1.53 ms, 504 TFLOP/s
+// of result and 1.01 PFLOP/s of products; 512 over 4,609 in 48 us. A tile takes 7,400 cycles, of
 // which the MMAs are 4,100: the chain of one half (its maximum 700, its weights 3,700, the rest of
 // P V 900, Q K^T 1,450) bounds it. The weights' 128 exponentials alone are 1,024 cycles of the
 // special-function unit, and their broadcast reads of the row scales from shared memory wait behind
@@ -310,8 +310,8 @@ struct PcItem {
 };
 // Finds it, the same in every thread, or returns false. Every CTA counts the row tiles of all sequences (their
 // extents are on the device) and takes the splits for what there is, not for the declared maxima: with one chunk of
-// 512 rows beside 63 single tokens that had left the chunk on 24 SMs (196 us; 46 alone), and an empty CTA takes
-// 3 us of an SM. `sh` is shared memory that the caller uses for nothing else before its next barrier.
+// 512 rows beside 63 single tokens that had left the chunk on 24 SMs (196 us, now 95; 48 alone), and an empty CTA
+// takes 3 us of an SM. `sh` is shared memory that the caller uses for nothing else before its next barrier.
 __device__ __forceinline__ bool pc_item(const PagedChunkArgs &a, int *sh, PcItem &it) {
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;

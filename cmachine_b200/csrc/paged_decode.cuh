@@ -18,8 +18,8 @@
 // straight into registers instead left the compiler spilling loads in flight, which made
 // every one of them a wait: 64 sessions of up to 8192 byte rows took 66 us so.
 //
-// Measured (attention alone): 64 sessions of up to 8192 byte rows, 70 MB, 25 us; 16 of 20,000 to
-// 32,768 BF16 rows, 443 MB, 80 us (87 % of copy bandwidth); one of 32,749 byte rows, 17 MB, 20 us.
+// Measured (attention alone): 63 sessions of up to 8192 byte rows, 70 MB, 26 us; 16 of 20,000 to
+// 32,768 BF16 rows, 443 MB, 83 us (84 % of copy bandwidth); one of 32,749 byte rows, 17 MB, 21 us.
 // Of the first, the loop takes 12 us at about the memory's rate; the rest is the start (finding the
 // stretch, the first rows and queries: 4 us), the merges (2 us) and the launch.
 //

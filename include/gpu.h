@@ -154,22 +154,26 @@ typedef struct {
     int table_stride;
 } TcmPagedBatch;
 /* All three return 0 when launched, or -1 with a message on stderr for sizes,
- * strides or alignment they do not take, and launch nothing; they never wait for
- * the device. What only the device can see is reported in *status (a device word
- * the kernels OR into and never clear; may be NULL): 1 a row was appended that
- * the pool cannot hold, 2 a page id outside the pool for a row that was needed, 4 extents that
- * do not fit rows, max_new, max_length or the table, 8 a wait inside the attention
- * ran out (qwen_b200_wait_limit): its outputs are not to be used. A row without a page is not
- * written, reads as zeros and is visible to no query; a sequence with bad extents
- * is left out, its rows of the outputs untouched. Row buffers are FP32, strides
- * count floats from one row to the next (multiples of 4), buffers are 16-byte
- * aligned; rows of no sequence are neither read nor written.
+ * strides or alignment they do not take, and launch nothing; they do not wait for
+ * the device, but for a call of attention whose scratch grows. What only the device
+ * can see is reported in *status (a device word, 4-byte aligned, that the kernels OR
+ * into and never clear; may be NULL): 1 a row was appended that the pool cannot hold,
+ * 2 a page id outside the pool for a row that was needed, 4 extents that do not fit
+ * rows, max_new, max_length or the table, 8 a wait inside the attention ran out
+ * (qwen_b200_wait_limit): its outputs are not to be used. A row without a page is
+ * not written, reads as zeros and is visible to no query; a sequence with bad
+ * extents is left out, its rows of the outputs untouched. Row buffers are FP32,
+ * strides count floats from one row to the next (multiples of 4), buffers are
+ * 16-byte aligned; rows of no sequence are neither read nor written.
  *
  * Write the new rows: k and v hold [kvheads][dim] a row, `stride` apart (both). A
  * row of one KV head with a non-finite value, or one whose stored form would be
  * infinite (BF16 from 2^128 - 2^119 on, bytes FP32's largest number), is stored as
- * zeros and reported. New rows at negative places (count > length) are skipped. What two sequences of one call that
- * write the same row of a shared page leave there is unspecified. */
+ * zeros and reported; bytes hold the ring's codes and scales, but for a row whose
+ * max|x| / 127 underflows: the ring refuses it, here it is stored as zeros with
+ * scale 0. New rows at negative places (count > length) are skipped. What two
+ * sequences of one call that write the same row of a shared page leave there is
+ * unspecified. */
 int gpu_paged_append(const TcmPagedCache *, const TcmPagedBatch *, const float *k, const float *v, long long stride,
                      int *status);
 /* Read the same rows back as the FP32 values they stand for. */
@@ -179,9 +183,19 @@ int gpu_paged_read(const TcmPagedCache *, const TcmPagedBatch *, float *k, float
  * q . k / sqrt(dim). q and out hold [qheads][dim] a row; query head h reads KV head
  * h / (qheads / kvheads); at most 8 query heads per KV head. A query that sees no
  * row gets zeros. Outputs that see a row with a non-finite value are unspecified;
- * no other output is touched by it. Deterministic. Scratch belongs to the handle and grows on
- * demand (the growing call allocates): calls with one handle follow one another on
- * the library's stream, and another thread needs a handle of its own. */
+ * no other output is touched by it.
+ * Precision: FP32 in and out, for magnitudes of queries and rows up to 1e30. The
+ * tensor cores get queries and weights as parts of 22 bits or more: over byte rows
+ * queries are 23 bits of the row's largest element for few new rows and FP16 pairs
+ * for chunks, weights FP16 pairs; over BF16 rows three BF16 parts for few new rows,
+ * FP16 pairs for chunks. A weight's step is 2^-28 of the size (max |v|) of the row
+ * that counts most for the query, whatever rows within 2^100 of it hold, seen or
+ * not. At most 32 truncating steps of 16 rows follow one another; longer sums are
+ * FP32, rounded to nearest.
+ * Deterministic, but a sequence's result depends on its batch in the last bits.
+ * Scratch belongs to the handle and grows on demand, to some 165 MB at most; a call
+ * that grows it allocates and waits for the device. Calls with one handle follow one
+ * another on the library's stream, and another thread needs a handle of its own. */
 int gpu_paged_attention(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
                         const TcmPagedCache *, const TcmPagedBatch *, int qheads, int window, int sinks, int *status);
 
