@@ -623,10 +623,11 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
                 if (__any_sync(0xffffffffu, moves)) {
                     float shrink = 1.f;
                     if constexpr (kBytes) {
+                        const int was = v_exp;
+                        const bool first_rows = v_top == 0.f;
                         if (!wide && v_most > v_top) {  // the same in every lane
-                            const int was = v_exp;
                             v_exp = max(-100, exponent_of(v_most) + 1);
-                            shrink = v_top == 0.f ? 0.f : power_of_two(was - v_exp);
+                            shrink = first_rows ? 0.f : power_of_two(was - v_exp);
                             v_top = power_of_two(v_exp);
                             v_factor = power_of_two(kPdWeightTop - v_exp);
                         }
@@ -637,8 +638,9 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
 #pragma unroll
                                 for (int mt = 0; mt < M; mt++)
 #pragma unroll
-                                    for (int r = 0; r < RL; r++)
-                                        own_scale[warp][16 * mt + 8 * r + g] = make_float2((float)v_exp, m[mt][r] + ((float)v_exp + kPdSlack));
+                                    for (int r = 0; r < RL; r++)  // the steps before this one were bounded by the scale before it
+                                        own_scale[warp][16 * mt + 8 * r + g] =
+                                            make_float2((float)v_exp, first_rows ? -INFINITY : m[mt][r] + ((float)was + kPdSlack));
                             __syncwarp();
                         }
                     }

@@ -299,3 +299,25 @@ def test_scores_of_one_sign(new):
         worst.append(np.abs(got[:, h, 0] - out) * 2 / (1 - out**2) / s[:, 0])
     assert np.mean(worst) <= 6 * 2.0**-23, np.mean(worst) * 2**23
     p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("power", [30, 60])
+@pytest.mark.parametrize("news,length,places", [(4, 600, [598]), (4, 600, [300, 598]), (2, 700, [0, 699]), (12, 500, [493])])
+def test_a_huge_row_late_in_a_warp_s_steps(kind, power, news, length, places):
+    """So many sequences that no segment is split: a warp meets the huge row after steps of ordinary ones, whose sums
+    it must neither lose nor count as huge."""
+    p = Pool(kind, (16, 8, 64), 16, [news] * 40, [length] * 40, seed=power + news)
+    for s in range(40):
+        for place in places:
+            at = (p.table[s, place // 16], slice(None), place % 16)
+            if kind == BYTES:
+                p.scales[1][at] *= np.float32(2.0**power)
+            else:
+                p.host[1][at] = np.where(p.host[1][at] & 0x7F80, p.host[1][at] + (power << 7), 0)
+    p.put()
+    p.values = [p.values(0), p.values(1)].__getitem__  # once, not for each sequence
+    q = p.queries()
+    check_by_query(p, p.attend(q), q)
+    assert p.flags() == 0
+    p.free()
