@@ -67,6 +67,16 @@ class PagedBatch(Structure):
         ("starts", c_void_p), ("lengths", c_void_p), ("table", c_void_p), ("table_stride", c_int)]
 
 
+class HeadRotation(Structure):
+    """TcmHeadRotation (include/gpu.h): qnorm and knorm are device pointers or None."""
+    _fields_ = [("qnorm", c_void_p), ("knorm", c_void_p), ("eps", c_float), ("theta", c_float), ("rotary", c_int)]
+
+
+class Sampling(Structure):
+    """TcmSampling (include/gpu.h); the calls take device arrays of it."""
+    _fields_ = [("temperature", c_float), ("top_k", c_int), ("top_p", c_float), ("min_p", c_float)]
+
+
 def qwen_shape(layers: int = 28, max_position: int = 32768) -> Shape:
     """Qwen2.5-1.5B geometry (hidden 1536, 12/2 heads of 128, MLP 8960, vocab 151936)."""
     return Shape(1536, layers, 12, 2, 128, 8960, 151936, max_position, 1e-6, 1e6)
@@ -148,6 +158,12 @@ def _declare(L, strict: bool = True):
         "gpu_paged_read": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), P, P, c_longlong, P]),
         "gpu_paged_attention": (c_int, [P, P, c_longlong, P, c_longlong, POINTER(PagedCache), POINTER(PagedBatch), c_int,
                                         c_int, c_int, P]),
+        "gpu_paged_rotate_append": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(HeadRotation), P, c_longlong, P, P,
+                                            P, c_longlong, c_int, P]),
+        "gpu_paged_bounds": (c_int, [POINTER(PagedCache), POINTER(PagedBatch), P, P]),
+        "gpu_paged_sparse_attention": (c_int, [P, P, c_longlong, P, c_longlong, POINTER(PagedCache), POINTER(PagedBatch), P,
+                                               c_int, c_int, c_int, c_int, P, P]),
+        "gpu_sample": (c_int, [P, P, P, P, P, c_longlong, c_int, c_int, P, P, P]),
         # include/bounded_cache.h
         "ring_open": (c_int, [P, P, P, c_int, c_int, c_int, c_int, c_int]),
         "ring_begin": (c_int, [P, c_int]), "ring_abort": (c_int, [P]), "ring_finish": (c_int, [P]),

@@ -7,7 +7,7 @@
 #include "paged.cuh"
 #include "paged_decode.cuh"
 #include "paged_chunk.cuh"
-#include "kernels.h"
+#include "paged_host.cuh"
 #include "../../include/qwen_b200.h"
 #include "../../include/tcm_seeded.h"
 #include <math.h>
@@ -74,8 +74,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, 
                     zero = fmaf(y[c], 0.f, zero);  // NaN once a value is not finite
                     m = fmaxf(m, fabsf(y[c]));
                 }
-                // BF16 rounds from 2^128 - 2^119 on to infinity; 127 times FP32's largest number over 127 is one too.
-                if (!__all_sync(0xffffffffu, zero == 0.f && m < (KIND == kPagedBytes ? 0x1.fffffep127f : 0x1.ffp127f))) {
+                if (!__all_sync(0xffffffffu, zero == 0.f && paged_holds<KIND>(m))) {
                     bad |= kPagedNonFinite;
                     m = 0.f;
 #pragma unroll
@@ -86,23 +85,8 @@ __global__ void __launch_bounds__(kRowThreads) paged_append_kernel(PagedView v, 
                 if constexpr (KIND == kPagedBytes) {
                     m = warp_max(m);
                     const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
-                    // A row so small that m / 127 underflows stands for zeros (scale 0, codes 0).
-                    // The quotient by a reciprocal is within 5e-5 of the divided one; only where it comes near a
-                    // half does the division decide (all of them by division: 26 us instead of 20 for 42,000 rows).
-                    // The largest scale, 2^128 / 127, still has a reciprocal.
                     int8_t q[E];
-                    const float up = __fdividef(1.f, scale);
-                    bool near_half = false;
-#pragma unroll
-                    for (int c = 0; c < E; c++) {
-                        const float quotient = y[c] * up, code = rintf(quotient);
-                        near_half |= !(fabsf(quotient - code) <= 0.4999f);
-                        q[c] = (int8_t)fminf(127.f, fmaxf(-127.f, code));
-                    }
-                    if (near_half)
-#pragma unroll
-                        for (int c = 0; c < E; c++)
-                            q[c] = scale > 0.f ? (int8_t)fminf(127.f, fmaxf(-127.f, roundf(__fdiv_rn(y[c], scale)))) : (int8_t)0;
+                    paged_codes(y, scale, q);
                     if constexpr (E == 4)
                         *reinterpret_cast<char4 *>(static_cast<int8_t *>(dst) + to) = make_char4(q[0], q[1], q[2], q[3]);
                     else
@@ -167,48 +151,6 @@ __global__ void __launch_bounds__(kRowThreads) paged_read_kernel(PagedView v, fl
 }
 
 // ---------------------------------------------------------------- host
-int refuse(const char *call, const char *why) {
-    fprintf(stderr, "%s: %s\n", call, why);
-    return -1;
-}
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
-// The call's descriptors as a view; 0, or -1 with a message.
-int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBatch *b, const int *status, PagedView *v) {
-    if (!c || !b) return refuse(call, "no cache or no batch");
-    if (c->kind != kPagedBf16 && c->kind != kPagedBytes) return refuse(call, "kind is 2 (BF16) or 3 (bytes)");
-    if (c->dim != 64 && c->dim != 128) return refuse(call, "dim is 64 or 128");
-    if (c->pages < 1 || c->page < 1 || c->page > 65536 || c->kvheads < 1 || c->kvheads > 1024)
-        return refuse(call, "pages, page or kvheads out of range");
-    if (!c->keys || !c->values || !aligned16(c->keys) || !aligned16(c->values))
-        return refuse(call, "keys and values are 16-byte aligned device memory");
-    if (c->kind == kPagedBytes && (!c->scales || ((uintptr_t)c->scales & 3))) return refuse(call, "a byte cache has scales");
-    if (b->sequences < 0 || b->sequences > 65535 || b->rows < 0 || b->max_new < 0 || b->max_length < 0 ||
-        b->max_length > 1 << 30)
-        return refuse(call, "sequences, rows, max_new or max_length out of range");
-    if (b->sequences && (!b->starts || !b->lengths || !b->table || b->table_stride < 1))
-        return refuse(call, "a batch has starts, lengths and a table");
-    if (((uintptr_t)b->starts | (uintptr_t)b->lengths | (uintptr_t)b->table) & 3)
-        return refuse(call, "starts, lengths and table are 4-byte aligned");
-    if ((uintptr_t)status & 3) return refuse(call, "status is 4-byte aligned");
-    const int max_new = b->max_new < b->rows ? b->max_new : b->rows;
-    // No sequence is longer than its table either.
-    const long long held = (long long)b->table_stride * c->page;
-    const int max_length = b->max_length < held ? b->max_length : (int)held;
-    if ((long long)max_new * c->kvheads > 0x7fffffff / 8) return refuse(call, "too many new rows for one call");
-    *v = PagedView{c->kind, c->pages, c->page, c->kvheads, c->dim, c->keys, c->values, c->scales, b->sequences, b->rows,
-                   max_new, max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0};
-    paged_divider(v);
-    return 0;
-}
-int check_rows(const char *call, const void *p, long long stride, int heads, int dim) {
-    if (!p || !aligned16(p)) return refuse(call, "row buffers are 16-byte aligned device memory");
-    if (stride < (long long)heads * dim || stride % 4) return refuse(call, "a row stride is a multiple of 4 and holds a row");
-    return 0;
-}
-// Nothing to do: no sequence, or none that may have a new row.
-bool nothing(const PagedView &v) { return !v.sequences || !v.rows || !v.max_new; }
-
 // Sequences with at most this many query rows a KV head are the decode kernel's, in row tiles of 8, 16
 // or 32, those with more the chunk kernel's. Measured with 32 sequences of 4096 rows, 8 KV heads of 128
 // (decode kernel, chunk kernel): 32 rows of BF16 183 and 425 us, 64 rows 353 and 428; of bytes 154 and
@@ -245,7 +187,7 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
         for (a.head0 = 0; a.head0 < all.kvheads; a.head0 += heads) {
             a.heads = all.kvheads - a.head0 < heads ? all.kvheads - a.head0 : heads;
             a.v.sequences = all.sequences - s < most ? all.sequences - s : most;
-            a.v.starts = all.starts + s;
+            a.v.starts = all.starts + ((int64_t)s << all.pairs);
             a.v.lengths = all.lengths + s;
             a.v.table = all.table + (int64_t)s * all.table_stride;
             launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
@@ -297,22 +239,6 @@ template <int KIND, int DIM> void chunk_launch(TcmGpu *gpu, PagedChunkArgs a, Pa
         launch(paged_chunk_join_kernel<DIM>, dim3((unsigned)(joins < most ? joins : most)), dim3(kPcJoinThreads), 0, stream(), true, a);
 }
 
-unsigned blocks_of(long long items, int a_block) {
-    const long long blocks = (items + a_block - 1) / a_block;
-    return (unsigned)(blocks < 4096 ? blocks : 4096);
-}
-
-#define PAGED_DISPATCH(view, call)                                      \
-    do {                                                                \
-        if ((view).kind == kPagedBf16) {                                \
-            if ((view).dim == 64) { call(kPagedBf16, 64); }             \
-            else { call(kPagedBf16, 128); }                             \
-        } else {                                                        \
-            if ((view).dim == 64) { call(kPagedBytes, 64); }            \
-            else { call(kPagedBytes, 128); }                            \
-        }                                                               \
-    } while (0)
-
 // gpu_paged_attention, and its self-check.
 int attention(const char *name, TcmGpu *gpu, float *out, long long out_stride, const float *q, long long q_stride,
               const TcmPagedCache *cache, const TcmPagedBatch *batch, int qheads, int window, int sinks, int *status,
@@ -346,6 +272,12 @@ int attention(const char *name, TcmGpu *gpu, float *out, long long out_stride, c
 }
 
 }  // namespace
+
+void paged_decode_rows(TcmGpu *gpu, const PagedDecodeArgs &args) {
+#define CALL(K, D) decode_launch<K, D>(gpu, args)
+    PAGED_DISPATCH(args.v, CALL);
+#undef CALL
+}
 
 void set_wait_limit_paged(unsigned long long ns) { set_module_wait_limit(ns); }
 

@@ -22,7 +22,7 @@ struct TcmGpu {
     unsigned *attn_counters;
     size_t attn_part_floats;
     int attn_kv;
-    PagedScratch paged[2];  // of the paged attention's decode and chunk kernels (grown on demand)
+    PagedScratch paged[3];  // of the paged attention's decode and chunk kernels, and of the choice of pages (grown on demand)
 };
 
 namespace tcm {

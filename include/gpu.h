@@ -199,6 +199,81 @@ int gpu_paged_read(const TcmPagedCache *, const TcmPagedBatch *, float *k, float
 int gpu_paged_attention(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
                         const TcmPagedCache *, const TcmPagedBatch *, int qheads, int window, int sinks, int *status);
 
+/* What stands between a projection and the cache: the queries and keys of each head
+ * normed (y = x / sqrt(mean x^2 + eps) times qnorm or knorm, [dim] device floats;
+ * NULL: not normed) and then rotated to their row's place p: with R = rotary, elements
+ * d and d + R / 2, d < R / 2, turn by the angle p theta^(-2d / R); elements from R on
+ * stay. rotary is a multiple of 4, at most dim; 0 rotates nothing. */
+typedef struct {
+    const float *qnorm, *knorm;
+    float eps, theta;
+    int rotary;
+} TcmHeadRotation;
+/* gpu_paged_append of rows as a projection leaves them: norms and rotates each new row's
+ * queries (into q_out, which may be q with the same stride) and keys, and writes keys
+ * and values to the pool as gpu_paged_append does, with its limits, status bits and
+ * treatment of rows that the pool cannot hold. q, k and v share one stride; they may be
+ * parts of one row. Queries of a row without a page, or at a negative place, are
+ * written all the same. Norms, angles and rotations are carried in 64 bits and rounded
+ * once to FP32, from which the stored form is taken (gpu_rope's angles are FP32: at
+ * place 32768 the two differ by up to 2e-3). A query head with a non-finite value is
+ * unspecified, the others are not touched by it. eps is finite and not negative, theta
+ * finite and positive; norms are 8-byte aligned. */
+int gpu_paged_rotate_append(const TcmPagedCache *, const TcmPagedBatch *, const TcmHeadRotation *, float *q_out,
+                            long long q_out_stride, const float *q, const float *k, const float *v, long long stride,
+                            int qheads, int *status);
+/* Bounds of the keys of each page, for gpu_paged_sparse_attention: bounds is
+ * [pages][kvheads][2][dim] BF16 (16-byte aligned), the least and the largest value of
+ * every key element over the page's rows, rounded down and up. The call brings every
+ * page that holds a new row of the batch up to date, from all rows of the page below its
+ * sequence's length; others are not touched. Call it behind each append (a batch whose
+ * counts are the lengths does whole sequences). A NaN bounds nothing. What two
+ * sequences of one call with different lengths leave of a page that both bring rows of
+ * is unspecified. */
+int gpu_paged_bounds(const TcmPagedCache *, const TcmPagedBatch *, uint16_t *bounds, int *status);
+/* gpu_paged_attention of each query over few pages of its sequence. The query at place p
+ * stands in page P = p / page of its sequence. Where P < blocks it sees all rows j <= p.
+ * Otherwise every KV head has `blocks` pages: the `first` first ones, the `recent` last
+ * ones up to P, and of those between the ones whose score
+ *     max over the KV head's query heads of sum_d max(q_d low_d, q_d high_d)
+ * is largest, an upper bound of the products of the page's keys with its queries; equal
+ * scores go to the lower page, a score that is NaN is lowest, and so is a page without
+ * a page id in the pool. Scores are summed in 64 bits, so the choice is that of exact
+ * arithmetic unless two scores agree to some 15 digits. blocks >= first + recent,
+ * first >= 0, recent >= 1, blocks <= 8192; sequences of more than 16384 pages are
+ * reported as bad extents (4) and left out. selected may be NULL; else it is
+ * [rows][kvheads][blocks] and gets the pages of every new row in ascending order, -1
+ * behind the last (rows at negative places: -1). Contract, limits, precision and scratch
+ * as gpu_paged_attention (bounds of pages below P must be up to date: a stale or wild
+ * one changes the choice, nothing else); its scratch is some 100 MB at most more. */
+int gpu_paged_sparse_attention(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
+                               const TcmPagedCache *, const TcmPagedBatch *, const uint16_t *bounds, int qheads, int blocks,
+                               int first, int recent, int *selected, int *status);
+
+/* ---- Sampling (no counterpart in the reference; gpu_top2 is the greedy readout) ----
+ * Each row's settings, in device memory: temperature >= 0 (0: the largest logit, the
+ * lowest id among equals), top_k (<= 0: off), top_p (>= 1: off), min_p (<= 0: off). */
+typedef struct {
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+} TcmSampling;
+/* Draw one token a row: logits[r * stride .. + vocab), FP32, -infinity for tokens that
+ * may not come. With w_i = exp((logit_i - largest) / temperature) and tokens ranked by
+ * logit, equal ones by lower id, kept is the least of: the top_k first; of those, the
+ * fewest first ones whose w add up to top_p of theirs or more (one at least); those with
+ * w >= min_p. The token is the first kept one, by id, at which the sum of the kept w
+ * passes uniforms[r] in [0, 1) times their whole sum. ids, logprobs (the log of the
+ * token's share of that sum) and kept (how many are) are [rows]; logprobs and kept may
+ * be NULL. stride >= vocab, or 0: every row draws from the same logits. vocab is 1 to
+ * 524288. Weights and sums are carried to 2^-30 of themselves or better and added
+ * exactly, in any order, so the same call gives the same tokens. A row that has no
+ * token gets id -1, logprob 0, kept 0, and a bit of *status (as above; may be NULL): 1 a
+ * logit is NaN or +infinity, 2 no logit is above -infinity, 4 its settings or its uniform
+ * are out of range. Returns 0 when launched, or -1 with a message on stderr. */
+int gpu_sample(TcmGpu *, int *ids, float *logprobs, int *kept, const float *logits, long long stride, int rows, int vocab,
+               const TcmSampling *params, const float *uniforms, int *status);
+
 #ifdef __cplusplus
 }
 #endif
