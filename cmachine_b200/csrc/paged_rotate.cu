@@ -16,7 +16,7 @@
 namespace tcm {
 namespace {
 
-constexpr int kTurnThreads = 256, kTurnRows = 8;  // rows a CTA forms the cosines of together, at most
+constexpr int kTurnTile = 8;  // rows of a CTA at a time, where there are many
 
 struct PagedTurnArgs {
     PagedView v;
@@ -25,132 +25,171 @@ struct PagedTurnArgs {
     long long stride, q_out_stride;
     const float *qnorm, *knorm;
     double eps;
-    int qheads, half, tile;  // half: pairs that turn; tile: rows of a CTA at a time
+    int qheads, half;  // half: pairs that turn
     int *status;
     double rate[64];  // half turns a place: theta^(-2d/R) / pi
 };
 
-template <int KIND, int DIM>
-__global__ void __launch_bounds__(kTurnThreads) paged_turn_kernel(const __grid_constant__ PagedTurnArgs a) {
-    constexpr int L = DIM / 4, H = 32 / L, W = kTurnThreads / 32;  // lanes a head, heads a warp, warps
-    __shared__ __align__(16) double2 turn[kTurnRows][DIM / 2];     // cosine, sine
+// x over the L lanes of a head, of R = 4 rows at once: two exchanges leave every lane with one row's, so that a quarter
+// of the warp adds up, and forms the root of, a row each. turn_row says which, turn_of brings a row's value back.
+template <int L> __device__ __forceinline__ double turn_sum(const double (&x)[4], int lane) {
+    const bool far = lane & (L / 2), odd = lane & (L / 4);
+    const double y0 = (far ? x[2] : x[0]) + __shfl_xor_sync(0xffffffffu, far ? x[0] : x[2], L / 2);
+    const double y1 = (far ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, far ? x[1] : x[3], L / 2);
+    double y = (odd ? y1 : y0) + __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, L / 4);
+#pragma unroll
+    for (int o = L / 8; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    return y;
+}
+template <int L> __device__ __forceinline__ double turn_of(double y, int row, int lane) {
+    return __shfl_sync(0xffffffffu, y, (lane & ~(L - 1)) + (row >> 1) * (L / 2) + (row & 1) * (L / 4));
+}
+template <int L> __device__ __forceinline__ double turn_sum(const double (&x)[1], int) {
+    double y = x[0];
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    return y;
+}
+
+// R rows of a head at a time. R = 4: tiles of kTurnTile rows, their cosines in shared memory. R = 1: single tokens; a
+// warp forms the cosines that it needs while its row is on the way, and waits for no other.
+template <int KIND, int DIM, int R>
+__global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 1 : 3) paged_turn_kernel(const __grid_constant__ PagedTurnArgs a) {
+    constexpr int T = R == 1 ? 512 : 256, L = DIM / 4, H = 32 / L, W = T / 32;  // threads; lanes a head, heads a warp, warps
+    constexpr int kTile = R == 1 ? 1 : kTurnTile;
+    __shared__ __align__(16) double2 turn[R == 1 ? 1 : kTile][R == 1 ? 1 : DIM / 2];  // cosine, sine
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / L, pair = 2 * (lane % L), s = blockIdx.y;
-    const unsigned mine = L == 32 ? 0xffffffffu : 0xffffu << (lane & 16);
     // Where the lane's two pieces of two elements lie in a head.
     const bool turns = pair < a.half;
     const int e0 = turns ? pair : 2 * pair, e1 = turns ? a.half + pair : 2 * pair + 2;
-    const int heads = a.qheads + 2 * v.kvheads, groups = (heads + H - 1) / H;
+    const int heads = a.qheads + 2 * v.kvheads;
     pdl_trigger();
     pdl_wait();
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
-    for (int first = blockIdx.x * a.tile; first < e.count; first += gridDim.x * a.tile) {
-        const int rows = min(a.tile, e.count - first), items = rows * groups, place = e.length - e.count + first;
-        struct Item {
-            float2 x[2];
-            int64_t row;  // of the pool, for keys and values
-            int head, at;
-        };
-        auto load = [&](int it) {
-            Item r;
-            r.at = it / groups;
-            r.head = (it - r.at * groups) * H + sub;
-            r.row = -1;
-            r.x[0] = r.x[1] = make_float2(0.f, 0.f);
-            if (it < items && r.head < heads) {
-                const bool key = r.head < a.qheads + v.kvheads;
-                const float *src = r.head < a.qheads ? a.q + r.head * DIM
-                                   : key             ? a.k + (r.head - a.qheads) * DIM
-                                                     : a.values + (r.head - a.qheads - v.kvheads) * DIM;
-                src += (long long)(e.start + first + r.at) * a.stride;
-                r.x[0] = *reinterpret_cast<const float2 *>(src + e0);
-                r.x[1] = *reinterpret_cast<const float2 *>(src + e1);
-                const int j = place + r.at;
-                if (r.head >= a.qheads && j >= 0 &&
-                    (r.row = paged_slot(&v, s, j, r.head - a.qheads - (key ? 0 : v.kvheads))) < 0)
-                    bad |= kPagedBadPage;
+    for (int first = blockIdx.x * kTile; first < e.count; first += gridDim.x * kTile) {
+        const int rows = min(kTile, e.count - first), place = e.length - e.count + first;
+        if constexpr (R > 1) {
+            for (int i = tid; i < rows * (DIM / 2); i += T) {
+                const int r = i / (DIM / 2), d = i % (DIM / 2);
+                double sn, cs;
+                if (d < a.half) {
+                    sincospi((double)(place + r) * a.rate[d], &sn, &cs);
+                    turn[r][d] = make_double2(cs, sn);
+                }
             }
-            return r;
-        };
-        Item next = load(warp);
-        for (int i = tid; i < rows * (DIM / 2); i += kTurnThreads) {
-            const int r = i / (DIM / 2), d = i % (DIM / 2);
-            double sn, cs;
-            if (d < a.half) {
-                sincospi((double)(place + r) * a.rate[d], &sn, &cs);
-                turn[r][d] = make_double2(cs, sn);
-            }
+            __syncthreads();
         }
-        __syncthreads();
-        for (int it = warp; it < items; it += W) {
-            const Item c = next;
-            next = load(it + W);
-            const bool there = c.head < heads, is_q = c.head < a.qheads, is_k = !is_q && c.head < a.qheads + v.kvheads;
-            float y[4] = {c.x[0].x, c.x[0].y, c.x[1].x, c.x[1].y};
-            if (__any_sync(0xffffffffu, there && (is_q || is_k))) {
-                double z[4] = {y[0], y[1], y[2], y[3]};
-                const float *norm = is_q ? a.qnorm : is_k ? a.knorm : nullptr;
-                if (a.qnorm || a.knorm) {
-                    double sum = z[0] * z[0] + z[1] * z[1] + (z[2] * z[2] + z[3] * z[3]);
+        for (int group = warp; group * H < heads; group += W) {
+            const int head = group * H + sub, kv_head = head - a.qheads;
+            const bool there = head < heads, is_q = kv_head < 0, is_k = !is_q && kv_head < v.kvheads;
+            const bool moves = there && (is_q || is_k);
+            const int h = is_k ? kv_head : kv_head - v.kvheads;  // of the pool
+            const float *src = is_q ? a.q + head * DIM : (is_k ? a.k : a.values) + h * DIM;
+            const float *norm = !moves ? nullptr : is_q ? a.qnorm : a.knorm;
+            const bool any_moves = __any_sync(0xffffffffu, moves), any_norm = __any_sync(0xffffffffu, norm != nullptr);
+            const bool any_stored = __any_sync(0xffffffffu, there && !is_q);
+            for (int r0 = 0; r0 < rows; r0 += R) {
+                float y[R][4];
 #pragma unroll
-                    for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (norm) {
-                        const double r = rsqrt(sum * (1.0 / DIM) + a.eps);
-                        const float2 w0 = *reinterpret_cast<const float2 *>(norm + e0);
-                        const float2 w1 = *reinterpret_cast<const float2 *>(norm + e1);
-                        z[0] *= r * w0.x, z[1] *= r * w0.y, z[2] *= r * w1.x, z[3] *= r * w1.y;
+                for (int i = 0; i < R; i++) {
+                    float2 x0 = make_float2(0.f, 0.f), x1 = x0;
+                    if (there && (R == 1 || r0 + i < rows)) {
+                        const float *x = src + (long long)(e.start + first + r0 + i) * a.stride;
+                        x0 = *reinterpret_cast<const float2 *>(x + e0);
+                        x1 = *reinterpret_cast<const float2 *>(x + e1);
+                    }
+                    y[i][0] = x0.x, y[i][1] = x0.y, y[i][2] = x1.x, y[i][3] = x1.y;
+                }
+                if (any_moves) {
+                    double2 t0 = make_double2(1.0, 0.0), t1 = t0;
+                    if constexpr (R == 1)
+                        if (turns) {
+                            sincospi((double)place * a.rate[pair], &t0.y, &t0.x);
+                            sincospi((double)place * a.rate[pair + 1], &t1.y, &t1.x);
+                        }
+                    double root = 1.0;
+                    float2 w0 = make_float2(1.f, 1.f), w1 = w0;
+                    if (any_norm) {
+                        if (norm) {
+                            w0 = *reinterpret_cast<const float2 *>(norm + e0);
+                            w1 = *reinterpret_cast<const float2 *>(norm + e1);
+                        }
+                        double sum[R];
+#pragma unroll
+                        for (int i = 0; i < R; i++) {
+                            const double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                            sum[i] = z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3);
+                        }
+                        root = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
+                    }
+#pragma unroll
+                    for (int i = 0; i < R; i++) {
+                        double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                        if (any_norm) {
+                            double r = root;
+                            if constexpr (R > 1) r = turn_of<L>(root, i, lane);
+                            if (norm) z0 *= r * w0.x, z1 *= r * w0.y, z2 *= r * w1.x, z3 *= r * w1.y;
+                        }
+                        if (turns && moves) {
+                            if constexpr (R > 1) t0 = turn[min(r0 + i, kTile - 1)][pair], t1 = turn[min(r0 + i, kTile - 1)][pair + 1];
+                            const double u0 = z0, u1 = z1;
+                            z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
+                            z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
+                        }
+                        if (moves) y[i][0] = (float)z0, y[i][1] = (float)z1, y[i][2] = (float)z2, y[i][3] = (float)z3;
                     }
                 }
-                if (turns && (is_q || is_k)) {
-                    const double2 t0 = turn[c.at][pair], t1 = turn[c.at][pair + 1];
-                    const double a0 = z[0], a1 = z[1], b0 = z[2], b1 = z[3];
-                    z[0] = a0 * t0.x - b0 * t0.y, z[1] = a1 * t1.x - b1 * t1.y;
-                    z[2] = b0 * t0.x + a0 * t0.y, z[3] = b1 * t1.x + a1 * t1.y;
+                if (there && is_q)
+#pragma unroll
+                    for (int i = 0; i < R; i++)
+                        if (R == 1 || r0 + i < rows) {
+                            float *dst = a.q_out + (long long)(e.start + first + r0 + i) * a.q_out_stride + head * DIM;
+                            *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[i][0], y[i][1]);
+                            *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[i][2], y[i][3]);
+                        }
+                if (!any_stored) continue;
+                // ---- keys and values in their stored form
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    const int j = place + r0 + i;
+                    int64_t row = -1;
+                    if (there && !is_q && r0 + i < rows && j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
+                    // The largest magnitude by its bits: a NaN's are above infinity's.
+                    uint32_t most = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) most = max(most, __float_as_uint(y[i][c]) & 0x7fffffffu);
+                    if constexpr (L == 32) most = __reduce_max_sync(0xffffffffu, most);
+                    else
+#pragma unroll
+                        for (int o = L / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    float m = __uint_as_float(most);
+                    if (row < 0) continue;
+                    if (!paged_holds<KIND>(m)) {
+                        bad |= kPagedNonFinite;
+                        m = 0.f;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) y[i][c] = 0.f;
+                    }
+                    void *dst = is_k ? v.keys : v.values;
+                    const int64_t to = row * DIM;
+                    if constexpr (KIND == kPagedBytes) {
+                        const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
+                        int8_t code[4];
+                        paged_codes(y[i], scale, code);
+                        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e0) = make_char2(code[0], code[1]);
+                        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e1) = make_char2(code[2], code[3]);
+                        if (lane % L == 0) v.scales[(is_k ? 0 : (int64_t)v.pages * v.kvheads * v.page) + row] = scale;
+                    } else {
+                        uint16_t *d = static_cast<uint16_t *>(dst) + to;
+                        *reinterpret_cast<uint32_t *>(d + e0) = (uint32_t)tcm_bf16_rne(y[i][0]) | ((uint32_t)tcm_bf16_rne(y[i][1]) << 16);
+                        *reinterpret_cast<uint32_t *>(d + e1) = (uint32_t)tcm_bf16_rne(y[i][2]) | ((uint32_t)tcm_bf16_rne(y[i][3]) << 16);
+                    }
                 }
-                if (is_q || is_k)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] = (float)z[i];
-            }
-            if (there && is_q) {
-                float *dst = a.q_out + (long long)(e.start + first + c.at) * a.q_out_stride + c.head * DIM;
-                *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[0], y[1]);
-                *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[2], y[3]);
-            }
-            // ---- keys and values in their stored form
-            if (!__any_sync(0xffffffffu, c.row >= 0)) continue;
-            float m = 0.f, zero = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                zero = fmaf(y[i], 0.f, zero);  // NaN once a value is not finite
-                m = fmaxf(m, fabsf(y[i]));
-            }
-            if ((__ballot_sync(0xffffffffu, zero == 0.f && paged_holds<KIND>(m)) & mine) != mine) {
-                if (c.row >= 0) bad |= kPagedNonFinite;
-                m = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = 0.f;
-            }
-            void *dst = is_k ? v.keys : v.values;
-            const int64_t to = c.row * DIM;
-            if constexpr (KIND == kPagedBytes) {
-#pragma unroll
-                for (int o = 1; o < L; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
-                int8_t code[4];
-                paged_codes(y, scale, code);
-                if (c.row >= 0) {
-                    *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e0) = make_char2(code[0], code[1]);
-                    *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e1) = make_char2(code[2], code[3]);
-                    if (lane % L == 0) v.scales[(is_k ? 0 : (int64_t)v.pages * v.kvheads * v.page) + c.row] = scale;
-                }
-            } else if (c.row >= 0) {
-                uint16_t *d = static_cast<uint16_t *>(dst) + to;
-                *reinterpret_cast<uint32_t *>(d + e0) = (uint32_t)tcm_bf16_rne(y[0]) | ((uint32_t)tcm_bf16_rne(y[1]) << 16);
-                *reinterpret_cast<uint32_t *>(d + e1) = (uint32_t)tcm_bf16_rne(y[2]) | ((uint32_t)tcm_bf16_rne(y[3]) << 16);
             }
         }
-        __syncthreads();
+        if constexpr (R > 1) __syncthreads();
     }
     paged_report(a.status, bad);
 }
@@ -197,11 +236,12 @@ extern "C" int gpu_paged_rotate_append(const TcmPagedCache *cache, const TcmPage
     a.qnorm = turn->qnorm, a.knorm = turn->knorm, a.eps = turn->eps;
     a.qheads = qheads, a.half = turn->rotary / 2, a.status = status;
     rates(a.rate, turn->theta, turn->rotary);
-    // A row a CTA while that leaves SMs free, up to eight where there are many.
-    const int each = a.v.rows / (3 * sm_count());
-    a.tile = each < 1 ? 1 : each > kTurnRows ? kTurnRows : each;
-    const dim3 grid(blocks_of(a.v.max_new, a.tile), a.v.sequences);
-#define CALL(K, D) launch(paged_turn_kernel<K, D>, grid, dim3(kTurnThreads), 0, stream(), true, a)
+    // Tiles of rows only where they leave no SM without work, and sequences have the rows to fill them.
+    const bool tiles = a.v.max_new >= 4 && a.v.rows >= 4 * sm_count();
+    const dim3 grid(blocks_of(a.v.max_new, tiles ? kTurnTile : 1), a.v.sequences);
+#define CALL(K, D)                                                                                        \
+    if (tiles) launch(paged_turn_kernel<K, D, 4>, grid, dim3(256), 0, stream(), true, a);                 \
+    else launch(paged_turn_kernel<K, D, 1>, grid, dim3(512), 0, stream(), true, a)
     PAGED_DISPATCH(a.v, CALL);
 #undef CALL
     return 0;
