@@ -15,7 +15,7 @@
 //
 // Weights exp((l - max) / T) are whole numbers, 2^44 for the largest: their sums are exact whatever the order, so that
 // atomics and the CTAs' shares leave results the same from call to call, and a sum of 2^19 of them stays below 2^64.
-// What bounds it: the weights' 15 FP64 instructions an element (28 cycles of an SM's quarter) beside HBM.
+// What bounds it: the weights' 13 FP64 instructions an element (26 cycles of an SM's quarter) beside HBM.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/gpu.h"
@@ -50,8 +50,8 @@ struct SampleArgs {
 
 // What a CTA of the cluster tells the others of its slice.
 struct SampleSlice {
-    float most, least;  // of the logits above -infinity
-    int live, bad;      // logits above -infinity; a NaN or +infinity among them
+    uint32_t most, least;  // keys of the logits above -infinity
+    int live, bad;         // logits above -infinity; a NaN or +infinity among them
 };
 struct SampleSums {
     u64 all, above, kept;  // weights: of the tokens that top-p takes a share of, above its bins, and above all bins and min-p
@@ -69,11 +69,17 @@ struct SampleShared {
     u64 warp_mass[kSampleWarps], warp_more[kSampleWarps], warp_kept[kSampleWarps];
     int warp_count[kSampleWarps];
     float warp_low[kSampleWarps], warp_high[kSampleWarps];
+    u64 whole, before, heavier, everything;  // of the row: see SampleSums; before: kept in CTAs before this one
     u64 list_before, list_kept, at_first, at_last;
-    int listed, list_count;
+    int kept, listed, list_count;
     int bin, above, in_bin;  // of top-k's cut
-    int mass_bin;            // of top-p's, estimated
-    int cut;                 // index in the list
+    float mass_whole;        // what top-p takes its share of, estimated
+    int mass_from, mass_to;  // top-p's bins, first and last,
+    int list_from, list_to;  // and the tokens above the first, up to the last
+    int cut;                 // index in the list of top-p's last token
+    int settled;             // whether the cut is in the list
+    uint32_t cut_key;
+    unsigned cut_id;
     u64 slow_mass;
 };
 
@@ -91,15 +97,9 @@ __device__ __forceinline__ float sample_value(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// 2^f = sum of (f ln 2)^k / k!: for |f| <= 1/2 the terms from the tenth on are below 2^-37 together.
-struct SampleSeries {
-    double c[10];
-    constexpr SampleSeries() : c() {
-        c[0] = 1.0;
-        for (int k = 1; k < 10; k++) c[k] = c[k - 1] * 0.69314718055994530942 / k;
-    }
-};
-__device__ constexpr SampleSeries kSampleSeries{};
+// (2^f - 1) / f for |f| <= 1/2, interpolated at the seven Chebyshev points there: 2^f is off by 2^-33 at most.
+__device__ constexpr double kSampleSeries[7] = {0.6931471805599453,    0.24022650922288757,   0.055504108839096185,  0.009618056678524632,
+                                                0.0013333502386162978, 0.00015461444698571227, 1.5297323760649362e-05};
 
 struct SampleRow {
     double top, cold, slope;  // the largest logit, 1 / T, log2(e) / T
@@ -109,9 +109,10 @@ struct SampleRow {
         // At most zero; from -64 on (its upper word decides) nothing is left of it.
         const double y = __hiloint2double((int)min((unsigned)__double2hiint(y0), 0xc0500000u), __double2loint(y0));
         const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
-        double z = kSampleSeries.c[9];
+        double z = kSampleSeries[6];
 #pragma unroll
-        for (int k = 8; k >= 0; k--) z = fma(z, f, kSampleSeries.c[k]);
+        for (int k = 5; k >= 0; k--) z = fma(z, f, kSampleSeries[k]);
+        z = fma(z, f, 1.0);
         z = __hiloint2double(__double2hiint(z) + (__double2loint(t) << 20), __double2loint(z));
         return (u64)(__double_as_longlong(z + 0x1.8p8) - __double_as_longlong(0x1.8p8));  // in units of 2^-44
     }
@@ -132,7 +133,7 @@ struct SampleBins {
         const int b = __float_as_int(fmaf(high - l * unit, scale, 0x1p23f)) & 0x7fffff;
         return l < from ? last : b;
     }
-    __device__ double middle(int b) const { return scale > 0.f ? (double)b / ((double)scale * (double)unit) : 0.0; }  // below high
+    __device__ float width() const { return scale > 0.f ? 1.f / scale / unit : 0.f; }  // a bin's
 };
 
 // The cut by repeated histograms of the cluster: counts and weights in bins of the range in which it must lie, then of the
@@ -358,6 +359,10 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     });
 }
 
+// The first kResolve threads of a CTA settle the list.
+constexpr int kResolve = 128;
+__device__ __forceinline__ void resolve_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kResolve) : "memory"); }
+
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) float slice_memory[];
     __shared__ __align__(16) SampleShared sh;
@@ -372,96 +377,96 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const TcmSampling p = a.params[row];
     const float u = a.uniforms[row];
 
-    // ---- the slice, and what there is in it. It starts in shared memory as far from a 16-byte boundary as in global memory.
-    const int off = (int)((uintptr_t)src >> 2) & 3;
+    // ---- the slice, and what there is in it. It starts in shared memory as far from a 16-byte boundary as in global
+    // memory, with -infinity around it, so that everything after this goes by whole quads.
+    const int off = (int)((uintptr_t)src >> 2) & 3, quads = (off + n + 3) / 4;
     float *x = slice_memory + off;
+    float4 *x4 = reinterpret_cast<float4 *>(slice_memory);
     float most = -INFINITY, least = INFINITY;
     bool bad = false;
     auto meet = [&](float l) {
         bad |= !(l < INFINITY);
         most = fmaxf(most, l), least = fminf(least, l);
     };
-    const int head = min(n, (4 - off) & 3), quads = (n - head) / 4;
-    if (tid < head) {
-        const float l = src[tid];
-        x[tid] = l;
-        meet(l);
-    }
+    const int q0 = off ? 1 : 0, q1 = (off + n) / 4;  // whole quads
 #pragma unroll 4
-    for (int i = tid; i < quads; i += kSampleThreads) {
-        const float4 l = __ldcg(reinterpret_cast<const float4 *>(src + head) + i);
-        reinterpret_cast<float4 *>(x + head)[i] = l;
+    for (int q = q0 + tid; q < q1; q += kSampleThreads) {
+        const float4 l = __ldcg(reinterpret_cast<const float4 *>(src - off) + q);
+        x4[q] = l;
         meet(l.x), meet(l.y), meet(l.z), meet(l.w);
     }
-    if (tid < (n - head) % 4) {
-        const int i = head + 4 * quads + tid;
-        const float l = src[i];
-        x[i] = l;
-        meet(l);
+    if (warp == 0) {  // the ends: lanes 0 .. 3 the first quad, 4 .. 7 the last
+        const int i = (lane < 4 ? 0 : 4 * q1) + lane % 4 - off;  // of the slice
+        if ((lane < 4 && q0) || (lane >= 4 && lane < 8 && q1 < quads && (q1 || !q0))) {
+            const bool there = i >= 0 && i < n;
+            const float l = there ? src[i] : -INFINITY;
+            x[i] = l;
+            if (there) meet(l);
+        }
     }
-    most = warp_max(most);
-    least = -warp_max(-least);
+    const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
+    uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
     bad = __any_sync(0xffffffffu, bad);
-    if (lane == 0) sh.warp_high[warp] = most, sh.warp_low[warp] = least, sh.warp_count[warp] = bad;
-    __syncthreads();
-    int live = n;
-    {
-        float low = INFINITY;
-        for (int w = 0; w < kSampleWarps; w++) low = fminf(low, sh.warp_low[w]);
-        if (low == -INFINITY) {  // masked tokens: what else there is
-            int count = 0;
-            least = INFINITY;
-            for (int i = tid; i < n; i += kSampleThreads)
-                if (x[i] > -INFINITY) count++, least = fminf(least, x[i]);
-            least = -warp_max(-least);
-            count = __reduce_add_sync(0xffffffffu, count);
-            __syncthreads();
-            if (lane == 0) sh.warp_low[warp] = least, sh.warp_mass[warp] = count;
-            __syncthreads();
-            live = 0;
-            for (int w = 0; w < kSampleWarps; w++) live += (int)sh.warp_mass[w];
-        }
+    int live = 0;
+    const bool masked = __syncthreads_or(least == -INFINITY);
+    if (masked) {  // what there is beside masked tokens
+        least = INFINITY;
+        for (int i = tid; i < n; i += kSampleThreads)
+            if (x[i] > -INFINITY) live++, least = fminf(least, x[i]);
+        warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
+        live = __reduce_add_sync(0xffffffffu, live);
     }
-    cluster.barrier_wait(std::move(started));
-    if (tid < C) {  // thread c tells CTA c
-        SampleSlice z = {-INFINITY, INFINITY, live, 0};
-        for (int w = 0; w < kSampleWarps; w++) {
-            z.most = fmaxf(z.most, sh.warp_high[w]), z.least = fminf(z.least, sh.warp_low[w]);
-            z.bad |= sh.warp_count[w];
-        }
-        cluster.map_shared_rank(sh.slices, tid)[rank] = z;
+    if (lane == 0) {
+        sh.warp_count[warp] = live;
+        reinterpret_cast<uint32_t *>(sh.warp_high)[warp] = warp_most, reinterpret_cast<uint32_t *>(sh.warp_low)[warp] = warp_least;
+        sh.warp_mass[warp] = bad;
     }
-    for (int i = tid; i < kSampleBins / 2; i += kSampleThreads) sh.buffer[0][i] = 0;
+    const bool ranked = p.top_k > 0 || p.top_p < 1.f;
+    if (ranked)
+        for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = 0;
+    __syncthreads();
+    cluster.barrier_wait(std::move(started));
+    if (warp == 0) {  // lane c tells CTA c
+        const int w = lane % kSampleWarps;
+        SampleSlice z;
+        z.most = __reduce_max_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_high)[w]);
+        z.least = __reduce_min_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_low)[w]);
+        z.live = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? sh.warp_count[w] : 0);
+        z.bad = __any_sync(0xffffffffu, sh.warp_mass[w] != 0);
+        if (!masked) z.live = n;
+        if (lane < C) cluster.map_shared_rank(sh.slices, lane)[rank] = z;
+    }
     cluster.sync();
-    SampleSlice all = sh.slices[0];
-    for (int c = 1; c < C; c++) {
-        const SampleSlice &z = sh.slices[c];
-        all.most = fmaxf(all.most, z.most), all.least = fminf(all.least, z.least);
-        all.live += z.live;
-        all.bad |= z.bad;
+    float high, low;
+    int all_live;
+    {
+        const SampleSlice z = sh.slices[lane < C ? lane : 0];
+        high = sample_value(__reduce_max_sync(0xffffffffu, z.most)), low = sample_value(__reduce_min_sync(0xffffffffu, z.least));
+        all_live = __reduce_add_sync(0xffffffffu, lane < C ? z.live : 0);
+        bad = __any_sync(0xffffffffu, z.bad);
     }
     const bool wrong = !(p.temperature >= 0.f && p.temperature < INFINITY && u >= 0.f && u < 1.f && p.min_p <= 1.f) ||
                        p.top_p != p.top_p;
-    if (all.bad || !all.live || wrong) {  // the whole cluster alike
+    if (bad || !all_live || wrong) {  // the whole cluster alike
         if (rank == 0 && tid == 0) {
             a.ids[row] = -1;
             if (a.logprobs) a.logprobs[row] = 0.f;
             if (a.kept) a.kept[row] = 0;
-            if (a.status) atomicOr(a.status, (all.bad ? 1 : 0) | (!all.bad && !all.live ? 2 : 0) | (wrong ? 4 : 0));
+            if (a.status) atomicOr(a.status, (bad ? 1 : 0) | (!bad && !all_live ? 2 : 0) | (wrong ? 4 : 0));
         }
         return;
     }
     if (p.temperature == 0.f) {
         int first = 0x7fffffff;
         for (int i = tid; i < n; i += kSampleThreads)
-            if (x[i] == all.most) first = min(first, base + i);
+            if (x[i] == high) first = min(first, base + i);
         first = __reduce_min_sync(0xffffffffu, first);
         if (lane == 0) sh.warp_count[warp] = first;
         __syncthreads();
-        if (tid == 0) {
-            for (int w = 0; w < kSampleWarps; w++) first = min(first, sh.warp_count[w]);
-            cluster.map_shared_rank(sh.first, 0)[rank] = first;
+        if (warp == 0) {
+            first = __reduce_min_sync(0xffffffffu, sh.warp_count[lane % kSampleWarps]);
+            if (lane == 0) cluster.map_shared_rank(sh.first, 0)[rank] = first;
         }
         cluster.sync();
         if (rank == 0 && tid == 0) {
@@ -474,7 +479,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
 
     SampleRow r;
-    r.top = all.most, r.cold = 1.0 / (double)p.temperature, r.slope = 1.4426950408889634074 * r.cold;
+    r.top = high, r.cold = 1.0 / (double)p.temperature, r.slope = 1.4426950408889634074 * r.cold;
     // min-p as the least logit that it keeps: next to the one that arithmetic gives, the one that satisfies the definition.
     float min_logit = -FLT_MAX;
     if (p.min_p > 0.f) {
@@ -482,40 +487,54 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         float l = fmaxf((float)(r.top + coldest * (double)p.temperature), -FLT_MAX);
         if (!(r.exponent(l) >= coldest)) l = nextafterf(l, INFINITY);
         else if (l > -FLT_MAX && r.exponent(nextafterf(l, -INFINITY)) >= coldest) l = nextafterf(l, -INFINITY);
-        min_logit = fminf(l, all.most);
+        min_logit = fminf(l, high);
     }
 
     // ---- the bins in which the cuts lie
-    const bool by_count = p.top_k > 0 && p.top_k < all.live, by_mass = p.top_p < 1.f;
+    const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f;
     const float reach = (float)(r.top - 32.0 * (double)p.temperature);
-    const SampleBins bins(all.least < reach && reach < all.most ? reach : all.least, all.most, kSampleBins);
+    const SampleBins bins(low < reach && reach < high ? reach : low, high, kSampleBins);
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
-    int listed_all = 0;
+    int listed = 0;
     if (by_count || by_mass) {
         unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
-        for (int i = tid; i < n; i += kSampleThreads)
-            if (x[i] > -INFINITY) atomicAdd(&own[bins.of(x[i])], 1u);
+        for (int q = tid; q < quads; q += kSampleThreads) {
+            const float4 l = x4[q];
+            if (l.x > -INFINITY) atomicAdd(&own[bins.of(l.x)], 1u);
+            if (l.y > -INFINITY) atomicAdd(&own[bins.of(l.y)], 1u);
+            if (l.z > -INFINITY) atomicAdd(&own[bins.of(l.z)], 1u);
+            if (l.w > -INFINITY) atomicAdd(&own[bins.of(l.w)], 1u);
+        }
         cluster.sync();
         // Each CTA adds up its share of the bins and tells the others.
         const int share_of = kSampleBins / C;
-        for (int i = tid; i < share_of; i += kSampleThreads) {
+        for (int i = 4 * tid; i < share_of; i += 4 * kSampleThreads) {
             const int b = rank * share_of + i;
-            unsigned c = 0;
+            uint4 c = make_uint4(0, 0, 0, 0);
 #pragma unroll 8
-            for (int k = 0; k < C; k++) c += cluster.map_shared_rank(own, k)[b];
+            for (int k = 0; k < C; k++) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(own, k) + b);
+                c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
+            }
 #pragma unroll 8
-            for (int k = 0; k < C; k++) cluster.map_shared_rank(counts, k)[b] = c;
+            for (int k = 0; k < C; k++) *reinterpret_cast<uint4 *>(cluster.map_shared_rank(counts, k) + b) = c;
         }
+        if (tid == 0) sh.bin = kSampleBins, sh.mass_from = sh.mass_to = kSampleBins - 1;
         cluster.sync();
         constexpr int each = kSampleBins / kSampleThreads;
         unsigned c[each], upto = 0;
         float mass[each], total = 0.f;
+        const float step = -bins.width() * (float)r.slope;
+#pragma unroll
+        for (int k = 0; k < each; k += 4) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(counts + tid * each + k);
+            c[k] = y.x, c[k + 1] = y.y, c[k + 2] = y.z, c[k + 3] = y.w;
+        }
 #pragma unroll
         for (int k = 0; k < each; k++) {
             const int b = tid * each + k;
-            c[k] = counts[b];
-            mass[k] = b == bins.last ? 0.f : (float)c[k] * exp2f((float)(-bins.middle(b) * r.slope));
+            mass[k] = b == kSampleBins - 1 ? 0.f : (float)c[k] * exp2f((float)b * step);
             upto += c[k], total += mass[k];
         }
         const unsigned mine = upto;
@@ -527,10 +546,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             if (lane >= o) upto += y, total += z;
         }
         if (lane == 31) sh.warp_count[warp] = (int)upto, sh.warp_high[warp] = total;
-        if (tid == 0) sh.mass_bin = bins.last, sh.bin = kSampleBins;
         __syncthreads();
         unsigned before = upto - mine;
         float lighter = total - mine_mass, whole = 0.f;
+#pragma unroll
         for (int w = 0; w < kSampleWarps; w++) {
             if (w < warp) before += (unsigned)sh.warp_count[w], lighter += sh.warp_high[w];
             whole += sh.warp_high[w];
@@ -544,114 +563,131 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 for (int b = 0; b < each; b++) {
                     if (above < k && k <= above + c[b]) {
                         sh.bin = tid * each + b, sh.above = (int)above, sh.in_bin = (int)c[b];
-                        sh.ends[0].x = heavier + mass[b] * ((float)(k - above) / (float)c[b]);
+                        sh.mass_whole = heavier + mass[b] * ((float)(k - above) / (float)c[b]);
                     }
                     above += c[b], heavier += mass[b];
                 }
             }
             __syncthreads();
             count_bin = sh.bin, tokens_left = p.top_k - sh.above, in_count_bin = sh.in_bin;
-            whole = sh.ends[0].x;
+            whole = sh.mass_whole;
         }
+        listed = in_count_bin;
         if (by_mass) {
-            const float share = fmaxf(p.top_p, 0.f) * whole;
-            int here = kSampleBins;
-#pragma unroll
-            for (int b = each - 1; b >= 0; b--) {
-                float sum = lighter;
-#pragma unroll
-                for (int m = 0; m <= b; m++) sum += mass[m];
-                if (c[b] && sum >= share) here = tid * each + b;
-            }
-            if (here < kSampleBins && (lighter < share || !(share > 0.f))) atomicMin(&sh.mass_bin, here);
-            __syncthreads();
-            const int bin = min(sh.mass_bin, count_bin < kSampleBins ? count_bin : bins.last);
-            mass_from = max(bin - 1, 0), mass_to = min(bin + 1, count_bin < kSampleBins ? count_bin : bins.last);
-        }
-        // How many tokens these bins hold: within a list, or the slow way. The estimate's neighbours only where they fit.
-        for (int tries = 0; tries < 2; tries++) {
-            int listed = 0;
+            // The bins at which the estimated sum passes the share, a little before and a little behind it.
+            const float share = fmaxf(p.top_p, 0.f) * whole, slack = 2e-5f * whole;
+            const int last = min(kSampleBins - 1, count_bin);
+            float sum = lighter;
 #pragma unroll
             for (int k = 0; k < each; k++) {
                 const int b = tid * each + k;
-                if ((b >= mass_from && b <= mass_to) || b == count_bin) listed += (int)c[k];
+                const float next = sum + mass[k];
+                if (c[k]) {
+                    if (sum < share - slack || before == 0) {
+                        if (next >= share - slack) atomicMin(&sh.mass_from, b);
+                    }
+                    if ((sum < share + slack || before == 0) && next >= share + slack) atomicMin(&sh.mass_to, b);
+                }
+                before += c[k], sum = next;
             }
-            listed = __reduce_add_sync(0xffffffffu, listed);
+            before -= mine;
             __syncthreads();
-            if (lane == 0) sh.warp_count[warp] = listed;
+            mass_from = min(sh.mass_from, last), mass_to = min(sh.mass_to, last);
+            if (mass_to < mass_from) mass_to = mass_from;
+            // How many tokens they hold: those up to the last but not above the first.
+#pragma unroll
+            for (int k = 0; k < each; k++) {
+                const int b = tid * each + k;
+                if (b == mass_from) sh.list_from = (int)before;
+                before += c[k];
+                if (b == mass_to) sh.list_to = (int)before;
+            }
             __syncthreads();
-            listed_all = 0;
-            for (int w = 0; w < kSampleWarps; w++) listed_all += sh.warp_count[w];
-            if (listed_all <= kSampleList || !by_mass || tries) break;
-            mass_from = mass_to = min(sh.mass_bin, count_bin < kSampleBins ? count_bin : bins.last);
+            listed = sh.list_to - sh.list_from + (mass_to < count_bin ? in_count_bin : 0);
         }
-        if (listed_all > kSampleList) {
-            sample_slowly(a, r, sh, x, n, base, row, all.least, all.most, all.live, min_logit);
+        if (listed > kSampleList) {
+            sample_slowly(a, r, sh, x, n, base, row, low, high, all_live, min_logit);
             return;
         }
     }
 
     // ---- weights above the bins, and the list of what is in them. A warp has a contiguous stretch of ids.
     const int kept_to = by_mass ? mass_from : count_bin;  // bins below this are kept whole
-    const int per_warp = (n + kSampleWarps - 1) / kSampleWarps, w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
+    const int per_warp = (quads + kSampleWarps - 1) / kSampleWarps, w0 = min(quads, warp * per_warp), w1 = min(quads, w0 + per_warp);
     u64 *own_list = sh.buffer[0], *list = sh.buffer[1];
-    SampleSums sums = {0, 0, 0, 0, 0};
+    u64 sum_all = 0, sum_above = 0, sum_kept = 0;
+    int kept = 0;
     if (by_count || by_mass) {
-        const int needed = max(by_mass ? mass_to : 0, by_count ? count_bin : by_mass ? bins.last : 0);  // weights end here
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const float l = x[i];
-            const int b = l > -INFINITY ? bins.of(l) : kSampleBins;
-            if (b > needed) continue;
-            if ((b >= mass_from && b <= mass_to) || b == count_bin)
-                own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << 32) | (unsigned)(base + i);
-            const bool below = b < kept_to;
-            if (!by_mass && !below) continue;
-            const u64 w = r.weight(l);
-            if (b < count_bin) sums.all += w;
-            if (below) {
-                sums.above += w;
-                if (l >= min_logit) sums.kept += w, sums.kept_count++;
+        const int needed = by_count ? count_bin : kSampleBins - 1;  // weights end here
+        for (int q = w0 + lane; q < w1; q += 32) {
+            const float4 y = x4[q];
+            const float l[4] = {y.x, y.y, y.z, y.w};
+            int b[4];
+            bool any = false;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                b[k] = l[k] > -INFINITY ? bins.of(l[k]) : kSampleBins;
+                any |= b[k] <= needed;
+            }
+            if (!any) continue;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if ((b[k] >= mass_from && b[k] <= mass_to) || (b[k] == count_bin && by_count))
+                    own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l[k]) << 32) | (unsigned)(base + 4 * q + k - off);
+            u64 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = r.weight(l[k]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (b[k] < count_bin) sum_all += w[k];
+                if (b[k] < kept_to) {
+                    sum_above += w[k];
+                    if (l[k] >= min_logit) sum_kept += w[k], kept++;
+                }
             }
         }
     } else {
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const float l = x[i];
-            if (l >= min_logit) sums.kept += r.weight(l), sums.kept_count++;
+        for (int q = w0 + lane; q < w1; q += 32) {
+            const float4 y = x4[q];
+            const float l[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const u64 w = r.weight(l[k]);
+                if (l[k] >= min_logit) sum_kept += w, kept++;
+            }
         }
     }
-    sums.all = warp_sum64(sums.all), sums.above = warp_sum64(sums.above), sums.kept = warp_sum64(sums.kept);
-    sums.kept_count = __reduce_add_sync(0xffffffffu, sums.kept_count);
-    const u64 warp_kept = sums.kept;
+    if (by_mass) sum_all = warp_sum64(sum_all), sum_above = warp_sum64(sum_above);
+    sum_kept = warp_sum64(sum_kept);
+    kept = __reduce_add_sync(0xffffffffu, kept);
     if (lane == 0) {
-        sh.warp_mass[warp] = sums.all, sh.warp_more[warp] = sums.above, sh.warp_kept[warp] = sums.kept;
-        sh.warp_count[warp] = sums.kept_count;
+        sh.warp_mass[warp] = sum_all, sh.warp_more[warp] = sum_above, sh.warp_kept[warp] = sum_kept;
+        sh.warp_count[warp] = kept;
     }
     __syncthreads();
-    if (tid < C) {
-        SampleSums z = {0, 0, 0, 0, sh.listed};
-        for (int w = 0; w < kSampleWarps; w++) {
-            z.all += sh.warp_mass[w], z.above += sh.warp_more[w], z.kept += sh.warp_kept[w];
-            z.kept_count += sh.warp_count[w];
-        }
-        cluster.map_shared_rank(sh.sums, tid)[rank] = z;
+    if (warp == 0) {  // lane c tells CTA c
+        const int w = lane % kSampleWarps;
+        SampleSums z = {0, 0, 0, 0, 0};
+        if (lane < kSampleWarps) z.all = sh.warp_mass[w], z.above = sh.warp_more[w], z.kept = sh.warp_kept[w], z.kept_count = sh.warp_count[w];
+        if (by_mass) z.all = warp_sum64(z.all), z.above = warp_sum64(z.above);
+        z.kept = warp_sum64(z.kept);
+        z.kept_count = __reduce_add_sync(0xffffffffu, z.kept_count);
+        z.listed = sh.listed;
+        if (lane < C) cluster.map_shared_rank(sh.sums, lane)[rank] = z;
     }
     cluster.sync();
-    u64 whole = 0, before = 0, heavier = 0, everything = 0;
-    int kept = 0;
-    for (int c = 0; c < C; c++) {
-        const SampleSums &z = sh.sums[c];
-        if (c < rank) before += z.kept;
-        whole += z.kept, heavier += z.above, everything += z.all;
-        kept += z.kept_count;
+    if (warp == 1) {
+        SampleSums z = {0, 0, 0, 0, 0};
+        if (lane < C) z = sh.sums[lane];
+        const u64 before = warp_sum64(lane < rank ? z.kept : 0), whole = warp_sum64(z.kept);
+        if (by_mass) z.above = warp_sum64(z.above), z.all = warp_sum64(z.all);
+        z.kept_count = __reduce_add_sync(0xffffffffu, z.kept_count);
+        if (lane == 0) sh.before = before, sh.whole = whole, sh.heavier = z.above, sh.everything = z.all, sh.kept = z.kept_count, sh.cut = kSampleList;
     }
-    for (int w = 0; w < warp; w++) before += sh.warp_kept[w];
-    float cut_value = -INFINITY;
-    unsigned cut_id = 0;
-    u64 warp_listed = 0;  // kept weights of the list in this warp's stretch
-    bool gathered = false;
+    if (lane == 0) sh.warp_more[warp] = 0;
+    // ---- the list of the cluster, sorted by a few warps: logits descending, ids ascending
     if (by_count || by_mass) {
-        // ---- the list of the cluster, sorted: logits descending, ids ascending
-        const int m = listed_all;
+        const int m = listed;
         for (int c = 0, to = 0; c < C; c++) {
             const int k = sh.sums[c].listed;
             const u64 *from = cluster.map_shared_rank(own_list, c);
@@ -659,126 +695,144 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             to += k;
         }
         cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
-        gathered = true;
         int size = 32;
         while (size < m) size <<= 1;
         for (int i = m + tid; i < size; i += kSampleThreads) list[i] = ~0ull;
-        for (int k = 2; k <= size; k <<= 1)
-            for (int j = k >> 1; j; j >>= 1) {
-                __syncthreads();
-                for (int i = tid; i < size / 2; i += kSampleThreads) {
-                    const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                    const u64 y = list[lo], z = list[hi];
-                    if ((y > z) == ((lo & k) == 0)) list[lo] = z, list[hi] = y;
+        __syncthreads();
+        if (tid < kResolve) {
+            for (int k = 2; k <= size; k <<= 1)
+                for (int j = k >> 1; j; j >>= 1) {
+                    for (int i = tid; i < size / 2; i += kResolve) {
+                        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                        const u64 y = list[lo], z = list[hi];
+                        if ((y > z) == ((lo & k) == 0)) list[lo] = z, list[hi] = y;
+                    }
+                    resolve_barrier();
+                }
+            auto logit_at = [&](int i) { return sample_value(~(uint32_t)(list[i] >> 32)); };
+            const int each = size > kResolve ? size / kResolve : 1, i0 = min(m, tid * each), i1 = min(m, i0 + each);
+            int cut = tokens_left - 1;
+            bool fine = true;
+            if (by_mass) {
+                // Sums of weights up to each thread's places.
+                u64 mine = 0;
+                for (int i = i0; i < i1; i++) mine += r.weight(logit_at(i));
+                u64 upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                if (lane == 31) sh.warp_mass[warp] = upto;
+                resolve_barrier();
+                upto -= mine;
+                for (int k = 0; k < warp; k++) upto += sh.warp_mass[k];
+                u64 all_of = sh.everything;
+                const int first = m - in_count_bin, last = first + tokens_left - 1;  // of top-k's bin, its tokens
+                if (by_count) {
+                    u64 sum = upto;
+                    for (int i = i0; i < i1; i++) {
+                        if (i == first) sh.at_first = sum;
+                        sum += r.weight(logit_at(i));
+                        if (i == last) sh.at_last = sum;
+                    }
+                    resolve_barrier();
+                    all_of += sh.at_last - sh.at_first;
+                }
+                const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
+                fine = mass_from == 0 || (double)sh.heavier < share;
+                u64 sum = sh.heavier + upto;
+                int i = i0;
+                for (; i < i1; i++) {
+                    sum += r.weight(logit_at(i));
+                    if ((double)sum >= share) break;
+                }
+                if (i < i1 && (i == 0 || (double)(sum - r.weight(logit_at(i))) < share)) sh.cut = i;
+                resolve_barrier();
+                cut = sh.cut;
+                // In top-p's bins, or the estimate was wrong.
+                fine = fine && cut < m && (!by_count || cut <= last);
+                if (fine) fine = bins.of(logit_at(cut)) <= mass_to;
+            }
+            if (tid == 0) {
+                sh.settled = fine;
+                if (fine) sh.cut_key = ~(uint32_t)(list[cut] >> 32), sh.cut_id = (unsigned)list[cut];
+            }
+            if (fine) {  // what is kept of the list, by where it is
+                for (int i = i0; i < i1 && i <= cut; i++) {
+                    const float l = logit_at(i);
+                    if (l < min_logit) continue;
+                    const u64 w = r.weight(l);
+                    const int at = (int)(unsigned)list[i] - base;
+                    atomicAdd(&sh.list_kept, w);
+                    atomicAdd(&sh.list_count, 1);
+                    if (at < 0) atomicAdd(&sh.list_before, w);
+                    else if (at < n) atomicAdd(&sh.warp_more[(at + off) / 4 / per_warp], w);
                 }
             }
-        __syncthreads();
-        // Sums of weights up to each place of the list, four places a thread.
-        constexpr int each = kSampleList / kSampleThreads;
-        u64 w[each], upto = 0;
-#pragma unroll
-        for (int k = 0; k < each; k++) {
-            const int i = tid * each + k;
-            w[k] = i < m && (by_mass || by_count) ? r.weight(sample_value(~(uint32_t)(list[min(i, kSampleList - 1)] >> 32))) : 0;
-            upto += w[k];
         }
-        const u64 mine = upto;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == 31) sh.warp_mass[warp] = upto;
-        if (tid == 0) sh.cut = kSampleList, sh.at_first = 0;
-        __syncthreads();
-        upto -= mine;
-        for (int k = 0; k < warp; k++) upto += sh.warp_mass[k];
-        int cut = kSampleList;
-        bool fine = true;
-        const int first_counted = m - in_count_bin, last_counted = first_counted + tokens_left - 1;  // of top-k's bin
-        if (by_count) cut = last_counted;
-        if (by_mass) {
-            u64 all_of = everything;
-            if (by_count) {
-                u64 sum = upto;
-#pragma unroll
-                for (int k = 0; k < each; k++) {
-                    if (tid * each + k == first_counted) sh.at_first = sum;
-                    sum += w[k];
-                    if (tid * each + k == last_counted) sh.at_last = sum;
-                }
-                __syncthreads();
-                all_of += sh.at_last - sh.at_first;
-            }
-            const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
-            fine = mass_from == 0 || (double)heavier < share;
-            u64 sum = heavier + upto;
-            int here = kSampleList;
-#pragma unroll
-            for (int k = 0; k < each; k++) {
-                sum += w[k];
-                if (here == kSampleList && tid * each + k < m && (double)sum >= share) here = tid * each + k;
-            }
-            if (here < kSampleList) atomicMin(&sh.cut, here);
-            __syncthreads();
-            cut = sh.cut;
-            // In top-p's bins, or the estimate was wrong.
-            fine = fine && cut < m && (!by_count || cut <= last_counted);
-            if (fine) fine = bins.of(sample_value(~(uint32_t)(list[cut] >> 32))) <= mass_to;
-        }
-        if (!fine) {  // the whole cluster alike
+    }
+    __syncthreads();
+    float cut_value = -INFINITY;
+    unsigned cut_id = 0;
+    u64 whole = sh.whole, before = sh.before;
+    if (by_count || by_mass) {
+        if (!sh.settled) {  // the whole cluster alike
             cluster.barrier_wait();
-            sample_slowly(a, r, sh, x, n, base, row, all.least, all.most, all.live, min_logit);
+            sample_slowly(a, r, sh, x, n, base, row, low, high, all_live, min_logit);
             return;
         }
-        const u64 last = list[cut];
-        cut_value = sample_value(~(uint32_t)(last >> 32)), cut_id = (unsigned)last;
-        // What is kept of the list, by where it is.
-        if (lane == 0) sh.warp_more[warp] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < each; k++) {
-            const int i = tid * each + k;
-            if (i > cut || i >= m) continue;
-            const u64 y = list[i];
-            if (sample_value(~(uint32_t)(y >> 32)) < min_logit) continue;
-            const int at = (int)(unsigned)y - base;
-            atomicAdd(&sh.list_kept, w[k]);
-            atomicAdd(&sh.list_count, 1);
-            if (at < 0) atomicAdd(&sh.list_before, w[k]);
-            else if (at < n) atomicAdd(&sh.warp_more[at / per_warp], w[k]);
-        }
-        __syncthreads();
-        whole += sh.list_kept, kept += sh.list_count, before += sh.list_before;
-        for (int k = 0; k < warp; k++) before += sh.warp_more[k];
-        warp_listed = sh.warp_more[warp];
+        cut_value = sample_value(sh.cut_key), cut_id = sh.cut_id;
+        whole += sh.list_kept, before += sh.list_before;
     }
     u64 target = (u64)((double)u * (double)whole);
     if (target >= whole) target = whole - 1;
-    if (target >= before && target < before + warp_kept + warp_listed) {  // one warp of the cluster has the token
-        for (int i0 = w0; i0 < w1; i0 += 32) {
-            const int i = i0 + lane;
-            const float l = i < w1 ? x[i] : -INFINITY;
-            const bool stays = (l > cut_value || (l == cut_value && (unsigned)(base + i) <= cut_id)) && l >= min_logit;
-            u64 upto = stays ? r.weight(l) : 0;
+    {
+        const u64 w = lane < kSampleWarps ? sh.warp_kept[lane] + sh.warp_more[lane] : 0;  // of each warp's stretch
+        before += warp_sum64(lane < warp ? w : 0);
+        const u64 own = __shfl_sync(0xffffffffu, w, warp);
+        if (target >= before && target < before + own) {  // one warp of the cluster has the token
+            for (int q0 = w0; q0 < w1; q0 += 32) {
+                const int q = q0 + lane;
+                const float4 y = q < w1 ? x4[q] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float l[4] = {y.x, y.y, y.z, y.w};
+                u64 w4[4], mine = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
-            if (reached) {
-                if (lane == __ffs(reached) - 1) {
-                    a.ids[row] = base + i;
-                    if (a.logprobs) a.logprobs[row] = (float)(r.exponent(l) - log((double)whole / kSampleOne));
-                    if (a.kept) a.kept[row] = kept;
+                for (int k = 0; k < 4; k++) {
+                    const unsigned id = (unsigned)(base + 4 * q + k - off);
+                    const bool stays = (l[k] > cut_value || (l[k] == cut_value && id <= cut_id)) && l[k] >= min_logit;
+                    w4[k] = r.weight(l[k]);
+                    if (!stays) w4[k] = 0;
+                    mine += w4[k];
                 }
-                break;
+                u64 upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 z = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += z;
+                }
+                const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
+                if (reached) {
+                    if (lane == __ffs(reached) - 1) {
+                        u64 sum = before + upto;
+                        int id = 0;
+                        float logit = 0.f;
+#pragma unroll
+                        for (int k = 3; k >= 0; k--) {  // the first of the four at which the sum passes the target
+                            if (sum > target && w4[k]) id = base + 4 * q + k - off, logit = l[k];
+                            sum -= w4[k];
+                        }
+                        a.ids[row] = id;
+                        if (a.logprobs) a.logprobs[row] = (float)(r.exponent(logit) - log((double)whole / kSampleOne));
+                        if (a.kept) a.kept[row] = sh.kept + ((by_count || by_mass) ? sh.list_count : 0);
+                    }
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
-    if (gathered) cluster.barrier_wait();
+    if (by_count || by_mass) cluster.barrier_wait();
 }
 
 int refuse(const char *why) {
@@ -804,7 +858,7 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
         return refuse("arrays are 4-byte aligned");
     static PerDeviceOnce once;
     once.run([] {
-        TCM_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSampleSlice + 4) * 4));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSampleSlice + 8) * 4));
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
     // Few rows take all the SMs that help; many rows the fewest CTAs whose slices leave room for two an SM.
@@ -815,7 +869,7 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * cluster);
     cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = (size_t)(slice + 4) * 4;
+    cfg.dynamicSmemBytes = (size_t)(slice + 8) * 4;
     cfg.stream = stream();
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
