@@ -30,9 +30,9 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024;
+constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
-constexpr int kSampleSlice = kSampleVocab / kSampleCluster;  // logits a CTA holds at most
+constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 72 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 constexpr double kSampleOne = 0x1p44;
 typedef unsigned long long u64;
 
@@ -70,16 +70,17 @@ struct SampleShared {
     int warp_count[kSampleWarps];
     float warp_low[kSampleWarps], warp_high[kSampleWarps];
     u64 whole, before, heavier, everything;  // of the row: see SampleSums; before: kept in CTAs before this one
-    u64 list_before, list_kept, at_first, at_last;
+    u64 list_before, list_kept, list_counted;
     int kept, listed, list_count;
     int bin, above, in_bin;  // of top-k's cut
     float mass_whole;        // what top-p takes its share of, estimated
     int mass_from, mass_to;  // top-p's bins, first and last,
     int list_from, list_to;  // and the tokens above the first, up to the last
-    int cut;                 // index in the list of top-p's last token
-    int settled;             // whether the cut is in the list
-    uint32_t cut_key;
-    unsigned cut_id;
+    // The search for the cut in the list.
+    u64 sub_mass[kSubBins], few[32], few_mass[32], found, found_mass;
+    unsigned sub_count[kSubBins];
+    uint32_t sub_least, sub_most;
+    int sub_bin, sub_above, few_count;
     u64 slow_mass;
 };
 
@@ -133,17 +134,68 @@ struct SampleBins {
         const int b = __float_as_int(fmaf(high - l * unit, scale, 0x1p23f)) & 0x7fffff;
         return l < from ? last : b;
     }
-    __device__ float width() const { return scale > 0.f ? 1.f / scale / unit : 0.f; }  // a bin's
+    __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
 };
+
+// A CTA's slice of the row: `off` elements behind a 16-byte boundary, in shared memory with -infinity around it, or where
+// it is in global memory, read again by every pass (from L2, mostly).
+template <bool RESIDENT> struct SampleLogits {
+    const float *x;  // of the first element's quad
+    int off, n;
+    __device__ float at(int i) const { return RESIDENT ? x[off + i] : __ldcg(x + off + i); }
+    __device__ float4 quad(int q) const {
+        if constexpr (RESIDENT) return reinterpret_cast<const float4 *>(x)[q];
+        else {
+            if (4 * q >= off && 4 * q + 3 < off + n) return __ldcg(reinterpret_cast<const float4 *>(x) + q);
+            float l[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) l[k] = 4 * q + k >= off && 4 * q + k < off + n ? __ldcg(x + 4 * q + k) : -INFINITY;
+            return make_float4(l[0], l[1], l[2], l[3]);
+        }
+    }
+};
+
+// f(q, quad) for the quads q of [from, to) a thread at a time, `step` apart. Those in global memory come through a ring of
+// the thread's own in shared memory, kRing of them ahead: HBM and L2 are some 2000 cycles away. (Four ahead in registers
+// left the weights' pass of 256 rows waiting half of its 85 us.)
+constexpr int kRing = 8;
+template <bool RESIDENT, typename F>
+__device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float4 *ring, int from, int to, int step, F f) {
+    if constexpr (RESIDENT) {
+        for (int q = from; q < to; q += step) f(q, x.quad(q));
+    } else {
+        float4 *mine = ring + threadIdx.x;
+        const uint32_t slots = (uint32_t)__cvta_generic_to_shared(mine);
+        auto whole = [&](int q) { return 4 * q >= x.off && 4 * q + 3 < x.off + x.n; };
+        auto copy = [&](int q, int slot) {
+            if (q < to && whole(q))
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + slot * (kSampleThreads * 16)), "l"(x.x + 4 * q) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kRing; i++) copy(from + i * step, i);
+        int slot = 0;
+        for (int q = from; q < to; q += step) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+            const float4 y = whole(q) ? mine[slot * kSampleThreads] : x.quad(q);
+            copy(q + kRing * step, slot);
+            slot = slot == kRing - 1 ? 0 : slot + 1;
+            f(q, y);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+}
 
 // The cut by repeated histograms of the cluster: counts and weights in bins of the range in which it must lie, then of the
 // bin that it falls into, until that holds one value. Then who is kept, and the token. All threads of the cluster call it.
-__device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow &r, SampleShared &sh, const float *x, int n, int base,
-                                           int row, float low_all, float high_all, int live, float min_logit) {
+template <bool RESIDENT>
+__device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow &r, SampleShared &sh, const SampleLogits<RESIDENT> &x, int base, int row,
+                                            float low_all, float high_all, int live, float min_logit) {
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const TcmSampling p = a.params[row];
+    const int n = x.n;
     u64 *mass = sh.buffer[0], *all_mass = sh.buffer[1];
     unsigned *count = reinterpret_cast<unsigned *>(mass + kSlowBins), *all_count = reinterpret_cast<unsigned *>(all_mass + kSlowBins);
     static_assert(kSampleList * 8 >= kSlowBins * 12, "the slow search's bins fit the buffers");
@@ -170,10 +222,10 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
             for (int i = tid; i < kSlowBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += kSampleThreads)
-                if (open(x[i])) {
-                    const int b = bins.of(x[i]);
+                if (const float l = x.at(i); open(l)) {
+                    const int b = bins.of(l);
                     atomicAdd(&count[b], 1u);
-                    atomicAdd(&mass[b], r.weight(x[i]));
+                    atomicAdd(&mass[b], r.weight(l));
                 }
             cluster.sync();
             // Each CTA adds up its share of the bins and tells the others.
@@ -215,7 +267,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
             cut.weight = sh.slow_mass;
             float down = INFINITY, up = -INFINITY;
             for (int i = tid; i < n; i += kSampleThreads)
-                if (open(x[i]) && bins.of(x[i]) == bin) down = fminf(down, x[i]), up = fmaxf(up, x[i]);
+                if (const float l = x.at(i); open(l) && bins.of(l) == bin) down = fminf(down, l), up = fmaxf(up, l);
             down = -warp_max(-down), up = warp_max(up);
             if (lane == 0) sh.warp_low[warp] = down, sh.warp_high[warp] = up;
             __syncthreads();
@@ -250,7 +302,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
         u64 whole = cut.weight;
         if (cut.value == -INFINITY) {  // of the row
             u64 m = 0;
-            for (int i = tid; i < n; i += kSampleThreads) m += r.weight(x[i]);
+            for (int i = tid; i < n; i += kSampleThreads) m += r.weight(x.at(i));
             m = warp_sum64(m);
             __syncthreads();
             if (lane == 0) sh.warp_mass[warp] = m;
@@ -283,7 +335,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     int ties_before = 0;
     if (cut.ties) {
         int t = 0;
-        for (int i = w0 + lane; i < w1; i += 32) t += x[i] == cut.value;
+        for (int i = w0 + lane; i < w1; i += 32) t += x.at(i) == cut.value;
         t = __reduce_add_sync(0xffffffffu, t);
         cluster.sync();  // the search's sums have been read
         if (lane == 0) sh.warp_count[warp] = t;
@@ -302,7 +354,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
         int level = ties_before;
         for (int i0 = w0; i0 < w1; i0 += 32) {
             const int i = i0 + lane;
-            const float l = i < w1 ? x[i] : -INFINITY;
+            const float l = i < w1 ? x.at(i) : -INFINITY;
             const bool tie = cut.ties && l == cut.value && i < w1;
             const unsigned tied = __ballot_sync(0xffffffffu, tie);
             const bool keep = l > cut.value || (tie && level + __popc(tied & ((1u << lane) - 1u)) < cut.ties);
@@ -351,7 +403,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
         const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
         if (reached && lane == __ffs(reached) - 1) {
             a.ids[row] = base + i;
-            if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x[i]) - log((double)whole / kSampleOne));
+            if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x.at(i)) - log((double)whole / kSampleOne));
             if (a.kept) a.kept[row] = kept;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -359,11 +411,106 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     });
 }
 
-// The first kResolve threads of a CTA settle the list.
-constexpr int kResolve = 128;
-__device__ __forceinline__ void resolve_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kResolve) : "memory"); }
+// A CTA's share of the cluster's list: every thread holds up to four tokens, as (descending logit, id) in one number.
+constexpr int kEach = kSampleList / kSampleThreads;
 
-__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
+// Of the tokens marked as members, the first in order with which `tokens` of them are reached (by_mass false), or with
+// which `heavier` and their weights make `share`: bins over the range of their numbers, until one holds 32 of them at
+// most. All threads call it; ~0 where there is none. Numbers are unique, so it ends.
+__device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u64 (&w)[kEach], const bool (&member)[kEach], bool by_mass,
+                           int tokens, double share, u64 heavier) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __syncthreads();
+    if (tid == 0) sh.sub_least = 0xffffffffu, sh.sub_most = 0;
+    __syncthreads();
+    uint32_t least = 0xffffffffu, most = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (member[k]) least = min(least, (uint32_t)(token[k] >> 32)), most = max(most, (uint32_t)(token[k] >> 32));
+    least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && least <= most) atomicMin(&sh.sub_least, least), atomicMax(&sh.sub_most, most);
+    __syncthreads();
+    if (sh.sub_least > sh.sub_most) return ~0ull;
+    u64 base = (u64)sh.sub_least << 32, width = ((u64)(sh.sub_most - sh.sub_least) << 32) | 0xffffffffu;
+    int shift = 64 - __clzll((long long)width) - 8;
+    for (;;) {
+        for (int i = tid; i < kSubBins; i += kSampleThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
+        if (tid == 0) sh.few_count = 0, sh.sub_bin = -1;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kEach; k++)
+            if (member[k] && token[k] - base <= width) {
+                const int b = (int)((token[k] - base) >> shift);
+                atomicAdd(&sh.sub_count[b], 1u);
+                if (by_mass) atomicAdd(&sh.sub_mass[b], w[k]);
+            }
+        __syncthreads();
+        if (warp == 0) {
+            constexpr int per_lane = kSubBins / 32;
+            unsigned c[per_lane], upto = 0;
+            u64 m[per_lane], sum = 0;
+#pragma unroll
+            for (int k = 0; k < per_lane; k++) {
+                c[k] = sh.sub_count[lane * per_lane + k], m[k] = sh.sub_mass[lane * per_lane + k];
+                upto += c[k], sum += m[k];
+            }
+            const unsigned mine = upto;
+            const u64 mine_mass = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+                const u64 z = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) upto += y, sum += z;
+            }
+            const bool here = by_mass ? mine && (double)(heavier + sum) >= share : upto >= (unsigned)tokens;
+            const unsigned reached = __ballot_sync(0xffffffffu, here);
+            if (reached && lane == __ffs(reached) - 1) {
+                unsigned above = upto - mine;
+                u64 mass = heavier + sum - mine_mass;
+#pragma unroll
+                for (int k = 0; k < per_lane; k++) {
+                    if (sh.sub_bin < 0 && c[k] && (by_mass ? (double)(mass + m[k]) >= share : above + c[k] >= (unsigned)tokens))
+                        sh.sub_bin = lane * per_lane + k, sh.sub_above = (int)above, sh.found_mass = mass;
+                    above += c[k], mass += m[k];
+                }
+            }
+        }
+        __syncthreads();
+        const int bin = sh.sub_bin;
+        if (bin < 0) return ~0ull;
+        tokens -= sh.sub_above;
+        if (by_mass) heavier = sh.found_mass;
+        base += (u64)bin << shift;
+        width = ((u64)1 << shift) - 1;
+        if (sh.sub_count[bin] <= 32) break;
+        shift = shift > 8 ? shift - 8 : 0;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (member[k] && token[k] - base <= width) {
+            const int i = atomicAdd(&sh.few_count, 1);
+            sh.few[i] = token[k], sh.few_mass[i] = w[k];
+        }
+    __syncthreads();
+    if (warp == 0) {
+        const int few = sh.few_count;
+        const u64 mine = lane < few ? sh.few[lane] : ~0ull, mass = lane < few ? sh.few_mass[lane] : 0;
+        int above = 0;
+        for (int i = 0; i < few; i++)
+            if (sh.few[i] < mine) above++, heavier += sh.few_mass[i];
+        const bool reached = lane < few && (by_mass ? (double)(heavier + mass) >= share : above + 1 >= tokens);
+        // The first of those that reach it.
+        unsigned who = __ballot_sync(0xffffffffu, reached);
+        const int least_above = __reduce_min_sync(0xffffffffu, reached ? above : 64);
+        who = __ballot_sync(0xffffffffu, reached && above == least_above);
+        if (lane == __ffs(who) - 1) sh.found = mine;
+    }
+    __syncthreads();
+    return sh.found;
+}
+
+template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) float slice_memory[];
     __shared__ __align__(16) SampleShared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -377,32 +524,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const TcmSampling p = a.params[row];
     const float u = a.uniforms[row];
 
-    // ---- the slice, and what there is in it. It starts in shared memory as far from a 16-byte boundary as in global
-    // memory, with -infinity around it, so that everything after this goes by whole quads.
+    // ---- what there is in the slice. In shared memory it starts as far from a 16-byte boundary as in global memory, so
+    // that everything goes by whole quads.
     const int off = (int)((uintptr_t)src >> 2) & 3, quads = (off + n + 3) / 4;
-    float *x = slice_memory + off;
-    float4 *x4 = reinterpret_cast<float4 *>(slice_memory);
+    const SampleLogits<RESIDENT> x = {RESIDENT ? slice_memory : src - off, off, n};
+    const SampleLogits<false> global = {src - off, off, n};
+    float4 *ring = reinterpret_cast<float4 *>(slice_memory);  // where the slice is not there
     float most = -INFINITY, least = INFINITY;
     bool bad = false;
-    auto meet = [&](float l) {
-        bad |= !(l < INFINITY);
-        most = fmaxf(most, l), least = fminf(least, l);
+    auto look = [&](int q, const float4 &l) {
+        bad |= !(l.x < INFINITY) | !(l.y < INFINITY) | !(l.z < INFINITY) | !(l.w < INFINITY);
+        most = fmaxf(fmaxf(fmaxf(most, l.x), fmaxf(l.y, l.z)), l.w);
+        if (4 * q >= off && 4 * q + 3 < off + n) least = fminf(fminf(fminf(least, l.x), fminf(l.y, l.z)), l.w);
+        else  // the ends' padding is no masked token
+            for (int i = max(4 * q, off); i < min(4 * q + 4, off + n); i++) least = fminf(least, global.at(i - off));
     };
-    const int q0 = off ? 1 : 0, q1 = (off + n) / 4;  // whole quads
+    if constexpr (RESIDENT) {
 #pragma unroll 4
-    for (int q = q0 + tid; q < q1; q += kSampleThreads) {
-        const float4 l = __ldcg(reinterpret_cast<const float4 *>(src - off) + q);
-        x4[q] = l;
-        meet(l.x), meet(l.y), meet(l.z), meet(l.w);
-    }
-    if (warp == 0) {  // the ends: lanes 0 .. 3 the first quad, 4 .. 7 the last
-        const int i = (lane < 4 ? 0 : 4 * q1) + lane % 4 - off;  // of the slice
-        if ((lane < 4 && q0) || (lane >= 4 && lane < 8 && q1 < quads && (q1 || !q0))) {
-            const bool there = i >= 0 && i < n;
-            const float l = there ? src[i] : -INFINITY;
-            x[i] = l;
-            if (there) meet(l);
+        for (int q = tid; q < quads; q += kSampleThreads) {
+            const float4 l = global.quad(q);
+            reinterpret_cast<float4 *>(slice_memory)[q] = l;
+            look(q, l);
         }
+    } else {
+        each_quad(x, ring, tid, quads, kSampleThreads, look);
     }
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
     uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
@@ -412,7 +557,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (masked) {  // what there is beside masked tokens
         least = INFINITY;
         for (int i = tid; i < n; i += kSampleThreads)
-            if (x[i] > -INFINITY) live++, least = fminf(least, x[i]);
+            if (const float l = x.at(i); l > -INFINITY) live++, least = fminf(least, l);
         warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
         live = __reduce_add_sync(0xffffffffu, live);
     }
@@ -424,7 +569,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const bool ranked = p.top_k > 0 || p.top_p < 1.f;
     if (ranked)
         for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = 0;
+    if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = sh.list_counted = 0;
     __syncthreads();
     cluster.barrier_wait(std::move(started));
     if (warp == 0) {  // lane c tells CTA c
@@ -459,8 +604,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     if (p.temperature == 0.f) {
         int first = 0x7fffffff;
-        for (int i = tid; i < n; i += kSampleThreads)
-            if (x[i] == high) first = min(first, base + i);
+        if (high == sample_value(sh.slices[rank].most))
+#pragma unroll 4
+            for (int q = tid; q < quads; q += kSampleThreads) {
+                const float4 y = x.quad(q);
+                const int id = base + 4 * q - off;
+                if (y.w == high) first = min(first, id + 3);
+                if (y.z == high) first = min(first, id + 2);
+                if (y.y == high) first = min(first, id + 1);
+                if (y.x == high) first = min(first, id);
+            }
         first = __reduce_min_sync(0xffffffffu, first);
         if (lane == 0) sh.warp_count[warp] = first;
         __syncthreads();
@@ -491,41 +644,45 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
 
     // ---- the bins in which the cuts lie
-    const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f;
+    const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f, cuts = by_count || by_mass;
     const float reach = (float)(r.top - 32.0 * (double)p.temperature);
     const SampleBins bins(low < reach && reach < high ? reach : low, high, kSampleBins);
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
     int listed = 0;
-    if (by_count || by_mass) {
+    if (cuts) {
         unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
-        for (int q = tid; q < quads; q += kSampleThreads) {
-            const float4 l = x4[q];
+        each_quad(x, ring, tid, quads, kSampleThreads, [&](int, const float4 &l) {
             if (l.x > -INFINITY) atomicAdd(&own[bins.of(l.x)], 1u);
             if (l.y > -INFINITY) atomicAdd(&own[bins.of(l.y)], 1u);
             if (l.z > -INFINITY) atomicAdd(&own[bins.of(l.z)], 1u);
             if (l.w > -INFINITY) atomicAdd(&own[bins.of(l.w)], 1u);
-        }
-        cluster.sync();
-        // Each CTA adds up its share of the bins and tells the others.
-        const int share_of = kSampleBins / C;
-        for (int i = 4 * tid; i < share_of; i += 4 * kSampleThreads) {
-            const int b = rank * share_of + i;
-            uint4 c = make_uint4(0, 0, 0, 0);
-#pragma unroll 8
-            for (int k = 0; k < C; k++) {
-                const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(own, k) + b);
-                c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
-            }
-#pragma unroll 8
-            for (int k = 0; k < C; k++) *reinterpret_cast<uint4 *>(cluster.map_shared_rank(counts, k) + b) = c;
-        }
+        });
         if (tid == 0) sh.bin = kSampleBins, sh.mass_from = sh.mass_to = kSampleBins - 1;
-        cluster.sync();
+        if (C > 1) {
+            cluster.sync();
+            // Each CTA adds up its share of the bins and tells the others.
+            const int share_of = kSampleBins / C;
+            for (int i = 4 * tid; i < share_of; i += 4 * kSampleThreads) {
+                const int b = rank * share_of + i;
+                uint4 c = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+                for (int k = 0; k < C; k++) {
+                    const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(own, k) + b);
+                    c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
+                }
+#pragma unroll 8
+                for (int k = 0; k < C; k++) *reinterpret_cast<uint4 *>(cluster.map_shared_rank(counts, k) + b) = c;
+            }
+            cluster.sync();
+        } else {
+            __syncthreads();
+            counts = own;
+        }
         constexpr int each = kSampleBins / kSampleThreads;
         unsigned c[each], upto = 0;
-        float mass[each], total = 0.f;
-        const float step = -bins.width() * (float)r.slope;
+        float mass[each], total = 0.f, squares = 0.f;
+        const float step = (float)(-bins.width() * r.slope);
 #pragma unroll
         for (int k = 0; k < each; k += 4) {
             const uint4 y = *reinterpret_cast<const uint4 *>(counts + tid * each + k);
@@ -534,8 +691,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 #pragma unroll
         for (int k = 0; k < each; k++) {
             const int b = tid * each + k;
-            mass[k] = b == kSampleBins - 1 ? 0.f : (float)c[k] * exp2f((float)b * step);
-            upto += c[k], total += mass[k];
+            const float weight = b == kSampleBins - 1 ? 0.f : exp2f((float)b * step);
+            mass[k] = (float)c[k] * weight;
+            upto += c[k], total += mass[k], squares += mass[k] * weight;
         }
         const unsigned mine = upto;
         const float mine_mass = total;
@@ -545,12 +703,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             const float z = __shfl_up_sync(0xffffffffu, total, o);
             if (lane >= o) upto += y, total += z;
         }
-        if (lane == 31) sh.warp_count[warp] = (int)upto, sh.warp_high[warp] = total;
+        squares = warp_sum(squares);
+        if (lane == 31) sh.warp_count[warp] = (int)upto, sh.warp_high[warp] = total, sh.warp_low[warp] = squares;
         __syncthreads();
         unsigned before = upto - mine;
         float lighter = total - mine_mass, whole = 0.f;
+        squares = 0.f;
 #pragma unroll
         for (int w = 0; w < kSampleWarps; w++) {
+            squares += sh.warp_low[w];
             if (w < warp) before += (unsigned)sh.warp_count[w], lighter += sh.warp_high[w];
             whole += sh.warp_high[w];
         }
@@ -575,7 +736,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         listed = in_count_bin;
         if (by_mass) {
             // The bins at which the estimated sum passes the share, a little before and a little behind it.
-            const float share = fmaxf(p.top_p, 0.f) * whole, slack = 2e-5f * whole;
+            // A token's weight is estimated within half a bin's width, so a sum of independent ones within some 0.3 widths
+            // of the root of their squares' sum; four times that, and what FP32 sums are off by.
+            const float share = fmaxf(p.top_p, 0.f) * whole, slack = -0.8f * step * sqrtf(squares) + 2e-5f * whole;
             const int last = min(kSampleBins - 1, count_bin);
             float sum = lighter;
 #pragma unroll
@@ -583,17 +746,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 const int b = tid * each + k;
                 const float next = sum + mass[k];
                 if (c[k]) {
-                    if (sum < share - slack || before == 0) {
-                        if (next >= share - slack) atomicMin(&sh.mass_from, b);
-                    }
+                    if ((sum < share - slack || before == 0) && next >= share - slack) atomicMin(&sh.mass_from, b);
                     if ((sum < share + slack || before == 0) && next >= share + slack) atomicMin(&sh.mass_to, b);
                 }
                 before += c[k], sum = next;
             }
             before -= mine;
             __syncthreads();
-            mass_from = min(sh.mass_from, last), mass_to = min(sh.mass_to, last);
-            if (mass_to < mass_from) mass_to = mass_from;
+            mass_from = min(sh.mass_from, last), mass_to = max(min(sh.mass_to, last), mass_from);
             // How many tokens they hold: those up to the last but not above the first.
 #pragma unroll
             for (int k = 0; k < each; k++) {
@@ -606,62 +766,69 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             listed = sh.list_to - sh.list_from + (mass_to < count_bin ? in_count_bin : 0);
         }
         if (listed > kSampleList) {
-            sample_slowly(a, r, sh, x, n, base, row, low, high, all_live, min_logit);
+            sample_slowly(a, r, sh, x, base, row, low, high, all_live, min_logit);
             return;
         }
+        if (C == 1) __syncthreads();  // the counts have been read: the list takes their place
     }
 
     // ---- weights above the bins, and the list of what is in them. A warp has a contiguous stretch of ids.
     const int kept_to = by_mass ? mass_from : count_bin;  // bins below this are kept whole
     const int per_warp = (quads + kSampleWarps - 1) / kSampleWarps, w0 = min(quads, warp * per_warp), w1 = min(quads, w0 + per_warp);
-    u64 *own_list = sh.buffer[0], *list = sh.buffer[1];
-    u64 sum_all = 0, sum_above = 0, sum_kept = 0;
+    u64 *own_list = sh.buffer[0], *list = C > 1 ? sh.buffer[1] : own_list;
+    u64 sum_above = 0, sum_below = 0, sum_kept = 0;
     int kept = 0;
-    if (by_count || by_mass) {
+    if (cuts) {
         const int needed = by_count ? count_bin : kSampleBins - 1;  // weights end here
-        for (int q = w0 + lane; q < w1; q += 32) {
-            const float4 y = x4[q];
+        const unsigned span = (unsigned)(mass_to - mass_from);      // (wraps where there is no top-p)
+        const bool least_logit = p.min_p > 0.f;
+        // No token of these bins is lower (of the first, by half a bin's width, whatever rounding does).
+        const float lowest = needed == kSampleBins - 1 ? -FLT_MAX : __double2float_rd((double)high - ((double)needed + 1.0) * bins.width());
+        each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+            if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= lowest)) return;
             const float l[4] = {y.x, y.y, y.z, y.w};
             int b[4];
-            bool any = false;
+            bool some = false;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 b[k] = l[k] > -INFINITY ? bins.of(l[k]) : kSampleBins;
-                any |= b[k] <= needed;
+                some |= (by_mass && (unsigned)(b[k] - mass_from) <= span) || (by_count && b[k] == count_bin);
             }
-            if (!any) continue;
+            if (some)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if ((b[k] >= mass_from && b[k] <= mass_to) || (b[k] == count_bin && by_count))
-                    own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l[k]) << 32) | (unsigned)(base + 4 * q + k - off);
+                for (int k = 0; k < 4; k++)
+                    if ((by_mass && (unsigned)(b[k] - mass_from) <= span) || (by_count && b[k] == count_bin))
+                        own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l[k]) << 32) | (unsigned)(base + 4 * q + k - off);
             u64 w[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) w[k] = r.weight(l[k]);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                if (b[k] < count_bin) sum_all += w[k];
-                if (b[k] < kept_to) {
-                    sum_above += w[k];
-                    if (l[k] >= min_logit) sum_kept += w[k], kept++;
-                }
+                if (b[k] < kept_to) sum_above += w[k], kept++;
+                else if (b[k] < count_bin) sum_below += w[k];
             }
-        }
+            if (least_logit)  // of the first, those that min-p takes away
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (b[k] < kept_to && l[k] < min_logit) sum_kept += w[k], kept--;
+        });
+        sum_kept = sum_above - sum_kept;
+        sum_below += sum_above;
     } else {
-        for (int q = w0 + lane; q < w1; q += 32) {
-            const float4 y = x4[q];
+        each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {
             const float l[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const u64 w = r.weight(l[k]);
                 if (l[k] >= min_logit) sum_kept += w, kept++;
             }
-        }
+        });
     }
-    if (by_mass) sum_all = warp_sum64(sum_all), sum_above = warp_sum64(sum_above);
+    if (by_mass) sum_below = warp_sum64(sum_below), sum_above = warp_sum64(sum_above);
     sum_kept = warp_sum64(sum_kept);
     kept = __reduce_add_sync(0xffffffffu, kept);
     if (lane == 0) {
-        sh.warp_mass[warp] = sum_all, sh.warp_more[warp] = sum_above, sh.warp_kept[warp] = sum_kept;
+        sh.warp_mass[warp] = sum_below, sh.warp_more[warp] = sum_above, sh.warp_kept[warp] = sum_kept;
         sh.warp_count[warp] = kept;
     }
     __syncthreads();
@@ -682,130 +849,125 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const u64 before = warp_sum64(lane < rank ? z.kept : 0), whole = warp_sum64(z.kept);
         if (by_mass) z.above = warp_sum64(z.above), z.all = warp_sum64(z.all);
         z.kept_count = __reduce_add_sync(0xffffffffu, z.kept_count);
-        if (lane == 0) sh.before = before, sh.whole = whole, sh.heavier = z.above, sh.everything = z.all, sh.kept = z.kept_count, sh.cut = kSampleList;
+        if (lane == 0) sh.before = before, sh.whole = whole, sh.heavier = z.above, sh.everything = z.all, sh.kept = z.kept_count;
     }
     if (lane == 0) sh.warp_more[warp] = 0;
-    // ---- the list of the cluster, sorted by a few warps: logits descending, ids ascending
-    if (by_count || by_mass) {
+    // ---- the cut in the cluster's list
+    u64 cut = 0;
+    if (cuts) {
         const int m = listed;
-        for (int c = 0, to = 0; c < C; c++) {
-            const int k = sh.sums[c].listed;
-            const u64 *from = cluster.map_shared_rank(own_list, c);
-            for (int i = tid; i < k; i += kSampleThreads) list[to + i] = from[i];
-            to += k;
+        if (C > 1) {
+            for (int c = 0, to = 0; c < C; c++) {
+                const int k = sh.sums[c].listed;
+                const u64 *from = cluster.map_shared_rank(own_list, c);
+                for (int i = tid; i < k; i += kSampleThreads) list[to + i] = from[i];
+                to += k;
+            }
+            cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
         }
-        cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
-        int size = 32;
-        while (size < m) size <<= 1;
-        for (int i = m + tid; i < size; i += kSampleThreads) list[i] = ~0ull;
         __syncthreads();
-        if (tid < kResolve) {
-            for (int k = 2; k <= size; k <<= 1)
-                for (int j = k >> 1; j; j >>= 1) {
-                    for (int i = tid; i < size / 2; i += kResolve) {
-                        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                        const u64 y = list[lo], z = list[hi];
-                        if ((y > z) == ((lo & k) == 0)) list[lo] = z, list[hi] = y;
-                    }
-                    resolve_barrier();
-                }
-            auto logit_at = [&](int i) { return sample_value(~(uint32_t)(list[i] >> 32)); };
-            const int each = size > kResolve ? size / kResolve : 1, i0 = min(m, tid * each), i1 = min(m, i0 + each);
-            int cut = tokens_left - 1;
-            bool fine = true;
-            if (by_mass) {
-                // Sums of weights up to each thread's places.
-                u64 mine = 0;
-                for (int i = i0; i < i1; i++) mine += r.weight(logit_at(i));
-                u64 upto = mine;
+        u64 token[kEach], w[kEach];
+        bool member[kEach], counted[kEach];
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += y;
-                }
-                if (lane == 31) sh.warp_mass[warp] = upto;
-                resolve_barrier();
-                upto -= mine;
-                for (int k = 0; k < warp; k++) upto += sh.warp_mass[k];
-                u64 all_of = sh.everything;
-                const int first = m - in_count_bin, last = first + tokens_left - 1;  // of top-k's bin, its tokens
-                if (by_count) {
-                    u64 sum = upto;
-                    for (int i = i0; i < i1; i++) {
-                        if (i == first) sh.at_first = sum;
-                        sum += r.weight(logit_at(i));
-                        if (i == last) sh.at_last = sum;
-                    }
-                    resolve_barrier();
-                    all_of += sh.at_last - sh.at_first;
-                }
-                const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
-                fine = mass_from == 0 || (double)sh.heavier < share;
-                u64 sum = sh.heavier + upto;
-                int i = i0;
-                for (; i < i1; i++) {
-                    sum += r.weight(logit_at(i));
-                    if ((double)sum >= share) break;
-                }
-                if (i < i1 && (i == 0 || (double)(sum - r.weight(logit_at(i))) < share)) sh.cut = i;
-                resolve_barrier();
-                cut = sh.cut;
-                // In top-p's bins, or the estimate was wrong.
-                fine = fine && cut < m && (!by_count || cut <= last);
-                if (fine) fine = bins.of(logit_at(cut)) <= mass_to;
+        for (int k = 0; k < kEach; k++) {
+            const int i = tid + k * kSampleThreads;
+            token[k] = i < m ? list[i] : ~0ull;
+            w[k] = 0;
+            counted[k] = member[k] = false;
+            if (i < m) {
+                const float l = sample_value(~(uint32_t)(token[k] >> 32));
+                w[k] = r.weight(l);
+                counted[k] = by_count && bins.of(l) == count_bin, member[k] = true;
             }
-            if (tid == 0) {
-                sh.settled = fine;
-                if (fine) sh.cut_key = ~(uint32_t)(list[cut] >> 32), sh.cut_id = (unsigned)list[cut];
-            }
-            if (fine) {  // what is kept of the list, by where it is
-                for (int i = i0; i < i1 && i <= cut; i++) {
-                    const float l = logit_at(i);
-                    if (l < min_logit) continue;
-                    const u64 w = r.weight(l);
-                    const int at = (int)(unsigned)list[i] - base;
-                    atomicAdd(&sh.list_kept, w);
-                    atomicAdd(&sh.list_count, 1);
-                    if (at < 0) atomicAdd(&sh.list_before, w);
-                    else if (at < n) atomicAdd(&sh.warp_more[(at + off) / 4 / per_warp], w);
+        }
+        cut = ~0ull;
+        if (by_count) cut = search_list(sh, token, w, counted, false, tokens_left, 0.0, 0);
+        if (by_mass) {
+            u64 all_of = sh.everything;
+            if (by_count) {
+#pragma unroll
+                for (int k = 0; k < kEach; k++) {
+                    member[k] = member[k] && token[k] <= cut;
+                    if (counted[k] && member[k]) atomicAdd(&sh.list_counted, w[k]);
                 }
+                __syncthreads();
+                all_of += sh.list_counted;
             }
+            const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
+            const u64 last = search_list(sh, token, w, member, true, 0, share, sh.heavier);
+            // In top-p's bins, or the estimate was wrong.
+            const bool fine = (mass_from == 0 || (double)sh.heavier < share) && last != ~0ull &&
+                              bins.of(sample_value(~(uint32_t)(last >> 32))) <= mass_to;
+            if (!fine) {  // the whole cluster alike
+                if (C > 1) cluster.barrier_wait();
+                sample_slowly(a, r, sh, x, base, row, low, high, all_live, min_logit);
+                return;
+            }
+            cut = last;
+        }
+        // What is kept of the list, by where it is.
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            if (!member[k] || token[k] > cut || sample_value(~(uint32_t)(token[k] >> 32)) < min_logit) continue;
+            const int at = (int)(unsigned)token[k] - base;
+            atomicAdd(&sh.list_kept, w[k]);
+            atomicAdd(&sh.list_count, 1);
+            if (at < 0) atomicAdd(&sh.list_before, w[k]);
+            else if (at < n) atomicAdd(&sh.warp_more[(at + off) / 4 / per_warp], w[k]);
         }
     }
     __syncthreads();
-    float cut_value = -INFINITY;
-    unsigned cut_id = 0;
     u64 whole = sh.whole, before = sh.before;
-    if (by_count || by_mass) {
-        if (!sh.settled) {  // the whole cluster alike
-            cluster.barrier_wait();
-            sample_slowly(a, r, sh, x, n, base, row, low, high, all_live, min_logit);
-            return;
-        }
-        cut_value = sample_value(sh.cut_key), cut_id = sh.cut_id;
-        whole += sh.list_kept, before += sh.list_before;
-    }
+    const float cut_value = cuts ? sample_value(~(uint32_t)(cut >> 32)) : -INFINITY;
+    const unsigned cut_id = (unsigned)cut;
+    if (cuts) whole += sh.list_kept, before += sh.list_before;
     u64 target = (u64)((double)u * (double)whole);
     if (target >= whole) target = whole - 1;
-    {
-        const u64 w = lane < kSampleWarps ? sh.warp_kept[lane] + sh.warp_more[lane] : 0;  // of each warp's stretch
-        before += warp_sum64(lane < warp ? w : 0);
-        const u64 own = __shfl_sync(0xffffffffu, w, warp);
-        if (target >= before && target < before + own) {  // one warp of the cluster has the token
-            for (int q0 = w0; q0 < w1; q0 += 32) {
-                const int q = q0 + lane;
-                const float4 y = q < w1 ? x4[q] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                const float l[4] = {y.x, y.y, y.z, y.w};
-                u64 w4[4], mine = 0;
+
+    // ---- the token: the warp's stretch that holds it, in 16 parts for the warps, then the part by one warp
+    auto weights = [&](int q, u64 (&w)[4]) {  // what is kept of a quad
+        const float4 y = x.quad(q);
+        const float l[4] = {y.x, y.y, y.z, y.w};
+        u64 sum = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const unsigned id = (unsigned)(base + 4 * q + k - off);
-                    const bool stays = (l[k] > cut_value || (l[k] == cut_value && id <= cut_id)) && l[k] >= min_logit;
-                    w4[k] = r.weight(l[k]);
-                    if (!stays) w4[k] = 0;
-                    mine += w4[k];
-                }
-                u64 upto = mine;
+        for (int k = 0; k < 4; k++) {
+            const unsigned id = (unsigned)(base + 4 * q + k - off);
+            const bool stays = (l[k] > cut_value || (l[k] == cut_value && id <= cut_id)) && l[k] >= min_logit;
+            w[k] = r.weight(l[k]);
+            if (!stays) w[k] = 0;
+            sum += w[k];
+        }
+        return sum;
+    };
+    // Which of 16 consecutive sums passes the target; -1: none. `before` moves to its start.
+    auto holder = [&](u64 mine) {
+        u64 upto = mine;
+#pragma unroll
+        for (int o = 1; o < kSampleWarps; o <<= 1) {
+            const u64 z = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += z;
+        }
+        const unsigned reached = __ballot_sync(0xffffffffu, lane < kSampleWarps && target >= before + upto - mine && target < before + upto);
+        const int who = __ffs(reached) - 1;
+        if (who >= 0) before += __shfl_sync(0xffffffffu, upto - mine, who);
+        return who;
+    };
+    const int who = holder(lane < kSampleWarps ? sh.warp_kept[lane] + sh.warp_more[lane] : 0);
+    if (who >= 0) {  // this CTA has it
+        const int s0 = min(quads, who * per_warp), s1 = min(quads, s0 + per_warp), part = (s1 - s0 + kSampleWarps - 1) / kSampleWarps;
+        u64 w[4], sum = 0;
+        for (int q = s0 + warp * part + lane; q < min(s1, s0 + (warp + 1) * part); q += 32) sum += weights(q, w);
+        sum = warp_sum64(sum);
+        if (lane == 0) sh.warp_mass[warp] = sum;
+        __syncthreads();
+        const int mine = holder(lane < kSampleWarps ? sh.warp_mass[lane] : 0);
+        if (warp == mine) {
+            const int q1 = min(s1, s0 + (warp + 1) * part);
+            for (int q0 = s0 + warp * part; q0 < q1; q0 += 32) {
+                const int q = q0 + lane;
+                w[0] = w[1] = w[2] = w[3] = 0;
+                const u64 own = q < q1 ? weights(q, w) : 0;
+                u64 upto = own;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const u64 z = __shfl_up_sync(0xffffffffu, upto, o);
@@ -814,17 +976,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
                 const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
                 if (reached) {
                     if (lane == __ffs(reached) - 1) {
-                        u64 sum = before + upto;
+                        u64 to = before + upto;
                         int id = 0;
-                        float logit = 0.f;
 #pragma unroll
                         for (int k = 3; k >= 0; k--) {  // the first of the four at which the sum passes the target
-                            if (sum > target && w4[k]) id = base + 4 * q + k - off, logit = l[k];
-                            sum -= w4[k];
+                            if (to > target && w[k]) id = 4 * q + k - off;
+                            to -= w[k];
                         }
-                        a.ids[row] = id;
-                        if (a.logprobs) a.logprobs[row] = (float)(r.exponent(logit) - log((double)whole / kSampleOne));
-                        if (a.kept) a.kept[row] = sh.kept + ((by_count || by_mass) ? sh.list_count : 0);
+                        a.ids[row] = base + id;
+                        if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x.at(id)) - log((double)whole / kSampleOne));
+                        if (a.kept) a.kept[row] = sh.kept + (cuts ? sh.list_count : 0);
                     }
                     break;
                 }
@@ -832,7 +993,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             }
         }
     }
-    if (by_count || by_mass) cluster.barrier_wait();
+    if (cuts && C > 1) cluster.barrier_wait();
 }
 
 int refuse(const char *why) {
@@ -858,18 +1019,23 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
         return refuse("arrays are 4-byte aligned");
     static PerDeviceOnce once;
     once.run([] {
-        TCM_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSampleSlice + 8) * 4));
-        TCM_CUDA(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleOwnSm));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing * kSampleThreads * 16));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
-    // Few rows take all the SMs that help; many rows the fewest CTAs whose slices leave room for two an SM.
+    // As many CTAs a row as run at once for all rows, of 1024 tokens at least.
     int cluster = kSampleCluster;
-    while (cluster > 1 && (vocab < cluster * 1024 || (rows * cluster > 2 * sm_count() && vocab <= cluster / 2 * 19456))) cluster /= 2;
+    while (cluster > 1 && (vocab < cluster * 1024 || (long long)rows * cluster > 2 * sm_count())) cluster /= 2;
     const int slice = ((vocab + cluster - 1) / cluster + 3) / 4 * 4;
+    // In shared memory where that takes no CTA off its SM.
+    const long long smem = (slice + 8) * 4ll;
+    const bool resident = smem <= ((long long)rows * cluster <= sm_count() ? kSampleOwnSm : kSampleHalfSm);
     const SampleArgs args = {ids, logprobs, kept, logits, stride, vocab, slice, params, uniforms, status};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * cluster);
     cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = (size_t)(slice + 8) * 4;
+    cfg.dynamicSmemBytes = resident ? (size_t)smem : kRing * kSampleThreads * 16;
     cfg.stream = stream();
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -878,6 +1044,7 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    TCM_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel, args));
+    if (resident) TCM_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<true>, args));
+    else TCM_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<false>, args));
     return 0;
 }
