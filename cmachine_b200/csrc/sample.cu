@@ -30,7 +30,7 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256;
+constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 72 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 constexpr double kSampleOne = 0x1p44;
@@ -77,10 +77,12 @@ struct SampleShared {
     int mass_from, mass_to;  // top-p's bins, first and last,
     int list_from, list_to;  // and the tokens above the first, up to the last
     // The search for the cut in the list.
-    u64 sub_mass[kSubBins], few[32], few_mass[32], found, found_mass;
+    u64 sub_mass[kSubBins], few[kFew], few_mass[kFew], found, found_mass;
     unsigned sub_count[kSubBins];
     uint32_t sub_least, sub_most;
     int sub_bin, sub_above, few_count;
+    float border[4];
+    int list_start[kSampleCluster];
     u64 slow_mass;
 };
 
@@ -415,77 +417,83 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
 constexpr int kEach = kSampleList / kSampleThreads;
 
 // Of the tokens marked as members, the first in order with which `tokens` of them are reached (by_mass false), or with
-// which `heavier` and their weights make `share`: bins over the range of their numbers, until one holds 32 of them at
-// most. All threads call it; ~0 where there is none. Numbers are unique, so it ends.
-__device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u64 (&w)[kEach], const bool (&member)[kEach], bool by_mass,
-                           int tokens, double share, u64 heavier) {
+// which `heavier` and their weights make `share`: bins over the range of their numbers, until one holds kFew of them at
+// most (there are `most_members` in all at most), which are compared with one another. All threads call it; ~0
+// where there is none. Numbers are unique, so it ends.
+__device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u64 (&w)[kEach], const bool (&member)[kEach], int most_members,
+                           bool by_mass, int tokens, double share, u64 heavier) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 base = 0, width = ~0ull;
     __syncthreads();
-    if (tid == 0) sh.sub_least = 0xffffffffu, sh.sub_most = 0;
-    __syncthreads();
-    uint32_t least = 0xffffffffu, most = 0;
-#pragma unroll
-    for (int k = 0; k < kEach; k++)
-        if (member[k]) least = min(least, (uint32_t)(token[k] >> 32)), most = max(most, (uint32_t)(token[k] >> 32));
-    least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0 && least <= most) atomicMin(&sh.sub_least, least), atomicMax(&sh.sub_most, most);
-    __syncthreads();
-    if (sh.sub_least > sh.sub_most) return ~0ull;
-    u64 base = (u64)sh.sub_least << 32, width = ((u64)(sh.sub_most - sh.sub_least) << 32) | 0xffffffffu;
-    int shift = 64 - __clzll((long long)width) - 8;
-    for (;;) {
-        for (int i = tid; i < kSubBins; i += kSampleThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
-        if (tid == 0) sh.few_count = 0, sh.sub_bin = -1;
+    if (tid == 0) sh.few_count = 0, sh.found = ~0ull;
+    if (most_members > kFew) {
+        if (tid == 0) sh.sub_least = 0xffffffffu, sh.sub_most = 0;
         __syncthreads();
+        uint32_t least = 0xffffffffu, most = 0;
 #pragma unroll
         for (int k = 0; k < kEach; k++)
-            if (member[k] && token[k] - base <= width) {
-                const int b = (int)((token[k] - base) >> shift);
-                atomicAdd(&sh.sub_count[b], 1u);
-                if (by_mass) atomicAdd(&sh.sub_mass[b], w[k]);
-            }
+            if (member[k]) least = min(least, (uint32_t)(token[k] >> 32)), most = max(most, (uint32_t)(token[k] >> 32));
+        least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0 && least <= most) atomicMin(&sh.sub_least, least), atomicMax(&sh.sub_most, most);
         __syncthreads();
-        if (warp == 0) {
-            constexpr int per_lane = kSubBins / 32;
-            unsigned c[per_lane], upto = 0;
-            u64 m[per_lane], sum = 0;
+        if (sh.sub_least > sh.sub_most) return ~0ull;
+        base = (u64)sh.sub_least << 32, width = ((u64)(sh.sub_most - sh.sub_least) << 32) | 0xffffffffu;
+        int shift = 64 - __clzll((long long)width) - 8;
+        for (;;) {
+            for (int i = tid; i < kSubBins; i += kSampleThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
+            if (tid == 0) sh.sub_bin = -1;
+            __syncthreads();
 #pragma unroll
-            for (int k = 0; k < per_lane; k++) {
-                c[k] = sh.sub_count[lane * per_lane + k], m[k] = sh.sub_mass[lane * per_lane + k];
-                upto += c[k], sum += m[k];
-            }
-            const unsigned mine = upto;
-            const u64 mine_mass = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
-                const u64 z = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) upto += y, sum += z;
-            }
-            const bool here = by_mass ? mine && (double)(heavier + sum) >= share : upto >= (unsigned)tokens;
-            const unsigned reached = __ballot_sync(0xffffffffu, here);
-            if (reached && lane == __ffs(reached) - 1) {
-                unsigned above = upto - mine;
-                u64 mass = heavier + sum - mine_mass;
+            for (int k = 0; k < kEach; k++)
+                if (member[k] && token[k] - base <= width) {
+                    const int b = (int)((token[k] - base) >> shift);
+                    atomicAdd(&sh.sub_count[b], 1u);
+                    if (by_mass) atomicAdd(&sh.sub_mass[b], w[k]);
+                }
+            __syncthreads();
+            if (warp == 0) {
+                constexpr int per_lane = kSubBins / 32;
+                unsigned c[per_lane], upto = 0;
+                u64 m[per_lane], sum = 0;
 #pragma unroll
                 for (int k = 0; k < per_lane; k++) {
-                    if (sh.sub_bin < 0 && c[k] && (by_mass ? (double)(mass + m[k]) >= share : above + c[k] >= (unsigned)tokens))
-                        sh.sub_bin = lane * per_lane + k, sh.sub_above = (int)above, sh.found_mass = mass;
-                    above += c[k], mass += m[k];
+                    c[k] = sh.sub_count[lane * per_lane + k], m[k] = sh.sub_mass[lane * per_lane + k];
+                    upto += c[k], sum += m[k];
+                }
+                const unsigned mine = upto;
+                const u64 mine_mass = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+                    const u64 z = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (lane >= o) upto += y, sum += z;
+                }
+                const bool here = by_mass ? mine && (double)(heavier + sum) >= share : upto >= (unsigned)tokens;
+                const unsigned reached = __ballot_sync(0xffffffffu, here);
+                if (reached && lane == __ffs(reached) - 1) {
+                    unsigned above = upto - mine;
+                    u64 mass = heavier + sum - mine_mass;
+#pragma unroll
+                    for (int k = 0; k < per_lane; k++) {
+                        if (sh.sub_bin < 0 && c[k] && (by_mass ? (double)(mass + m[k]) >= share : above + c[k] >= (unsigned)tokens))
+                            sh.sub_bin = lane * per_lane + k, sh.sub_above = (int)above, sh.found_mass = mass;
+                        above += c[k], mass += m[k];
+                    }
                 }
             }
+            __syncthreads();
+            const int bin = sh.sub_bin;
+            if (bin < 0) return ~0ull;
+            tokens -= sh.sub_above;
+            if (by_mass) heavier = sh.found_mass;
+            base += (u64)bin << shift;
+            width = ((u64)1 << shift) - 1;
+            if (sh.sub_count[bin] <= kFew) break;
+            shift = shift > 8 ? shift - 8 : 0;
+            __syncthreads();
         }
-        __syncthreads();
-        const int bin = sh.sub_bin;
-        if (bin < 0) return ~0ull;
-        tokens -= sh.sub_above;
-        if (by_mass) heavier = sh.found_mass;
-        base += (u64)bin << shift;
-        width = ((u64)1 << shift) - 1;
-        if (sh.sub_count[bin] <= 32) break;
-        shift = shift > 8 ? shift - 8 : 0;
-        __syncthreads();
     }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEach; k++)
         if (member[k] && token[k] - base <= width) {
@@ -493,18 +501,14 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
             sh.few[i] = token[k], sh.few_mass[i] = w[k];
         }
     __syncthreads();
-    if (warp == 0) {
-        const int few = sh.few_count;
-        const u64 mine = lane < few ? sh.few[lane] : ~0ull, mass = lane < few ? sh.few_mass[lane] : 0;
+    const int few = sh.few_count;
+    if (tid < few) {
+        const u64 mine = sh.few[tid], mass = sh.few_mass[tid];
         int above = 0;
         for (int i = 0; i < few; i++)
             if (sh.few[i] < mine) above++, heavier += sh.few_mass[i];
-        const bool reached = lane < few && (by_mass ? (double)(heavier + mass) >= share : above + 1 >= tokens);
-        // The first of those that reach it.
-        unsigned who = __ballot_sync(0xffffffffu, reached);
-        const int least_above = __reduce_min_sync(0xffffffffu, reached ? above : 64);
-        who = __ballot_sync(0xffffffffu, reached && above == least_above);
-        if (lane == __ffs(who) - 1) sh.found = mine;
+        // The first at which it is reached: the one before it does not reach it.
+        if (by_mass ? (double)(heavier + mass) >= share && (!above || (double)heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
     }
     __syncthreads();
     return sh.found;
@@ -650,6 +654,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
     int listed = 0;
+    bool all_listed = false;
     if (cuts) {
         unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
         each_quad(x, ring, tid, quads, kSampleThreads, [&](int, const float4 &l) {
@@ -732,9 +737,13 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             __syncthreads();
             count_bin = sh.bin, tokens_left = p.top_k - sh.above, in_count_bin = sh.in_bin;
             whole = sh.mass_whole;
+            all_listed = sh.above + sh.in_bin <= kSampleList;
         }
         listed = in_count_bin;
-        if (by_mass) {
+        if (all_listed) {  // a small k: all tokens down to its bin, and no estimate
+            mass_from = 0, mass_to = count_bin;
+            listed += sh.above, tokens_left = p.top_k;
+        } else if (by_mass) {
             // The bins at which the estimated sum passes the share, a little before and a little behind it.
             // A token's weight is estimated within half a bin's width, so a sum of independent ones within some 0.3 widths
             // of the root of their squares' sum; four times that, and what FP32 sums are off by.
@@ -773,47 +782,59 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     }
 
     // ---- weights above the bins, and the list of what is in them. A warp has a contiguous stretch of ids.
-    const int kept_to = by_mass ? mass_from : count_bin;  // bins below this are kept whole
     const int per_warp = (quads + kSampleWarps - 1) / kSampleWarps, w0 = min(quads, warp * per_warp), w1 = min(quads, w0 + per_warp);
-    u64 *own_list = sh.buffer[0], *list = C > 1 ? sh.buffer[1] : own_list;
+    u64 *own_list = sh.buffer[0];
     u64 sum_above = 0, sum_below = 0, sum_kept = 0;
     int kept = 0;
     if (cuts) {
-        const int needed = by_count ? count_bin : kSampleBins - 1;  // weights end here
-        const unsigned span = (unsigned)(mass_to - mass_from);      // (wraps where there is no top-p)
+        // The bins' borders as logits: the least of a bin and those above it, found by halving as the arithmetic of bins.of()
+        // has it. Tokens from `sure` on are above the bins in question and kept; from `in_from` down to `in_to` in top-p's,
+        // from `count_from` down to `count_to` in top-k's.
+        if (warp == 0) {
+            const int b = lane == 0 ? (by_mass || all_listed ? mass_from : count_bin) - 1 : lane == 1 ? mass_to : lane == 2 ? count_bin - 1 : count_bin;
+            uint32_t down = sample_key(-FLT_MAX), up = sample_key(high);  // bins.of(up) <= b, or none is
+            if (b < 0) down = up = sample_key(INFINITY);
+            else if (bins.of(-FLT_MAX) <= b) up = down;
+            while (down < up) {
+                const uint32_t mid = down + (up - down) / 2;
+                if (bins.of(sample_value(mid)) <= b) up = mid;
+                else down = mid + 1;
+            }
+            if (lane < 4) sh.border[lane] = sample_value(up);
+        }
+        __syncthreads();
+        const bool ranged = by_mass || all_listed;
+        const float sure = sh.border[0], in_to = ranged ? sh.border[1] : INFINITY;
+        const float count_from = by_count ? sh.border[2] : -FLT_MAX, count_to = by_count ? sh.border[3] : INFINITY;
+        const float lowest = by_count ? count_to : -FLT_MAX;
         const bool least_logit = p.min_p > 0.f;
-        // No token of these bins is lower (of the first, by half a bin's width, whatever rounding does).
-        const float lowest = needed == kSampleBins - 1 ? -FLT_MAX : __double2float_rd((double)high - ((double)needed + 1.0) * bins.width());
+        auto append = [&](float l, int i) { own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << 32) | (unsigned)(base + i); };
+        auto in_question = [&](float l) { return (l < sure && l >= in_to) || (l < count_from && l >= count_to); };
         each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
             if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= lowest)) return;
             const float l[4] = {y.x, y.y, y.z, y.w};
-            int b[4];
             bool some = false;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                b[k] = l[k] > -INFINITY ? bins.of(l[k]) : kSampleBins;
-                some |= (by_mass && (unsigned)(b[k] - mass_from) <= span) || (by_count && b[k] == count_bin);
-            }
+            for (int k = 0; k < 4; k++) some |= in_question(l[k]);
             if (some)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    if ((by_mass && (unsigned)(b[k] - mass_from) <= span) || (by_count && b[k] == count_bin))
-                        own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l[k]) << 32) | (unsigned)(base + 4 * q + k - off);
+                    if (in_question(l[k])) append(l[k], 4 * q + k - off);
+            if (all_listed) return;
             u64 w[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) w[k] = r.weight(l[k]);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                if (b[k] < kept_to) sum_above += w[k], kept++;
-                else if (b[k] < count_bin) sum_below += w[k];
+                if (l[k] >= sure) sum_above += w[k], kept++;
+                if (l[k] >= count_from) sum_below += w[k];
             }
             if (least_logit)  // of the first, those that min-p takes away
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    if (b[k] < kept_to && l[k] < min_logit) sum_kept += w[k], kept--;
+                    if (l[k] >= sure && l[k] < min_logit) sum_kept += w[k], kept--;
         });
         sum_kept = sum_above - sum_kept;
-        sum_below += sum_above;
     } else {
         each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {
             const float l[4] = {y.x, y.y, y.z, y.w};
@@ -850,51 +871,58 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         if (by_mass) z.above = warp_sum64(z.above), z.all = warp_sum64(z.all);
         z.kept_count = __reduce_add_sync(0xffffffffu, z.kept_count);
         if (lane == 0) sh.before = before, sh.whole = whole, sh.heavier = z.above, sh.everything = z.all, sh.kept = z.kept_count;
+        int upto = z.listed;
+#pragma unroll
+        for (int o = 1; o < kSampleCluster; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane < C) sh.list_start[lane] = upto - z.listed;
     }
     if (lane == 0) sh.warp_more[warp] = 0;
     // ---- the cut in the cluster's list
     u64 cut = 0;
     if (cuts) {
         const int m = listed;
-        if (C > 1) {
-            for (int c = 0, to = 0; c < C; c++) {
-                const int k = sh.sums[c].listed;
-                const u64 *from = cluster.map_shared_rank(own_list, c);
-                for (int i = tid; i < k; i += kSampleThreads) list[to + i] = from[i];
-                to += k;
-            }
-            cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
-        }
         __syncthreads();
         u64 token[kEach], w[kEach];
         bool member[kEach], counted[kEach];
 #pragma unroll
         for (int k = 0; k < kEach; k++) {
             const int i = tid + k * kSampleThreads;
-            token[k] = i < m ? list[i] : ~0ull;
-            w[k] = 0;
-            counted[k] = member[k] = false;
-            if (i < m) {
-                const float l = sample_value(~(uint32_t)(token[k] >> 32));
-                w[k] = r.weight(l);
-                counted[k] = by_count && bins.of(l) == count_bin, member[k] = true;
+            token[k] = ~0ull;
+            member[k] = i < m;
+            if (member[k]) {
+                int c = 0;
+                while (c + 1 < C && sh.list_start[c + 1] <= i) c++;
+                token[k] = cluster.map_shared_rank(own_list, c)[i - sh.list_start[c]];
             }
         }
+#pragma unroll
+        for (int k = 0; k < kEach; k++) {
+            const float l = sample_value(~(uint32_t)(token[k] >> 32));
+            w[k] = member[k] ? r.weight(l) : 0;
+            counted[k] = member[k] && by_count && bins.of(l) <= count_bin && (all_listed || bins.of(l) == count_bin);
+        }
+        if (C > 1) cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
         cut = ~0ull;
-        if (by_count) cut = search_list(sh, token, w, counted, false, tokens_left, 0.0, 0);
+        if (by_count) cut = search_list(sh, token, w, counted, m, false, tokens_left, 0.0, 0);
         if (by_mass) {
             u64 all_of = sh.everything;
             if (by_count) {
+                u64 sum = 0;
 #pragma unroll
                 for (int k = 0; k < kEach; k++) {
                     member[k] = member[k] && token[k] <= cut;
-                    if (counted[k] && member[k]) atomicAdd(&sh.list_counted, w[k]);
+                    if (counted[k] && member[k]) sum += w[k];
                 }
+                sum = warp_sum64(sum);
+                if (lane == 0 && sum) atomicAdd(&sh.list_counted, sum);
                 __syncthreads();
                 all_of += sh.list_counted;
             }
             const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
-            const u64 last = search_list(sh, token, w, member, true, 0, share, sh.heavier);
+            const u64 last = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
             // In top-p's bins, or the estimate was wrong.
             const bool fine = (mass_from == 0 || (double)sh.heavier < share) && last != ~0ull &&
                               bins.of(sample_value(~(uint32_t)(last >> 32))) <= mass_to;
@@ -906,14 +934,22 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             cut = last;
         }
         // What is kept of the list, by where it is.
+        u64 sum = 0, ahead = 0;
+        int count = 0;
 #pragma unroll
         for (int k = 0; k < kEach; k++) {
             if (!member[k] || token[k] > cut || sample_value(~(uint32_t)(token[k] >> 32)) < min_logit) continue;
             const int at = (int)(unsigned)token[k] - base;
-            atomicAdd(&sh.list_kept, w[k]);
-            atomicAdd(&sh.list_count, 1);
-            if (at < 0) atomicAdd(&sh.list_before, w[k]);
+            sum += w[k], count++;
+            if (at < 0) ahead += w[k];
             else if (at < n) atomicAdd(&sh.warp_more[(at + off) / 4 / per_warp], w[k]);
+        }
+        sum = warp_sum64(sum), ahead = warp_sum64(ahead);
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (lane == 0 && count) {
+            atomicAdd(&sh.list_kept, sum);
+            atomicAdd(&sh.list_count, count);
+            if (ahead) atomicAdd(&sh.list_before, ahead);
         }
     }
     __syncthreads();
