@@ -32,7 +32,7 @@ namespace {
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
-constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 72 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
+constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 constexpr double kSampleOne = 0x1p44;
 typedef unsigned long long u64;
 
@@ -77,8 +77,7 @@ struct SampleShared {
     int mass_from, mass_to;  // top-p's bins, first and last,
     int list_from, list_to;  // and the tokens above the first, up to the last
     // The search for the cut in the list.
-    u64 sub_mass[kSubBins], few[kFew], few_mass[kFew], found, found_mass;
-    unsigned sub_count[kSubBins];
+    u64 found, found_mass;
     uint32_t sub_least, sub_most;
     int sub_bin, sub_above, few_count;
     float border[4];
@@ -413,6 +412,13 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     });
 }
 
+// The memory of the search for the cut in the list, in the place of the cluster's counts.
+struct SampleSearch {
+    u64 mass[kSubBins], few[kFew], few_mass[kFew];
+    unsigned count[kSubBins];
+};
+static_assert(sizeof(SampleSearch) <= sizeof(SampleShared::buffer[1]), "the search's memory fits the buffer");
+
 // A CTA's share of the cluster's list: every thread holds up to four tokens, as (descending logit, id) in one number.
 constexpr int kEach = kSampleList / kSampleThreads;
 
@@ -423,6 +429,7 @@ constexpr int kEach = kSampleList / kSampleThreads;
 __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u64 (&w)[kEach], const bool (&member)[kEach], int most_members,
                            bool by_mass, int tokens, double share, u64 heavier) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    SampleSearch &in = *reinterpret_cast<SampleSearch *>(sh.buffer[1]);
     u64 base = 0, width = ~0ull;
     __syncthreads();
     if (tid == 0) sh.few_count = 0, sh.found = ~0ull;
@@ -440,15 +447,15 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
         base = (u64)sh.sub_least << 32, width = ((u64)(sh.sub_most - sh.sub_least) << 32) | 0xffffffffu;
         int shift = 64 - __clzll((long long)width) - 8;
         for (;;) {
-            for (int i = tid; i < kSubBins; i += kSampleThreads) sh.sub_count[i] = 0, sh.sub_mass[i] = 0;
+            for (int i = tid; i < kSubBins; i += kSampleThreads) in.count[i] = 0, in.mass[i] = 0;
             if (tid == 0) sh.sub_bin = -1;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kEach; k++)
                 if (member[k] && token[k] - base <= width) {
                     const int b = (int)((token[k] - base) >> shift);
-                    atomicAdd(&sh.sub_count[b], 1u);
-                    if (by_mass) atomicAdd(&sh.sub_mass[b], w[k]);
+                    atomicAdd(&in.count[b], 1u);
+                    if (by_mass) atomicAdd(&in.mass[b], w[k]);
                 }
             __syncthreads();
             if (warp == 0) {
@@ -457,7 +464,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
                 u64 m[per_lane], sum = 0;
 #pragma unroll
                 for (int k = 0; k < per_lane; k++) {
-                    c[k] = sh.sub_count[lane * per_lane + k], m[k] = sh.sub_mass[lane * per_lane + k];
+                    c[k] = in.count[lane * per_lane + k], m[k] = in.mass[lane * per_lane + k];
                     upto += c[k], sum += m[k];
                 }
                 const unsigned mine = upto;
@@ -488,7 +495,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
             if (by_mass) heavier = sh.found_mass;
             base += (u64)bin << shift;
             width = ((u64)1 << shift) - 1;
-            if (sh.sub_count[bin] <= kFew) break;
+            if (in.count[bin] <= kFew) break;
             shift = shift > 8 ? shift - 8 : 0;
             __syncthreads();
         }
@@ -498,15 +505,15 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
     for (int k = 0; k < kEach; k++)
         if (member[k] && token[k] - base <= width) {
             const int i = atomicAdd(&sh.few_count, 1);
-            sh.few[i] = token[k], sh.few_mass[i] = w[k];
+            in.few[i] = token[k], in.few_mass[i] = w[k];
         }
     __syncthreads();
     const int few = sh.few_count;
     if (tid < few) {
-        const u64 mine = sh.few[tid], mass = sh.few_mass[tid];
+        const u64 mine = in.few[tid], mass = in.few_mass[tid];
         int above = 0;
         for (int i = 0; i < few; i++)
-            if (sh.few[i] < mine) above++, heavier += sh.few_mass[i];
+            if (in.few[i] < mine) above++, heavier += in.few_mass[i];
         // The first at which it is reached: the one before it does not reach it.
         if (by_mass ? (double)(heavier + mass) >= share && (!above || (double)heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
     }
@@ -1060,13 +1067,15 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
-    // As many CTAs a row as run at once for all rows, of 1024 tokens at least.
-    int cluster = kSampleCluster;
+    // As many CTAs a row as run at once for all rows, of 1024 tokens at least; 16 only where every CTA has an SM of its own.
+    // Measured with rows of 151,936 and top-p, us for 1, 2, 4, 8, 16 CTAs a row: 1 row 120, 71, 38, 29, 25; 16 rows 121, 80, 39,
+    // 39, 52; 64 rows 158, 107, 73, 80, 143; 256 rows 205, 224, 264, 330, 541.
+    int cluster = (long long)rows * kSampleCluster <= sm_count() ? kSampleCluster : kSampleCluster / 2;
     while (cluster > 1 && (vocab < cluster * 1024 || (long long)rows * cluster > 2 * sm_count())) cluster /= 2;
     const int slice = ((vocab + cluster - 1) / cluster + 3) / 4 * 4;
     // In shared memory where that takes no CTA off its SM.
     const long long smem = (slice + 8) * 4ll;
-    const bool resident = smem <= ((long long)rows * cluster <= sm_count() ? kSampleOwnSm : kSampleHalfSm);
+    const bool resident = smem <= ((long long)rows * cluster <= sm_count() && smem > kSampleHalfSm ? kSampleOwnSm : kSampleHalfSm);
     const SampleArgs args = {ids, logprobs, kept, logits, stride, vocab, slice, params, uniforms, status};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * cluster);
