@@ -543,12 +543,15 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     float4 *ring = reinterpret_cast<float4 *>(slice_memory);  // where the slice is not there
     float most = -INFINITY, least = INFINITY;
     bool bad = false;
-    auto look = [&](int q, const float4 &l) {
-        bad |= !(l.x < INFINITY) | !(l.y < INFINITY) | !(l.z < INFINITY) | !(l.w < INFINITY);
-        most = fmaxf(fmaxf(fmaxf(most, l.x), fmaxf(l.y, l.z)), l.w);
-        if (4 * q >= off && 4 * q + 3 < off + n) least = fminf(fminf(fminf(least, l.x), fminf(l.y, l.z)), l.w);
-        else  // the ends' padding is no masked token
-            for (int i = max(4 * q, off); i < min(4 * q + 4, off + n); i++) least = fminf(least, global.at(i - off));
+    int live = 0;
+    auto look = [&](int, const float4 &y) {
+        const float l[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            bad |= !(l[k] < INFINITY);
+            most = fmaxf(most, l[k]);
+            if (l[k] > -INFINITY) live++, least = fminf(least, l[k]);
+        }
     };
     if constexpr (RESIDENT) {
 #pragma unroll 4
@@ -561,17 +564,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         each_quad(x, ring, tid, quads, kSampleThreads, look);
     }
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
-    uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
+    const uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
     bad = __any_sync(0xffffffffu, bad);
-    int live = 0;
-    const bool masked = __syncthreads_or(least == -INFINITY);
-    if (masked) {  // what there is beside masked tokens
-        least = INFINITY;
-        for (int i = tid; i < n; i += kSampleThreads)
-            if (const float l = x.at(i); l > -INFINITY) live++, least = fminf(least, l);
-        warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
-        live = __reduce_add_sync(0xffffffffu, live);
-    }
+    live = __reduce_add_sync(0xffffffffu, live);
     if (lane == 0) {
         sh.warp_count[warp] = live;
         reinterpret_cast<uint32_t *>(sh.warp_high)[warp] = warp_most, reinterpret_cast<uint32_t *>(sh.warp_low)[warp] = warp_least;
@@ -590,7 +585,6 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         z.least = __reduce_min_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_low)[w]);
         z.live = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? sh.warp_count[w] : 0);
         z.bad = __any_sync(0xffffffffu, sh.warp_mass[w] != 0);
-        if (!masked) z.live = n;
         if (lane < C) cluster.map_shared_rank(sh.slices, lane)[rank] = z;
     }
     cluster.sync();
@@ -791,7 +785,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     // ---- weights above the bins, and the list of what is in them. A warp has a contiguous stretch of ids.
     const int per_warp = (quads + kSampleWarps - 1) / kSampleWarps, w0 = min(quads, warp * per_warp), w1 = min(quads, w0 + per_warp);
     u64 *own_list = sh.buffer[0];
-    u64 sum_above = 0, sum_below = 0, sum_kept = 0;
+    u64 sum_above = 0, sum_all = 0, sum_kept = 0;
     int kept = 0;
     if (cuts) {
         // The bins' borders as logits: the least of a bin and those above it, found by halving as the arithmetic of bins.of()
@@ -810,53 +804,84 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             if (lane < 4) sh.border[lane] = sample_value(up);
         }
         __syncthreads();
-        const bool ranged = by_mass || all_listed;
-        const float sure = sh.border[0], in_to = ranged ? sh.border[1] : INFINITY;
-        const float count_from = by_count ? sh.border[2] : -FLT_MAX, count_to = by_count ? sh.border[3] : INFINITY;
-        const float lowest = by_count ? count_to : -FLT_MAX;
-        const bool least_logit = p.min_p > 0.f;
+        const float sure = sh.border[0], in_to = by_mass || all_listed ? sh.border[1] : INFINITY;
         auto append = [&](float l, int i) { own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << 32) | (unsigned)(base + i); };
-        auto in_question = [&](float l) { return (l < sure && l >= in_to) || (l < count_from && l >= count_to); };
-        each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
-            if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= lowest)) return;
-            const float l[4] = {y.x, y.y, y.z, y.w};
-            bool some = false;
-#pragma unroll
-            for (int k = 0; k < 4; k++) some |= in_question(l[k]);
-            if (some)
+        // Lists those of a quad that `in` marks.
+        auto append_some = [&](int q, const float (&l)[4], auto in) {
+            if (in(l[0]) || in(l[1]) || in(l[2]) || in(l[3]))
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    if (in_question(l[k])) append(l[k], 4 * q + k - off);
-            if (all_listed) return;
-            u64 w[4];
+                    if (in(l[k])) append(l[k], 4 * q + k - off);
+        };
+        if (all_listed) {
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+                const float l[4] = {y.x, y.y, y.z, y.w};
+                append_some(q, l, [&](float z) { return z >= in_to; });
+            });
+        } else if (by_count) {
+            const float count_from = sh.border[2], count_to = sh.border[3];
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+                if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= count_to)) return;
+                const float l[4] = {y.x, y.y, y.z, y.w};
+                append_some(q, l, [&](float z) { return (z < sure && z >= in_to) || (z < count_from && z >= count_to); });
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = r.weight(l[k]);
+                for (int k = 0; k < 4; k++) {
+                    const u64 w = r.weight(l[k]);
+                    if (l[k] >= count_from) sum_all += w;
+                    if (l[k] >= sure) sum_above += w;
+                    if (l[k] >= sure && l[k] < min_logit) sum_kept += w, kept--;
+                }
+            });
+        } else if (p.min_p > 0.f) {
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+                const float l[4] = {y.x, y.y, y.z, y.w};
+                append_some(q, l, [&](float z) { return z < sure && z >= in_to; });
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (l[k] >= sure) sum_above += w[k], kept++;
-                if (l[k] >= count_from) sum_below += w[k];
-            }
-            if (least_logit)  // of the first, those that min-p takes away
+                for (int k = 0; k < 4; k++) {
+                    const u64 w = r.weight(l[k]);
+                    sum_all += w;
+                    if (l[k] >= sure) sum_above += w;
+                    if (l[k] >= sure && l[k] < min_logit) sum_kept += w, kept--;
+                }
+            });
+        } else {
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+                const float l[4] = {y.x, y.y, y.z, y.w};
+                append_some(q, l, [&](float z) { return z < sure && z >= in_to; });
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (l[k] >= sure && l[k] < min_logit) sum_kept += w[k], kept--;
-        });
+                for (int k = 0; k < 4; k++) {
+                    const u64 w = r.weight(l[k]);
+                    sum_all += w;
+                    if (l[k] >= sure) sum_above += w;
+                }
+            });
+        }
+        // How many there are above the bins is known of the whole row; sum_kept and kept are what min-p takes away of them.
+        if (rank == 0 && tid == 0) kept += all_listed ? 0 : by_mass ? sh.list_from : sh.above;
         sum_kept = sum_above - sum_kept;
     } else {
-        each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {
-            const float l[4] = {y.x, y.y, y.z, y.w};
+        if (p.min_p > 0.f)
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {
+                if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= min_logit)) return;
+                const float l[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const u64 w = r.weight(l[k]);
-                if (l[k] >= min_logit) sum_kept += w, kept++;
-            }
-        });
+                for (int k = 0; k < 4; k++) {
+                    const u64 w = r.weight(l[k]);
+                    if (l[k] >= min_logit) sum_kept += w, kept++;
+                }
+            });
+        else {
+            each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {  // masked tokens weigh nothing
+                sum_kept += (r.weight(y.x) + r.weight(y.y)) + (r.weight(y.z) + r.weight(y.w));
+            });
+            if (rank == 0 && tid == 0) kept = all_live;
+        }
     }
-    if (by_mass) sum_below = warp_sum64(sum_below), sum_above = warp_sum64(sum_above);
+    if (by_mass) sum_all = warp_sum64(sum_all), sum_above = warp_sum64(sum_above);
     sum_kept = warp_sum64(sum_kept);
     kept = __reduce_add_sync(0xffffffffu, kept);
     if (lane == 0) {
-        sh.warp_mass[warp] = sum_below, sh.warp_more[warp] = sum_above, sh.warp_kept[warp] = sum_kept;
+        sh.warp_mass[warp] = sum_all, sh.warp_more[warp] = sum_above, sh.warp_kept[warp] = sum_kept;
         sh.warp_count[warp] = kept;
     }
     __syncthreads();
