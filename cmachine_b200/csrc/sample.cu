@@ -750,18 +750,21 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             // of the root of their squares' sum; four times that, and what FP32 sums are off by.
             const float share = fmaxf(p.top_p, 0.f) * whole, slack = -0.8f * step * sqrtf(squares) + 2e-5f * whole;
             const int last = min(kSampleBins - 1, count_bin);
-            float sum = lighter;
+            // A thread's last sum is the next one's first, so that every value is passed by one of them.
+            float behind = __shfl_down_sync(0xffffffffu, lighter, 1), sum = lighter;
+            if (lane == 31) {
+                behind = 0.f;
+                for (int w = 0; w <= warp; w++) behind += sh.warp_high[w];
+            }
 #pragma unroll
             for (int k = 0; k < each; k++) {
                 const int b = tid * each + k;
-                const float next = sum + mass[k];
-                if (c[k]) {
-                    if ((sum < share - slack || before == 0) && next >= share - slack) atomicMin(&sh.mass_from, b);
-                    if ((sum < share + slack || before == 0) && next >= share + slack) atomicMin(&sh.mass_to, b);
-                }
-                before += c[k], sum = next;
+                const float next = k == each - 1 ? behind : sum + mass[k];
+                if (sum < share - slack && next >= share - slack) atomicMin(&sh.mass_from, b);
+                if (sum < share + slack && next >= share + slack) atomicMin(&sh.mass_to, b);
+                sum = next;
             }
-            before -= mine;
+            if (tid == 0 && !(share > slack)) atomicMin(&sh.mass_from, 0);
             __syncthreads();
             mass_from = min(sh.mass_from, last), mass_to = max(min(sh.mass_to, last), mass_from);
             // How many tokens they hold: those up to the last but not above the first.
