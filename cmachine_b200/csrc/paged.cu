@@ -187,7 +187,7 @@ template <int KIND, int DIM, int R> void decode_launch_rows(TcmGpu *gpu, PagedDe
         for (a.head0 = 0; a.head0 < all.kvheads; a.head0 += heads) {
             a.heads = all.kvheads - a.head0 < heads ? all.kvheads - a.head0 : heads;
             a.v.sequences = all.sequences - s < most ? all.sequences - s : most;
-            a.v.starts = all.starts + ((int64_t)s << all.pairs);
+            a.v.starts = all.starts + s;
             a.v.lengths = all.lengths + s;
             a.v.table = all.table + (int64_t)s * all.table_stride;
             launch(paged_decode_kernel<KIND, DIM, R>, dim3(ctas), dim3(kPdThreads), smem, stream(), true, a);
@@ -272,12 +272,6 @@ int attention(const char *name, TcmGpu *gpu, float *out, long long out_stride, c
 }
 
 }  // namespace
-
-void paged_decode_rows(TcmGpu *gpu, const PagedDecodeArgs &args) {
-#define CALL(K, D) decode_launch<K, D>(gpu, args)
-    PAGED_DISPATCH(args.v, CALL);
-#undef CALL
-}
 
 void set_wait_limit_paged(unsigned long long ns) { set_module_wait_limit(ns); }
 

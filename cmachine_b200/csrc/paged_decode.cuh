@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
             auto page_of = [&](int k) -> int {    // the page id of step k, or (pages that end inside steps) of lane % 16's row
                 if (k >= k1) return -1;
                 const int j = min(paged_tile(tiles, k) * 16 + (whole ? 0 : lane & 15), last);
-                return v.table[(int64_t)s * v.table_stride + (int64_t)h * v.table_head + paged_div(&v, j)];
+                return v.table[(int64_t)s * v.table_stride + paged_div(&v, j)];
             };
             // Copies step k into its stage; returns which of its 16 places have a row. One copy group a
             // call, empty behind the last step.
@@ -954,8 +954,5 @@ __global__ void __launch_bounds__(kPdThreads, (kPdCtas<KIND, DIM, R>)) paged_dec
     if (a.beside) pdl_wait();
     if (bad) paged_report(a.status, bad);
 }
-
-// Launches the kernel above for sequences of at most `few` new rows each (paged.cu).
-void paged_decode_rows(TcmGpu *gpu, const PagedDecodeArgs &args);
 
 }  // namespace tcm

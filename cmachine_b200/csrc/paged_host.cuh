@@ -36,7 +36,7 @@ inline int open_view(const char *call, const TcmPagedCache *c, const TcmPagedBat
     const int max_length = b->max_length < held ? b->max_length : (int)held;
     if ((long long)max_new * c->kvheads > 0x7fffffff / 8) return refuse(call, "too many new rows for one call");
     *v = PagedView{c->kind, c->pages, c->page, c->kvheads, c->dim, c->keys, c->values, c->scales, b->sequences, b->rows,
-                   max_new, max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0, 0, 0};
+                   max_new, max_length, b->table_stride, b->starts, b->lengths, b->table, 0, 0};
     paged_divider(v);
     return 0;
 }

@@ -28,9 +28,6 @@ typedef struct {
     const int *starts, *lengths, *table;
     uint32_t page_mul;
     int page_shift;
-    /* Zero for a batch as callers give it. With `pairs`, starts holds two words a sequence, its first row and the
-     * one behind its last; with table_head, every KV head has a table of its own, that many entries on. */
-    int pairs, table_head;
 } PagedView;
 
 /* x / page as (hi32(mul * x) + x) >> shift for 0 <= x < 2^31: with l = ceil(log2 page),
@@ -71,8 +68,7 @@ TCM_HD int paged_extent_of(const PagedView *v, int start, int end, int length, P
     return 0;
 }
 TCM_HD int paged_extent(const PagedView *v, int s, PagedExtent *e) {
-    const int *p = v->starts + ((int64_t)s << v->pairs);
-    return paged_extent_of(v, p[0], p[1], v->lengths[s], e);
+    return paged_extent_of(v, v->starts[s], v->starts[s + 1], v->lengths[s], e);
 }
 
 /* Row j >= 0 of KV head h under page id `id`, in rows of the [pages][kvheads][page]
@@ -84,7 +80,7 @@ TCM_HD int64_t paged_row(const PagedView *v, int id, int j, int j_page, int h) {
 /* The same through the table, for 0 <= j < a sequence's length. */
 TCM_HD int64_t paged_slot(const PagedView *v, int s, int j, int h) {
     const int p = paged_div(v, j);
-    return paged_row(v, v->table[(int64_t)s * v->table_stride + (int64_t)h * v->table_head + p], j, p, h);
+    return paged_row(v, v->table[(int64_t)s * v->table_stride + p], j, p, h);
 }
 
 /* Does the query at place `at` see row j of its sequence? */

@@ -1,11 +1,11 @@
-// Attention over few pages of a paged K/V cache: the pages' bounds, the choice of each query's pages, and the decode
-// kernel (paged_decode.cuh) over what was chosen.
+// Attention over few pages of a paged K/V cache: the pages' bounds, the choice of each query's pages, and the attention
+// over what was chosen (paged_chosen.cuh).
 //
-// The choice leaves each query row a sequence of its own: one new row, a table for every KV head that names the chosen
-// pages, and the length that they make. Its own page is the last of them and the only one that may be partly filled, so
-// the decode kernel needs no other mask than its own.
+// The choice leaves each query row and KV head a table that names the chosen pages in order, and the number of rows that
+// they hold. The query's own page is the last of them and the only one that may be partly filled, so all those rows are
+// visible.
 #include "paged_host.cuh"
-#include "paged_decode.cuh"
+#include "paged_chosen.cuh"
 #include <float.h>
 #include <math.h>
 
@@ -100,7 +100,7 @@ struct PagedChoiceArgs {
     int group, blocks, first, recent;
     int row0, rows;       // the slab
     int pages;            // scores that a row has room for
-    int *starts, *lengths, *table;  // the slab's: [rows][2], [rows], [rows][kvheads][blocks]
+    int *lengths, *table;  // the slab's: rows chosen, -1 for no row of the batch; [rows][kvheads][blocks]
     int *selected;        // [rows][kvheads][blocks] of all rows, or null
     int *status;
 };
@@ -184,10 +184,8 @@ __global__ void __launch_bounds__(kChoiceThreads<R>, R == 1 ? 1 : 2) paged_choic
         const int at0 = live ? e.length - e.count + (a.row0 + tile0 + i0 - e.start) : 0;  // the first row's place
         if (h == 0)
             for (int i = i0 + tid; i < i1; i += T) {
-                const int r = tile0 + i, at = at0 + i - i0, own = at < 0 ? -1 : paged_div(&v, at);
-                a.starts[2 * r] = live ? a.row0 + r : 0;
-                a.starts[2 * r + 1] = live ? a.row0 + r + 1 : 0;
-                a.lengths[r] = !live || at < 0 ? 0 : (min(own + 1, a.blocks) - 1) * v.page + at - own * v.page + 1;
+                const int at = at0 + i - i0, own = at < 0 ? -1 : paged_div(&v, at);
+                a.lengths[tile0 + i] = !live ? -1 : at < 0 ? 0 : (min(own + 1, a.blocks) - 1) * v.page + at - own * v.page + 1;
             }
         if (!live) continue;
         const int *ids = v.table + (int64_t)s * v.table_stride;
@@ -530,6 +528,33 @@ template <int DIM, int R> void choice_launch(const PagedChoiceArgs &a) {
            stream(), true, a);
 }
 
+// CTAs an item: as many as run at once for all items while a warp has two steps, and so that no warp has more than
+// kPdChain, which needs no sums of its own for each.
+template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int rows, long long steps) {
+    constexpr size_t smem = PsGeo<KIND, DIM>::kSmem;
+    static PerDeviceOnce once;
+    once.run([] {
+        TCM_CUDA(cudaFuncSetAttribute(paged_chosen_kernel<KIND, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        TCM_CUDA(cudaFuncSetAttribute(paged_chosen_kernel<KIND, DIM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    });
+    const long long items = (long long)rows * a.v.kvheads;
+    int c = 1;
+    while (c < kPsCluster && ((items * 2 * c <= kPsCtas * sm_count() && steps >= 16 * c) || steps > (long long)kPdChain * kPsWarps * c)) c *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c, a.v.kvheads, rows);
+    cfg.blockDim = dim3(kPsThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream();
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)c, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    TCM_CUDA(cudaLaunchKernelEx(&cfg, paged_chosen_kernel<KIND, DIM>, a));
+}
+
 }  // namespace
 }  // namespace tcm
 
@@ -566,10 +591,9 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     if (check_rows(call, q, q_stride, qheads, view.dim) || check_rows(call, out, out_stride, qheads, view.dim)) return -1;
     const int group = qheads / view.kvheads;
     // Rows in slabs whose tables stay within 64 MB.
-    const long long a_row = (long long)view.kvheads * blocks + 3;
+    const long long a_row = (long long)view.kvheads * blocks + 1;
     long long slab = (64ll << 20) / 4 / a_row;
-    slab = slab < 1 ? 1 : slab > 65535 ? 65535 : slab;
-    if (slab > kPdSequences) slab = slab / kPdSequences * kPdSequences;
+    slab = slab < 4 ? 4 : slab > 65532 ? 65532 : slab / 4 * 4;
     if (slab > view.rows) slab = view.rows;
     float *part;
     float2 *ml;
@@ -579,23 +603,21 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     const int pages = (int)(most < kChoicePages ? most : kChoicePages);
     // Rows of one sequence share the loads of its bounds, where there are rows enough and their scores leave room for two CTAs an SM.
     const bool four = view.max_new >= 4 && (long long)view.rows * view.kvheads >= 4ll * sm_count() && choice_smem(view.dim, 4, pages) <= 100 * 1024;
-    PagedChoiceArgs c = {view, q, q_stride, bounds, group, blocks, first, recent, 0, 0, pages, reinterpret_cast<int *>(words),
-                         reinterpret_cast<int *>(words) + 2 * slab, reinterpret_cast<int *>(words) + 3 * slab, selected, status};
-    // What was chosen, as a batch: one row a sequence.
-    PagedDecodeArgs d = {view, out, q, out_stride, q_stride, group, 0, 0, 0, 0, 1, 1.44269504088896340736f / sqrtf((float)view.dim),
-                         nullptr, nullptr, nullptr, status, 0};
-    d.v.starts = c.starts, d.v.lengths = c.lengths, d.v.table = c.table;
-    d.v.pairs = 1, d.v.table_head = blocks, d.v.table_stride = view.kvheads * blocks;
-    d.v.max_new = 1;
+    int *lengths = reinterpret_cast<int *>(words);
+    PagedChoiceArgs c = {view, q, q_stride, bounds, group, blocks, first, recent, 0, 0, pages, lengths, lengths + slab, selected, status};
+    PagedChosenArgs d = {view, q, out, q_stride, out_stride, group, blocks, 0, lengths, lengths + slab,
+                         1.44269504088896340736f / sqrtf((float)view.dim), status};
     const long long held = (long long)blocks * view.page;
-    d.v.max_length = held < view.max_length ? (int)held : view.max_length;
+    const long long steps = ((held < view.max_length ? held : view.max_length) + 15) / 16;
     for (long long r = 0; r < view.rows; r += slab) {
         const int rows = (int)(view.rows - r < slab ? view.rows - r : slab);
         c.row0 = (int)r, c.rows = rows;
         if (view.dim == 64) four ? choice_launch<64, 4>(c) : choice_launch<64, 1>(c);
         else four ? choice_launch<128, 4>(c) : choice_launch<128, 1>(c);
-        d.v.sequences = rows;
-        paged_decode_rows(gpu, d);
+        d.row0 = (int)r;
+#define CALL(K, D) chosen_launch<K, D>(d, rows, steps)
+        PAGED_DISPATCH(view, CALL);
+#undef CALL
     }
     return 0;
 }
