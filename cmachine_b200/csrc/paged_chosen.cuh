@@ -1,7 +1,7 @@
 // Attention of single query rows over pages chosen for them, one KV head at a time (paged_sparse.cu writes the choice).
 //
 // An item is a query row and a KV head: up to eight query heads, a table of pages of its own, and the number of rows
-// that they hold, all of them visible. A cluster of CTAs has an item and shares its rows out in steps of 16; every warp
+// that they hold, all of them visible. A cluster of CTAs has an item and shares its rows out in steps of 32; every warp
 // takes steps in turn, each with its own online softmax, and the parts meet in shared memory, the CTAs' in one
 // another's. No item waits for another, and nothing is left in global memory in between.
 //
@@ -36,8 +36,8 @@ constexpr int kPsWarps = 4, kPsThreads = kPsWarps * 32, kPsCtas = 3, kPsCluster 
 constexpr float kPsMost = 32768.f;  // of a byte row's scaled weight, inside FP16
 template <int KIND, int DIM> struct PsGeo {
     static constexpr int kRow = DIM * (KIND == kPagedBytes ? 1 : 2);               // bytes of a stored row
-    static constexpr int kUnit = 16 * kRow + (KIND == kPagedBytes ? 64 : 0) + 16;  // 16 rows, their scales, which are there
-    static constexpr int kAhead = KIND == kPagedBf16 && DIM == 128 ? 2 : 4;        // steps in a warp's ring: three CTAs an SM fit
+    static constexpr int kUnit = 32 * kRow + (KIND == kPagedBytes ? 128 : 0) + 16;  // 32 rows, their scales, which are there
+    static constexpr int kAhead = KIND == kPagedBf16 && DIM == 128 ? 1 : 2;         // steps in a warp's ring: three CTAs an SM fit
     static constexpr int kSteps = kRow / 32;                                       // k-steps of Q K^T
     static constexpr size_t kRing = (size_t)kPsWarps * 2 * kAhead * kUnit;
     static constexpr size_t kFrag = (size_t)2 * kSteps * 32 * 16;
@@ -75,66 +75,69 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         return;
     }
     const int *table = a.table + ((int64_t)r * v.kvheads + h) * a.blocks;
-    const int steps = (n + 15) / 16;
+    const int steps = (n + 31) / 32;
     const int k0 = (int)((int64_t)steps * part / C), k1 = (int)((int64_t)steps * (part + 1) / C);
 
     // ---- the copies of this warp's steps k0 + warp, + W, ...: unit i is K (even i) or V of the i / 2-th. A lane copies 16
     // bytes of every kRpl-th row; where they lie in a unit goes by pd_swizzle, whose change from one of its rows to the
     // next is the same in every lane.
-    constexpr int kLpr = G::kRow / 16, kRpl = 32 / kLpr, kRowsCopied = 16 / kRpl;  // lanes a row, rows at a time, rows of a lane
-    const bool whole = v.page % 16 == 0;  // a step lies inside one page
+    constexpr int kLpr = G::kRow / 16, kRpl = 32 / kLpr, kRowsCopied = 32 / kRpl;  // lanes a row, rows at a time, rows of a lane
+    const bool whole = v.page % 16 == 0;  // 16 rows lie inside one page
     const bool wide = whole && (!kBytes || ((uintptr_t)v.scales & 15) == 0);  // scales by 16 bytes as well
     const uint32_t lane_to = (uint32_t)(lane / kLpr * G::kRow + pd_swizzle<G::kRow>(lane / kLpr, lane % kLpr) * 16);
     unsigned char *const ring = ps_smem + warp * 2 * A * G::kUnit;
     const char *const keys = static_cast<const char *>(v.keys) + lane * 16, *const values = static_cast<const char *>(v.values) + lane * 16;
     const int page_rows = v.kvheads * v.page, head_row = h * v.page;  // rows of a page, and before this head's in it
     int bad = 0;
-    auto id_of = [&](int k) -> int {  // the page id of step k, or (pages that end inside steps) of lane % 16's row
-        if (k >= k1) return -1;
-        return table[paged_div(&v, min(16 * k + (whole ? 0 : lane & 15), n - 1))];
-    };
-    // Of the step that is copied next: its number, where its rows are in the pool (lane % 16's row, where pages end inside
-    // steps; -1: nowhere), which are there, the unit that takes its K rows, and the page id of the step behind it.
+    // The lane's place in step k: its half's first row, or (pages that end inside 16 rows) its own; and the page id of it.
+    auto place_of = [&](int k) { return 32 * k + (whole ? lane & 16 : lane); };
+    auto id_of = [&](int k) -> int { return k < k1 ? table[paged_div(&v, min(place_of(k), n - 1))] : -1; };
+    // Of the step that is copied next: its number, where the two halves' rows, or the lane's, are in the pool (-1:
+    // nowhere), which are there, the unit that takes its K rows, and the page id of the step behind it.
     int ahead = k0 + warp, next_id = id_of(ahead);
-    int64_t row = -1;
+    int64_t row[2] = {-1, -1};
     unsigned there = 0;
     uint32_t to = smem_addr(ring);
     const uint32_t ring_end = to + 2 * A * G::kUnit;
     auto copy = [&](const char *pool, const float *scales, uint32_t unit) {
-        if (wide && there == 0xffffu) {
-            const char *src = pool + row * G::kRow;
+        auto row_to = [&](int i) { return unit + (lane_to ^ (uint32_t)(pd_swizzle<G::kRow>(i * kRpl, 0) * 16)) + (uint32_t)(i * 512); };
+        if (wide && there == 0xffffffffu) {
 #pragma unroll
-            for (int i = 0; i < kRowsCopied; i++)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                 unit + (lane_to ^ (uint32_t)(pd_swizzle<G::kRow>(i * kRpl, 0) * 16)) + (uint32_t)(i * 512)),
-                             "l"(src + i * 512) : "memory");
+            for (int half = 0; half < 2; half++) {
+                const char *src = pool + row[half] * G::kRow;
+#pragma unroll
+                for (int i = 0; i < kRowsCopied / 2; i++)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(row_to(half * kRowsCopied / 2 + i)), "l"(src + i * 512) : "memory");
+            }
             if constexpr (kBytes)
-                if (lane < 4)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(unit + 16 * G::kRow + lane * 16),
-                                 "l"(scales + row + lane * 4) : "memory");
+                if (lane < 8)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(unit + 32 * G::kRow + lane * 16),
+                                 "l"(scales + (lane < 4 ? row[0] : row[1]) + lane % 4 * 4) : "memory");
         } else {
 #pragma unroll
             for (int i = 0; i < kRowsCopied; i++) {
                 const int rr = i * kRpl + lane / kLpr;
                 const bool has = (there >> rr) & 1;
-                const int64_t from = whole ? row + rr : __shfl_sync(0xffffffffu, row, rr);
-                pd_copy16(unit + (lane_to ^ (uint32_t)(pd_swizzle<G::kRow>(i * kRpl, 0) * 16)) + (uint32_t)(i * 512),
-                          has ? pool - lane * 16 + from * G::kRow + lane % kLpr * 16 : pool, has);
+                const int64_t from = whole ? row[i >= kRowsCopied / 2] + rr % 16 : __shfl_sync(0xffffffffu, row[0], rr);
+                pd_copy16(row_to(i), has ? pool - lane * 16 + from * G::kRow + lane % kLpr * 16 : pool, has);
             }
-            if constexpr (kBytes)
-                if (lane < 16) {
-                    const bool has = (there >> lane) & 1;
-                    pd_copy4(unit + 16 * G::kRow + lane * 4, scales + (has ? row + (whole ? lane : 0) : 0), has);
-                }
+            if constexpr (kBytes) {
+                const bool has = (there >> lane) & 1;
+                pd_copy4(unit + 32 * G::kRow + lane * 4, scales + (!has ? 0 : whole ? (lane < 16 ? row[0] : row[1]) + lane % 16 : row[0]), has);
+            }
         }
     };
     auto copy_keys = [&]() {
         if (ahead < k1) {
-            const int j = 16 * ahead + (whole ? 0 : lane & 15), p = paged_div(&v, j);
-            row = next_id < 0 || next_id >= v.pages || j >= n ? -1 : (int64_t)next_id * page_rows + (head_row + j - p * v.page);
-            if (row < 0 && j < n) bad |= kPagedBadPage;
-            if (whole) there = row < 0 ? 0u : n - j >= 16 ? 0xffffu : (1u << (n - j)) - 1u;
-            else there = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+            const int j = place_of(ahead), p = paged_div(&v, j), last = whole ? j + (lane & 15) : j;
+            int64_t mine = -1;
+            if (j < n) {
+                if (next_id < 0 || next_id >= v.pages) bad |= kPagedBadPage;
+                else mine = (int64_t)next_id * page_rows + (head_row + j - p * v.page);
+            }
+            there = __ballot_sync(0xffffffffu, mine >= 0 && last < n);
+            row[0] = mine;
+            if (whole) row[0] = __shfl_sync(0xffffffffu, mine, 0), row[1] = __shfl_sync(0xffffffffu, mine, 16);
             next_id = id_of(ahead + W);
             copy(keys, v.scales, to);
             if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + G::kUnit - 16), "r"(there) : "memory");
@@ -225,7 +228,7 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
     }
     __syncthreads();
 
-    // ---- the steps. Lane (g, t) has the scores of query head g and places 2t, 2t + 1, 8 + 2t and 9 + 2t
+    // ---- the steps. Lane (g, t) has the scores of query head g: x[i] of place 8 (i / 2) + 2t + i % 2
     float o[DV][4], m = -INFINITY, l = 0.f, ref = 0.f;  // ref: m, 0 before the first
     int v_exp = -100;                                   // byte rows: weights times scales count in units of 2^(v_exp - 12)
     float v_up = power_of_two(kPdWeightTop + 100);
@@ -240,8 +243,8 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
 #pragma unroll
             for (int c = 0; c < 4; c++) o[j][c] *= keep;
     };
-    const bool long_sum = k1 - k0 > kPdChain * W;
-    // Where a lane's pieces of K rows g and g + 8, and of V rows 2t, 2t + 1, 8 + 2t and 9 + 2t, lie in a unit.
+    const bool long_sum = 2 * (k1 - k0) > kPdChain * W;  // steps of the tensor cores are 16 rows
+    // Where a lane's pieces of K rows g, g + 8, ..., and of V rows 2t, 2t + 1, 8 + 2t, 9 + 2t, ..., lie in a unit.
     const unsigned char *unit = ring;
     const int k_at = g * G::kRow + pd_swizzle<G::kRow>(g, t) * 16;
     const int v_at = 2 * t * G::kRow + pd_swizzle<G::kRow>(2 * t, g * (DV * ES) / 16) * 16 + g * (DV * ES) % 16;
@@ -252,22 +255,22 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * A - 1) : "memory");
         __syncwarp();
         const unsigned has = *reinterpret_cast<const unsigned *>(unit + G::kUnit - 16);
-        float x[4];
+        float x[8];
         {
-            int ci[kBytes ? 2 : 1][2][4] = {};
-            float cf[2][4] = {};
-            uint4 kr[2];
+            int ci[kBytes ? 2 : 1][4][4] = {};
+            float cf[4][4] = {};
+            uint4 kr[4];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 if (ks % 2 == 0)
 #pragma unroll
-                    for (int gr = 0; gr < 2; gr++)
+                    for (int gr = 0; gr < 4; gr++)
                         kr[gr] = *reinterpret_cast<const uint4 *>(unit + (k_at ^ (ks / 2 * 64)) + gr * 8 * G::kRow);
 #pragma unroll
                 for (int p = 1; p >= 0; p--) {
                     const uint4 f = qf[p][ks][lane];
 #pragma unroll
-                    for (int gr = 0; gr < 2; gr++) {
+                    for (int gr = 0; gr < 4; gr++) {
                         const uint32_t b0 = ks % 2 ? kr[gr].z : kr[gr].x, b1 = ks % 2 ? kr[gr].w : kr[gr].y;
                         if constexpr (kBytes) mma_s8(ci[p][gr], f, b0, b1);
                         else mma_bf16(cf[gr], f.x, f.y, f.z, f.w, b0, b1);
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 8; i++) {
                 const int gr = i >> 1, c = i & 1;
                 if constexpr (kBytes)  // each sum is below 2^21, the lower two together below 2^30
                     x[i] = fmaf((float)ci[0][gr][c], 0x1p-8f, (float)(ci[0][gr][2 + c] * 256 + ci[1][gr][c]) * 0x1p-24f);
@@ -283,21 +286,27 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
             }
         }
         if constexpr (kBytes) {
-            const float *scales = reinterpret_cast<const float *>(unit + 16 * G::kRow) + 2 * t;
-            const float2 s0 = *reinterpret_cast<const float2 *>(scales), s1 = *reinterpret_cast<const float2 *>(scales + 8);
-            x[0] *= s0.x, x[1] *= s0.y, x[2] *= s1.x, x[3] *= s1.y;
+            const float *scales = reinterpret_cast<const float *>(unit + 32 * G::kRow) + 2 * t;
+#pragma unroll
+            for (int gr = 0; gr < 4; gr++) {
+                const float2 y = *reinterpret_cast<const float2 *>(scales + 8 * gr);
+                x[2 * gr] *= y.x, x[2 * gr + 1] *= y.y;
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] *= sc;
-        if (has != 0xffffu)
+        for (int i = 0; i < 8; i++) x[i] *= sc;
+        if (has != 0xffffffffu)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 8; i++)
                 if (!((has >> ((i >> 1) * 8 + 2 * t + (i & 1))) & 1)) x[i] = -INFINITY;
         __syncwarp();  // every lane has read the unit before it is copied into again
         copy_keys();
 
         // ---- weights. The reference moves rarely: when the maximum has passed it by 2^3.
-        float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        auto most_of = [](const float (&y)[8]) {
+            return fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+        };
+        float top = most_of(x);
         if (__any_sync(0xffffffffu, top > m + kPdSlack)) {
             top = quad_max(top);
             float keep = 1.f;
@@ -314,9 +323,9 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
             }
             rescale(keep);
         }
-        float w[4];
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 8; i++) {
             w[i] = ex2(x[i] - ref);
             l += w[i];
         }
@@ -325,10 +334,13 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * A - 1) : "memory");
         __syncwarp();
         if constexpr (kBytes) {  // (rows that are not there have scale 0)
-            const float *scales = reinterpret_cast<const float *>(unit + G::kUnit + 16 * G::kRow) + 2 * t;
-            const float2 s0 = *reinterpret_cast<const float2 *>(scales), s1 = *reinterpret_cast<const float2 *>(scales + 8);
-            w[0] *= s0.x, w[1] *= s0.y, w[2] *= s1.x, w[3] *= s1.y;
-            const float most = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+            const float *scales = reinterpret_cast<const float *>(unit + G::kUnit + 32 * G::kRow) + 2 * t;
+#pragma unroll
+            for (int gr = 0; gr < 4; gr++) {
+                const float2 y = *reinterpret_cast<const float2 *>(scales + 8 * gr);
+                w[2 * gr] *= y.x, w[2 * gr + 1] *= y.y;
+            }
+            const float most = most_of(w);
             if (__any_sync(0xffffffffu, most * v_up > kPsMost)) {
                 const float all = quad_max(most);
                 float keep = 1.f;
@@ -341,18 +353,18 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 rescale(keep);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] *= v_up;
+            for (int i = 0; i < 8; i++) w[i] *= v_up;
         }
-        uint32_t pa[2][P];
-        split_pair<KIND>(w[0], w[1], pa[0]);
-        split_pair<KIND>(w[2], w[3], pa[1]);
-        auto pv = [&](int j, uint32_t b0, uint32_t b1, auto apart) {
+        uint32_t pa[4][P];
+#pragma unroll
+        for (int i = 0; i < 4; i++) split_pair<KIND>(w[2 * i], w[2 * i + 1], pa[i]);
+        auto pv = [&](int j, int q, uint32_t b0, uint32_t b1, auto apart) {  // rows 16 q .. 16 q + 15
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
             float(&acc)[4] = decltype(apart)::value ? sum : o[j];
-            if constexpr (kBytes) mma_f16(acc, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b0, b1);
+            if constexpr (kBytes) mma_f16(acc, pa[2 * q][0], pa[2 * q][1], pa[2 * q + 1][0], pa[2 * q + 1][1], b0, b1);
             else {
-                mma_bf16(acc, 0u, pa[0][P - 1], 0u, pa[1][P - 1], b0, b1);
-                mma_bf16(acc, pa[0][0], pa[0][1], pa[1][0], pa[1][1], b0, b1);
+                mma_bf16(acc, 0u, pa[2 * q][P - 1], 0u, pa[2 * q + 1][P - 1], b0, b1);
+                mma_bf16(acc, pa[2 * q][0], pa[2 * q][1], pa[2 * q + 1][0], pa[2 * q + 1][1], b0, b1);
             }
             if constexpr (decltype(apart)::value)
 #pragma unroll
@@ -361,11 +373,13 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         auto add_values = [&](auto apart) {
             uint4 vr[4];
 #pragma unroll
+            for (int q = 0; q < 2; q++)
+#pragma unroll
             for (int c = 0; c < VW; c++) {
                 if (c % 4 == 0)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const unsigned char *p = value_at(i & 1, i >> 1, c / 4);
+                        const unsigned char *p = value_at(i & 1, 2 * q + (i >> 1), c / 4);
                         if constexpr (VW == 2) {
                             const uint2 y = *reinterpret_cast<const uint2 *>(p);
                             vr[i] = make_uint4(y.x, y.y, 0, 0);
@@ -379,13 +393,13 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 if constexpr (kBytes) {
                     const uint32_t lo0 = __byte_perm(y[0], y[1], 0x5140) ^ 0x80808080u, hi0 = __byte_perm(y[0], y[1], 0x7362) ^ 0x80808080u;
                     const uint32_t lo1 = __byte_perm(y[2], y[3], 0x5140) ^ 0x80808080u, hi1 = __byte_perm(y[2], y[3], 0x7362) ^ 0x80808080u;
-                    pv(4 * c, codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140), apart);
-                    pv(4 * c + 1, codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342), apart);
-                    pv(4 * c + 2, codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140), apart);
-                    pv(4 * c + 3, codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342), apart);
+                    pv(4 * c, q, codes_f16(lo0, 0x4140), codes_f16(lo1, 0x4140), apart);
+                    pv(4 * c + 1, q, codes_f16(lo0, 0x4342), codes_f16(lo1, 0x4342), apart);
+                    pv(4 * c + 2, q, codes_f16(hi0, 0x4140), codes_f16(hi1, 0x4140), apart);
+                    pv(4 * c + 3, q, codes_f16(hi0, 0x4342), codes_f16(hi1, 0x4342), apart);
                 } else {
-                    pv(2 * c, __byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), apart);
-                    pv(2 * c + 1, __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632), apart);
+                    pv(2 * c, q, __byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), apart);
+                    pv(2 * c + 1, q, __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632), apart);
                 }
             }
         };

@@ -528,8 +528,8 @@ template <int DIM, int R> void choice_launch(const PagedChoiceArgs &a) {
            stream(), true, a);
 }
 
-// CTAs an item: as many as run at once for all items while a warp has two steps, and so that no warp has more than
-// kPdChain, which needs no sums of its own for each.
+// CTAs an item: as many as run at once for all items while a warp has two steps, eight at most; and so that no warp sums
+// more than kPdChain steps of 16 rows in the tensor cores, which needs no sums of its own for each.
 template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int rows, long long steps) {
     constexpr size_t smem = PsGeo<KIND, DIM>::kSmem;
     static PerDeviceOnce once;
@@ -538,10 +538,13 @@ template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int ro
         TCM_CUDA(cudaFuncSetAttribute(paged_chosen_kernel<KIND, DIM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
     const long long items = (long long)rows * a.v.kvheads;
-    int c = 1;
-    while (c < kPsCluster && ((items * 2 * c <= kPsCtas * sm_count() && steps >= 16 * c) || steps > (long long)kPdChain * kPsWarps * c)) c *= 2;
+    const long long fit = kPsCtas * sm_count() / items, worth = steps / (2 * kPsWarps), need = (2 * steps + kPdChain * kPsWarps - 1) / (kPdChain * kPsWarps);
+    long long c = fit < worth ? fit : worth;
+    c = c > 8 ? 8 : c;
+    c = c < need ? need : c;
+    c = c < 1 ? 1 : c > kPsCluster ? kPsCluster : c;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(c, a.v.kvheads, rows);
+    cfg.gridDim = dim3((unsigned)c, a.v.kvheads, rows);
     cfg.blockDim = dim3(kPsThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream();
@@ -608,7 +611,7 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     PagedChosenArgs d = {view, q, out, q_stride, out_stride, group, blocks, 0, lengths, lengths + slab,
                          1.44269504088896340736f / sqrtf((float)view.dim), status};
     const long long held = (long long)blocks * view.page;
-    const long long steps = ((held < view.max_length ? held : view.max_length) + 15) / 16;
+    const long long steps = ((held < view.max_length ? held : view.max_length) + 31) / 32;
     for (long long r = 0; r < view.rows; r += slab) {
         const int rows = (int)(view.rows - r < slab ? view.rows - r : slab);
         c.row0 = (int)r, c.rows = rows;
