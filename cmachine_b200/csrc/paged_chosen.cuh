@@ -1,7 +1,7 @@
 // Attention of single query rows over pages chosen for them, one KV head at a time (paged_sparse.cu writes the choice).
 //
 // An item is a query row and a KV head: up to eight query heads, a table of pages of its own, and the number of rows
-// that they hold, all of them visible. A cluster of CTAs has an item and shares its rows out in steps of 32; every warp
+// that they hold, all of them visible. A cluster of CTAs has an item and shares its rows out in steps of 16 or 32; every warp
 // takes steps in turn, each with its own online softmax, and the parts meet in shared memory, the CTAs' in one
 // another's. No item waits for another, and nothing is left in global memory in between.
 //
@@ -36,8 +36,11 @@ constexpr int kPsWarps = 4, kPsThreads = kPsWarps * 32, kPsCtas = 3, kPsCluster 
 constexpr float kPsMost = 32768.f;  // of a byte row's scaled weight, inside FP16
 template <int KIND, int DIM> struct PsGeo {
     static constexpr int kRow = DIM * (KIND == kPagedBytes ? 1 : 2);               // bytes of a stored row
-    static constexpr int kUnit = 32 * kRow + (KIND == kPagedBytes ? 128 : 0) + 16;  // 32 rows, their scales, which are there
-    static constexpr int kAhead = KIND == kPagedBf16 && DIM == 128 ? 1 : 2;         // steps in a warp's ring: three CTAs an SM fit
+    // Rows of a step: 32 cost a quarter fewer instructions a row than 16 (493 and 400 of byte rows, measured), but leave no
+    // room for a second step in the ring beside BF16 rows of 128 (32 sequences of 5 tokens: 117 us, 111 with 16).
+    static constexpr int kStep = KIND == kPagedBf16 && DIM == 128 ? 16 : 32;
+    static constexpr int kUnit = kStep * kRow + (KIND == kPagedBytes ? kStep * 4 : 0) + 16;  // rows, their scales, which are there
+    static constexpr int kAhead = 2;                                                      // steps in a warp's ring: three CTAs an SM fit
     static constexpr int kSteps = kRow / 32;                                       // k-steps of Q K^T
     static constexpr size_t kRing = (size_t)kPsWarps * 2 * kAhead * kUnit;
     static constexpr size_t kFrag = (size_t)2 * kSteps * 32 * 16;
@@ -49,7 +52,8 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
     constexpr bool kBytes = KIND == kPagedBytes;
     using G = PsGeo<KIND, DIM>;
     constexpr int W = kPsWarps, T = kPsThreads, ES = kBytes ? 1 : 2, DV = DIM / 8, VW = DV * ES / 4, KS = G::kSteps;
-    constexpr int P = kPdParts<KIND>, A = G::kAhead;
+    constexpr int P = kPdParts<KIND>, A = G::kAhead, S = G::kStep;
+    constexpr unsigned kAll = S == 32 ? 0xffffffffu : 0xffffu;
     extern __shared__ __align__(16) unsigned char ps_smem[];
     uint4(*qf)[KS][32] = reinterpret_cast<uint4(*)[KS][32]>(ps_smem + G::kRing);   // the queries' fragments
     float4(*wo)[8][DIM / 4] = reinterpret_cast<float4(*)[8][DIM / 4]>(ps_smem);     // the warps' outputs, then the CTAs'
@@ -75,13 +79,13 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         return;
     }
     const int *table = a.table + ((int64_t)r * v.kvheads + h) * a.blocks;
-    const int steps = (n + 31) / 32;
+    const int steps = (n + S - 1) / S;
     const int k0 = (int)((int64_t)steps * part / C), k1 = (int)((int64_t)steps * (part + 1) / C);
 
     // ---- the copies of this warp's steps k0 + warp, + W, ...: unit i is K (even i) or V of the i / 2-th. A lane copies 16
     // bytes of every kRpl-th row; where they lie in a unit goes by pd_swizzle, whose change from one of its rows to the
     // next is the same in every lane.
-    constexpr int kLpr = G::kRow / 16, kRpl = 32 / kLpr, kRowsCopied = 32 / kRpl;  // lanes a row, rows at a time, rows of a lane
+    constexpr int kLpr = G::kRow / 16, kRpl = 32 / kLpr, kRowsCopied = S / kRpl;  // lanes a row, rows at a time, rows of a lane
     const bool whole = v.page % 16 == 0;  // 16 rows lie inside one page
     const bool wide = whole && (!kBytes || ((uintptr_t)v.scales & 15) == 0);  // scales by 16 bytes as well
     const uint32_t lane_to = (uint32_t)(lane / kLpr * G::kRow + pd_swizzle<G::kRow>(lane / kLpr, lane % kLpr) * 16);
@@ -89,10 +93,10 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
     const char *const keys = static_cast<const char *>(v.keys) + lane * 16, *const values = static_cast<const char *>(v.values) + lane * 16;
     const int page_rows = v.kvheads * v.page, head_row = h * v.page;  // rows of a page, and before this head's in it
     int bad = 0;
-    // The lane's place in step k: its half's first row, or (pages that end inside 16 rows) its own; and the page id of it.
-    auto place_of = [&](int k) { return 32 * k + (whole ? lane & 16 : lane); };
+    // The lane's place in step k: its 16 rows' first, or (pages that end inside 16 rows) its own; and the page id of it.
+    auto place_of = [&](int k) { return S * k + (whole ? lane & (S - 16) : lane & (S - 1)); };
     auto id_of = [&](int k) -> int { return k < k1 ? table[paged_div(&v, min(place_of(k), n - 1))] : -1; };
-    // Of the step that is copied next: its number, where the two halves' rows, or the lane's, are in the pool (-1:
+    // Of the step that is copied next: its number, where its 16 rows, or the lane's one, are in the pool (-1:
     // nowhere), which are there, the unit that takes its K rows, and the page id of the step behind it.
     int ahead = k0 + warp, next_id = id_of(ahead);
     int64_t row[2] = {-1, -1};
@@ -101,29 +105,29 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
     const uint32_t ring_end = to + 2 * A * G::kUnit;
     auto copy = [&](const char *pool, const float *scales, uint32_t unit) {
         auto row_to = [&](int i) { return unit + (lane_to ^ (uint32_t)(pd_swizzle<G::kRow>(i * kRpl, 0) * 16)) + (uint32_t)(i * 512); };
-        if (wide && there == 0xffffffffu) {
+        if (wide && there == kAll) {
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
+            for (int half = 0; half < S / 16; half++) {
                 const char *src = pool + row[half] * G::kRow;
 #pragma unroll
-                for (int i = 0; i < kRowsCopied / 2; i++)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(row_to(half * kRowsCopied / 2 + i)), "l"(src + i * 512) : "memory");
+                for (int i = 0; i < 16 / kRpl; i++)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(row_to(half * (16 / kRpl) + i)), "l"(src + i * 512) : "memory");
             }
             if constexpr (kBytes)
-                if (lane < 8)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(unit + 32 * G::kRow + lane * 16),
+                if (lane < S / 4)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(unit + S * G::kRow + lane * 16),
                                  "l"(scales + (lane < 4 ? row[0] : row[1]) + lane % 4 * 4) : "memory");
         } else {
 #pragma unroll
             for (int i = 0; i < kRowsCopied; i++) {
                 const int rr = i * kRpl + lane / kLpr;
                 const bool has = (there >> rr) & 1;
-                const int64_t from = whole ? row[i >= kRowsCopied / 2] + rr % 16 : __shfl_sync(0xffffffffu, row[0], rr);
+                const int64_t from = whole ? row[i >= 16 / kRpl] + rr % 16 : __shfl_sync(0xffffffffu, row[0], rr);
                 pd_copy16(row_to(i), has ? pool - lane * 16 + from * G::kRow + lane % kLpr * 16 : pool, has);
             }
             if constexpr (kBytes) {
                 const bool has = (there >> lane) & 1;
-                pd_copy4(unit + 32 * G::kRow + lane * 4, scales + (!has ? 0 : whole ? (lane < 16 ? row[0] : row[1]) + lane % 16 : row[0]), has);
+                if (lane < S) pd_copy4(unit + S * G::kRow + lane * 4, scales + (!has ? 0 : whole ? (lane < 16 ? row[0] : row[1]) + lane % 16 : row[0]), has);
             }
         }
     };
@@ -135,9 +139,9 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 if (next_id < 0 || next_id >= v.pages) bad |= kPagedBadPage;
                 else mine = (int64_t)next_id * page_rows + (head_row + j - p * v.page);
             }
-            there = __ballot_sync(0xffffffffu, mine >= 0 && last < n);
+            there = __ballot_sync(0xffffffffu, mine >= 0 && last < n) & kAll;
             row[0] = mine;
-            if (whole) row[0] = __shfl_sync(0xffffffffu, mine, 0), row[1] = __shfl_sync(0xffffffffu, mine, 16);
+            if (whole) row[0] = __shfl_sync(0xffffffffu, mine, 0), row[1] = __shfl_sync(0xffffffffu, mine, S - 16);
             next_id = id_of(ahead + W);
             copy(keys, v.scales, to);
             if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + G::kUnit - 16), "r"(there) : "memory");
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
 #pragma unroll
             for (int c = 0; c < 4; c++) o[j][c] *= keep;
     };
-    const bool long_sum = 2 * (k1 - k0) > kPdChain * W;  // steps of the tensor cores are 16 rows
+    const bool long_sum = S / 16 * (k1 - k0) > kPdChain * W;  // steps of the tensor cores are 16 rows
     // Where a lane's pieces of K rows g, g + 8, ..., and of V rows 2t, 2t + 1, 8 + 2t, 9 + 2t, ..., lie in a unit.
     const unsigned char *unit = ring;
     const int k_at = g * G::kRow + pd_swizzle<G::kRow>(g, t) * 16;
@@ -255,22 +259,22 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * A - 1) : "memory");
         __syncwarp();
         const unsigned has = *reinterpret_cast<const unsigned *>(unit + G::kUnit - 16);
-        float x[8];
+        float x[S / 4];
         {
-            int ci[kBytes ? 2 : 1][4][4] = {};
-            float cf[4][4] = {};
-            uint4 kr[4];
+            int ci[kBytes ? 2 : 1][S / 8][4] = {};
+            float cf[S / 8][4] = {};
+            uint4 kr[S / 8];
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 if (ks % 2 == 0)
 #pragma unroll
-                    for (int gr = 0; gr < 4; gr++)
+                    for (int gr = 0; gr < S / 8; gr++)
                         kr[gr] = *reinterpret_cast<const uint4 *>(unit + (k_at ^ (ks / 2 * 64)) + gr * 8 * G::kRow);
 #pragma unroll
                 for (int p = 1; p >= 0; p--) {
                     const uint4 f = qf[p][ks][lane];
 #pragma unroll
-                    for (int gr = 0; gr < 4; gr++) {
+                    for (int gr = 0; gr < S / 8; gr++) {
                         const uint32_t b0 = ks % 2 ? kr[gr].z : kr[gr].x, b1 = ks % 2 ? kr[gr].w : kr[gr].y;
                         if constexpr (kBytes) mma_s8(ci[p][gr], f, b0, b1);
                         else mma_bf16(cf[gr], f.x, f.y, f.z, f.w, b0, b1);
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < S / 4; i++) {
                 const int gr = i >> 1, c = i & 1;
                 if constexpr (kBytes)  // each sum is below 2^21, the lower two together below 2^30
                     x[i] = fmaf((float)ci[0][gr][c], 0x1p-8f, (float)(ci[0][gr][2 + c] * 256 + ci[1][gr][c]) * 0x1p-24f);
@@ -286,25 +290,28 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
             }
         }
         if constexpr (kBytes) {
-            const float *scales = reinterpret_cast<const float *>(unit + 32 * G::kRow) + 2 * t;
+            const float *scales = reinterpret_cast<const float *>(unit + S * G::kRow) + 2 * t;
 #pragma unroll
-            for (int gr = 0; gr < 4; gr++) {
+            for (int gr = 0; gr < S / 8; gr++) {
                 const float2 y = *reinterpret_cast<const float2 *>(scales + 8 * gr);
                 x[2 * gr] *= y.x, x[2 * gr + 1] *= y.y;
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= sc;
-        if (has != 0xffffffffu)
+        for (int i = 0; i < S / 4; i++) x[i] *= sc;
+        if (has != kAll)
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < S / 4; i++)
                 if (!((has >> ((i >> 1) * 8 + 2 * t + (i & 1))) & 1)) x[i] = -INFINITY;
         __syncwarp();  // every lane has read the unit before it is copied into again
         copy_keys();
 
         // ---- weights. The reference moves rarely: when the maximum has passed it by 2^3.
-        auto most_of = [](const float (&y)[8]) {
-            return fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+        auto most_of = [](const float (&y)[S / 4]) {
+            float z = y[0];
+#pragma unroll
+            for (int i = 1; i < S / 4; i++) z = fmaxf(z, y[i]);
+            return z;
         };
         float top = most_of(x);
         if (__any_sync(0xffffffffu, top > m + kPdSlack)) {
@@ -323,9 +330,9 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
             }
             rescale(keep);
         }
-        float w[8];
+        float w[S / 4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < S / 4; i++) {
             w[i] = ex2(x[i] - ref);
             l += w[i];
         }
@@ -334,9 +341,9 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * A - 1) : "memory");
         __syncwarp();
         if constexpr (kBytes) {  // (rows that are not there have scale 0)
-            const float *scales = reinterpret_cast<const float *>(unit + G::kUnit + 32 * G::kRow) + 2 * t;
+            const float *scales = reinterpret_cast<const float *>(unit + G::kUnit + S * G::kRow) + 2 * t;
 #pragma unroll
-            for (int gr = 0; gr < 4; gr++) {
+            for (int gr = 0; gr < S / 8; gr++) {
                 const float2 y = *reinterpret_cast<const float2 *>(scales + 8 * gr);
                 w[2 * gr] *= y.x, w[2 * gr + 1] *= y.y;
             }
@@ -353,11 +360,11 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
                 rescale(keep);
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] *= v_up;
+            for (int i = 0; i < S / 4; i++) w[i] *= v_up;
         }
-        uint32_t pa[4][P];
+        uint32_t pa[S / 8][P];
 #pragma unroll
-        for (int i = 0; i < 4; i++) split_pair<KIND>(w[2 * i], w[2 * i + 1], pa[i]);
+        for (int i = 0; i < S / 8; i++) split_pair<KIND>(w[2 * i], w[2 * i + 1], pa[i]);
         auto pv = [&](int j, int q, uint32_t b0, uint32_t b1, auto apart) {  // rows 16 q .. 16 q + 15
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
             float(&acc)[4] = decltype(apart)::value ? sum : o[j];
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(kPsThreads, kPsCtas) paged_chosen_kernel(const
         auto add_values = [&](auto apart) {
             uint4 vr[4];
 #pragma unroll
-            for (int q = 0; q < 2; q++)
+            for (int q = 0; q < S / 16; q++)
 #pragma unroll
             for (int c = 0; c < VW; c++) {
                 if (c % 4 == 0)

@@ -530,7 +530,7 @@ template <int DIM, int R> void choice_launch(const PagedChoiceArgs &a) {
 
 // CTAs an item: as many as run at once for all items while a warp has two steps, eight at most; and so that no warp sums
 // more than kPdChain steps of 16 rows in the tensor cores, which needs no sums of its own for each.
-template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int rows, long long steps) {
+template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int rows, long long most_rows) {
     constexpr size_t smem = PsGeo<KIND, DIM>::kSmem;
     static PerDeviceOnce once;
     once.run([] {
@@ -538,7 +538,8 @@ template <int KIND, int DIM> void chosen_launch(const PagedChosenArgs &a, int ro
         TCM_CUDA(cudaFuncSetAttribute(paged_chosen_kernel<KIND, DIM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
     const long long items = (long long)rows * a.v.kvheads;
-    const long long fit = kPsCtas * sm_count() / items, worth = steps / (2 * kPsWarps), need = (2 * steps + kPdChain * kPsWarps - 1) / (kPdChain * kPsWarps);
+    const long long steps = (most_rows + 15) / 16;
+    const long long fit = kPsCtas * sm_count() / items, worth = steps / (PsGeo<KIND, DIM>::kStep / 8 * kPsWarps), need = (steps + kPdChain * kPsWarps - 1) / (kPdChain * kPsWarps);
     long long c = fit < worth ? fit : worth;
     c = c > 8 ? 8 : c;
     c = c < need ? need : c;
@@ -611,14 +612,14 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     PagedChosenArgs d = {view, q, out, q_stride, out_stride, group, blocks, 0, lengths, lengths + slab,
                          1.44269504088896340736f / sqrtf((float)view.dim), status};
     const long long held = (long long)blocks * view.page;
-    const long long steps = ((held < view.max_length ? held : view.max_length) + 31) / 32;
+    const long long most_rows = held < view.max_length ? held : view.max_length;
     for (long long r = 0; r < view.rows; r += slab) {
         const int rows = (int)(view.rows - r < slab ? view.rows - r : slab);
         c.row0 = (int)r, c.rows = rows;
         if (view.dim == 64) four ? choice_launch<64, 4>(c) : choice_launch<64, 1>(c);
         else four ? choice_launch<128, 4>(c) : choice_launch<128, 1>(c);
         d.row0 = (int)r;
-#define CALL(K, D) chosen_launch<K, D>(d, rows, steps)
+#define CALL(K, D) chosen_launch<K, D>(d, rows, most_rows)
         PAGED_DISPATCH(view, CALL);
 #undef CALL
     }
