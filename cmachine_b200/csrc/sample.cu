@@ -30,7 +30,7 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 4096, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
+constexpr int kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 constexpr double kSampleOne = 0x1p44;
@@ -50,7 +50,7 @@ struct SampleArgs {
 
 // What a CTA of the cluster tells the others of its slice.
 struct SampleSlice {
-    uint32_t most, least;  // keys of the logits above -infinity
+    uint32_t most, least, counted;  // keys of the logits above -infinity: the largest, the least, the least that the first pass counted
     int live, bad;         // logits above -infinity; a NaN or +infinity among them
 };
 struct SampleSums {
@@ -120,21 +120,31 @@ struct SampleRow {
     }
 };
 
-// Bins over [from, high]: 0 for `high`, and not falling as l falls; all below `from` are the last.
+// Bins of the logits: 0 for the largest, and not falling as l falls; `last` for all that lie so many bins lower, or lower.
+constexpr float kSampleRound = 0x1.8p23f;  // FP32 sums with it are whole numbers, one to one with their bits
+constexpr float kSampleReach = 0x1p19f;
 struct SampleBins {
-    float from, high, unit, scale;
-    int last;
-    __device__ SampleBins(float from_, float high_, int bins) : from(from_), high(high_), last(bins - 1) {
+    float unit, origin, scale, least;
+    int top, last;
+    // Of equal width over [from, high]; what lies below `from` is the last but one at most.
+    __device__ SampleBins(float from, float high, int bins) : last(bins - 1) {
         // Differences in a power of two at which neither they nor the scale leave FP32's range.
         const float span = high - from;
-        unit = span > 1e30f ? 0.25f : span < 1e-25f ? 0x1p100f : 1.f;
-        scale = span > 0.f ? (float)(bins - 2) * 0.999999f / (high * unit - from * unit) : 0.f;
-        high *= unit;
+        unit = span > 1e30f ? 0.25f : span > 0.f && span < 1e-25f ? 0x1p100f : 1.f;
+        origin = high * unit;
+        scale = span > 0.f ? (float)(bins - 2) * 0.999999f / (origin - from * unit) : 0.f;
+        top = __float_as_int(kSampleRound);
+        least = kSampleRound - (float)last;
     }
-    __device__ int of(float l) const {
-        const int b = __float_as_int(fmaf(high - l * unit, scale, 0x1p23f)) & 0x7fffff;
-        return l < from ? last : b;
+    // Of a width given beforehand, 1 / scale, with borders that do not move with the row: slot() tells one of kSampleSlots in a
+    // circle without knowing `high`. |high * scale| is below kSampleReach.
+    static __device__ int slot(float l, float scale) { return __float_as_int(fmaf(l, scale, kSampleRound)) & (kSampleSlots - 1); }
+    __device__ SampleBins(float high, float scale_) : unit(1.f), origin(0.f), scale(scale_), last(kSampleBins - 1) {
+        const float t = fmaf(high, scale, kSampleRound);
+        top = __float_as_int(t);
+        least = t - (float)last;
     }
+    __device__ int of(float l) const { return top - __float_as_int(fmaxf(fmaf(fmaf(l, unit, -origin), scale, kSampleRound), least)); }
     __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
 };
 
@@ -156,31 +166,42 @@ template <bool RESIDENT> struct SampleLogits {
     }
 };
 
-// f(q, quad) for the quads q of [from, to) a thread at a time, `step` apart. Those in global memory come through a ring of
+// f(q, quad) for the quads from, from + STEP, ... below `to`, of a thread. Those in global memory come through a ring of
 // the thread's own in shared memory, kRing of them ahead: HBM and L2 are some 2000 cycles away. (Four ahead in registers
 // left the weights' pass of 256 rows waiting half of its 85 us.)
 constexpr int kRing = 8;
-template <bool RESIDENT, typename F>
-__device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float4 *ring, int from, int to, int step, F f) {
+template <int STEP, bool RESIDENT, typename F>
+__device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float4 *ring, int from, int to, F f) {
     if constexpr (RESIDENT) {
-        for (int q = from; q < to; q += step) f(q, x.quad(q));
+        for (int q = from; q < to; q += STEP) f(q, x.quad(q));
     } else {
+        // Quads that the row's ends cut, then whole ones.
+        if (from == 0 && x.off && to > 0) {
+            f(0, x.quad(0));
+            from += STEP;
+        }
+        const int whole = (x.off + x.n) / 4;
+        if (to > whole) {
+            if (from <= whole && (whole - from) % STEP == 0) f(whole, x.quad(whole));
+            to = whole;
+        }
         float4 *mine = ring + threadIdx.x;
         const uint32_t slots = (uint32_t)__cvta_generic_to_shared(mine);
-        auto whole = [&](int q) { return 4 * q >= x.off && 4 * q + 3 < x.off + x.n; };
-        auto copy = [&](int q, int slot) {
-            if (q < to && whole(q))
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + slot * (kSampleThreads * 16)), "l"(x.x + 4 * q) : "memory");
+        const float4 *src = reinterpret_cast<const float4 *>(x.x) + from;
+        int ahead = from, at = 0;
+        auto copy = [&](int slot) {
+            if (ahead < to) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + slot), "l"(src) : "memory");
             asm volatile("cp.async.commit_group;" ::: "memory");
+            ahead += STEP, src += STEP;
         };
+        constexpr int slot_bytes = kSampleThreads * 16;
 #pragma unroll
-        for (int i = 0; i < kRing; i++) copy(from + i * step, i);
-        int slot = 0;
-        for (int q = from; q < to; q += step) {
+        for (int i = 0; i < kRing; i++) copy(i * slot_bytes);
+        for (int q = from; q < to; q += STEP) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-            const float4 y = whole(q) ? mine[slot * kSampleThreads] : x.quad(q);
-            copy(q + kRing * step, slot);
-            slot = slot == kRing - 1 ? 0 : slot + 1;
+            const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(mine) + at);
+            copy(at);
+            at = (at + slot_bytes) & (kRing * slot_bytes - 1);
             f(q, y);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -529,6 +550,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
+    for (int i = tid; i < (C > 1 ? 1 : 2) * kSampleList / 2; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = sh.list_counted = 0;
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
     const float *src = a.logits + (long long)row * a.stride + base;
@@ -541,9 +565,23 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const SampleLogits<RESIDENT> x = {RESIDENT ? slice_memory : src - off, off, n};
     const SampleLogits<false> global = {src - off, off, n};
     float4 *ring = reinterpret_cast<float4 *>(slice_memory);  // where the slice is not there
-    float most = -INFINITY, least = INFINITY;
+    // Where cuts are asked for, tokens are counted as they come, in bins of a 128th of the temperature whose borders do not
+    // depend on the row: a circle of 8192, as numbers of 16 bits where a slice has no more tokens than they count. Tokens
+    // that are masked with a large number, -1e4 or -FLT_MAX, are left out.
+    unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
+    const float fixed_scale = 128.f / p.temperature;
+    const bool early = (p.top_k > 0 || p.top_p < 1.f) && fixed_scale > 0.f && fixed_scale < INFINITY && (C == 1 || a.slice <= 0xffff);
+    const float fixed_floor = -kSampleReach / fixed_scale;
+    float most = -INFINITY, least = INFINITY, least_counted = INFINITY;
     bool bad = false;
     int live = 0;
+    auto count = [&](float l) {
+        const int b = SampleBins::slot(l, fixed_scale);
+        if (l > fixed_floor) {
+            least_counted = fminf(least_counted, l);
+            atomicAdd(&own[C > 1 ? b / 2 : b], C > 1 ? 1u << b % 2 * 16 : 1u);
+        }
+    };
     auto look = [&](int, const float4 &y) {
         const float l[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -552,6 +590,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             most = fmaxf(most, l[k]);
             if (l[k] > -INFINITY) live++, least = fminf(least, l[k]);
         }
+        if (early)
+#pragma unroll
+            for (int k = 0; k < 4; k++) count(l[k]);
     };
     if constexpr (RESIDENT) {
 #pragma unroll 4
@@ -561,21 +602,19 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             look(q, l);
         }
     } else {
-        each_quad(x, ring, tid, quads, kSampleThreads, look);
+        each_quad<kSampleThreads>(x, ring, tid, quads, look);
     }
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
     const uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
+    const uint32_t warp_counted = __reduce_min_sync(0xffffffffu, sample_key(least_counted));
     bad = __any_sync(0xffffffffu, bad);
     live = __reduce_add_sync(0xffffffffu, live);
     if (lane == 0) {
         sh.warp_count[warp] = live;
         reinterpret_cast<uint32_t *>(sh.warp_high)[warp] = warp_most, reinterpret_cast<uint32_t *>(sh.warp_low)[warp] = warp_least;
+        sh.warp_more[warp] = warp_counted;
         sh.warp_mass[warp] = bad;
     }
-    const bool ranked = p.top_k > 0 || p.top_p < 1.f;
-    if (ranked)
-        for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = sh.list_counted = 0;
     __syncthreads();
     cluster.barrier_wait(std::move(started));
     if (warp == 0) {  // lane c tells CTA c
@@ -583,16 +622,18 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         SampleSlice z;
         z.most = __reduce_max_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_high)[w]);
         z.least = __reduce_min_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_low)[w]);
+        z.counted = __reduce_min_sync(0xffffffffu, (uint32_t)sh.warp_more[w]);
         z.live = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? sh.warp_count[w] : 0);
         z.bad = __any_sync(0xffffffffu, sh.warp_mass[w] != 0);
         if (lane < C) cluster.map_shared_rank(sh.slices, lane)[rank] = z;
     }
     cluster.sync();
-    float high, low;
+    float high, low, low_counted;
     int all_live;
     {
         const SampleSlice z = sh.slices[lane < C ? lane : 0];
         high = sample_value(__reduce_max_sync(0xffffffffu, z.most)), low = sample_value(__reduce_min_sync(0xffffffffu, z.least));
+        low_counted = sample_value(__reduce_min_sync(0xffffffffu, z.counted));
         all_live = __reduce_add_sync(0xffffffffu, lane < C ? z.live : 0);
         bad = __any_sync(0xffffffffu, z.bad);
     }
@@ -650,58 +691,63 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
 
     // ---- the bins in which the cuts lie
     const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f, cuts = by_count || by_mass;
+    // Counts of the first pass hold where the largest token is among them and no slot has two bins.
+    const auto bin_of = [&](float l) { return __float_as_int(fmaf(l, fixed_scale, kSampleRound)); };
     const float reach = (float)(r.top - 32.0 * (double)p.temperature);
-    const SampleBins bins(low < reach && reach < high ? reach : low, high, kSampleBins);
+    bool fixed = early && high > fixed_floor && fabsf(high) * fixed_scale < kSampleReach && bin_of(high) - bin_of(low_counted) < kSampleSlots;
+    SampleBins bins(high, fixed_scale);
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
     int listed = 0;
     bool all_listed = false;
-    if (cuts) {
-        unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
-        each_quad(x, ring, tid, quads, kSampleThreads, [&](int, const float4 &l) {
-            if (l.x > -INFINITY) atomicAdd(&own[bins.of(l.x)], 1u);
-            if (l.y > -INFINITY) atomicAdd(&own[bins.of(l.y)], 1u);
-            if (l.z > -INFINITY) atomicAdd(&own[bins.of(l.z)], 1u);
-            if (l.w > -INFINITY) atomicAdd(&own[bins.of(l.w)], 1u);
-        });
+    for (; cuts; fixed = false) {  // again, with bins over the row's own range, where those hold too many or not at all
+        if (!fixed) {
+            bins = SampleBins(low < reach && reach < high ? reach : low, high, kSampleBins);
+            __syncthreads();
+            for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(own)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+            each_quad<kSampleThreads>(x, ring, tid, quads, [&](int, const float4 &l) {
+                if (l.x > -INFINITY) atomicAdd(&own[bins.of(l.x)], 1u);
+                if (l.y > -INFINITY) atomicAdd(&own[bins.of(l.y)], 1u);
+                if (l.z > -INFINITY) atomicAdd(&own[bins.of(l.z)], 1u);
+                if (l.w > -INFINITY) atomicAdd(&own[bins.of(l.w)], 1u);
+            });
+            if (C > 1) cluster.sync();
+            else __syncthreads();
+        }
         if (tid == 0) sh.bin = kSampleBins, sh.mass_from = sh.mass_to = kSampleBins - 1;
         if (C > 1) {
-            cluster.sync();
             // Each CTA adds up its share of the bins and tells the others.
             const int share_of = kSampleBins / C;
-            for (int i = 4 * tid; i < share_of; i += 4 * kSampleThreads) {
-                const int b = rank * share_of + i;
-                uint4 c = make_uint4(0, 0, 0, 0);
+            for (int i = tid; i < share_of; i += kSampleThreads) {
+                const int b = rank * share_of + i, at = fixed ? (bins.top - b) & (kSampleSlots - 1) : b;
+                unsigned c = 0;
 #pragma unroll 8
                 for (int k = 0; k < C; k++) {
-                    const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(own, k) + b);
-                    c.x += y.x, c.y += y.y, c.z += y.z, c.w += y.w;
+                    const unsigned *theirs = cluster.map_shared_rank(own, k);
+                    c += fixed ? reinterpret_cast<const unsigned short *>(theirs)[at] : theirs[at];
                 }
 #pragma unroll 8
-                for (int k = 0; k < C; k++) *reinterpret_cast<uint4 *>(cluster.map_shared_rank(counts, k) + b) = c;
+                for (int k = 0; k < C; k++) cluster.map_shared_rank(counts, k)[b] = c;
             }
             cluster.sync();
         } else {
             __syncthreads();
-            counts = own;
         }
         constexpr int each = kSampleBins / kSampleThreads;
         unsigned c[each], upto = 0;
         float mass[each], total = 0.f, squares = 0.f;
         const float step = (float)(-bins.width() * r.slope);
 #pragma unroll
-        for (int k = 0; k < each; k += 4) {
-            const uint4 y = *reinterpret_cast<const uint4 *>(counts + tid * each + k);
-            c[k] = y.x, c[k + 1] = y.y, c[k + 2] = y.z, c[k + 3] = y.w;
-        }
-#pragma unroll
         for (int k = 0; k < each; k++) {
             const int b = tid * each + k;
+            c[k] = C > 1 ? counts[b] : fixed ? own[(bins.top - b) & (kSampleSlots - 1)] : own[b];
+            if (b == kSampleBins - 1) c[k] = 0;  // and all that lie lower: what the others leave
             const float weight = b == kSampleBins - 1 ? 0.f : exp2f((float)b * step);
             mass[k] = (float)c[k] * weight;
             upto += c[k], total += mass[k], squares += mass[k] * weight;
         }
-        const unsigned mine = upto;
+        unsigned mine = upto;
         const float mine_mass = total;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -721,6 +767,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             if (w < warp) before += (unsigned)sh.warp_count[w], lighter += sh.warp_high[w];
             whole += sh.warp_high[w];
         }
+        if (tid == kSampleThreads - 1) c[each - 1] = (unsigned)all_live - before - mine, mine += c[each - 1];
         if (by_count) {
             const unsigned k = (unsigned)p.top_k;
             if (before < k && k <= before + mine) {
@@ -738,8 +785,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             __syncthreads();
             count_bin = sh.bin, tokens_left = p.top_k - sh.above, in_count_bin = sh.in_bin;
             whole = sh.mass_whole;
-            all_listed = sh.above + sh.in_bin <= kSampleList;
         }
+        all_listed = by_count && sh.above + sh.in_bin <= kSampleList;
         listed = in_count_bin;
         if (all_listed) {  // a small k: all tokens down to its bin, and no estimate
             mass_from = 0, mass_to = count_bin;
@@ -778,11 +825,12 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             __syncthreads();
             listed = sh.list_to - sh.list_from + (mass_to < count_bin ? in_count_bin : 0);
         }
-        if (listed > kSampleList) {
+        if (C == 1) __syncthreads();  // the counts have been read: the list takes their place
+        if (listed <= kSampleList) break;
+        if (!fixed) {
             sample_slowly(a, r, sh, x, base, row, low, high, all_live, min_logit);
             return;
         }
-        if (C == 1) __syncthreads();  // the counts have been read: the list takes their place
     }
 
     // ---- weights above the bins, and the list of what is in them. A warp has a contiguous stretch of ids.
@@ -817,13 +865,13 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                     if (in(l[k])) append(l[k], 4 * q + k - off);
         };
         if (all_listed) {
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 const float l[4] = {y.x, y.y, y.z, y.w};
                 append_some(q, l, [&](float z) { return z >= in_to; });
             });
         } else if (by_count) {
             const float count_from = sh.border[2], count_to = sh.border[3];
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= count_to)) return;
                 const float l[4] = {y.x, y.y, y.z, y.w};
                 append_some(q, l, [&](float z) { return (z < sure && z >= in_to) || (z < count_from && z >= count_to); });
@@ -836,9 +884,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 }
             });
         } else if (p.min_p > 0.f) {
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 const float l[4] = {y.x, y.y, y.z, y.w};
-                append_some(q, l, [&](float z) { return z < sure && z >= in_to; });
+                append_some(q, l, [&](float z) { return !(z >= sure) && z >= in_to; });
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const u64 w = r.weight(l[k]);
@@ -848,9 +896,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 }
             });
         } else {
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int q, const float4 &y) {
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 const float l[4] = {y.x, y.y, y.z, y.w};
-                append_some(q, l, [&](float z) { return z < sure && z >= in_to; });
+                append_some(q, l, [&](float z) { return !(z >= sure) && z >= in_to; });
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const u64 w = r.weight(l[k]);
@@ -864,7 +912,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         sum_kept = sum_above - sum_kept;
     } else {
         if (p.min_p > 0.f)
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int, const float4 &y) {
                 if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= min_logit)) return;
                 const float l[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -874,7 +922,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 }
             });
         else {
-            each_quad(x, ring, w0 + lane, w1, 32, [&](int, const float4 &y) {  // masked tokens weigh nothing
+            each_quad<32>(x, ring, w0 + lane, w1, [&](int, const float4 &y) {  // masked tokens weigh nothing
                 sum_kept += (r.weight(y.x) + r.weight(y.y)) + (r.weight(y.z) + r.weight(y.w));
             });
             if (rank == 0 && tid == 0) kept = all_live;

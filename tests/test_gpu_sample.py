@@ -154,6 +154,32 @@ def test_logits_of_any_size(scale):
               rng.random(6).astype(np.float32))
 
 
+@pytest.mark.parametrize("vocab", [700, 30000, 151936, 400000])
+def test_ranges_of_every_width(vocab):
+    """Rows that are narrow and wide against their temperature, far from zero, with tokens masked by large numbers."""
+    rng = np.random.default_rng(vocab)
+    rows = []
+    for t in (1.0, 0.6):
+        for spread, at in ((0.02, 0), (0.3, -40), (1.5, 15), (6.0, 0), (9.0, 300), (30.0, 0), (2.0, 3900), (2.0, 5000), (2.0, -60000)):
+            x = (rng.standard_normal(vocab) * spread + at).astype(np.float32)
+            for fill in (None, -1e4, -3000.0, LOW):
+                y = x.copy()
+                if fill is not None:
+                    y[rng.random(vocab) < 0.4] = fill
+                rows.append((y, t))
+    settings = [(0, 0.9), (50, 1.0), (0, 0.5), (5000, 0.97)]
+    for i in range(0, len(rows), 36):
+        part = rows[i:i + 36]
+        check(np.stack([x for x, _ in part]), [(t, *settings[(i + j + j // 4) % 4], 0.0) for j, (_, t) in enumerate(part)],
+              rng.random(len(part)).astype(np.float32), pad=i % 4)
+
+
+@pytest.mark.parametrize("value", [0.0, 5.0, -4096.0, 1e10, -1e30, 3e38])
+def test_one_value_of_any_size(value):
+    logits = np.full((4, 5000), value, np.float32)
+    check(logits, [(1.0, 0, 0.9, 0.0), (1e-3, 100, 1.0, 0.0), (1e30, 100, 0.3, 0.0), (1e-38, 0, 0.7, 0.5)], np.array([0.3, 0.9, 0.77, 0.1], np.float32))
+
+
 def test_logits_that_halve():
     """Values that fall by powers of two: each pass over the range cuts off the few largest."""
     x = (2.0 ** -np.arange(240)).astype(np.float32) * np.float32(2.0**100)
