@@ -22,6 +22,7 @@
 #include <cooperative_groups.h>
 #include <float.h>
 #include <math.h>
+#include <type_traits>
 #include <utility>
 
 namespace cg = cooperative_groups;
@@ -120,7 +121,7 @@ struct SampleRow {
     }
 };
 
-// Bins of the logits: 0 for the largest, and not falling as l falls; `last` for all that lie so many bins lower, or lower.
+// Bins of the logits: one of the first eight for the largest, and not falling as l falls; `last` for all that lie so many bins lower, or lower.
 constexpr float kSampleRound = 0x1.8p23f;  // FP32 sums with it are whole numbers, one to one with their bits
 constexpr float kSampleReach = 0x1p19f;
 struct SampleBins {
@@ -140,9 +141,8 @@ struct SampleBins {
     // circle without knowing `high`. |high * scale| is below kSampleReach.
     static __device__ int slot(float l, float scale) { return __float_as_int(fmaf(l, scale, kSampleRound)) & (kSampleSlots - 1); }
     __device__ SampleBins(float high, float scale_) : unit(1.f), origin(0.f), scale(scale_), last(kSampleBins - 1) {
-        const float t = fmaf(high, scale, kSampleRound);
-        top = __float_as_int(t);
-        least = t - (float)last;
+        top = __float_as_int(fmaf(high, scale, kSampleRound)) | 7;  // so that a thread's eight slots are two aligned quads
+        least = __int_as_float(top) - (float)last;
     }
     __device__ int of(float l) const { return top - __float_as_int(fmaxf(fmaf(fmaf(l, unit, -origin), scale, kSampleRound), least)); }
     __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
@@ -448,7 +448,7 @@ constexpr int kEach = kSampleList / kSampleThreads;
 // most (there are `most_members` in all at most), which are compared with one another. All threads call it; ~0
 // where there is none. Numbers are unique, so it ends.
 __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u64 (&w)[kEach], const bool (&member)[kEach], int most_members,
-                           bool by_mass, int tokens, double share, u64 heavier) {
+                           bool by_mass, int tokens, u64 share, u64 heavier) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     SampleSearch &in = *reinterpret_cast<SampleSearch *>(sh.buffer[1]);
     u64 base = 0, width = ~0ull;
@@ -496,14 +496,14 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
                     const u64 z = __shfl_up_sync(0xffffffffu, sum, o);
                     if (lane >= o) upto += y, sum += z;
                 }
-                const bool here = by_mass ? mine && (double)(heavier + sum) >= share : upto >= (unsigned)tokens;
+                const bool here = by_mass ? mine && heavier + sum >= share : upto >= (unsigned)tokens;
                 const unsigned reached = __ballot_sync(0xffffffffu, here);
                 if (reached && lane == __ffs(reached) - 1) {
                     unsigned above = upto - mine;
                     u64 mass = heavier + sum - mine_mass;
 #pragma unroll
                     for (int k = 0; k < per_lane; k++) {
-                        if (sh.sub_bin < 0 && c[k] && (by_mass ? (double)(mass + m[k]) >= share : above + c[k] >= (unsigned)tokens))
+                        if (sh.sub_bin < 0 && c[k] && (by_mass ? mass + m[k] >= share : above + c[k] >= (unsigned)tokens))
                             sh.sub_bin = lane * per_lane + k, sh.sub_above = (int)above, sh.found_mass = mass;
                         above += c[k], mass += m[k];
                     }
@@ -536,7 +536,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
         for (int i = 0; i < few; i++)
             if (in.few[i] < mine) above++, heavier += in.few_mass[i];
         // The first at which it is reached: the one before it does not reach it.
-        if (by_mass ? (double)(heavier + mass) >= share && (!above || (double)heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
+        if (by_mass ? heavier + mass >= share && (!above || heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
     }
     __syncthreads();
     return sh.found;
@@ -575,35 +575,38 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     float most = -INFINITY, least = INFINITY, least_counted = INFINITY;
     bool bad = false;
     int live = 0;
-    auto count = [&](float l) {
-        const int b = SampleBins::slot(l, fixed_scale);
-        if (l > fixed_floor) {
-            least_counted = fminf(least_counted, l);
-            atomicAdd(&own[C > 1 ? b / 2 : b], C > 1 ? 1u << b % 2 * 16 : 1u);
-        }
-    };
-    auto look = [&](int, const float4 &y) {
-        const float l[4] = {y.x, y.y, y.z, y.w};
+    auto first_pass = [&](auto early, auto packed) {
+        auto look = [&](int, const float4 &y) {
+            const float l[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            bad |= !(l[k] < INFINITY);
-            most = fmaxf(most, l[k]);
-            if (l[k] > -INFINITY) live++, least = fminf(least, l[k]);
-        }
-        if (early)
-#pragma unroll
-            for (int k = 0; k < 4; k++) count(l[k]);
-    };
-    if constexpr (RESIDENT) {
+            for (int k = 0; k < 4; k++) {
+                bad |= !(l[k] < INFINITY);
+                most = fmaxf(most, l[k]);
+                if (l[k] > -INFINITY) live++, least = fminf(least, l[k]);
+                if constexpr (decltype(early)::value) {
+                    const int b = SampleBins::slot(l[k], fixed_scale);
+                    if (l[k] > fixed_floor) {
+                        least_counted = fminf(least_counted, l[k]);
+                        if constexpr (decltype(packed)::value) atomicAdd(&own[b / 2], 1u << b % 2 * 16);
+                        else atomicAdd(&own[b], 1u);
+                    }
+                }
+            }
+        };
+        if constexpr (RESIDENT) {
 #pragma unroll 4
-        for (int q = tid; q < quads; q += kSampleThreads) {
-            const float4 l = global.quad(q);
-            reinterpret_cast<float4 *>(slice_memory)[q] = l;
-            look(q, l);
+            for (int q = tid; q < quads; q += kSampleThreads) {
+                const float4 l = global.quad(q);
+                reinterpret_cast<float4 *>(slice_memory)[q] = l;
+                look(q, l);
+            }
+        } else {
+            each_quad<kSampleThreads>(x, ring, tid, quads, look);
         }
-    } else {
-        each_quad<kSampleThreads>(x, ring, tid, quads, look);
-    }
+    };
+    if (!early) first_pass(std::false_type{}, std::false_type{});
+    else if (C > 1) first_pass(std::true_type{}, std::true_type{});
+    else first_pass(std::true_type{}, std::false_type{});
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
     const uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
     const uint32_t warp_counted = __reduce_min_sync(0xffffffffu, sample_key(least_counted));
@@ -691,11 +694,11 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
 
     // ---- the bins in which the cuts lie
     const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f, cuts = by_count || by_mass;
-    // Counts of the first pass hold where the largest token is among them and no slot has two bins.
-    const auto bin_of = [&](float l) { return __float_as_int(fmaf(l, fixed_scale, kSampleRound)); };
     const float reach = (float)(r.top - 32.0 * (double)p.temperature);
-    bool fixed = early && high > fixed_floor && fabsf(high) * fixed_scale < kSampleReach && bin_of(high) - bin_of(low_counted) < kSampleSlots;
     SampleBins bins(high, fixed_scale);
+    // Counts of the first pass hold where the largest token is among them and no slot has two bins.
+    bool fixed = early && high > fixed_floor && fabsf(high) * fixed_scale < kSampleReach &&
+                 bins.top - __float_as_int(fmaf(low_counted, fixed_scale, kSampleRound)) < kSampleSlots;
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
     int listed = 0;
@@ -738,10 +741,15 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         unsigned c[each], upto = 0;
         float mass[each], total = 0.f, squares = 0.f;
         const float step = (float)(-bins.width() * r.slope);
+        static_assert(each == 8, "two quads");
+        const bool circle = C == 1 && fixed;  // in which bins go down
+        const unsigned *from = C > 1 ? counts + tid * each : circle ? own + ((bins.top - tid * each - (each - 1)) & (kSampleSlots - 1)) : own + tid * each;
+        const uint4 some_low = reinterpret_cast<const uint4 *>(from)[0], some_high = reinterpret_cast<const uint4 *>(from)[1];
+        const unsigned some[each] = {some_low.x, some_low.y, some_low.z, some_low.w, some_high.x, some_high.y, some_high.z, some_high.w};
 #pragma unroll
         for (int k = 0; k < each; k++) {
             const int b = tid * each + k;
-            c[k] = C > 1 ? counts[b] : fixed ? own[(bins.top - b) & (kSampleSlots - 1)] : own[b];
+            c[k] = circle ? some[7 - k] : some[k];
             if (b == kSampleBins - 1) c[k] = 0;  // and all that lie lower: what the others leave
             const float weight = b == kSampleBins - 1 ? 0.f : exp2f((float)b * step);
             mass[k] = (float)c[k] * weight;
@@ -839,20 +847,21 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     u64 sum_above = 0, sum_all = 0, sum_kept = 0;
     int kept = 0;
     if (cuts) {
-        // The bins' borders as logits: the least of a bin and those above it, found by halving as the arithmetic of bins.of()
+        // The bins' borders as logits: the least of a bin and those above it, found by trial as the arithmetic of bins.of()
         // has it. Tokens from `sure` on are above the bins in question and kept; from `in_from` down to `in_to` in top-p's,
         // from `count_from` down to `count_to` in top-k's.
-        if (warp == 0) {
-            const int b = lane == 0 ? (by_mass || all_listed ? mass_from : count_bin) - 1 : lane == 1 ? mass_to : lane == 2 ? count_bin - 1 : count_bin;
+        if (warp < 4) {  // a warp a border: 32 numbers at a time cut the range into 33
+            const int b = warp == 0 ? (by_mass || all_listed ? mass_from : count_bin) - 1 : warp == 1 ? mass_to : warp == 2 ? count_bin - 1 : count_bin;
             uint32_t down = sample_key(-FLT_MAX), up = sample_key(high);  // bins.of(up) <= b, or none is
-            if (b < 0) down = up = sample_key(INFINITY);
-            else if (bins.of(-FLT_MAX) <= b) up = down;
+            if (b < bins.of(high)) down = up = sample_key(INFINITY);
             while (down < up) {
-                const uint32_t mid = down + (up - down) / 2;
-                if (bins.of(sample_value(mid)) <= b) up = mid;
-                else down = mid + 1;
+                const uint32_t step = (up - down) / 33 + 1, at = up - down > (lane + 1) * step ? up - (lane + 1) * step : down;
+                const unsigned in = __ballot_sync(0xffffffffu, bins.of(sample_value(at)) <= b);  // the first lanes
+                const uint32_t most = up - down, passed = __popc(in);
+                up = most > passed * step ? up - passed * step : down;
+                if (passed < 32) down = most > (passed + 1) * step ? up - step + 1 : down + 1;
             }
-            if (lane < 4) sh.border[lane] = sample_value(up);
+            if (lane == 0) sh.border[warp] = sample_value(up);
         }
         __syncthreads();
         const float sure = sh.border[0], in_to = by_mass || all_listed ? sh.border[1] : INFINITY;
@@ -977,19 +986,22 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             member[k] = i < m;
             if (member[k]) {
                 int c = 0;
-                while (c + 1 < C && sh.list_start[c + 1] <= i) c++;
+#pragma unroll
+                for (int j = 1; j < kSampleCluster; j++) c += j < C && sh.list_start[j] <= i;
                 token[k] = cluster.map_shared_rank(own_list, c)[i - sh.list_start[c]];
             }
         }
 #pragma unroll
         for (int k = 0; k < kEach; k++) {
+            w[k] = 0, counted[k] = false;
+            if (k * kSampleThreads + warp * 32 >= m) continue;
             const float l = sample_value(~(uint32_t)(token[k] >> 32));
             w[k] = member[k] ? r.weight(l) : 0;
             counted[k] = member[k] && by_count && bins.of(l) <= count_bin && (all_listed || bins.of(l) == count_bin);
         }
         if (C > 1) cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
         cut = ~0ull;
-        if (by_count) cut = search_list(sh, token, w, counted, m, false, tokens_left, 0.0, 0);
+        if (by_count) cut = search_list(sh, token, w, counted, m, false, tokens_left, 0, 0);
         if (by_mass) {
             u64 all_of = sh.everything;
             if (by_count) {
@@ -1004,10 +1016,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 __syncthreads();
                 all_of += sh.list_counted;
             }
-            const double share = fmax(0.0, (double)p.top_p) * (double)all_of;
+            const u64 share = (u64)ceil(fmax(0.0, (double)p.top_p) * (double)all_of);  // no sum is nearer to it than its rounding
             const u64 last = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
             // In top-p's bins, or the estimate was wrong.
-            const bool fine = (mass_from == 0 || (double)sh.heavier < share) && last != ~0ull &&
+            const bool fine = (mass_from == 0 || sh.heavier < share) && last != ~0ull &&
                               bins.of(sample_value(~(uint32_t)(last >> 32))) <= mass_to;
             if (!fine) {  // the whole cluster alike
                 if (C > 1) cluster.barrier_wait();
@@ -1044,8 +1056,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     if (target >= whole) target = whole - 1;
 
     // ---- the token: the warp's stretch that holds it, in 16 parts for the warps, then the part by one warp
-    auto weights = [&](int q, u64 (&w)[4]) {  // what is kept of a quad
-        const float4 y = x.quad(q);
+    auto weights = [&](int q, const float4 &y, u64 (&w)[4]) {  // what is kept of a quad
         const float l[4] = {y.x, y.y, y.z, y.w};
         u64 sum = 0;
 #pragma unroll
@@ -1075,26 +1086,35 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     if (who >= 0) {  // this CTA has it
         const int s0 = min(quads, who * per_warp), s1 = min(quads, s0 + per_warp), part = (s1 - s0 + kSampleWarps - 1) / kSampleWarps;
         u64 w[4], sum = 0;
-        for (int q = s0 + warp * part + lane; q < min(s1, s0 + (warp + 1) * part); q += 32) sum += weights(q, w);
+        each_quad<32>(x, ring, s0 + warp * part + lane, min(s1, s0 + (warp + 1) * part), [&](int q, const float4 &y) { sum += weights(q, y, w); });
         sum = warp_sum64(sum);
         if (lane == 0) sh.warp_mass[warp] = sum;
         __syncthreads();
         const int mine = holder(lane < kSampleWarps ? sh.warp_mass[lane] : 0);
         if (warp == mine) {
             const int q1 = min(s1, s0 + (warp + 1) * part);
-            for (int q0 = s0 + warp * part; q0 < q1; q0 += 32) {
-                const int q = q0 + lane;
-                w[0] = w[1] = w[2] = w[3] = 0;
-                const u64 own = q < q1 ? weights(q, w) : 0;
-                u64 upto = own;
+            bool found = false;
+            constexpr int kLoads = 4;  // at a time
+            for (int q0 = s0 + warp * part; q0 < q1 && !found; q0 += 32 * kLoads) {
+                float4 y[kLoads];
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 z = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += z;
+                for (int i = 0; i < kLoads; i++) {
+                    const int q = q0 + 32 * i + lane;
+                    y[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (q < q1) y[i] = x.quad(q);
                 }
-                const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
-                if (reached) {
-                    if (lane == __ffs(reached) - 1) {
+#pragma unroll
+                for (int i = 0; i < kLoads; i++) {
+                    const int q = q0 + 32 * i + lane;
+                    w[0] = w[1] = w[2] = w[3] = 0;
+                    u64 upto = q < q1 ? weights(q, y[i], w) : 0;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 z = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += z;
+                    }
+                    const unsigned reached = found ? 0 : __ballot_sync(0xffffffffu, before + upto > target);
+                    if (reached && lane == __ffs(reached) - 1) {
                         u64 to = before + upto;
                         int id = 0;
 #pragma unroll
@@ -1106,9 +1126,9 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                         if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x.at(id)) - log((double)whole / kSampleOne));
                         if (a.kept) a.kept[row] = sh.kept + (cuts ? sh.list_count : 0);
                     }
-                    break;
+                    found |= reached != 0;
+                    before += __shfl_sync(0xffffffffu, upto, 31);
                 }
-                before += __shfl_sync(0xffffffffu, upto, 31);
             }
         }
     }
