@@ -34,7 +34,6 @@ constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
-constexpr double kSampleOne = 0x1p44;
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -51,7 +50,7 @@ struct SampleArgs {
 
 // What a CTA of the cluster tells the others of its slice.
 struct SampleSlice {
-    uint32_t most, least, counted;  // keys of the logits above -infinity: the largest, the least, the least that the first pass counted
+    uint32_t most, counted;  // keys of the logits above -infinity: the largest, the least that the first pass counted
     int live, bad;         // logits above -infinity; a NaN or +infinity among them
 };
 struct SampleSums {
@@ -64,7 +63,7 @@ struct SampleShared {
     SampleSlice slices[kSampleCluster];
     SampleSums sums[kSampleCluster];
     int first[kSampleCluster];       // greedy rows: the lowest id of the largest logit
-    float2 ends[kSampleCluster];     // least and largest logit of the slow search's bin
+    float2 ends[kSampleCluster];     // least and largest logit above -infinity, or of the slow search's bin
     u64 part_mass[kSampleCluster];
     int part_count[kSampleCluster];
     u64 warp_mass[kSampleWarps], warp_more[kSampleWarps], warp_kept[kSampleWarps];
@@ -101,15 +100,24 @@ __device__ __forceinline__ float sample_value(uint32_t key) {
 }
 
 // (2^f - 1) / f for |f| <= 1/2, interpolated at the seven Chebyshev points there: 2^f is off by 2^-33 at most.
-__device__ constexpr double kSampleSeries[7] = {0.6931471805599453,    0.24022650922288757,   0.055504108839096185,  0.009618056678524632,
-                                                0.0013333502386162978, 0.00015461444698571227, 1.5297323760649362e-05};
+__constant__ double kSampleSeries[7] = {0.6931471805599453,    0.24022650922288757,   0.055504108839096185,  0.009618056678524632,
+                                        0.0013333502386162978, 0.00015461444698571227, 1.5297323760649362e-05};
 
 struct SampleRow {
-    double top, cold, slope;  // the largest logit, 1 / T, log2(e) / T
+    double top, cold;      // the largest logit, 1 / T
+    double slope, offset;  // log2(e) / T, and -top times that
+    // The product is off by 2^-53 of itself, 2^-23 at most as no slope is larger than 2^30 / |top|, at which FP32's next lower
+    // number weighs nothing. All weights of the row are off by that one factor, and weight(top) by the same.
+    __device__ SampleRow(float high, float temperature) : top(high), cold(1.0 / (double)temperature) {
+        slope = 1.4426950408889634074 * cold;
+        if (slope * fabs(top) > 0x1p30) slope = 0x1p30 / fabs(top);
+        offset = -top * slope;
+    }
     __device__ double exponent(float l) const { return ((double)l - top) * cold; }
+    __device__ float logprob(float l, u64 whole) const { return (float)(exponent(l) - log((double)whole / (double)weight((float)top))); }
     __device__ u64 weight(float l) const {
-        const double y0 = ((double)l - top) * slope;
-        // At most zero; from -64 on (its upper word decides) nothing is left of it.
+        const double y0 = fma((double)l, slope, offset);
+        // At most 2^-23; from -64 on (its upper word decides) nothing is left of it.
         const double y = __hiloint2double((int)min((unsigned)__double2hiint(y0), 0xc0500000u), __double2loint(y0));
         const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
         double z = kSampleSeries[6];
@@ -121,9 +129,10 @@ struct SampleRow {
     }
 };
 
-// Bins of the logits: one of the first eight for the largest, and not falling as l falls; `last` for all that lie so many bins lower, or lower.
-constexpr float kSampleRound = 0x1.8p23f;  // FP32 sums with it are whole numbers, one to one with their bits
-constexpr float kSampleReach = 0x1p19f;
+// Bins of the logits: one of the first eight for the largest, and not falling as l falls; `last` for all that lie so many
+// bins lower, or lower. FP32 sums with kSampleRound are whole numbers, one to one with their bits;
+// they go to the nearest, and to even ones from between, so that bins are not off to one side of logits of 16 bits.
+constexpr float kSampleRound = 0x1.8p23f, kSampleReach = 0x1p19f;
 struct SampleBins {
     float unit, origin, scale, least;
     int top, last;
@@ -142,11 +151,16 @@ struct SampleBins {
     static __device__ int slot(float l, float scale) { return __float_as_int(fmaf(l, scale, kSampleRound)) & (kSampleSlots - 1); }
     __device__ SampleBins(float high, float scale_) : unit(1.f), origin(0.f), scale(scale_), last(kSampleBins - 1) {
         top = __float_as_int(fmaf(high, scale, kSampleRound)) | 7;  // so that a thread's eight slots are two aligned quads
-        least = __int_as_float(top) - (float)last;
+        least = __int_as_float(top - last);
     }
     __device__ int of(float l) const { return top - __float_as_int(fmaxf(fmaf(fmaf(l, unit, -origin), scale, kSampleRound), least)); }
     __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
 };
+
+// Adds to a word of shared memory where `is`, without a branch.
+__device__ __forceinline__ void count_if(bool is, uint32_t address, unsigned x) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %0, 0;\n @p red.shared.add.u32 [%1], %2;\n}" ::"r"((unsigned)is), "r"(address), "r"(x) : "memory");
+}
 
 // A CTA's slice of the row: `off` elements behind a 16-byte boundary, in shared memory with -infinity around it, or where
 // it is in global memory, read again by every pass (from L2, mostly).
@@ -175,16 +189,14 @@ __device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float
     if constexpr (RESIDENT) {
         for (int q = from; q < to; q += STEP) f(q, x.quad(q));
     } else {
-        // Quads that the row's ends cut, then whole ones.
+        // Quads that the slice's ends cut, and whole ones between.
         if (from == 0 && x.off && to > 0) {
             f(0, x.quad(0));
             from += STEP;
         }
         const int whole = (x.off + x.n) / 4;
-        if (to > whole) {
-            if (from <= whole && (whole - from) % STEP == 0) f(whole, x.quad(whole));
-            to = whole;
-        }
+        const bool cut = to > whole && from <= whole && (whole - from) % STEP == 0;
+        to = min(to, whole);
         float4 *mine = ring + threadIdx.x;
         const uint32_t slots = (uint32_t)__cvta_generic_to_shared(mine);
         const float4 *src = reinterpret_cast<const float4 *>(x.x) + from;
@@ -205,6 +217,7 @@ __device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float
             f(q, y);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (cut) f(whole, x.quad(whole));
     }
 }
 
@@ -212,7 +225,7 @@ __device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float
 // bin that it falls into, until that holds one value. Then who is kept, and the token. All threads of the cluster call it.
 template <bool RESIDENT>
 __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow &r, SampleShared &sh, const SampleLogits<RESIDENT> &x, int base, int row,
-                                            float low_all, float high_all, int live, float min_logit) {
+                                            float high_all, int live, float min_logit) {
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -232,7 +245,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     // There is one.
     auto find = [&](bool by_mass, int tokens, double share, float floor) {
         Cut cut = {0.f, 0, 0, 0};
-        float low = fmaxf(low_all, floor), high = high_all;
+        float low = fmaxf(-FLT_MAX, floor), high = high_all;
         // Weights end 32 temperatures below the largest; what lies lower is one bin until the cut is known to be there.
         const float reach = (float)(r.top - 32.0 * (double)p.temperature);
         float from = low < reach && reach < high ? reach : low;
@@ -425,7 +438,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
         const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
         if (reached && lane == __ffs(reached) - 1) {
             a.ids[row] = base + i;
-            if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x.at(i)) - log((double)whole / kSampleOne));
+            if (a.logprobs) a.logprobs[row] = r.logprob(x.at(i), whole);
             if (a.kept) a.kept[row] = kept;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -435,12 +448,21 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
 
 // The memory of the search for the cut in the list, in the place of the cluster's counts.
 struct SampleSearch {
-    u64 mass[kSubBins], few[kFew], few_mass[kFew];
-    unsigned count[kSubBins];
+    // A bin's count above its weight's upper bits, and the next 21 and 21 of it, so that native atomics add them up: a loop
+    // for 64 bits took 31 us where 400 equal logits met in a bin.
+    unsigned top[kSubBins], middle[kSubBins], low[kSubBins];
+    u64 few[kFew], few_mass[kFew];
+    __device__ unsigned count(int b) const { return top[b] >> 16; }
+    __device__ u64 mass(int b) const { return ((u64)(top[b] & 0xffff) << 42) + ((u64)middle[b] << 21) + low[b]; }
 };
+static_assert(kSampleList * 8 <= 0xffff && (u64)kSampleList << 21 <= 1ull << 32, "the parts' sums fit");
 static_assert(sizeof(SampleSearch) <= sizeof(SampleShared::buffer[1]), "the search's memory fits the buffer");
 
 // A CTA's share of the cluster's list: every thread holds up to four tokens, as (descending logit, id) in one number.
+constexpr int kIdBits = 19;
+static_assert(kSampleVocab == 1 << kIdBits, "ids fit");
+__device__ __forceinline__ float token_logit(u64 token) { return sample_value(~(uint32_t)(token >> kIdBits)); }
+__device__ __forceinline__ int token_id(u64 token) { return (int)(token & (kSampleVocab - 1)); }
 constexpr int kEach = kSampleList / kSampleThreads;
 
 // Of the tokens marked as members, the first in order with which `tokens` of them are reached (by_mass false), or with
@@ -460,23 +482,23 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
         uint32_t least = 0xffffffffu, most = 0;
 #pragma unroll
         for (int k = 0; k < kEach; k++)
-            if (member[k]) least = min(least, (uint32_t)(token[k] >> 32)), most = max(most, (uint32_t)(token[k] >> 32));
+            if (member[k]) least = min(least, (uint32_t)(token[k] >> kIdBits)), most = max(most, (uint32_t)(token[k] >> kIdBits));
         least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0 && least <= most) atomicMin(&sh.sub_least, least), atomicMax(&sh.sub_most, most);
         __syncthreads();
         if (sh.sub_least > sh.sub_most) return ~0ull;
-        base = (u64)sh.sub_least << 32, width = ((u64)(sh.sub_most - sh.sub_least) << 32) | 0xffffffffu;
+        base = (u64)sh.sub_least << kIdBits, width = ((u64)(sh.sub_most - sh.sub_least) << kIdBits) | (kSampleVocab - 1);
         int shift = 64 - __clzll((long long)width) - 8;
         for (;;) {
-            for (int i = tid; i < kSubBins; i += kSampleThreads) in.count[i] = 0, in.mass[i] = 0;
+            for (int i = tid; i < kSubBins; i += kSampleThreads) in.top[i] = in.middle[i] = in.low[i] = 0;
             if (tid == 0) sh.sub_bin = -1;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kEach; k++)
                 if (member[k] && token[k] - base <= width) {
                     const int b = (int)((token[k] - base) >> shift);
-                    atomicAdd(&in.count[b], 1u);
-                    if (by_mass) atomicAdd(&in.mass[b], w[k]);
+                    atomicAdd(&in.top[b], 0x10000u + (unsigned)(w[k] >> 42));
+                    if (by_mass) atomicAdd(&in.middle[b], (unsigned)(w[k] >> 21) & 0x1fffffu), atomicAdd(&in.low[b], (unsigned)w[k] & 0x1fffffu);
                 }
             __syncthreads();
             if (warp == 0) {
@@ -485,7 +507,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
                 u64 m[per_lane], sum = 0;
 #pragma unroll
                 for (int k = 0; k < per_lane; k++) {
-                    c[k] = in.count[lane * per_lane + k], m[k] = in.mass[lane * per_lane + k];
+                    c[k] = in.count(lane * per_lane + k), m[k] = in.mass(lane * per_lane + k);
                     upto += c[k], sum += m[k];
                 }
                 const unsigned mine = upto;
@@ -516,7 +538,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
             if (by_mass) heavier = sh.found_mass;
             base += (u64)bin << shift;
             width = ((u64)1 << shift) - 1;
-            if (in.count[bin] <= kFew) break;
+            if (in.count(bin) <= kFew) break;
             shift = shift > 8 ? shift - 8 : 0;
             __syncthreads();
         }
@@ -572,24 +594,26 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const float fixed_scale = 128.f / p.temperature;
     const bool early = (p.top_k > 0 || p.top_p < 1.f) && fixed_scale > 0.f && fixed_scale < INFINITY && (C == 1 || a.slice <= 0xffff);
     const float fixed_floor = -kSampleReach / fixed_scale;
-    float most = -INFINITY, least = INFINITY, least_counted = INFINITY;
+    float most = -INFINITY, least_counted = INFINITY;
     bool bad = false;
-    int live = 0;
+    int live = 0, most_at = 0;  // for greedy rows: the first quad that has the largest
+    const uint32_t own_at = (uint32_t)__cvta_generic_to_shared(own);
     auto first_pass = [&](auto early, auto packed) {
-        auto look = [&](int, const float4 &y) {
+        auto look = [&](int q, const float4 &y) {
             const float l[4] = {y.x, y.y, y.z, y.w};
+            if constexpr (!decltype(early)::value)
+                if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) > most) most_at = q;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 bad |= !(l[k] < INFINITY);
                 most = fmaxf(most, l[k]);
-                if (l[k] > -INFINITY) live++, least = fminf(least, l[k]);
+                live += l[k] > -INFINITY;
                 if constexpr (decltype(early)::value) {
                     const int b = SampleBins::slot(l[k], fixed_scale);
-                    if (l[k] > fixed_floor) {
-                        least_counted = fminf(least_counted, l[k]);
-                        if constexpr (decltype(packed)::value) atomicAdd(&own[b / 2], 1u << b % 2 * 16);
-                        else atomicAdd(&own[b], 1u);
-                    }
+                    const bool is = l[k] > fixed_floor;
+                    least_counted = fminf(least_counted, is ? l[k] : INFINITY);
+                    if constexpr (decltype(packed)::value) count_if(is, own_at + (2 * b & ~3), b & 1 ? 0x10000u : 1u);
+                    else count_if(is, own_at + 4 * b, 1u);
                 }
             }
         };
@@ -608,14 +632,12 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     else if (C > 1) first_pass(std::true_type{}, std::true_type{});
     else first_pass(std::true_type{}, std::false_type{});
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
-    const uint32_t warp_least = __reduce_min_sync(0xffffffffu, sample_key(least));
     const uint32_t warp_counted = __reduce_min_sync(0xffffffffu, sample_key(least_counted));
     bad = __any_sync(0xffffffffu, bad);
     live = __reduce_add_sync(0xffffffffu, live);
     if (lane == 0) {
         sh.warp_count[warp] = live;
-        reinterpret_cast<uint32_t *>(sh.warp_high)[warp] = warp_most, reinterpret_cast<uint32_t *>(sh.warp_low)[warp] = warp_least;
-        sh.warp_more[warp] = warp_counted;
+        reinterpret_cast<uint32_t *>(sh.warp_high)[warp] = warp_most, reinterpret_cast<uint32_t *>(sh.warp_low)[warp] = warp_counted;
         sh.warp_mass[warp] = bad;
     }
     __syncthreads();
@@ -624,18 +646,17 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         const int w = lane % kSampleWarps;
         SampleSlice z;
         z.most = __reduce_max_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_high)[w]);
-        z.least = __reduce_min_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_low)[w]);
-        z.counted = __reduce_min_sync(0xffffffffu, (uint32_t)sh.warp_more[w]);
+        z.counted = __reduce_min_sync(0xffffffffu, reinterpret_cast<uint32_t *>(sh.warp_low)[w]);
         z.live = __reduce_add_sync(0xffffffffu, lane < kSampleWarps ? sh.warp_count[w] : 0);
         z.bad = __any_sync(0xffffffffu, sh.warp_mass[w] != 0);
         if (lane < C) cluster.map_shared_rank(sh.slices, lane)[rank] = z;
     }
     cluster.sync();
-    float high, low, low_counted;
+    float high, low_counted;
     int all_live;
     {
         const SampleSlice z = sh.slices[lane < C ? lane : 0];
-        high = sample_value(__reduce_max_sync(0xffffffffu, z.most)), low = sample_value(__reduce_min_sync(0xffffffffu, z.least));
+        high = sample_value(__reduce_max_sync(0xffffffffu, z.most));
         low_counted = sample_value(__reduce_min_sync(0xffffffffu, z.counted));
         all_live = __reduce_add_sync(0xffffffffu, lane < C ? z.live : 0);
         bad = __any_sync(0xffffffffu, z.bad);
@@ -653,16 +674,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     }
     if (p.temperature == 0.f) {
         int first = 0x7fffffff;
-        if (high == sample_value(sh.slices[rank].most))
-#pragma unroll 4
-            for (int q = tid; q < quads; q += kSampleThreads) {
-                const float4 y = x.quad(q);
-                const int id = base + 4 * q - off;
-                if (y.w == high) first = min(first, id + 3);
-                if (y.z == high) first = min(first, id + 2);
-                if (y.y == high) first = min(first, id + 1);
-                if (y.x == high) first = min(first, id);
-            }
+        if (most == high) {  // both zeros are one number
+            const float4 y = x.quad(most_at);
+            first = base + 4 * most_at - off + (y.x == high ? 0 : y.y == high ? 1 : y.z == high ? 2 : 3);
+        }
         first = __reduce_min_sync(0xffffffffu, first);
         if (lane == 0) sh.warp_count[warp] = first;
         __syncthreads();
@@ -680,8 +695,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         return;
     }
 
-    SampleRow r;
-    r.top = high, r.cold = 1.0 / (double)p.temperature, r.slope = 1.4426950408889634074 * r.cold;
+    const SampleRow r(high, p.temperature);
     // min-p as the least logit that it keeps: next to the one that arithmetic gives, the one that satisfies the definition.
     float min_logit = -FLT_MAX;
     if (p.min_p > 0.f) {
@@ -705,8 +719,24 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     bool all_listed = false;
     for (; cuts; fixed = false) {  // again, with bins over the row's own range, where those hold too many or not at all
         if (!fixed) {
-            bins = SampleBins(low < reach && reach < high ? reach : low, high, kSampleBins);
+            float low = INFINITY;
+            each_quad<kSampleThreads>(x, ring, tid, quads, [&](int, const float4 &y) {
+                const float l[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) low = fminf(low, l[k] > -INFINITY ? l[k] : INFINITY);
+            });
+            low = -warp_max(-low);
             __syncthreads();
+            if (lane == 0) sh.warp_low[warp] = low;
+            __syncthreads();
+            if (tid < C) {
+                for (int w = 0; w < kSampleWarps; w++) low = fminf(low, sh.warp_low[w]);
+                cluster.map_shared_rank(sh.ends, tid)[rank] = make_float2(low, high);
+            }
+            if (C > 1) cluster.sync();
+            else __syncthreads();
+            for (int c = 0; c < C; c++) low = fminf(low, sh.ends[c].x);
+            bins = SampleBins(low < reach && reach < high ? reach : low, high, kSampleBins);
             for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(own)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             each_quad<kSampleThreads>(x, ring, tid, quads, [&](int, const float4 &l) {
@@ -836,7 +866,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         if (C == 1) __syncthreads();  // the counts have been read: the list takes their place
         if (listed <= kSampleList) break;
         if (!fixed) {
-            sample_slowly(a, r, sh, x, base, row, low, high, all_live, min_logit);
+            sample_slowly(a, r, sh, x, base, row, high, all_live, min_logit);
             return;
         }
     }
@@ -865,10 +895,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         }
         __syncthreads();
         const float sure = sh.border[0], in_to = by_mass || all_listed ? sh.border[1] : INFINITY;
-        auto append = [&](float l, int i) { own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << 32) | (unsigned)(base + i); };
+        auto append = [&](float l, int i) { own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << kIdBits) | (unsigned)(base + i); };
         // Lists those of a quad that `in` marks.
         auto append_some = [&](int q, const float (&l)[4], auto in) {
-            if (in(l[0]) || in(l[1]) || in(l[2]) || in(l[3]))
+            if (in(l[0]) | in(l[1]) | in(l[2]) | in(l[3]))
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                     if (in(l[k])) append(l[k], 4 * q + k - off);
@@ -883,7 +913,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= count_to)) return;
                 const float l[4] = {y.x, y.y, y.z, y.w};
-                append_some(q, l, [&](float z) { return (z < sure && z >= in_to) || (z < count_from && z >= count_to); });
+                append_some(q, l, [&](float z) { return (!(z >= sure) & (z >= in_to)) | (!(z >= count_from) & (z >= count_to)); });
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const u64 w = r.weight(l[k]);
@@ -895,7 +925,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         } else if (p.min_p > 0.f) {
             each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 const float l[4] = {y.x, y.y, y.z, y.w};
-                append_some(q, l, [&](float z) { return !(z >= sure) && z >= in_to; });
+                append_some(q, l, [&](float z) { return !(z >= sure) & (z >= in_to); });
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const u64 w = r.weight(l[k]);
@@ -907,7 +937,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         } else {
             each_quad<32>(x, ring, w0 + lane, w1, [&](int q, const float4 &y) {
                 const float l[4] = {y.x, y.y, y.z, y.w};
-                append_some(q, l, [&](float z) { return !(z >= sure) && z >= in_to; });
+                append_some(q, l, [&](float z) { return !(z >= sure) & (z >= in_to); });
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const u64 w = r.weight(l[k]);
@@ -995,7 +1025,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         for (int k = 0; k < kEach; k++) {
             w[k] = 0, counted[k] = false;
             if (k * kSampleThreads + warp * 32 >= m) continue;
-            const float l = sample_value(~(uint32_t)(token[k] >> 32));
+            const float l = token_logit(token[k]);
             w[k] = member[k] ? r.weight(l) : 0;
             counted[k] = member[k] && by_count && bins.of(l) <= count_bin && (all_listed || bins.of(l) == count_bin);
         }
@@ -1020,10 +1050,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             const u64 last = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
             // In top-p's bins, or the estimate was wrong.
             const bool fine = (mass_from == 0 || sh.heavier < share) && last != ~0ull &&
-                              bins.of(sample_value(~(uint32_t)(last >> 32))) <= mass_to;
+                              bins.of(token_logit(last)) <= mass_to;
             if (!fine) {  // the whole cluster alike
                 if (C > 1) cluster.barrier_wait();
-                sample_slowly(a, r, sh, x, base, row, low, high, all_live, min_logit);
+                sample_slowly(a, r, sh, x, base, row, high, all_live, min_logit);
                 return;
             }
             cut = last;
@@ -1033,8 +1063,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         int count = 0;
 #pragma unroll
         for (int k = 0; k < kEach; k++) {
-            if (!member[k] || token[k] > cut || sample_value(~(uint32_t)(token[k] >> 32)) < min_logit) continue;
-            const int at = (int)(unsigned)token[k] - base;
+            if (!member[k] || token[k] > cut || token_logit(token[k]) < min_logit) continue;
+            const int at = token_id(token[k]) - base;
             sum += w[k], count++;
             if (at < 0) ahead += w[k];
             else if (at < n) atomicAdd(&sh.warp_more[(at + off) / 4 / per_warp], w[k]);
@@ -1049,8 +1079,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     }
     __syncthreads();
     u64 whole = sh.whole, before = sh.before;
-    const float cut_value = cuts ? sample_value(~(uint32_t)(cut >> 32)) : -INFINITY;
-    const unsigned cut_id = (unsigned)cut;
+    const float cut_value = cuts ? token_logit(cut) : -INFINITY;
+    const unsigned cut_id = token_id(cut);
     if (cuts) whole += sh.list_kept, before += sh.list_before;
     u64 target = (u64)((double)u * (double)whole);
     if (target >= whole) target = whole - 1;
@@ -1123,7 +1153,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                             to -= w[k];
                         }
                         a.ids[row] = base + id;
-                        if (a.logprobs) a.logprobs[row] = (float)(r.exponent(x.at(id)) - log((double)whole / kSampleOne));
+                        if (a.logprobs) a.logprobs[row] = r.logprob(x.at(id), whole);
                         if (a.kept) a.kept[row] = sh.kept + (cuts ? sh.list_count : 0);
                     }
                     found |= reached != 0;
