@@ -31,7 +31,7 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
+constexpr int kSampleShifts = 256, kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 typedef unsigned long long u64;
@@ -65,6 +65,7 @@ struct SampleShared {
     int first[kSampleCluster];       // greedy rows: the lowest id of the largest logit
     float2 ends[kSampleCluster];     // least and largest logit above -infinity, or of the slow search's bin
     u64 part_mass[kSampleCluster];
+    double shift[kSampleShifts];     // the row's: see SampleRow
     int part_count[kSampleCluster];
     u64 warp_mass[kSampleWarps], warp_more[kSampleWarps], warp_kept[kSampleWarps];
     int warp_count[kSampleWarps];
@@ -90,6 +91,18 @@ __device__ __forceinline__ u64 warp_sum64(u64 x) {
     for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
+// p * x, for p of [0, 1), down to a whole number, or up. FP64 would round x first, and a share that falls between two of
+// many equal weights be one token off.
+__device__ __forceinline__ u64 sample_share(float p, u64 x, bool up) {
+    const unsigned bits = __float_as_uint(p), e = bits >> 23;  // p is at least zero
+    if (!bits || bits >> 31) return 0;
+    const u64 m = (bits & 0x7fffffu) | (e ? 0x800000u : 0);
+    const int s = 150 - (int)(e ? e : 1);  // p = m / 2^s, s from 24 to 149
+    const u64 high = __umul64hi(m, x), low = m * x;
+    const u64 y = s < 64 ? high << (64 - s) | low >> s : s < 128 ? high >> (s - 64) : 0;
+    const u64 rest = s < 64 ? low << (64 - s) : s == 64 ? low : s < 128 ? low | high << (128 - s) : low | high;
+    return y + (up && rest);
+}
 // Floats in ascending order as unsigned numbers, and back. Both zeros are one number.
 __device__ __forceinline__ uint32_t sample_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.f);
@@ -103,28 +116,38 @@ __device__ __forceinline__ float sample_value(uint32_t key) {
 __constant__ double kSampleSeries[7] = {0.6931471805599453,    0.24022650922288757,   0.055504108839096185,  0.009618056678524632,
                                         0.0013333502386162978, 0.00015461444698571227, 1.5297323760649362e-05};
 
+constexpr int kSampleDown = 64;  // powers of two below the largest weight, at which nothing is left
 struct SampleRow {
-    double top, cold;      // the largest logit, 1 / T
-    double slope, offset;  // log2(e) / T, and -top times that
-    // The product is off by 2^-53 of itself, 2^-23 at most as no slope is larger than 2^30 / |top|, at which FP32's next lower
-    // number weighs nothing. All weights of the row are off by that one factor, and weight(top) by the same.
-    __device__ SampleRow(float high, float temperature) : top(high), cold(1.0 / (double)temperature) {
+    double top, cold;                   // the largest logit, 1 / T
+    double slope;                       // log2(e) / T
+    float high, lowest;                 // the largest logit, and one that is kSampleDown to 3 kSampleDown powers of two lower
+    float unit, origin, step;           // a power of two, `high` times that; slope / unit
+    const double *shift;                // [kSampleShifts]: n - top * slope
+    // The product is off by 2^-44 of itself, 2^-14 at most as no slope is larger than 2^30 / |top|, at which FP32's next lower
+    // number weighs nothing. All weights of the row are off by that one factor, and weight(high) by the same: the product's
+    // last bits are cut off so that adding n is exact. A thread writes a number of `table`.
+    __device__ SampleRow(float high_, float temperature, double *table) : top(high_), cold(1.0 / (double)temperature), high(high_), shift(table) {
         slope = 1.4426950408889634074 * cold;
         if (slope * fabs(top) > 0x1p30) slope = 0x1p30 / fabs(top);
-        offset = -top * slope;
+        // Differences, and what they are multiplied by, stay normal numbers of FP32.
+        unit = slope > 1e30 ? 0x1p100f : slope < 1e-30 ? 0.25f : 1.f;
+        origin = high * unit, step = (float)(slope / (double)unit);
+        lowest = fmaxf(__double2float_rd(top - kSampleDown / slope), -FLT_MAX);  // 2^7 powers of two are a step of FP32 at most
+        const double product = top * slope;
+        if (threadIdx.x < kSampleShifts) table[threadIdx.x] = threadIdx.x - __hiloint2double(__double2hiint(product), __double2loint(product) & ~0xff);
     }
     __device__ double exponent(float l) const { return ((double)l - top) * cold; }
-    __device__ float logprob(float l, u64 whole) const { return (float)(exponent(l) - log((double)whole / (double)weight((float)top))); }
-    __device__ u64 weight(float l) const {
-        const double y0 = fma((double)l, slope, offset);
-        // At most 2^-23; from -64 on (its upper word decides) nothing is left of it.
-        const double y = __hiloint2double((int)min((unsigned)__double2hiint(y0), 0xc0500000u), __double2loint(y0));
-        const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+    __device__ float logprob(float l, u64 whole) const { return (float)(exponent(l) - log((double)whole / (double)weight(high))); }
+    __device__ u64 weight(float l) const {  // of a logit no larger than `high`
+        // The power of two by FP32 arithmetic, and what is left to it, a half and little more at most, in FP64.
+        l = fmaxf(l, lowest);
+        const int n = __float_as_int(fmaf(fmaf(l, unit, -origin), step, 0x1.8p23f));  // its lower bits; 0 to -193
+        const double f = fma((double)l, slope, shift[__float_as_int(0x1.8p23f) - n]);
         double z = kSampleSeries[6];
 #pragma unroll
         for (int k = 5; k >= 0; k--) z = fma(z, f, kSampleSeries[k]);
         z = fma(z, f, 1.0);
-        z = __hiloint2double(__double2hiint(z) + (__double2loint(t) << 20), __double2loint(z));
+        z = __hiloint2double(__double2hiint(z) + (n << 20), __double2loint(z));
         return (u64)(__double_as_longlong(z + 0x1.8p8) - __double_as_longlong(0x1.8p8));  // in units of 2^-44
     }
 };
@@ -156,11 +179,6 @@ struct SampleBins {
     __device__ int of(float l) const { return top - __float_as_int(fmaxf(fmaf(fmaf(l, unit, -origin), scale, kSampleRound), least)); }
     __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
 };
-
-// Adds to a word of shared memory where `is`, without a branch.
-__device__ __forceinline__ void count_if(bool is, uint32_t address, unsigned x) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %0, 0;\n @p red.shared.add.u32 [%1], %2;\n}" ::"r"((unsigned)is), "r"(address), "r"(x) : "memory");
-}
 
 // A CTA's slice of the row: `off` elements behind a 16-byte boundary, in shared memory with -infinity around it, or where
 // it is in global memory, read again by every pass (from L2, mostly).
@@ -224,7 +242,7 @@ __device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float
 // The cut by repeated histograms of the cluster: counts and weights in bins of the range in which it must lie, then of the
 // bin that it falls into, until that holds one value. Then who is kept, and the token. All threads of the cluster call it.
 template <bool RESIDENT>
-__device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow &r, SampleShared &sh, const SampleLogits<RESIDENT> &x, int base, int row,
+__device__ __noinline__ void sample_slowly(const SampleArgs a, const SampleRow r, SampleShared &sh, const SampleLogits<RESIDENT> x, int base, int row,
                                             float high_all, int live, float min_logit) {
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -243,7 +261,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
     };
     // The least prefix of the tokens above `floor` that holds `tokens` of them (by_mass false) or weighs `share` or more.
     // There is one.
-    auto find = [&](bool by_mass, int tokens, double share, float floor) {
+    auto find = [&](bool by_mass, int tokens, u64 share, float floor) {
         Cut cut = {0.f, 0, 0, 0};
         float low = fmaxf(-FLT_MAX, floor), high = high_all;
         // Weights end 32 temperatures below the largest; what lies lower is one bin until the cut is known to be there.
@@ -285,7 +303,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
                         const u64 z = __shfl_up_sync(0xffffffffu, sum, o);
                         if (lane >= o) upto += y, sum += z;
                     }
-                    const bool here = by_mass ? c && (double)(heavier + sum) >= share : above + upto >= tokens;
+                    const bool here = by_mass ? c && heavier + sum >= share : above + upto >= tokens;
                     const unsigned reached = __ballot_sync(0xffffffffu, here);
                     if (reached) {
                         if (lane == __ffs(reached) - 1)
@@ -319,8 +337,8 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
                 int t;
                 if (!by_mass) t = tokens - cut.tokens;
                 else {
-                    const double need = ceil((share - (double)cut.weight) / (double)(w ? w : 1));
-                    t = need < 1.0 ? 1 : need > (double)in_bin ? in_bin : (int)need;
+                    const u64 need = share > cut.weight && w ? (share - cut.weight + w - 1) / w : 1;
+                    t = need > (u64)in_bin ? in_bin : (int)need;
                 }
                 cut.value = low, cut.ties = t;
                 cut.tokens += t;
@@ -332,7 +350,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
 
     // ---- top-k, then top-p of what it leaves
     Cut cut = {-INFINITY, 0, live, 0};
-    if (p.top_k > 0 && p.top_k < live) cut = find(false, p.top_k, 0.0, -INFINITY);
+    if (p.top_k > 0 && p.top_k < live) cut = find(false, p.top_k, 0, -INFINITY);
     if (p.top_p < 1.f) {
         u64 whole = cut.weight;
         if (cut.value == -INFINITY) {  // of the row
@@ -350,12 +368,12 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
             cluster.sync();
             for (int c = 0; c < C; c++) whole += sh.part_mass[c];
         }
-        const double share = fmax(0.0, (double)p.top_p) * (double)whole;
+        const u64 share = sample_share(p.top_p, whole, true);
         // Inside the ties of top-k's cut, or above them.
         const u64 w = cut.value == -INFINITY ? 0 : r.weight(cut.value), above = cut.weight - w * (u64)cut.ties;
-        if (cut.value != -INFINITY && (double)above < share) {
-            const double need = ceil((share - (double)above) / (double)(w ? w : 1));
-            const int t = need < 1.0 ? 1 : need > (double)cut.ties ? cut.ties : (int)need;
+        if (cut.value != -INFINITY && above < share) {
+            const u64 need = w ? (share - above + w - 1) / w : 1;
+            const int t = need > (u64)cut.ties ? cut.ties : (int)need;
             cut.tokens -= cut.ties - t;
             cut.ties = t;
         } else if (cut.value != -INFINITY && cut.tokens == cut.ties) {  // nothing above them
@@ -424,8 +442,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, const SampleRow 
         whole += sh.part_mass[c];
         kept += sh.part_count[c];
     }
-    u64 target = (u64)((double)a.uniforms[row] * (double)whole);
-    if (target >= whole) target = whole - 1;
+    const u64 target = sample_share(a.uniforms[row], whole, false);
     for (int w = 0; w < warp; w++) before += sh.warp_mass[w];
     if (target < before || target >= before + sum) return;  // one warp of the cluster has the token
     walk([&](int i, bool, u64 w) {
@@ -564,7 +581,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
     return sh.found;
 }
 
-template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs a) {
+template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
     extern __shared__ __align__(16) float slice_memory[];
     __shared__ __align__(16) SampleShared sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -597,24 +614,37 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     float most = -INFINITY, least_counted = INFINITY;
     bool bad = false;
     int live = 0, most_at = 0;  // for greedy rows: the first quad that has the largest
-    const uint32_t own_at = (uint32_t)__cvta_generic_to_shared(own);
     auto first_pass = [&](auto early, auto packed) {
+        constexpr bool kEarly = decltype(early)::value, kPacked = decltype(packed)::value;
+        const float floor = kEarly ? fixed_floor : -INFINITY;
         auto look = [&](int q, const float4 &y) {
             const float l[4] = {y.x, y.y, y.z, y.w};
-            if constexpr (!decltype(early)::value)
-                if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) > most) most_at = q;
+            const float largest = fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)), smallest = fminf(fminf(y.x, y.y), fminf(y.z, y.w));
+            if (!kEarly && largest > most) most_at = q;
+            most = fmaxf(most, largest);
+            if ((smallest > floor) & ((y.x + y.y) + (y.z + y.w) < INFINITY)) {  // four usual tokens: 20 instructions fewer
+                live += 4;
+                if constexpr (kEarly) {
+                    least_counted = fminf(least_counted, smallest);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int b = SampleBins::slot(l[k], fixed_scale);
+                        if constexpr (kPacked) atomicAdd(&own[b >> 1], b & 1 ? 0x10000u : 1u);
+                        else atomicAdd(&own[b], 1u);
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 bad |= !(l[k] < INFINITY);
-                most = fmaxf(most, l[k]);
                 live += l[k] > -INFINITY;
-                if constexpr (decltype(early)::value) {
-                    const int b = SampleBins::slot(l[k], fixed_scale);
-                    const bool is = l[k] > fixed_floor;
-                    least_counted = fminf(least_counted, is ? l[k] : INFINITY);
-                    if constexpr (decltype(packed)::value) count_if(is, own_at + (2 * b & ~3), b & 1 ? 0x10000u : 1u);
-                    else count_if(is, own_at + 4 * b, 1u);
-                }
+                if constexpr (kEarly)
+                    if (l[k] > floor) {
+                        const int b = SampleBins::slot(l[k], fixed_scale);
+                        least_counted = fminf(least_counted, l[k]);
+                        atomicAdd(&own[kPacked ? b >> 1 : b], kPacked && b & 1 ? 0x10000u : 1u);
+                    }
             }
         };
         if constexpr (RESIDENT) {
@@ -695,7 +725,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         return;
     }
 
-    const SampleRow r(high, p.temperature);
+    const SampleRow r(high, p.temperature, sh.shift);
+    __syncthreads();
     // min-p as the least logit that it keeps: next to the one that arithmetic gives, the one that satisfies the definition.
     float min_logit = -FLT_MAX;
     if (p.min_p > 0.f) {
@@ -1046,7 +1077,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 __syncthreads();
                 all_of += sh.list_counted;
             }
-            const u64 share = (u64)ceil(fmax(0.0, (double)p.top_p) * (double)all_of);  // no sum is nearer to it than its rounding
+            const u64 share = sample_share(p.top_p, all_of, true);
             const u64 last = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
             // In top-p's bins, or the estimate was wrong.
             const bool fine = (mass_from == 0 || sh.heavier < share) && last != ~0ull &&
@@ -1082,8 +1113,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const float cut_value = cuts ? token_logit(cut) : -INFINITY;
     const unsigned cut_id = token_id(cut);
     if (cuts) whole += sh.list_kept, before += sh.list_before;
-    u64 target = (u64)((double)u * (double)whole);
-    if (target >= whole) target = whole - 1;
+    const u64 target = sample_share(u, whole, false);
 
     // ---- the token: the warp's stretch that holds it, in 16 parts for the warps, then the part by one warp
     auto weights = [&](int q, const float4 &y, u64 (&w)[4]) {  // what is kept of a quad
