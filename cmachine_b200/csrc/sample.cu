@@ -59,6 +59,9 @@ struct SampleSums {
 };
 
 struct SampleShared {
+    TcmSampling set;             // the row's settings, its uniform number, 1 / T
+    float uniform;
+    double cold;
     u64 buffer[2][kSampleList];  // own counts, then own list; the cluster's counts, then its list
     SampleSlice slices[kSampleCluster];
     SampleSums sums[kSampleCluster];
@@ -118,15 +121,15 @@ __constant__ double kSampleSeries[7] = {0.6931471805599453,    0.240226509222887
 
 constexpr int kSampleDown = 64;  // powers of two below the largest weight, at which nothing is left
 struct SampleRow {
-    double top, cold;                   // the largest logit, 1 / T
     double slope;                       // log2(e) / T
-    float high, lowest;                 // the largest logit, and one that is kSampleDown to 3 kSampleDown powers of two lower
-    float unit, origin, step;           // a power of two, `high` times that; slope / unit
-    const double *shift;                // [kSampleShifts]: n - top * slope
+    float lowest;                       // a logit that is kSampleDown to 3 kSampleDown powers of two below the largest
+    float unit, origin, step;           // a power of two, the largest logit times that; slope / unit
+    uint32_t shift;                     // where in shared memory -top * slope - n is for the n whose bits are zero: n steps of 8 bytes
     // The product is off by 2^-44 of itself, 2^-14 at most as no slope is larger than 2^30 / |top|, at which FP32's next lower
     // number weighs nothing. All weights of the row are off by that one factor, and weight(high) by the same: the product's
     // last bits are cut off so that adding n is exact. A thread writes a number of `table`.
-    __device__ SampleRow(float high_, float temperature, double *table) : top(high_), cold(1.0 / (double)temperature), high(high_), shift(table) {
+    __device__ SampleRow(float high, double cold, double *table) {
+        const double top = high;
         slope = 1.4426950408889634074 * cold;
         if (slope * fabs(top) > 0x1p30) slope = 0x1p30 / fabs(top);
         // Differences, and what they are multiplied by, stay normal numbers of FP32.
@@ -134,16 +137,21 @@ struct SampleRow {
         origin = high * unit, step = (float)(slope / (double)unit);
         lowest = fmaxf(__double2float_rd(top - kSampleDown / slope), -FLT_MAX);  // 2^7 powers of two are a step of FP32 at most
         const double product = top * slope;
-        if (threadIdx.x < kSampleShifts) table[threadIdx.x] = threadIdx.x - __hiloint2double(__double2hiint(product), __double2loint(product) & ~0xff);
+        if (threadIdx.x < kSampleShifts)
+            table[kSampleShifts - 1 - threadIdx.x] = threadIdx.x - __hiloint2double(__double2hiint(product), __double2loint(product) & ~0xff);
+        shift = (uint32_t)__cvta_generic_to_shared(table + kSampleShifts - 1) - (__float_as_uint(0x1.8p23f) << 3);
     }
-    __device__ double exponent(float l) const { return ((double)l - top) * cold; }
-    __device__ float logprob(float l, u64 whole) const { return (float)(exponent(l) - log((double)whole / (double)weight(high))); }
-    __device__ u64 weight(float l) const {  // of a logit no larger than `high`
+    __device__ float logprob(float l, float high, double cold, u64 whole) const {
+        return (float)(((double)l - (double)high) * cold - log((double)whole / (double)weight(high)));
+    }
+    __device__ u64 weight(float l) const {  // of a logit no larger than the largest
         // The power of two by FP32 arithmetic, and what is left to it, a half and little more at most, in FP64.
         l = fmaxf(l, lowest);
         const int n = __float_as_int(fmaf(fmaf(l, unit, -origin), step, 0x1.8p23f));  // its lower bits; 0 to -193
-        const double f = fma((double)l, slope, shift[__float_as_int(0x1.8p23f) - n]);
-        double z = kSampleSeries[6];
+        double z, less;
+        asm volatile("ld.shared.f64 %0, [%1];" : "=d"(less) : "r"(shift + ((unsigned)n << 3)));
+        const double f = fma((double)l, slope, less);
+        z = kSampleSeries[6];
 #pragma unroll
         for (int k = 5; k >= 0; k--) z = fma(z, f, kSampleSeries[k]);
         z = fma(z, f, 1.0);
@@ -198,57 +206,71 @@ template <bool RESIDENT> struct SampleLogits {
     }
 };
 
-// f(q, quad) for the quads from, from + STEP, ... below `to`, of a thread. Those in global memory come through a ring of
-// the thread's own in shared memory, kRing of them ahead: HBM and L2 are some 2000 cycles away. (Four ahead in registers
-// left the weights' pass of 256 rows waiting half of its 85 us.)
-constexpr int kRing = 8;
-template <int STEP, bool RESIDENT, typename F>
-__device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float4 *ring, int from, int to, F f) {
-    if constexpr (RESIDENT) {
-        for (int q = from; q < to; q += STEP) f(q, x.quad(q));
-    } else {
-        // Quads that the slice's ends cut, and whole ones between.
-        if (from == 0 && x.off && to > 0) {
-            f(0, x.quad(0));
-            from += STEP;
-        }
+// The quads from, from + STEP, ... below `to` of a thread, out of global memory: kRing of them are on the way at a time, as
+// HBM and L2 are some 2000 cycles away, into a ring of the thread's own in shared memory or (KEEP) to where the quad stays
+// there. (Four ahead in registers left the weights' pass of 256 rows waiting half of its 85 us.) The copies start with
+// the constructor; run() calls f(q, quad).
+constexpr int kRing = 8, kRingBytes = kRing * kSampleThreads * 16;
+template <int STEP, bool KEEP> struct QuadStream {
+    const SampleLogits<false> x;
+    float4 *const memory;
+    int q, ahead, to;
+    bool cut_first, cut_last;  // quads that the slice's ends cut
+    uint32_t at;               // bytes from the memory's start to quad q
+    __device__ QuadStream(const SampleLogits<false> &x_, float4 *memory_, int from, int to_) : x(x_), memory(memory_) {
         const int whole = (x.off + x.n) / 4;
-        const bool cut = to > whole && from <= whole && (whole - from) % STEP == 0;
-        to = min(to, whole);
-        float4 *mine = ring + threadIdx.x;
-        const uint32_t slots = (uint32_t)__cvta_generic_to_shared(mine);
-        const float4 *src = reinterpret_cast<const float4 *>(x.x) + from;
-        int ahead = from, at = 0;
-        auto copy = [&](int slot) {
-            if (ahead < to) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slots + slot), "l"(src) : "memory");
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            ahead += STEP, src += STEP;
-        };
-        constexpr int slot_bytes = kSampleThreads * 16;
+        cut_first = from == 0 && x.off && to_ > 0;
+        cut_last = to_ > whole && from <= whole && (whole - from) % STEP == 0 && !(cut_first && whole == 0);
+        q = cut_first ? from + STEP : from, to = min(to_, whole), ahead = q, at = 16 * (KEEP ? q : threadIdx.x);
 #pragma unroll
-        for (int i = 0; i < kRing; i++) copy(i * slot_bytes);
-        for (int q = from; q < to; q += STEP) {
+        for (int i = 0; i < kRing; i++) copy(KEEP ? at + i * (STEP * 16) : at + i * (kSampleThreads * 16));
+    }
+    __device__ __forceinline__ void copy(uint32_t to_at) {
+        if (ahead < to)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(memory) + to_at),
+                         "l"(reinterpret_cast<const float4 *>(x.x) + ahead) : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += STEP;
+    }
+    template <typename F> __device__ __forceinline__ void run(F f) {
+        auto cut = [&](int quad) {
+            const float4 y = x.quad(quad);
+            if (KEEP) memory[quad] = y;
+            f(quad, y);
+        };
+        if (cut_first) cut(0);
+        for (; q < to; q += STEP) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-            const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(mine) + at);
-            copy(at);
-            at = (at + slot_bytes) & (kRing * slot_bytes - 1);
+            const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(memory) + at);
+            copy(KEEP ? at + kRing * STEP * 16 : at);
+            at = KEEP ? at + STEP * 16 : (at + kSampleThreads * 16) & (kRingBytes - 1);
             f(q, y);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (cut) f(whole, x.quad(whole));
+        if (cut_last) cut((x.off + x.n) / 4);
     }
+};
+// The same of a slice wherever it is.
+template <int STEP, bool RESIDENT, typename F>
+__device__ __forceinline__ void each_quad(const SampleLogits<RESIDENT> &x, float4 *ring, int from, int to, F f) {
+    if constexpr (RESIDENT)
+        for (int q = from; q < to; q += STEP) f(q, x.quad(q));
+    else QuadStream<STEP, false>(x, ring, from, to).run(f);
 }
 
 // The cut by repeated histograms of the cluster: counts and weights in bins of the range in which it must lie, then of the
 // bin that it falls into, until that holds one value. Then who is kept, and the token. All threads of the cluster call it.
 template <bool RESIDENT>
-__device__ __noinline__ void sample_slowly(const SampleArgs a, const SampleRow r, SampleShared &sh, const SampleLogits<RESIDENT> x, int base, int row,
-                                            float high_all, int live, float min_logit) {
+__device__ __noinline__ void sample_slowly(const SampleArgs &a, SampleShared &sh, float *slice_memory, int row, float high_all, int live, float min_logit) {
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const TcmSampling p = a.params[row];
-    const int n = x.n;
+    const TcmSampling p = sh.set;
+    const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
+    const float *src = a.logits + (long long)row * a.stride + base;
+    const int off = (int)((uintptr_t)src >> 2) & 3;
+    const SampleLogits<RESIDENT> x = {RESIDENT ? slice_memory : src - off, off, n};
+    const SampleRow r(high_all, sh.cold, sh.shift);  // `shift` as it is
     u64 *mass = sh.buffer[0], *all_mass = sh.buffer[1];
     unsigned *count = reinterpret_cast<unsigned *>(mass + kSlowBins), *all_count = reinterpret_cast<unsigned *>(all_mass + kSlowBins);
     static_assert(kSampleList * 8 >= kSlowBins * 12, "the slow search's bins fit the buffers");
@@ -265,7 +287,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs a, const SampleRow r
         Cut cut = {0.f, 0, 0, 0};
         float low = fmaxf(-FLT_MAX, floor), high = high_all;
         // Weights end 32 temperatures below the largest; what lies lower is one bin until the cut is known to be there.
-        const float reach = (float)(r.top - 32.0 * (double)p.temperature);
+        const float reach = (float)((double)high_all - 32.0 * (double)p.temperature);
         float from = low < reach && reach < high ? reach : low;
         // A pass narrows the range a thousandfold, and FP32's spans less than 2^280: 64 are never reached.
         for (int pass = 0;; pass++) {
@@ -442,7 +464,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs a, const SampleRow r
         whole += sh.part_mass[c];
         kept += sh.part_count[c];
     }
-    const u64 target = sample_share(a.uniforms[row], whole, false);
+    const u64 target = sample_share(sh.uniform, whole, false);
     for (int w = 0; w < warp; w++) before += sh.warp_mass[w];
     if (target < before || target >= before + sum) return;  // one warp of the cluster has the token
     walk([&](int i, bool, u64 w) {
@@ -455,7 +477,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs a, const SampleRow r
         const unsigned reached = __ballot_sync(0xffffffffu, before + upto > target);
         if (reached && lane == __ffs(reached) - 1) {
             a.ids[row] = base + i;
-            if (a.logprobs) a.logprobs[row] = r.logprob(x.at(i), whole);
+            if (a.logprobs) a.logprobs[row] = r.logprob(x.at(i), high_all, sh.cold, whole);
             if (a.kept) a.kept[row] = kept;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -589,14 +611,12 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int base = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - base);
-    for (int i = tid; i < (C > 1 ? 1 : 2) * kSampleList / 2; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < kSampleList; i += kSampleThreads) reinterpret_cast<uint4 *>(sh.buffer[0])[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) sh.listed = sh.list_count = 0, sh.list_before = sh.list_kept = sh.list_counted = 0;
     __syncthreads();
     pdl_trigger();
     pdl_wait();
     const float *src = a.logits + (long long)row * a.stride + base;
-    const TcmSampling p = a.params[row];
-    const float u = a.uniforms[row];
 
     // ---- what there is in the slice. In shared memory it starts as far from a 16-byte boundary as in global memory, so
     // that everything goes by whole quads.
@@ -604,12 +624,18 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const SampleLogits<RESIDENT> x = {RESIDENT ? slice_memory : src - off, off, n};
     const SampleLogits<false> global = {src - off, off, n};
     float4 *ring = reinterpret_cast<float4 *>(slice_memory);  // where the slice is not there
+    QuadStream<kSampleThreads, RESIDENT> stream(global, ring, tid, quads);
+    const TcmSampling &p = sh.set;
+    if (tid == 0) sh.set = a.params[row], sh.uniform = a.uniforms[row], sh.cold = 1.0 / (double)sh.set.temperature;
+    __syncthreads();
     // Where cuts are asked for, tokens are counted as they come, in bins of a 128th of the temperature whose borders do not
     // depend on the row: a circle of 8192, as numbers of 16 bits where a slice has no more tokens than they count. Tokens
     // that are masked with a large number, -1e4 or -FLT_MAX, are left out.
-    unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = reinterpret_cast<unsigned *>(sh.buffer[1]);
+    // Where they count more, the slice is not in shared memory, and the cluster's counts go to the ring.
+    const bool packed = C > 1 && a.slice <= 0xffff;
+    unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = RESIDENT || packed ? reinterpret_cast<unsigned *>(sh.buffer[1]) : reinterpret_cast<unsigned *>(slice_memory);
     const float fixed_scale = 128.f / p.temperature;
-    const bool early = (p.top_k > 0 || p.top_p < 1.f) && fixed_scale > 0.f && fixed_scale < INFINITY && (C == 1 || a.slice <= 0xffff);
+    const bool early = (p.top_k > 0 || p.top_p < 1.f) && fixed_scale > 0.f && fixed_scale < INFINITY;
     const float fixed_floor = -kSampleReach / fixed_scale;
     float most = -INFINITY, least_counted = INFINITY;
     bool bad = false;
@@ -647,19 +673,10 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                     }
             }
         };
-        if constexpr (RESIDENT) {
-#pragma unroll 4
-            for (int q = tid; q < quads; q += kSampleThreads) {
-                const float4 l = global.quad(q);
-                reinterpret_cast<float4 *>(slice_memory)[q] = l;
-                look(q, l);
-            }
-        } else {
-            each_quad<kSampleThreads>(x, ring, tid, quads, look);
-        }
+        stream.run(look);
     };
     if (!early) first_pass(std::false_type{}, std::false_type{});
-    else if (C > 1) first_pass(std::true_type{}, std::true_type{});
+    else if (packed) first_pass(std::true_type{}, std::true_type{});
     else first_pass(std::true_type{}, std::false_type{});
     const uint32_t warp_most = __reduce_max_sync(0xffffffffu, sample_key(most));
     const uint32_t warp_counted = __reduce_min_sync(0xffffffffu, sample_key(least_counted));
@@ -691,6 +708,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         all_live = __reduce_add_sync(0xffffffffu, lane < C ? z.live : 0);
         bad = __any_sync(0xffffffffu, z.bad);
     }
+    const float u = sh.uniform;
     const bool wrong = !(p.temperature >= 0.f && p.temperature < INFINITY && u >= 0.f && u < 1.f && p.min_p <= 1.f) ||
                        p.top_p != p.top_p;
     if (bad || !all_live || wrong) {  // the whole cluster alike
@@ -725,21 +743,22 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         return;
     }
 
-    const SampleRow r(high, p.temperature, sh.shift);
+    const SampleRow r(high, sh.cold, sh.shift);
     __syncthreads();
     // min-p as the least logit that it keeps: next to the one that arithmetic gives, the one that satisfies the definition.
     float min_logit = -FLT_MAX;
     if (p.min_p > 0.f) {
         const double coldest = log((double)p.min_p);
-        float l = fmaxf((float)(r.top + coldest * (double)p.temperature), -FLT_MAX);
-        if (!(r.exponent(l) >= coldest)) l = nextafterf(l, INFINITY);
-        else if (l > -FLT_MAX && r.exponent(nextafterf(l, -INFINITY)) >= coldest) l = nextafterf(l, -INFINITY);
+        auto exponent = [&](float l) { return ((double)l - (double)high) * sh.cold; };
+        float l = fmaxf((float)((double)high + coldest * (double)p.temperature), -FLT_MAX);
+        if (!(exponent(l) >= coldest)) l = nextafterf(l, INFINITY);
+        else if (l > -FLT_MAX && exponent(nextafterf(l, -INFINITY)) >= coldest) l = nextafterf(l, -INFINITY);
         min_logit = fminf(l, high);
     }
 
     // ---- the bins in which the cuts lie
     const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f, cuts = by_count || by_mass;
-    const float reach = (float)(r.top - 32.0 * (double)p.temperature);
+    const float reach = (float)((double)high - 32.0 * (double)p.temperature);
     SampleBins bins(high, fixed_scale);
     // Counts of the first pass hold where the largest token is among them and no slot has two bins.
     bool fixed = early && high > fixed_floor && fabsf(high) * fixed_scale < kSampleReach &&
@@ -789,7 +808,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
 #pragma unroll 8
                 for (int k = 0; k < C; k++) {
                     const unsigned *theirs = cluster.map_shared_rank(own, k);
-                    c += fixed ? reinterpret_cast<const unsigned short *>(theirs)[at] : theirs[at];
+                    c += fixed && packed ? reinterpret_cast<const unsigned short *>(theirs)[at] : theirs[at];
                 }
 #pragma unroll 8
                 for (int k = 0; k < C; k++) cluster.map_shared_rank(counts, k)[b] = c;
@@ -897,7 +916,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         if (C == 1) __syncthreads();  // the counts have been read: the list takes their place
         if (listed <= kSampleList) break;
         if (!fixed) {
-            sample_slowly(a, r, sh, x, base, row, high, all_live, min_logit);
+            sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
             return;
         }
     }
@@ -1084,7 +1103,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                               bins.of(token_logit(last)) <= mass_to;
             if (!fine) {  // the whole cluster alike
                 if (C > 1) cluster.barrier_wait();
-                sample_slowly(a, r, sh, x, base, row, high, all_live, min_logit);
+                sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
                 return;
             }
             cut = last;
@@ -1113,7 +1132,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     const float cut_value = cuts ? token_logit(cut) : -INFINITY;
     const unsigned cut_id = token_id(cut);
     if (cuts) whole += sh.list_kept, before += sh.list_before;
-    const u64 target = sample_share(u, whole, false);
+    const u64 target = sample_share(sh.uniform, whole, false);
 
     // ---- the token: the warp's stretch that holds it, in 16 parts for the warps, then the part by one warp
     auto weights = [&](int q, const float4 &y, u64 (&w)[4]) {  // what is kept of a quad
@@ -1183,7 +1202,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                             to -= w[k];
                         }
                         a.ids[row] = base + id;
-                        if (a.logprobs) a.logprobs[row] = r.logprob(x.at(id), whole);
+                        if (a.logprobs) a.logprobs[row] = r.logprob(x.at(id), high, sh.cold, whole);
                         if (a.kept) a.kept[row] = sh.kept + (cuts ? sh.list_count : 0);
                     }
                     found |= reached != 0;
@@ -1219,7 +1238,7 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
     static PerDeviceOnce once;
     once.run([] {
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleOwnSm));
-        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing * kSampleThreads * 16));
+        TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
@@ -1236,7 +1255,7 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * cluster);
     cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = resident ? (size_t)smem : kRing * kSampleThreads * 16;
+    cfg.dynamicSmemBytes = resident ? (size_t)smem : kRingBytes;
     cfg.stream = stream();
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
