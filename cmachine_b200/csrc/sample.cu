@@ -1,21 +1,28 @@
 // Sampling: one token a row of logits, with temperature, top-k, top-p and min-p, by a given uniform number.
 //
-// A thread-block cluster has one row. Each of its CTAs brings a contiguous slice of the row into shared memory, and
-// everything after that runs on chip: the row is read from HBM once. All three filters keep a prefix of the tokens in
-// descending order of their logits (equal ones by id), so what is kept is described by the last token that is, the cut:
-// a logit and an id. The row is never sorted:
-//   1. the largest logit (a cluster barrier);
-//   2. for top-k and top-p, how many tokens each of 4096 bins of the logits' range has (two barriers). The bin of the
-//      k-th token is known then; that of top-p's last token is estimated from the counts and the bins' middles;
-//   3. one pass adds up the weights above those bins, and lists the few tokens inside them (a barrier);
-//   4. every CTA sorts the list and finds the cut in it, then the id at which the kept weights pass the uniform number's
+// A thread-block cluster has one row. Each of its CTAs has a contiguous slice of it, in shared memory where it fits (the
+// row is read from HBM once then, twice otherwise). All three filters keep a prefix of the tokens in descending order of
+// their logits (equal ones by id), so what is kept is described by the last token that is, the cut: a logit and an id. The
+// row is never sorted:
+//   1. one pass finds the largest logit and, for top-k and top-p, counts the tokens in bins of a 128th of the temperature
+//      whose borders do not depend on the row: a circle of 8192 bins, of which the cluster adds up the 4096 below the
+//      largest logit. Where the row's range passes the circle, or its bins hold too many, a pass over the row's own range
+//      counts again;
+//   2. the bin of the k-th token is known then; that of top-p's last token is estimated from the counts and the bins'
+//      middles;
+//   3. one pass adds up the weights above those bins, and lists the few tokens inside them;
+//   4. every CTA searches the list for the cut, then finds the id at which the kept weights pass the uniform number's
 //      share; the warp that holds this id writes the result.
 // Where the estimate was wrong, or the bins hold more than a list (many equal logits), sample_slowly() narrows the range
 // bin by bin instead.
 //
-// Weights exp((l - max) / T) are whole numbers, 2^44 for the largest: their sums are exact whatever the order, so that
-// atomics and the CTAs' shares leave results the same from call to call, and a sum of 2^19 of them stays below 2^64.
-// What bounds it: the weights' 13 FP64 instructions an element (26 cycles of an SM's quarter) beside HBM.
+// Weights exp((l - max) / T) are whole numbers, 2^44 or next to it for the largest: their sums are exact whatever the order,
+// so that atomics and the CTAs' shares leave results the same from call to call, and a sum of 2^19 of them stays below 2^64.
+//
+// What bounds it (rows of 151,936): one row, five barriers of the cluster and the search, 1 to 5 us each (23 us; 11 with
+// neither top-k nor top-p). 256 rows with top-p, 138 us, an SM's two CTAs: 40 us of the first pass and 63 of the weights',
+// which take 9 FP64 instructions an element at two cycles or more of an SM's quarter, and some 25 others; the other 35 are
+// steps 2 and 4. A row's slices are as long as one another, so an SM with two CTAs is waited for by those with one.
 #include "common.cuh"
 #include "kernels.h"
 #include "../../include/gpu.h"
@@ -1242,10 +1249,11 @@ extern "C" int gpu_sample(TcmGpu *gpu, int *ids, float *logprobs, int *kept, con
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         TCM_CUDA(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     });
-    // As many CTAs a row as run at once for all rows, of 1024 tokens at least; 16 only where every CTA has an SM of its own.
-    // Measured with rows of 151,936 and top-p, us for 1, 2, 4, 8, 16 CTAs a row: 1 row 120, 71, 38, 29, 25; 16 rows 121, 80, 39,
-    // 39, 52; 64 rows 158, 107, 73, 80, 143; 256 rows 205, 224, 264, 330, 541.
-    int cluster = (long long)rows * kSampleCluster <= sm_count() ? kSampleCluster : kSampleCluster / 2;
+    // As many CTAs a row as run at once for all rows, of 1024 tokens at least; 8 and 16 only where every CTA has an SM of its own.
+    // Measured with rows of 151,936 and top-p, us for 1, 2, 4, 8, 16 CTAs a row: 1 row 81, 55, 35, 29, 26; 32 rows 91, 67, 36,
+    // 43, 74; 64 rows 109, 80, 57, 75, 132; 128 rows 128, 84, 115, 146, 249; 256 rows 136, 163, 212, 279, 480.
+    int cluster = kSampleCluster;
+    while (cluster > 4 && (long long)rows * cluster > sm_count()) cluster /= 2;
     while (cluster > 1 && (vocab < cluster * 1024 || (long long)rows * cluster > 2 * sm_count())) cluster /= 2;
     const int slice = ((vocab + cluster - 1) / cluster + 3) / 4 * 4;
     // In shared memory where that takes no CTA off its SM.
