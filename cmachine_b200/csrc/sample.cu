@@ -38,7 +38,7 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleShifts = 256, kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = 128;
+constexpr int kSampleShifts = 256, kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = kSampleThreads / 4;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 typedef unsigned long long u64;
@@ -598,11 +598,17 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
         }
     __syncthreads();
     const int few = sh.few_count;
-    if (tid < few) {
-        const u64 mine = in.few[tid], mass = in.few_mass[tid];
+    if (warp * 8 < few) {  // four lanes a token
+        const int at = min(tid / 4, few - 1);
+        const u64 mine = in.few[at], mass = in.few_mass[at];
         int above = 0;
-        for (int i = 0; i < few; i++)
-            if (in.few[i] < mine) above++, heavier += in.few_mass[i];
+        u64 sum = 0;
+#pragma unroll 4
+        for (int i = lane % 4; i < few; i += 4)
+            if (in.few[i] < mine) above++, sum += in.few_mass[i];
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o), sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        heavier += sum;
         // The first at which it is reached: the one before it does not reach it.
         if (by_mass ? heavier + mass >= share && (!above || heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
     }
