@@ -521,6 +521,142 @@ def test_wild_bounds_and_queries_stay_inside(kind):
 
 
 @KINDS
+@pytest.mark.parametrize("page", [7, 16, 24, 48, 100])
+@pytest.mark.parametrize("what", ["non-finite", "huge"])
+def test_what_no_query_sees_may_hold_anything(kind, page, what):
+    """Free pages and rows behind a sequence's last hold NaN and infinities, or numbers far larger than any other."""
+    news, lengths = [1, 3, 1], [1111, 500, page - 1]
+    p = Served(kind, QWEN, page, news, lengths, seed=20)
+    plain = Served(kind, QWEN, page, news, lengths, seed=20)
+    used = np.zeros((p.pages, page), bool)
+    for s, n in enumerate(lengths):
+        for j in range(n):
+            used[p.table[s, j // page], j % page] = True
+    hide = ~used[:, None, :]
+    if kind == BYTES:
+        for kk, bad in ((0, np.nan), (1, np.inf)) if what == "non-finite" else ((0, 1e30), (1, 1e30)):
+            p.scales[kk][np.broadcast_to(hide, p.scales[kk].shape)] = bad
+    else:
+        for kk, bad in ((0, 0x7FC0), (1, 0xFF80)) if what == "non-finite" else ((0, 0x7149), (1, 0xF149)):
+            p.host[kk][np.broadcast_to(hide, p.host[kk].shape[:3])] = bad
+    p.put()
+    p.whole()
+    marks = download(p.bounds, p.marks.shape, np.uint16)
+    q = p.queries()
+    got, which = p.sparse(q, 5, 1, 1)
+    plain.check_sparse(got, which, q, 5, 1, 1, marks)
+    assert p.flags() == 0
+    p.free()
+    plain.free()
+
+
+@KINDS
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-4, 12.0, 1e20])
+def test_queries_of_any_size(kind, scale):
+    p = Served(kind, QWEN, 32, [1, 3], [900, 700], seed=21, spread=0.3)
+    p.whole()
+    marks = download(p.bounds, p.marks.shape, np.uint16)
+    q = p.queries(scale)
+    q[0, :128] = 0
+    got, which = p.sparse(q, 6, 1, 1)
+    p.check_sparse(got, which, q, 6, 1, 1, marks)
+    p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("spread", [2.0, 5.0])
+@pytest.mark.parametrize("heads", [QWEN, ODD64])
+def test_rows_of_unlike_size(kind, heads, spread):
+    """K and V rows whose sizes differ by many powers of two, zero rows among them; the largest V row first, or last."""
+    for blocks in (5, 60):
+        p = Served(kind, heads, 16, [1, 2], [1500, 1600], seed=22, spread=spread)
+        for s, place in ((0, 3), (1, 1590)):
+            at = p.table[s, place // 16], slice(None), place % 16
+            if kind == BYTES:
+                p.scales[1][at] = 1e25
+            else:
+                p.host[1][at] = bf16(np.full(p.host[1][at].shape, 1e25, np.float32))
+        if kind == BYTES:
+            p.host[0][:, 0, 3], p.host[1][:, 1, 5] = 0, 0
+        else:
+            p.host[0][:, 0, 3], p.host[1][:, 1, 5] = 0, 0x8000
+        p.put()
+        p.whole()
+        marks = download(p.bounds, p.marks.shape, np.uint16)
+        q = p.queries(0.3 if spread < 3 else 0.01)
+        got, which = p.sparse(q, blocks, 1, 1)
+        p.check_sparse(got, which, q, blocks, 1, 1, marks)
+        p.free()
+
+
+@pytest.mark.parametrize("page", [16, 24, 64])
+def test_scales_at_any_float(page):
+    """Scales that start next to a 16-byte boundary."""
+    p = Served(BYTES, QWEN, page, [1, 2], [1000, 777], seed=23)
+    p.whole()
+    q = p.queries()
+    want, _ = p.sparse(q, 6, 1, 1)
+    for off in (1, 2, 3):
+        moved = upload(np.concatenate([np.full(off, np.nan, np.float32), p.scales.reshape(-1)]))
+        p.cache.scales = moved + 4 * off
+        got, _ = p.sparse(q, 6, 1, 1)
+        cm.lib().gpu_free(moved)
+        assert np.array_equal(got, want)
+    p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sums(kind, dim):
+    """So many rows of nearly equal weight that the largest cluster's warps add up more than one chain each; V of one sign."""
+    p = Served(kind, (2, 1, dim), 256, [1], [60000], seed=24)
+    if kind == BYTES:
+        p.host[1] = np.abs(p.host[1])
+    else:
+        p.host[1] = p.host[1] & np.uint16(0x7fff)
+    p.put()
+    p.whole()
+    marks = download(p.bounds, p.marks.shape, np.uint16)
+    q = p.queries(0.01)
+    got, which = p.sparse(q, 200, 1, 1)
+    p.check_sparse(got, which, q, 200, 1, 1, marks)
+    p.free()
+
+
+@KINDS
+def test_more_rows_than_one_pass_has_tables_for(kind):
+    p = Served(kind, (2, 2, 64), 1, [1, 1100], [9000, 1200], seed=25)
+    p.whole()
+    marks = download(p.bounds, p.marks.shape, np.uint16)
+    q = p.queries()
+    got, which = p.sparse(q, 8192, 2, 3)
+    p.check_sparse(got, which, q, 8192, 2, 3, marks)
+    p.free()
+
+
+@KINDS
+def test_thousands_of_equal_pages(kind):
+    """One row in every page: the choice goes by the ids of thousands of equal scores."""
+    p = Served(kind, (4, 2, 64), 1, [1, 1], [6000, 3000], seed=26)
+    for x in p.host:
+        x[:] = x[:1]
+    p.scales[:] = p.scales[:, :1]
+    x = p.table[0, [17, 5000]]  # two above the others
+    if kind == BYTES:
+        p.scales[0][x] *= 1.5
+    else:
+        p.host[0][x] = bf16(widen(p.host[0][x]) * np.float32(1.5))
+    p.put()
+    p.whole()
+    marks = download(p.bounds, p.marks.shape, np.uint16)
+    q = p.queries()
+    for blocks in (9, 1000):
+        got, which = p.sparse(q, blocks, 1, 1)
+        p.check_sparse(got, which, q, blocks, 1, 1, marks)
+    p.free()
+
+
+@KINDS
 def test_a_decoding_loop(kind):
     """Rotated append, bounds and attention over chosen pages, token by token and once more in one chunk: the same cache
     and bounds, and every token's attention held to its own cache."""
