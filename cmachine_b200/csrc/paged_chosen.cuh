@@ -7,13 +7,21 @@
 //
 // The MMAs are those of the decode kernel's tile of eight query rows (paged_decode.cuh): the queries' first and second
 // parts share an operand, and 16-byte pieces of the rows are the other one as they come. A warp's copies go through a
-// ring of half steps, K and V apart. Every row that a query has is visible, so nothing of a tile is ever masked but the
+// ring of two steps, K and V apart. Every row that a query has is visible, so nothing of a tile is ever masked but the
 // places behind the last row and pages without an id, which are copied as zeros.
 //
 // Precision is the decode kernel's: products exact, queries as three BF16 parts or three signed bytes, weights as three
 // BF16 parts, or over byte rows, whose scales they carry, as FP16 pairs: every head scales its own by a power of two
 // that follows the largest weight times scale so far, and falls when the maximum rises, so that no row sets it for what
 // comes after. Sums in the tensor cores truncate: no more than kPdChain steps of P V follow one another there.
+//
+// What bounds it: with many items the instructions of a row, 25 of bytes, at half of the issue slots, as three warps a
+// scheduler wait for one another's fixed latencies (512 rows of 4096 byte rows, 2 KV heads: 213 us; four CTAs an SM at 128
+// registers 222); over BF16 rows L2 (160 rows of 1280 rows, 8 KV heads: 111 us, 7.5 TB/s). With few items the chain of a
+// warp, 2 us a step, behind 3 us to the first rows and before 4 of joining (64 rows of 128 to 2048 byte rows, 2 KV heads:
+// 20 us; one row: 8). The same choice read by the decode kernel, a row a sequence, made whole calls of 298, 193 and 43 us
+// that take 247, 136 and 47 here: its line of equal stretches serves 64 unequal items better, its tiles of one row each the
+// others worse.
 #pragma once
 #include "paged_decode.cuh"
 #include <cooperative_groups.h>

@@ -237,15 +237,17 @@ int gpu_paged_bounds(const TcmPagedCache *, const TcmPagedBatch *, uint16_t *bou
  * ones up to P, and of those between the ones whose score
  *     max over the KV head's query heads of sum_d max(q_d low_d, q_d high_d)
  * is largest, an upper bound of the products of the page's keys with its queries; equal
- * scores go to the lower page, a score that is NaN is lowest, and so is a page without
- * a page id in the pool. Scores are summed in 64 bits, so the choice is that of exact
- * arithmetic unless two scores agree to some 15 digits. blocks >= first + recent,
+ * scores go to the lower page, and a page without a page id in the pool is lowest. The
+ * choice is that of sums in 64 bits, so of exact arithmetic unless two scores agree to
+ * some 15 digits; with a non-finite query or bound it is unspecified (still `blocks`
+ * pages of the sequence). blocks >= first + recent,
  * first >= 0, recent >= 1, blocks <= 8192; sequences of more than 16384 pages are
  * reported as bad extents (4) and left out. selected may be NULL; else it is
  * [rows][kvheads][blocks] and gets the pages of every new row in ascending order, -1
- * behind the last (rows at negative places: -1). Contract, limits, precision and scratch
- * as gpu_paged_attention (bounds of pages below P must be up to date: a stale or wild
- * one changes the choice, nothing else); its scratch is some 100 MB at most more. */
+ * behind the last (rows at negative places: -1). Contract, limits and precision as
+ * gpu_paged_attention (bounds of pages below P must be up to date: a stale or wild one
+ * changes the choice, nothing else). The handle's scratch holds the tables of as many
+ * rows as fit 64 MB, four at least; more rows go in turns. */
 int gpu_paged_sparse_attention(TcmGpu *, float *out, long long out_stride, const float *q, long long q_stride,
                                const TcmPagedCache *, const TcmPagedBatch *, const uint16_t *bounds, int qheads, int blocks,
                                int first, int recent, int *selected, int *status);
@@ -266,8 +268,8 @@ typedef struct {
  * passes uniforms[r] in [0, 1) times their whole sum. ids, logprobs (the log of the
  * token's share of that sum) and kept (how many are) are [rows]; logprobs and kept may
  * be NULL. stride >= vocab, or 0: every row draws from the same logits. vocab is 1 to
- * 524288. Weights and sums are carried to 2^-30 of themselves or better and added
- * exactly, in any order, so the same call gives the same tokens. A row that has no
+ * 524288. Weights are off by 2^-30 of themselves or 2^-44 of the largest at most, and
+ * added exactly, so the same call gives the same tokens. A row that has no
  * token gets id -1, logprob 0, kept 0, and a bit of *status (as above; may be NULL): 1 a
  * logit is NaN or +infinity, 2 no logit is above -infinity, 4 its settings or its uniform
  * are out of range. Returns 0 when launched, or -1 with a message on stderr. */
