@@ -16,11 +16,13 @@
 #include "../../include/tcm_seeded.h"
 #include <math.h>
 #include <string.h>
+#include <type_traits>
 
 namespace tcm {
 namespace {
 
-constexpr int kTurnTile = 8;  // rows of a CTA at a time, where there are many
+constexpr int kTurnTile = 8;               // rows of a CTA at a time, where there are many
+constexpr long long kTurnStride = 1 << 27;  // floats: a tile's offsets stay within 32 bits
 
 struct PagedTurnArgs {
     PagedView v;
@@ -55,13 +57,45 @@ template <int L> __device__ __forceinline__ double turn_sum(const double (&x)[1]
     return y;
 }
 
-// R rows of a head at a time. R = 4: tiles of kTurnTile rows, their cosines in shared memory. R = 1: single tokens; a
-// warp forms the cosines that it needs while its row is on the way, and waits for no other.
-template <int KIND, int DIM, int R>
-__global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 1 : 3) paged_turn_kernel(const __grid_constant__ PagedTurnArgs a) {
-    constexpr int T = R == 1 ? 512 : 256, L = DIM / 4, H = 32 / L, W = T / 32;  // threads; lanes a head, heads a warp, warps
-    constexpr int kTile = R == 1 ? 1 : kTurnTile;
-    __shared__ __align__(16) double2 turn[R == 1 ? 1 : kTile][R == 1 ? 1 : DIM / 2];  // cosine, sine
+// Keys and values of a lane's four elements in their stored form, at row `row` of the pool; a row that it cannot hold is zeros.
+template <int KIND, int DIM, int L>
+__device__ __forceinline__ void turn_store(const PagedView &v, float (&y)[4], bool is_k, int64_t row, int e0, int e1, int lane, int &bad) {
+    // The largest magnitude by its bits: a NaN's are above infinity's.
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < 4; c++) most = max(most, __float_as_uint(y[c]) & 0x7fffffffu);
+    if constexpr (L == 32) most = __reduce_max_sync(0xffffffffu, most);
+    else
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    float m = __uint_as_float(most);
+    if (row < 0) return;
+    if (!paged_holds<KIND>(m)) {
+        bad |= kPagedNonFinite;
+        m = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; c++) y[c] = 0.f;
+    }
+    void *dst = is_k ? v.keys : v.values;
+    const int64_t to = row * DIM;
+    if constexpr (KIND == kPagedBytes) {
+        const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
+        int8_t code[4];
+        paged_codes(y, scale, code);
+        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e0) = make_char2(code[0], code[1]);
+        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e1) = make_char2(code[2], code[3]);
+        if (lane % L == 0) v.scales[(is_k ? 0 : (int64_t)v.pages * v.kvheads * v.page) + row] = scale;
+    } else {
+        uint16_t *d = static_cast<uint16_t *>(dst) + to;
+        *reinterpret_cast<uint32_t *>(d + e0) = (uint32_t)tcm_bf16_rne(y[0]) | ((uint32_t)tcm_bf16_rne(y[1]) << 16);
+        *reinterpret_cast<uint32_t *>(d + e1) = (uint32_t)tcm_bf16_rne(y[2]) | ((uint32_t)tcm_bf16_rne(y[3]) << 16);
+    }
+}
+
+// Single tokens, a CTA each: a warp forms the cosines that it needs while its row is on the way, and waits for no other.
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(512) paged_turn_kernel(const __grid_constant__ PagedTurnArgs a) {
+    constexpr int L = DIM / 4, H = 32 / L, W = 512 / 32;  // lanes a head, heads a warp, warps
     const PagedView &v = a.v;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / L, pair = 2 * (lane % L), s = blockIdx.y;
     // Where the lane's two pieces of two elements lie in a head.
@@ -72,19 +106,8 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 1 : 3) paged_turn
     pdl_wait();
     PagedExtent e;
     int bad = paged_extent(&v, s, &e);
-    for (int first = blockIdx.x * kTile; first < e.count; first += gridDim.x * kTile) {
-        const int rows = min(kTile, e.count - first), place = e.length - e.count + first;
-        if constexpr (R > 1) {
-            for (int i = tid; i < rows * (DIM / 2); i += T) {
-                const int r = i / (DIM / 2), d = i % (DIM / 2);
-                double sn, cs;
-                if (d < a.half) {
-                    sincospi((double)(place + r) * a.rate[d], &sn, &cs);
-                    turn[r][d] = make_double2(cs, sn);
-                }
-            }
-            __syncthreads();
-        }
+    for (int first = blockIdx.x; first < e.count; first += gridDim.x) {
+        const int place = e.length - e.count + first;
         for (int group = warp; group * H < heads; group += W) {
             const int head = group * H + sub, kv_head = head - a.qheads;
             const bool there = head < heads, is_q = kv_head < 0, is_k = !is_q && kv_head < v.kvheads;
@@ -94,106 +117,158 @@ __global__ void __launch_bounds__(R == 1 ? 512 : 256, R == 1 ? 1 : 3) paged_turn
             const float *norm = !moves ? nullptr : is_q ? a.qnorm : a.knorm;
             const bool any_moves = __any_sync(0xffffffffu, moves), any_norm = __any_sync(0xffffffffu, norm != nullptr);
             const bool any_stored = __any_sync(0xffffffffu, there && !is_q);
-            for (int r0 = 0; r0 < rows; r0 += R) {
-                float y[R][4];
-#pragma unroll
-                for (int i = 0; i < R; i++) {
-                    float2 x0 = make_float2(0.f, 0.f), x1 = x0;
-                    if (there && (R == 1 || r0 + i < rows)) {
-                        const float *x = src + (long long)(e.start + first + r0 + i) * a.stride;
-                        x0 = *reinterpret_cast<const float2 *>(x + e0);
-                        x1 = *reinterpret_cast<const float2 *>(x + e1);
-                    }
-                    y[i][0] = x0.x, y[i][1] = x0.y, y[i][2] = x1.x, y[i][3] = x1.y;
+            float2 x0 = make_float2(0.f, 0.f), x1 = x0;
+            if (there) {
+                const float *x = src + (long long)(e.start + first) * a.stride;
+                x0 = *reinterpret_cast<const float2 *>(x + e0);
+                x1 = *reinterpret_cast<const float2 *>(x + e1);
+            }
+            float y[4] = {x0.x, x0.y, x1.x, x1.y};
+            if (any_moves) {
+                double2 t0 = make_double2(1.0, 0.0), t1 = t0;
+                if (turns) {
+                    sincospi((double)place * a.rate[pair], &t0.y, &t0.x);
+                    sincospi((double)place * a.rate[pair + 1], &t1.y, &t1.x);
                 }
-                if (any_moves) {
-                    double2 t0 = make_double2(1.0, 0.0), t1 = t0;
-                    if constexpr (R == 1)
-                        if (turns) {
-                            sincospi((double)place * a.rate[pair], &t0.y, &t0.x);
-                            sincospi((double)place * a.rate[pair + 1], &t1.y, &t1.x);
-                        }
-                    double root = 1.0;
-                    float2 w0 = make_float2(1.f, 1.f), w1 = w0;
-                    if (any_norm) {
-                        if (norm) {
-                            w0 = *reinterpret_cast<const float2 *>(norm + e0);
-                            w1 = *reinterpret_cast<const float2 *>(norm + e1);
-                        }
-                        double sum[R];
-#pragma unroll
-                        for (int i = 0; i < R; i++) {
-                            const double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
-                            sum[i] = z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3);
-                        }
-                        root = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
-                    }
-#pragma unroll
-                    for (int i = 0; i < R; i++) {
-                        double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
-                        if (any_norm) {
-                            double r = root;
-                            if constexpr (R > 1) r = turn_of<L>(root, i, lane);
-                            if (norm) z0 *= r * w0.x, z1 *= r * w0.y, z2 *= r * w1.x, z3 *= r * w1.y;
-                        }
-                        if (turns && moves) {
-                            if constexpr (R > 1) t0 = turn[min(r0 + i, kTile - 1)][pair], t1 = turn[min(r0 + i, kTile - 1)][pair + 1];
-                            const double u0 = z0, u1 = z1;
-                            z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
-                            z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
-                        }
-                        if (moves) y[i][0] = (float)z0, y[i][1] = (float)z1, y[i][2] = (float)z2, y[i][3] = (float)z3;
+                double z0 = y[0], z1 = y[1], z2 = y[2], z3 = y[3];
+                if (any_norm) {
+                    const double sum[1] = {z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3)};
+                    const double r = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
+                    if (norm) {
+                        const float2 w0 = *reinterpret_cast<const float2 *>(norm + e0), w1 = *reinterpret_cast<const float2 *>(norm + e1);
+                        z0 *= r * w0.x, z1 *= r * w0.y, z2 *= r * w1.x, z3 *= r * w1.y;
                     }
                 }
-                if (there && is_q)
+                if (turns) {
+                    const double u0 = z0, u1 = z1;
+                    z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
+                    z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
+                }
+                if (moves) y[0] = (float)z0, y[1] = (float)z1, y[2] = (float)z2, y[3] = (float)z3;
+            }
+            if (there && is_q) {
+                float *dst = a.q_out + (long long)(e.start + first) * a.q_out_stride + head * DIM;
+                *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[0], y[1]);
+                *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[2], y[3]);
+            }
+            if (!any_stored) continue;
+            int64_t row = -1;
+            if (there && !is_q && place >= 0 && (row = paged_slot(&v, s, place, h)) < 0) bad |= kPagedBadPage;
+            turn_store<KIND, DIM, L>(v, y, is_k, row, e0, e1, lane, bad);
+        }
+    }
+    paged_report(a.status, bad);
+}
+
+// Tiles of kTurnTile rows. Their cosines, and where their rows are in the pool, are in shared memory; a warp has a group of
+// heads of one sort, four rows of it at a time. Rows behind the tile's last are copies of it that nothing stores.
+enum { kTurnQ, kTurnK, kTurnV };
+struct TurnTile {
+    int rows;
+    const float *q, *k, *values;  // the first row's
+    float *q_out;
+};
+template <int KIND, int DIM>
+__global__ void __launch_bounds__(256, 3) paged_turn_tile_kernel(const __grid_constant__ PagedTurnArgs a) {
+    constexpr int T = 256, L = DIM / 4, H = 32 / L, W = T / 32;
+    __shared__ __align__(16) double2 turn[kTurnTile][DIM / 2];  // cosine, sine
+    __shared__ int64_t slot[kTurnTile];                         // of KV head 0; -1: nowhere
+    const PagedView &v = a.v;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / L, pair = 2 * (lane % L), s = blockIdx.y;
+    const bool turns = pair < a.half;
+    const int e0 = turns ? pair : 2 * pair, e1 = turns ? a.half + pair : 2 * pair + 2;
+    const int q_groups = (a.qheads + H - 1) / H, kv_groups = (v.kvheads + H - 1) / H;
+    const uint32_t stride = (uint32_t)a.stride, q_out_stride = (uint32_t)a.q_out_stride;  // of at most kTurnStride
+    pdl_trigger();
+    pdl_wait();
+    PagedExtent e;
+    int bad = paged_extent(&v, s, &e);
+    auto run = [&](auto sort, const TurnTile &tile, int group) {
+        constexpr int SORT = decltype(sort)::value;
+        const int head = group * H + sub;
+        const bool there = head < (SORT == kTurnQ ? a.qheads : v.kvheads);
+        const float *src = (SORT == kTurnQ ? tile.q : SORT == kTurnK ? tile.k : tile.values) + (there ? head * DIM : 0);
+        const float *norm = SORT == kTurnQ ? a.qnorm : a.knorm;
+        double w[4];
+        if (SORT != kTurnV && norm) {
+            const float2 w0 = *reinterpret_cast<const float2 *>(norm + e0), w1 = *reinterpret_cast<const float2 *>(norm + e1);
+            w[0] = w0.x, w[1] = w0.y, w[2] = w1.x, w[3] = w1.y;
+        }
+        for (int r0 = 0; r0 < tile.rows; r0 += 4) {
+            float y[4][4];
 #pragma unroll
-                    for (int i = 0; i < R; i++)
-                        if (R == 1 || r0 + i < rows) {
-                            float *dst = a.q_out + (long long)(e.start + first + r0 + i) * a.q_out_stride + head * DIM;
-                            *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[i][0], y[i][1]);
-                            *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[i][2], y[i][3]);
-                        }
-                if (!any_stored) continue;
-                // ---- keys and values in their stored form
+            for (int i = 0; i < 4; i++) {
+                const float *x = src + min(r0 + i, tile.rows - 1) * stride;
+                const float2 x0 = *reinterpret_cast<const float2 *>(x + e0), x1 = *reinterpret_cast<const float2 *>(x + e1);
+                y[i][0] = x0.x, y[i][1] = x0.y, y[i][2] = x1.x, y[i][3] = x1.y;
+            }
+            if (SORT != kTurnV && (norm || a.half)) {
+                double root = 1.0;
+                if (norm) {
+                    double sum[4];
 #pragma unroll
-                for (int i = 0; i < R; i++) {
-                    const int j = place + r0 + i;
-                    int64_t row = -1;
-                    if (there && !is_q && r0 + i < rows && j >= 0 && (row = paged_slot(&v, s, j, h)) < 0) bad |= kPagedBadPage;
-                    // The largest magnitude by its bits: a NaN's are above infinity's.
-                    uint32_t most = 0;
-#pragma unroll
-                    for (int c = 0; c < 4; c++) most = max(most, __float_as_uint(y[i][c]) & 0x7fffffffu);
-                    if constexpr (L == 32) most = __reduce_max_sync(0xffffffffu, most);
-                    else
-#pragma unroll
-                        for (int o = L / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    float m = __uint_as_float(most);
-                    if (row < 0) continue;
-                    if (!paged_holds<KIND>(m)) {
-                        bad |= kPagedNonFinite;
-                        m = 0.f;
-#pragma unroll
-                        for (int c = 0; c < 4; c++) y[i][c] = 0.f;
+                    for (int i = 0; i < 4; i++) {
+                        const double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                        sum[i] = z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3);
                     }
-                    void *dst = is_k ? v.keys : v.values;
-                    const int64_t to = row * DIM;
-                    if constexpr (KIND == kPagedBytes) {
-                        const float scale = m > 0.f ? __fdiv_rn(m, 127.0f) : 1.0f;
-                        int8_t code[4];
-                        paged_codes(y[i], scale, code);
-                        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e0) = make_char2(code[0], code[1]);
-                        *reinterpret_cast<char2 *>(static_cast<int8_t *>(dst) + to + e1) = make_char2(code[2], code[3]);
-                        if (lane % L == 0) v.scales[(is_k ? 0 : (int64_t)v.pages * v.kvheads * v.page) + row] = scale;
-                    } else {
-                        uint16_t *d = static_cast<uint16_t *>(dst) + to;
-                        *reinterpret_cast<uint32_t *>(d + e0) = (uint32_t)tcm_bf16_rne(y[i][0]) | ((uint32_t)tcm_bf16_rne(y[i][1]) << 16);
-                        *reinterpret_cast<uint32_t *>(d + e1) = (uint32_t)tcm_bf16_rne(y[i][2]) | ((uint32_t)tcm_bf16_rne(y[i][3]) << 16);
+                    root = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                    if (norm) {
+                        const double r = turn_of<L>(root, i, lane);
+                        z0 *= r * w[0], z1 *= r * w[1], z2 *= r * w[2], z3 *= r * w[3];
                     }
+                    if (turns) {
+                        const double2 t0 = turn[r0 + i][pair], t1 = turn[r0 + i][pair + 1];
+                        const double u0 = z0, u1 = z1;
+                        z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
+                        z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
+                    }
+                    y[i][0] = (float)z0, y[i][1] = (float)z1, y[i][2] = (float)z2, y[i][3] = (float)z3;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (SORT == kTurnQ) {
+                    if (there && r0 + i < tile.rows) {
+                        float *dst = tile.q_out + head * DIM + (r0 + i) * q_out_stride;
+                        *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[i][0], y[i][1]);
+                        *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[i][2], y[i][3]);
+                    }
+                } else {
+                    const int64_t at = slot[r0 + i];
+                    turn_store<KIND, DIM, L>(v, y[i], SORT == kTurnK, there && at >= 0 ? at + head * v.page : -1, e0, e1, lane, bad);
                 }
             }
         }
-        if constexpr (R > 1) __syncthreads();
+    };
+    for (int first = blockIdx.x * kTurnTile; first < e.count; first += gridDim.x * kTurnTile) {
+        const long long row = e.start + first;
+        const TurnTile tile = {min(kTurnTile, e.count - first), a.q + row * a.stride, a.k + row * a.stride, a.values + row * a.stride,
+                               a.q_out + row * a.q_out_stride};
+        const int place = e.length - e.count + first;
+        if (tid < kTurnTile) {
+            int64_t at = -1;
+            if (tid < tile.rows && place + tid >= 0 && (at = paged_slot(&v, s, place + tid, 0)) < 0) bad |= kPagedBadPage;
+            slot[tid] = at;
+        }
+        for (int i = tid; i < tile.rows * (DIM / 2); i += T) {
+            const int r = i / (DIM / 2), d = i % (DIM / 2);
+            if (d < a.half) {
+                double sn, cs;
+                sincospi((double)(place + r) * a.rate[d], &sn, &cs);
+                turn[r][d] = make_double2(cs, sn);
+            }
+        }
+        __syncthreads();
+        for (int group = warp; group < q_groups + 2 * kv_groups; group += W) {
+            if (group < q_groups) run(std::integral_constant<int, kTurnQ>{}, tile, group);
+            else if (group < q_groups + kv_groups) run(std::integral_constant<int, kTurnK>{}, tile, group - q_groups);
+            else run(std::integral_constant<int, kTurnV>{}, tile, group - q_groups - kv_groups);
+        }
+        __syncthreads();
     }
     paged_report(a.status, bad);
 }
@@ -241,11 +316,11 @@ extern "C" int gpu_paged_rotate_append(const TcmPagedCache *cache, const TcmPage
     a.qheads = qheads, a.half = turn->rotary / 2, a.status = status;
     rates(a.rate, turn->theta, turn->rotary);
     // Tiles of rows only where they leave no SM without work, and sequences have the rows to fill them.
-    const bool tiles = a.v.max_new >= 4 && a.v.rows >= 4 * sm_count();
+    const bool tiles = a.v.max_new >= 4 && a.v.rows >= 4 * sm_count() && stride <= kTurnStride && q_out_stride <= kTurnStride;
     const dim3 grid(blocks_of(a.v.max_new, tiles ? kTurnTile : 1), a.v.sequences);
 #define CALL(K, D)                                                                                        \
-    if (tiles) launch(paged_turn_kernel<K, D, 4>, grid, dim3(256), 0, stream(), true, a);                 \
-    else launch(paged_turn_kernel<K, D, 1>, grid, dim3(512), 0, stream(), true, a)
+    if (tiles) launch(paged_turn_tile_kernel<K, D>, grid, dim3(256), 0, stream(), true, a);               \
+    else launch(paged_turn_kernel<K, D>, grid, dim3(512), 0, stream(), true, a)
     PAGED_DISPATCH(a.v, CALL);
 #undef CALL
     return 0;
