@@ -3,15 +3,15 @@
 // A row of a projection holds query, key and value heads. A head of DIM elements belongs to DIM / 4 lanes, each with
 // two of its rotation's pairs (d, d + R / 2), so that a head is read once, its sum of squares is a reduction over those
 // lanes, and the pairs turn in registers. (Elements that do not turn, from R on, are dealt to the other lanes four at a
-// time.) The cosines of a row are shared by its heads: the CTA forms those of its rows first, in shared memory.
+// time.) Of many rows a CTA has four at a time: their heads share the cosines, and their reductions the exchanges.
 //
 // A row is read once, queries are written once, keys and values in their stored form. Sums, angles and rotations are
 // 64-bit: the choice of pages (paged_sparse.cu) and the codes of a stored row go by values next to borders.
 //
-// What bounds it: 21,149 rows of 12 query heads and 2 of keys and of values, byte rows, take 94 us, their bytes 48: 169
-// instructions a head's row (20 of them FP64, 8 conversions) at half of the issue slots, with 24 warps an SM. Rows through
-// a cp.async ring took 3 us less and two rows of a head at a time more. A single token takes 5 us, of which 3 are its
-// sequence's extent, its page and the row one after another.
+// What bounds it: 21,149 rows of 12 query heads and 2 of keys and of values, byte rows, take 78 us, their bytes 48: 160
+// instructions a head's row (24 of them FP64, 8 conversions), at 60 % of the issue slots. Without norm and rotation it is
+// 51. With eight rows a tile and 24 warps an SM it took 92, without the prefetch 83, at 9 or 10 CTAs an SM, in fewer
+// registers, 81 and 86. A single token takes 5 us, of which 3 are its sequence's extent, its page and the row one after another.
 #include "paged_host.cuh"
 #include "../../include/tcm_seeded.h"
 #include <math.h>
@@ -21,7 +21,7 @@
 namespace tcm {
 namespace {
 
-constexpr int kTurnTile = 8;               // rows of a CTA at a time, where there are many
+constexpr int kTurnTile = 4, kTurnThreads = 128, kTurnCtas = 8;  // rows of a CTA at a time, where there are many; CTAs an SM
 constexpr long long kTurnStride = 1 << 27;  // floats: a tile's offsets stay within 32 bits
 
 struct PagedTurnArgs {
@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(512) paged_turn_kernel(const __grid_constant__
     paged_report(a.status, bad);
 }
 
-// Tiles of kTurnTile rows. Their cosines, and where their rows are in the pool, are in shared memory; a warp has a group of
-// heads of one sort, four rows of it at a time. Rows behind the tile's last are copies of it that nothing stores.
+// Tiles of four rows. Their cosines, and where their rows are in the pool, are in shared memory; a warp has a group of heads
+// of one sort, all four rows of it at a time. Rows behind the tile's last are copies of it that nothing stores.
 enum { kTurnQ, kTurnK, kTurnV };
 struct TurnTile {
     int rows;
@@ -169,8 +169,8 @@ struct TurnTile {
     float *q_out;
 };
 template <int KIND, int DIM>
-__global__ void __launch_bounds__(256, 3) paged_turn_tile_kernel(const __grid_constant__ PagedTurnArgs a) {
-    constexpr int T = 256, L = DIM / 4, H = 32 / L, W = T / 32;
+__global__ void __launch_bounds__(kTurnThreads, kTurnCtas) paged_turn_tile_kernel(const __grid_constant__ PagedTurnArgs a) {
+    constexpr int T = kTurnThreads, L = DIM / 4, H = 32 / L, W = T / 32;
     __shared__ __align__(16) double2 turn[kTurnTile][DIM / 2];  // cosine, sine
     __shared__ int64_t slot[kTurnTile];                         // of KV head 0; -1: nowhere
     const PagedView &v = a.v;
@@ -194,53 +194,51 @@ __global__ void __launch_bounds__(256, 3) paged_turn_tile_kernel(const __grid_co
             const float2 w0 = *reinterpret_cast<const float2 *>(norm + e0), w1 = *reinterpret_cast<const float2 *>(norm + e1);
             w[0] = w0.x, w[1] = w0.y, w[2] = w1.x, w[3] = w1.y;
         }
-        for (int r0 = 0; r0 < tile.rows; r0 += 4) {
-            float y[4][4];
+        float y[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float *x = src + min(r0 + i, tile.rows - 1) * stride;
-                const float2 x0 = *reinterpret_cast<const float2 *>(x + e0), x1 = *reinterpret_cast<const float2 *>(x + e1);
-                y[i][0] = x0.x, y[i][1] = x0.y, y[i][2] = x1.x, y[i][3] = x1.y;
-            }
-            if (SORT != kTurnV && (norm || a.half)) {
-                double root = 1.0;
-                if (norm) {
-                    double sum[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
-                        sum[i] = z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3);
-                    }
-                    root = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
-                }
+        for (int i = 0; i < 4; i++) {
+            const float *x = src + min(i, tile.rows - 1) * stride;
+            const float2 x0 = *reinterpret_cast<const float2 *>(x + e0), x1 = *reinterpret_cast<const float2 *>(x + e1);
+            y[i][0] = x0.x, y[i][1] = x0.y, y[i][2] = x1.x, y[i][3] = x1.y;
+        }
+        if (SORT != kTurnV && (norm || a.half)) {
+            double root = 1.0;
+            if (norm) {
+                double sum[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
-                    if (norm) {
-                        const double r = turn_of<L>(root, i, lane);
-                        z0 *= r * w[0], z1 *= r * w[1], z2 *= r * w[2], z3 *= r * w[3];
-                    }
-                    if (turns) {
-                        const double2 t0 = turn[r0 + i][pair], t1 = turn[r0 + i][pair + 1];
-                        const double u0 = z0, u1 = z1;
-                        z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
-                        z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
-                    }
-                    y[i][0] = (float)z0, y[i][1] = (float)z1, y[i][2] = (float)z2, y[i][3] = (float)z3;
+                    const double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                    sum[i] = z0 * z0 + z1 * z1 + (z2 * z2 + z3 * z3);
                 }
+                root = rsqrt(turn_sum<L>(sum, lane) * (1.0 / DIM) + a.eps);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if constexpr (SORT == kTurnQ) {
-                    if (there && r0 + i < tile.rows) {
-                        float *dst = tile.q_out + head * DIM + (r0 + i) * q_out_stride;
-                        *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[i][0], y[i][1]);
-                        *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[i][2], y[i][3]);
-                    }
-                } else {
-                    const int64_t at = slot[r0 + i];
-                    turn_store<KIND, DIM, L>(v, y[i], SORT == kTurnK, there && at >= 0 ? at + head * v.page : -1, e0, e1, lane, bad);
+                double z0 = y[i][0], z1 = y[i][1], z2 = y[i][2], z3 = y[i][3];
+                if (norm) {
+                    const double r = turn_of<L>(root, i, lane);
+                    z0 *= r * w[0], z1 *= r * w[1], z2 *= r * w[2], z3 *= r * w[3];
                 }
+                if (turns) {
+                    const double2 t0 = turn[i][pair], t1 = turn[i][pair + 1];
+                    const double u0 = z0, u1 = z1;
+                    z0 = u0 * t0.x - z2 * t0.y, z1 = u1 * t1.x - z3 * t1.y;
+                    z2 = z2 * t0.x + u0 * t0.y, z3 = z3 * t1.x + u1 * t1.y;
+                }
+                y[i][0] = (float)z0, y[i][1] = (float)z1, y[i][2] = (float)z2, y[i][3] = (float)z3;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (SORT == kTurnQ) {
+                if (there && i < tile.rows) {
+                    float *dst = tile.q_out + head * DIM + i * q_out_stride;
+                    *reinterpret_cast<float2 *>(dst + e0) = make_float2(y[i][0], y[i][1]);
+                    *reinterpret_cast<float2 *>(dst + e1) = make_float2(y[i][2], y[i][3]);
+                }
+            } else {
+                const int64_t at = slot[i];
+                turn_store<KIND, DIM, L>(v, y[i], SORT == kTurnK, there && at >= 0 ? at + head * v.page : -1, e0, e1, lane, bad);
             }
         }
     };
@@ -249,6 +247,12 @@ __global__ void __launch_bounds__(256, 3) paged_turn_tile_kernel(const __grid_co
         const TurnTile tile = {min(kTurnTile, e.count - first), a.q + row * a.stride, a.k + row * a.stride, a.values + row * a.stride,
                                a.q_out + row * a.q_out_stride};
         const int place = e.length - e.count + first;
+        // The rows are on their way to L2 while the cosines are formed.
+        for (int i = tid; i < tile.rows * (a.qheads + 2 * v.kvheads) * (DIM / 32); i += T) {
+            const int heads = a.qheads + 2 * v.kvheads, unit = i / (DIM / 32), r = unit / heads, head = unit - r * heads, kv = head - a.qheads;
+            const float *x = kv < 0 ? tile.q + head * DIM : kv < v.kvheads ? tile.k + kv * DIM : tile.values + (kv - v.kvheads) * DIM;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(x + r * stride + i % (DIM / 32) * 32));
+        }
         if (tid < kTurnTile) {
             int64_t at = -1;
             if (tid < tile.rows && place + tid >= 0 && (at = paged_slot(&v, s, place + tid, 0)) < 0) bad |= kPagedBadPage;
@@ -319,7 +323,7 @@ extern "C" int gpu_paged_rotate_append(const TcmPagedCache *cache, const TcmPage
     const bool tiles = a.v.max_new >= 4 && a.v.rows >= 4 * sm_count() && stride <= kTurnStride && q_out_stride <= kTurnStride;
     const dim3 grid(blocks_of(a.v.max_new, tiles ? kTurnTile : 1), a.v.sequences);
 #define CALL(K, D)                                                                                        \
-    if (tiles) launch(paged_turn_tile_kernel<K, D>, grid, dim3(256), 0, stream(), true, a);               \
+    if (tiles) launch(paged_turn_tile_kernel<K, D>, grid, dim3(kTurnThreads), 0, stream(), true, a);      \
     else launch(paged_turn_kernel<K, D>, grid, dim3(512), 0, stream(), true, a)
     PAGED_DISPATCH(a.v, CALL);
 #undef CALL
