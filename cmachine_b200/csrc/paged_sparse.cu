@@ -93,8 +93,8 @@ __global__ void __launch_bounds__(kBoundThreads) paged_bounds_kernel(PagedView v
 // pages of 2 KV heads took 239 us, of one row 60; now 49 and 17.
 //
 // What bounds it: few CTAs, each a chain. 16 rows over 1024 pages of 2 KV heads: 7 us for the bounds (an SM's share of
-// 512 KB), 7 for extents, fragments, counts, cut, 64-bit sums and the table. Four rows at a time share the bounds' loads and
-// take 5 us more for each row after the first.
+// 512 KB), 7 for extents, fragments, counts, cut, 64-bit sums and the table. Rows at a time share the bounds' loads and take
+// 5 us more for each after the first.
 constexpr int kChoicePages = 16384, kChoiceBins = 256, kChoiceFew = 1024;
 
 struct PagedChoiceArgs {
@@ -132,8 +132,10 @@ __device__ __forceinline__ double choice_widen(uint32_t u) {
     return __hiloint2double((int)(((u & 0x7fffu) << 13) | ((u & 0x8000u) << 16)), 0);
 }
 
-// R rows of one KV head at a time; one where there are few.
-template <int R> constexpr int kChoiceThreads = R == 1 ? 512 : 256;
+// R rows of one KV head at a time: two where there are many, by CTAs of 128 threads, four of which have an SM, as most of a
+// row's time is waiting. (160 rows over 128 pages of 8 KV heads, and 512 over 512 of 2, whole calls: 131 and 248 us; four
+// rows by 256 threads 138 and 248, by 128 144 and 274; two rows by 256 139 and 254.)
+template <int R> constexpr int kChoiceThreads = R == 1 ? 512 : 128;
 template <int DIM> constexpr int kChoiceRow = 2 * (2 * DIM / 16) * 32;  // fragments of a row: [part][k-step][lane]
 constexpr size_t choice_smem(int dim, int r, long long pages) {
     return (size_t)r * (dim == 64 ? kChoiceRow<64> : kChoiceRow<128>) * 8 + (size_t)pages * (8 + 4 * r);
@@ -151,7 +153,7 @@ template <int T, typename V, typename F> __device__ __forceinline__ V block_fold
 }
 
 template <int DIM, int R>
-__global__ void __launch_bounds__(kChoiceThreads<R>, R == 1 ? 1 : 2) paged_choice_kernel(const __grid_constant__ PagedChoiceArgs a) {
+__global__ void __launch_bounds__(kChoiceThreads<R>, R == 1 ? 1 : 4) paged_choice_kernel(const __grid_constant__ PagedChoiceArgs a) {
     constexpr int T = kChoiceThreads<R>, W = T / 32, P = DIM / 32;  // threads, warps, stretches of 32 elements
     extern __shared__ __align__(16) unsigned char choice_smem_bytes[];
     uint2(*frag)[2][4 * P][32] = reinterpret_cast<uint2(*)[2][4 * P][32]>(choice_smem_bytes);  // [row][part][k-step][lane]
@@ -611,7 +613,7 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     const long long most = ((long long)view.max_length + view.page - 1) / view.page;
     const int pages = (int)(most < kChoicePages ? most : kChoicePages);
     // Rows of one sequence share the loads of its bounds, where there are rows enough and their scores leave room for two CTAs an SM.
-    const bool four = view.max_new >= 4 && (long long)view.rows * view.kvheads >= 4ll * sm_count() && choice_smem(view.dim, 4, pages) <= 100 * 1024;
+    const bool pair = view.max_new >= 2 && (long long)view.rows * view.kvheads >= 4ll * sm_count() && choice_smem(view.dim, 2, pages) <= 100 * 1024;
     int *lengths = reinterpret_cast<int *>(words);
     PagedChoiceArgs c = {view, q, q_stride, bounds, group, blocks, first, recent, 0, 0, pages, lengths, lengths + slab, selected, status};
     PagedChosenArgs d = {view, q, out, q_stride, out_stride, group, blocks, 0, lengths, lengths + slab,
@@ -621,8 +623,8 @@ int gpu_paged_sparse_attention(TcmGpu *gpu, float *out, long long out_stride, co
     for (long long r = 0; r < view.rows; r += slab) {
         const int rows = (int)(view.rows - r < slab ? view.rows - r : slab);
         c.row0 = (int)r, c.rows = rows;
-        if (view.dim == 64) four ? choice_launch<64, 4>(c) : choice_launch<64, 1>(c);
-        else four ? choice_launch<128, 4>(c) : choice_launch<128, 1>(c);
+        if (view.dim == 64) pair ? choice_launch<64, 2>(c) : choice_launch<64, 1>(c);
+        else pair ? choice_launch<128, 2>(c) : choice_launch<128, 1>(c);
         d.row0 = (int)r;
 #define CALL(K, D) chosen_launch<K, D>(d, rows, most_rows)
         PAGED_DISPATCH(view, CALL);
