@@ -19,7 +19,7 @@
 // Weights exp((l - max) / T) are whole numbers, 2^44 or next to it for the largest: their sums are exact whatever the order,
 // so that atomics and the CTAs' shares leave results the same from call to call, and a sum of 2^19 of them stays below 2^64.
 //
-// What bounds it (rows of 151,936): one row, five barriers of the cluster and the search, 1 to 5 us each (23 us; 11 with
+// What bounds it (rows of 151,936): one row, five barriers of the cluster and the search, 1 to 3 us each (20 us; 11 with
 // neither top-k nor top-p). 256 rows with top-p, 138 us, an SM's two CTAs: 40 us of the first pass and 63 of the weights',
 // which take 9 FP64 instructions an element at two cycles or more of an SM's quarter, and some 25 others; the other 35 are
 // steps 2 and 4. A row's slices are as long as one another, so an SM with two CTAs is waited for by those with one.
@@ -511,6 +511,17 @@ __device__ __forceinline__ float token_logit(u64 token) { return sample_value(~(
 __device__ __forceinline__ int token_id(u64 token) { return (int)(token & (kSampleVocab - 1)); }
 constexpr int kEach = kSampleList / kSampleThreads;
 
+// How many of the few come before `mine`, and their weights, added to what is there. Four lanes a token.
+__device__ __forceinline__ void rank_few(const SampleSearch &in, int few, u64 mine, int &above, u64 &heavier) {
+    u64 sum = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x % 4; i < few; i += 4)
+        if (in.few[i] < mine) above++, sum += in.few_mass[i];
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o), sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    heavier += sum;
+}
+
 // Of the tokens marked as members, the first in order with which `tokens` of them are reached (by_mass false), or with
 // which `heavier` and their weights make `share`: bins over the range of their numbers, until one holds kFew of them at
 // most (there are `most_members` in all at most), which are compared with one another. All threads call it; ~0
@@ -602,13 +613,7 @@ __device__ u64 search_list(SampleShared &sh, const u64 (&token)[kEach], const u6
         const int at = min(tid / 4, few - 1);
         const u64 mine = in.few[at], mass = in.few_mass[at];
         int above = 0;
-        u64 sum = 0;
-#pragma unroll 4
-        for (int i = lane % 4; i < few; i += 4)
-            if (in.few[i] < mine) above++, sum += in.few_mass[i];
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o), sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        heavier += sum;
+        rank_few(in, few, mine, above, heavier);
         // The first at which it is reached: the one before it does not reach it.
         if (by_mass ? heavier + mass >= share && (!above || heavier < share) : above + 1 == tokens) atomicMin(&sh.found, mine);
     }
@@ -1094,8 +1099,39 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         }
         if (C > 1) cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
         cut = ~0ull;
-        if (by_count) cut = search_list(sh, token, w, counted, m, false, tokens_left, 0, 0);
-        if (by_mass) {
+        // Few tokens are compared with one another once, for both cuts. (One row with top-k 40 and top-p: 20.3 us, 22.7 with two
+        // searches.)
+        const bool at_once = m > 0 && m <= kFew && (all_listed || !by_count);
+        u64 share = 0;
+        if (at_once) {
+            SampleSearch &in = *reinterpret_cast<SampleSearch *>(sh.buffer[1]);
+            if (tid < m) in.few[tid] = token[0], in.few_mass[tid] = w[0];
+            if (tid == 0) sh.found = ~0ull;
+            __syncthreads();
+            const int at = min(tid / 4, m - 1);
+            const u64 mine = in.few[at], mass = in.few_mass[at];
+            int above = 0;
+            u64 heavier = sh.heavier;
+            rank_few(in, m, mine, above, heavier);
+            const bool counts_in = !by_count || above < tokens_left;
+            if (by_mass) {
+                u64 all_of = sh.everything;
+                if (by_count) {
+                    const u64 sum = warp_sum64(counts_in && lane % 4 == 0 && tid / 4 < m ? mass : 0);
+                    if (lane == 0 && sum) atomicAdd(&sh.list_counted, sum);
+                    __syncthreads();
+                    all_of += sh.list_counted;
+                }
+                share = sample_share(p.top_p, all_of, true);
+                if (counts_in && heavier + mass >= share && (!above || heavier < share)) atomicMin(&sh.found, mine);
+            } else if (above + 1 == tokens_left) {
+                atomicMin(&sh.found, mine);
+            }
+            __syncthreads();
+            cut = sh.found;
+        }
+        if (by_count && !at_once) cut = search_list(sh, token, w, counted, m, false, tokens_left, 0, 0);
+        if (by_mass && !at_once) {
             u64 all_of = sh.everything;
             if (by_count) {
                 u64 sum = 0;
@@ -1109,17 +1145,18 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 __syncthreads();
                 all_of += sh.list_counted;
             }
-            const u64 share = sample_share(p.top_p, all_of, true);
-            const u64 last = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
+            share = sample_share(p.top_p, all_of, true);
+            cut = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
+        }
+        if (by_mass) {
             // In top-p's bins, or the estimate was wrong.
-            const bool fine = (mass_from == 0 || sh.heavier < share) && last != ~0ull &&
-                              bins.of(token_logit(last)) <= mass_to;
+            const bool fine = (mass_from == 0 || sh.heavier < share) && cut != ~0ull &&
+                              bins.of(token_logit(cut)) <= mass_to;
             if (!fine) {  // the whole cluster alike
                 if (C > 1) cluster.barrier_wait();
                 sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
                 return;
             }
-            cut = last;
         }
         // What is kept of the list, by where it is.
         u64 sum = 0, ahead = 0;
