@@ -20,7 +20,7 @@
 // registers 222); over BF16 rows L2 (160 rows of 1280 rows, 8 KV heads: 111 us, 7.5 TB/s). With few items the chain of a
 // warp, 2 us a step, behind 3 us to the first rows and before 4 of joining (64 rows of 128 to 2048 byte rows, 2 KV heads:
 // 20 us; one row: 8). The same choice read by the decode kernel, a row a sequence, made whole calls of 298, 193 and 43 us
-// that take 247, 136 and 47 here: its line of equal stretches serves 64 unequal items better, its tiles of one row each the
+// that take 249, 131 and 47 here: its line of equal stretches serves 64 unequal items better, its tiles of one row each the
 // others worse.
 #pragma once
 #include "paged_decode.cuh"

@@ -186,8 +186,11 @@ ROTATIONS = [(None, None, 1e-6, 1e6, 128), ("w", "w", 1e-6, 1e6, 128), ("w", Non
 @KINDS
 @pytest.mark.parametrize("rotation", ROTATIONS, ids=range(len(ROTATIONS)))
 @pytest.mark.parametrize("shape", [(QWEN, 16, [1], [1]), (QWEN, 64, [1, 1, 1], [300, 31, 32768]), (ODD64, 7, [3, 0, 5, 17], [3, 9, 90, 400]),
-                                   (GROUP3, 24, [2, 9], [40, 9]), (MQA, 100, [130], [130]), (MHA64, 3, [33, 40], [100, 64])],
-                         ids=["first", "single", "ragged", "odd", "chunk", "small"])
+                                   (GROUP3, 24, [2, 9], [40, 9]), (MQA, 100, [130], [130]), (MHA64, 3, [33, 40], [100, 64]),
+                                   # rows enough for tiles of four: whole ones, and sequences that leave one to three
+                                   (QWEN, 16, [650, 2], [700, 900]), (ODD64, 7, [601, 1, 0, 6], [601, 40, 3, 90]),
+                                   (GROUP3, 24, [299, 303, 5], [400, 303, 5]), (MQA, 100, [700], [1000])],
+                         ids=["first", "single", "ragged", "odd", "chunk", "small", "tiles", "ragged-tiles", "odd-tiles", "chunk-tiles"])
 def test_rotated_rows_match_float64(kind, rotation, shape):
     heads, page, news, lengths = shape
     p = Served(kind, heads, page, news, lengths, seed=sum(lengths), gap=2)
@@ -222,12 +225,15 @@ def test_rotated_rows_match_float64(kind, rotation, shape):
 
 
 @KINDS
-def test_rotation_in_place(kind):
-    p = Served(kind, QWEN, 16, [5, 1, 40], [5, 900, 77], seed=2)
+@pytest.mark.parametrize("heads", [QWEN, GROUP3])
+@pytest.mark.parametrize("most", [40, 603])
+def test_rotation_in_place(kind, heads, most):
+    p = Served(kind, heads, 16, [5, 1, most], [5, 900, most + 37], seed=2)
     rng = np.random.default_rng(3)
-    x = rng.standard_normal((p.rows, 16 * 128)).astype(np.float32)
-    w = np.ones(128, np.float32)
-    turn = (w, w, 1e-6, 1e6, 128)
+    d = heads[2]
+    x = rng.standard_normal((p.rows, (heads[0] + 2 * heads[1]) * d)).astype(np.float32)
+    w = np.ones(d, np.float32)
+    turn = (w, w, 1e-6, 1e6, d)
     a = p.rotate(x, turn, pad=8)
     first = p.get()
     b = p.rotate(x, turn, inplace=True, pad=8)
@@ -256,8 +262,9 @@ def test_far_places(place):
 
 
 @KINDS
-def test_rotation_reports_what_it_cannot_store(kind):
-    p = Served(kind, QWEN, 16, [3, 2, 4], [40, 1, 4], seed=8)  # the second has a row at place -1
+@pytest.mark.parametrize("more", [[], [600]], ids=["few", "tiles"])
+def test_rotation_reports_what_it_cannot_store(kind, more):
+    p = Served(kind, QWEN, 16, [3, 2, 4] + more, [40, 1, 4] + more, seed=8)  # the second has a row at place -1
     p.table[0, 2] = p.pages  # places 32 .. 47 of the first
     p.put()
     x = np.random.default_rng(4).standard_normal((p.rows, 16 * 128)).astype(np.float32)
@@ -285,7 +292,7 @@ def test_rotation_reports_what_it_cannot_store(kind):
     assert np.all(val(0, 2, 1) == 0) or np.all(np.isfinite(val(0, 2, 1)))
     for kk in range(2):  # rows without a page went nowhere
         changed = np.argwhere((after[0][kk] != before[0][kk]).any(-1))
-        assert {int(c[0]) for c in changed} <= {int(p.table[1, 0]), int(p.table[2, 0])}
+        assert {int(c[0]) for c in changed} <= {int(p.table[1, 0]), int(p.table[2, 0]), *p.table[3:].reshape(-1).tolist()}
     p.free()
 
 
@@ -370,7 +377,9 @@ def test_bounds_pass_over_nan_and_report_bad_pages(kind):
 CHOICES = [(QWEN, 16, [1], [1], 4, 1, 1), (QWEN, 16, [1, 1, 1], [64, 65, 80], 4, 1, 2), (QWEN, 64, [1] * 4, [4000, 31, 1025, 64], 6, 1, 2),
            (ODD64, 24, [1, 3, 7], [900, 700, 7], 5, 0, 1), (GROUP4, 32, [5, 5], [900, 300], 9, 2, 2), (MQA, 1, [1, 2], [200, 33], 40, 3, 5),
            (MHA64, 7, [40, 1], [300, 129], 12, 1, 4), (GROUP3, 100, [1, 130], [2000, 1500], 4, 0, 4), (QWEN, 16, [1], [5000], 100, 1, 1),
-           (QWEN, 16, [200, 1], [333, 1000], 3, 1, 1), (QWEN, 48, [3], [2], 5, 1, 1), ((1, 1, 64), 16, [1], [20000], 1, 0, 1)]
+           (QWEN, 16, [200, 1], [333, 1000], 3, 1, 1), (QWEN, 48, [3], [2], 5, 1, 1), ((1, 1, 64), 16, [1], [20000], 1, 0, 1),
+           # rows enough to go in pairs, which sequences' ends part
+           (QWEN, 16, [299, 1, 4], [900, 333, 40], 5, 1, 1), (GROUP3, 24, [201], [1500], 6, 0, 2), (QWEN, 16, [300], [3000], 150, 2, 5)]
 
 
 @KINDS
