@@ -90,7 +90,7 @@ def build_oracle(verbose: bool = False) -> None:
     ref = os.environ.get("CMACHINE_REFERENCE")
     if ref:
         make.append(f"REF={ref}")
-    _run(make + ["liboracle.so", "libpaged_cpu.so"])
+    _run(make + ["liboracle.so", "libpaged_cpu.so", "libsample_cpu.so"])
     _run(make + ["ref-if-present"])
     if verbose:
         print("oracle built")

@@ -25,6 +25,7 @@
 // steps 2 and 4. A row's slices are as long as one another, so an SM with two CTAs is waited for by those with one.
 #include "common.cuh"
 #include "kernels.h"
+#include "sample_bins.h"
 #include "../../include/gpu.h"
 #include <cooperative_groups.h>
 #include <float.h>
@@ -38,7 +39,7 @@ namespace tcm {
 namespace {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleShifts = 256, kSampleBins = 4096, kSampleSlots = 8192, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = kSampleThreads / 4;
+constexpr int kSampleShifts = 256, kSampleList = 2048, kSlowBins = 1024, kSubBins = 256, kFew = kSampleThreads / 4;
 constexpr int kSampleVocab = 1 << 19, kSampleCluster = 16;
 constexpr int kSampleOwnSm = 180 * 1024, kSampleHalfSm = 76 * 1024;  // bytes of a slice in shared memory: one CTA an SM, two
 typedef unsigned long long u64;
@@ -167,34 +168,6 @@ struct SampleRow {
     }
 };
 
-// Bins of the logits: one of the first eight for the largest, and not falling as l falls; `last` for all that lie so many
-// bins lower, or lower. FP32 sums with kSampleRound are whole numbers, one to one with their bits;
-// they go to the nearest, and to even ones from between, so that bins are not off to one side of logits of 16 bits.
-constexpr float kSampleRound = 0x1.8p23f, kSampleReach = 0x1p19f;
-struct SampleBins {
-    float unit, origin, scale, least;
-    int top, last;
-    // Of equal width over [from, high]; what lies below `from` is the last but one at most.
-    __device__ SampleBins(float from, float high, int bins) : last(bins - 1) {
-        // Differences in a power of two at which neither they nor the scale leave FP32's range.
-        const float span = high - from;
-        unit = span > 1e30f ? 0.25f : span > 0.f && span < 1e-25f ? 0x1p100f : 1.f;
-        origin = high * unit;
-        scale = span > 0.f ? (float)(bins - 2) * 0.999999f / (origin - from * unit) : 0.f;
-        top = __float_as_int(kSampleRound);
-        least = kSampleRound - (float)last;
-    }
-    // Of a width given beforehand, 1 / scale, with borders that do not move with the row: slot() tells one of kSampleSlots in a
-    // circle without knowing `high`. |high * scale| is below kSampleReach.
-    static __device__ int slot(float l, float scale) { return __float_as_int(fmaf(l, scale, kSampleRound)) & (kSampleSlots - 1); }
-    __device__ SampleBins(float high, float scale_) : unit(1.f), origin(0.f), scale(scale_), last(kSampleBins - 1) {
-        top = __float_as_int(fmaf(high, scale, kSampleRound)) | 7;  // so that a thread's eight slots are two aligned quads
-        least = __int_as_float(top - last);
-    }
-    __device__ int of(float l) const { return top - __float_as_int(fmaxf(fmaf(fmaf(l, unit, -origin), scale, kSampleRound), least)); }
-    __device__ double width() const { return scale > 0.f ? 1.0 / ((double)scale * (double)unit) : 0.0; }  // a bin's
-};
-
 // A CTA's slice of the row: `off` elements behind a 16-byte boundary, in shared memory with -infinity around it, or where
 // it is in global memory, read again by every pass (from L2, mostly).
 template <bool RESIDENT> struct SampleLogits {
@@ -298,14 +271,14 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, SampleShared &sh
         float from = low < reach && reach < high ? reach : low;
         // A pass narrows the range a thousandfold, and FP32's spans less than 2^280: 64 are never reached.
         for (int pass = 0;; pass++) {
-            const SampleBins bins(from, high, kSlowBins);
+            const SampleBins bins = sample_bins_over(from, high, kSlowBins);
             auto open = [&](float l) { return l <= high && l >= low && l > floor; };
             __syncthreads();
             for (int i = tid; i < kSlowBins; i += kSampleThreads) mass[i] = 0, count[i] = 0;
             __syncthreads();
             for (int i = tid; i < n; i += kSampleThreads)
                 if (const float l = x.at(i); open(l)) {
-                    const int b = bins.of(l);
+                    const int b = sample_bin(&bins, l);
                     atomicAdd(&count[b], 1u);
                     atomicAdd(&mass[b], r.weight(l));
                 }
@@ -349,7 +322,7 @@ __device__ __noinline__ void sample_slowly(const SampleArgs &a, SampleShared &sh
             cut.weight = sh.slow_mass;
             float down = INFINITY, up = -INFINITY;
             for (int i = tid; i < n; i += kSampleThreads)
-                if (const float l = x.at(i); open(l) && bins.of(l) == bin) down = fminf(down, l), up = fmaxf(up, l);
+                if (const float l = x.at(i); open(l) && sample_bin(&bins, l) == bin) down = fminf(down, l), up = fmaxf(up, l);
             down = -warp_max(-down), up = warp_max(up);
             if (lane == 0) sh.warp_low[warp] = down, sh.warp_high[warp] = up;
             __syncthreads();
@@ -648,13 +621,13 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     __syncthreads();
     // Where cuts are asked for, tokens are counted as they come, in bins of a 128th of the temperature whose borders do not
     // depend on the row: a circle of 8192, as numbers of 16 bits where a slice has no more tokens than they count. Tokens
-    // that are masked with a large number, -1e4 or -FLT_MAX, are left out.
+    // that are masked with a large number, -1e4 or -FLT_MAX, are left out (sample_slots_hold() says when they may be).
     // Where they count more, the slice is not in shared memory, and the cluster's counts go to the ring.
     const bool packed = C > 1 && a.slice <= 0xffff;
     unsigned *own = reinterpret_cast<unsigned *>(sh.buffer[0]), *counts = RESIDENT || packed ? reinterpret_cast<unsigned *>(sh.buffer[1]) : reinterpret_cast<unsigned *>(slice_memory);
     const float fixed_scale = 128.f / p.temperature;
     const bool early = (p.top_k > 0 || p.top_p < 1.f) && fixed_scale > 0.f && fixed_scale < INFINITY;
-    const float fixed_floor = -kSampleReach / fixed_scale;
+    const float fixed_floor = sample_floor(fixed_scale);
     float most = -INFINITY, least_counted = INFINITY;
     bool bad = false;
     int live = 0, most_at = 0;  // for greedy rows: the first quad that has the largest
@@ -672,7 +645,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                     least_counted = fminf(least_counted, smallest);
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const int b = SampleBins::slot(l[k], fixed_scale);
+                        const int b = sample_slot(l[k], fixed_scale);
                         if constexpr (kPacked) atomicAdd(&own[b >> 1], b & 1 ? 0x10000u : 1u);
                         else atomicAdd(&own[b], 1u);
                     }
@@ -685,7 +658,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
                 live += l[k] > -INFINITY;
                 if constexpr (kEarly)
                     if (l[k] > floor) {
-                        const int b = SampleBins::slot(l[k], fixed_scale);
+                        const int b = sample_slot(l[k], fixed_scale);
                         least_counted = fminf(least_counted, l[k]);
                         atomicAdd(&own[kPacked ? b >> 1 : b], kPacked && b & 1 ? 0x10000u : 1u);
                     }
@@ -777,10 +750,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     // ---- the bins in which the cuts lie
     const bool by_count = p.top_k > 0 && p.top_k < all_live, by_mass = p.top_p < 1.f, cuts = by_count || by_mass;
     const float reach = (float)((double)high - 32.0 * (double)p.temperature);
-    SampleBins bins(high, fixed_scale);
-    // Counts of the first pass hold where the largest token is among them and no slot has two bins.
-    bool fixed = early && high > fixed_floor && fabsf(high) * fixed_scale < kSampleReach &&
-                 bins.top - __float_as_int(fmaf(low_counted, fixed_scale, kSampleRound)) < kSampleSlots;
+    SampleBins bins = sample_bins_of(high, fixed_scale);
+    bool fixed = early && sample_slots_hold(&bins, high, low_counted);
     int count_bin = kSampleBins, mass_from = kSampleBins, mass_to = -1;  // top-k's bin; top-p's, first and last
     int tokens_left = 0, in_count_bin = 0;                               // of top-k in its bin, and how many that has
     int listed = 0;
@@ -804,14 +775,14 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             if (C > 1) cluster.sync();
             else __syncthreads();
             for (int c = 0; c < C; c++) low = fminf(low, sh.ends[c].x);
-            bins = SampleBins(low < reach && reach < high ? reach : low, high, kSampleBins);
+            bins = sample_bins_over(low < reach && reach < high ? reach : low, high, kSampleBins);
             for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) reinterpret_cast<uint4 *>(own)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             each_quad<kSampleThreads>(x, ring, tid, quads, [&](int, const float4 &l) {
-                if (l.x > -INFINITY) atomicAdd(&own[bins.of(l.x)], 1u);
-                if (l.y > -INFINITY) atomicAdd(&own[bins.of(l.y)], 1u);
-                if (l.z > -INFINITY) atomicAdd(&own[bins.of(l.z)], 1u);
-                if (l.w > -INFINITY) atomicAdd(&own[bins.of(l.w)], 1u);
+                if (l.x > -INFINITY) atomicAdd(&own[sample_bin(&bins, l.x)], 1u);
+                if (l.y > -INFINITY) atomicAdd(&own[sample_bin(&bins, l.y)], 1u);
+                if (l.z > -INFINITY) atomicAdd(&own[sample_bin(&bins, l.z)], 1u);
+                if (l.w > -INFINITY) atomicAdd(&own[sample_bin(&bins, l.w)], 1u);
             });
             if (C > 1) cluster.sync();
             else __syncthreads();
@@ -838,7 +809,8 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         constexpr int each = kSampleBins / kSampleThreads;
         unsigned c[each], upto = 0;
         float mass[each], total = 0.f, squares = 0.f;
-        const float step = (float)(-bins.width() * r.slope);
+        // A bin's width, in powers of two of weight.
+        const float step = bins.scale > 0.f ? (float)(-r.slope / ((double)bins.scale * (double)bins.unit)) : 0.f;
         static_assert(each == 8, "two quads");
         const bool circle = C == 1 && fixed;  // in which bins go down
         const unsigned *from = C > 1 ? counts + tid * each : circle ? own + ((bins.top - tid * each - (each - 1)) & (kSampleSlots - 1)) : own + tid * each;
@@ -945,16 +917,16 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
     u64 sum_above = 0, sum_all = 0, sum_kept = 0;
     int kept = 0;
     if (cuts) {
-        // The bins' borders as logits: the least of a bin and those above it, found by trial as the arithmetic of bins.of()
+        // The bins' borders as logits: the least of a bin and those above it, found by trial as the arithmetic of sample_bin(&bins, )
         // has it. Tokens from `sure` on are above the bins in question and kept; from `in_from` down to `in_to` in top-p's,
         // from `count_from` down to `count_to` in top-k's.
         if (warp < 4) {  // a warp a border: 32 numbers at a time cut the range into 33
             const int b = warp == 0 ? (by_mass || all_listed ? mass_from : count_bin) - 1 : warp == 1 ? mass_to : warp == 2 ? count_bin - 1 : count_bin;
-            uint32_t down = sample_key(-FLT_MAX), up = sample_key(high);  // bins.of(up) <= b, or none is
-            if (b < bins.of(high)) down = up = sample_key(INFINITY);
+            uint32_t down = sample_key(-FLT_MAX), up = sample_key(high);  // sample_bin(&bins, up) <= b, or none is
+            if (b < sample_bin(&bins, high)) down = up = sample_key(INFINITY);
             while (down < up) {
                 const uint32_t step = (up - down) / 33 + 1, at = up - down > (lane + 1) * step ? up - (lane + 1) * step : down;
-                const unsigned in = __ballot_sync(0xffffffffu, bins.of(sample_value(at)) <= b);  // the first lanes
+                const unsigned in = __ballot_sync(0xffffffffu, sample_bin(&bins, sample_value(at)) <= b);  // the first lanes
                 const uint32_t most = up - down, passed = __popc(in);
                 up = most > passed * step ? up - passed * step : down;
                 if (passed < 32) down = most > (passed + 1) * step ? up - step + 1 : down + 1;
@@ -1095,7 +1067,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             if (k * kSampleThreads + warp * 32 >= m) continue;
             const float l = token_logit(token[k]);
             w[k] = member[k] ? r.weight(l) : 0;
-            counted[k] = member[k] && by_count && bins.of(l) <= count_bin && (all_listed || bins.of(l) == count_bin);
+            counted[k] = member[k] && by_count && sample_bin(&bins, l) <= count_bin && (all_listed || sample_bin(&bins, l) == count_bin);
         }
         if (C > 1) cluster.barrier_arrive();  // the others' lists have been read; a CTA leaves when its own has
         cut = ~0ull;
@@ -1151,7 +1123,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         if (by_mass) {
             // In top-p's bins, or the estimate was wrong.
             const bool fine = (mass_from == 0 || sh.heavier < share) && cut != ~0ull &&
-                              bins.of(token_logit(cut)) <= mass_to;
+                              sample_bin(&bins, token_logit(cut)) <= mass_to;
             if (!fine) {  // the whole cluster alike
                 if (C > 1) cluster.barrier_wait();
                 sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
