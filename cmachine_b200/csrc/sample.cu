@@ -93,7 +93,7 @@ struct SampleShared {
     uint32_t sub_least, sub_most;
     int sub_bin, sub_above, few_count;
     float border[4];
-    int list_start[kSampleCluster];
+    int list_start[kSampleCluster], list_total;
     u64 slow_mass;
 };
 
@@ -935,7 +935,11 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         }
         __syncthreads();
         const float sure = sh.border[0], in_to = by_mass || all_listed ? sh.border[1] : INFINITY;
-        auto append = [&](float l, int i) { own_list[atomicAdd(&sh.listed, 1)] = ((u64)~sample_key(l) << kIdBits) | (unsigned)(base + i); };
+        // As many as the bins counted; whatever they counted, no more than there is room for.
+        auto append = [&](float l, int i) {
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < kSampleList) own_list[at] = ((u64)~sample_key(l) << kIdBits) | (unsigned)(base + i);
+        };
         // Lists those of a quad that `in` marks.
         auto append_some = [&](int q, const float (&l)[4], auto in) {
             if (in(l[0]) | in(l[1]) | in(l[2]) | in(l[3]))
@@ -1022,7 +1026,7 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
         if (by_mass) z.all = warp_sum64(z.all), z.above = warp_sum64(z.above);
         z.kept = warp_sum64(z.kept);
         z.kept_count = __reduce_add_sync(0xffffffffu, z.kept_count);
-        z.listed = sh.listed;
+        z.listed = min(sh.listed, kSampleList);
         if (lane < C) cluster.map_shared_rank(sh.sums, lane)[rank] = z;
     }
     cluster.sync();
@@ -1040,13 +1044,14 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             if (lane >= o) upto += y;
         }
         if (lane < C) sh.list_start[lane] = upto - z.listed;
+        if (lane == C - 1) sh.list_total = upto;
     }
     if (lane == 0) sh.warp_more[warp] = 0;
     // ---- the cut in the cluster's list
     u64 cut = 0;
     if (cuts) {
-        const int m = listed;
         __syncthreads();
+        const int m = min(listed, sh.list_total);  // tokens that are there, so each once: the search ends
         u64 token[kEach], w[kEach];
         bool member[kEach], counted[kEach];
 #pragma unroll
@@ -1120,15 +1125,12 @@ template <bool RESIDENT> __global__ void __launch_bounds__(kSampleThreads, 2) sa
             share = sample_share(p.top_p, all_of, true);
             cut = search_list(sh, token, w, member, m, true, 0, share, sh.heavier);
         }
-        if (by_mass) {
-            // In top-p's bins, or the estimate was wrong.
-            const bool fine = (mass_from == 0 || sh.heavier < share) && cut != ~0ull &&
-                              sample_bin(&bins, token_logit(cut)) <= mass_to;
-            if (!fine) {  // the whole cluster alike
-                if (C > 1) cluster.barrier_wait();
-                sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
-                return;
-            }
+        // There is one, top-p's in its bins, or the estimate or the counts were wrong.
+        const bool fine = cut != ~0ull && (!by_mass || ((mass_from == 0 || sh.heavier < share) && sample_bin(&bins, token_logit(cut)) <= mass_to));
+        if (!fine) {  // the whole cluster alike
+            if (C > 1) cluster.barrier_wait();
+            sample_slowly<RESIDENT>(a, sh, slice_memory, row, high, all_live, min_logit);
+            return;
         }
         // What is kept of the list, by where it is.
         u64 sum = 0, ahead = 0;
