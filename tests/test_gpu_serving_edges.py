@@ -62,3 +62,34 @@ def test_queries_and_bounds_that_are_not_finite(kind, value, bound):
             w = which[r, h]
             assert np.all(np.diff(w) > 0) and w[0] == 0 and w[-1] == at // 16 and w[-2] == at // 16 - 1
     p.free()
+
+
+@KINDS
+@pytest.mark.parametrize("most", [4, 640], ids=["single", "tiles"])
+@pytest.mark.parametrize("which", ["key", "value"])
+def test_a_row_that_its_rotation_takes_out_of_range_is_zeros(kind, most, which):
+    """3.4e38 (cos 2 - sin 2) = -4.5e38, beyond FP32: the only row of the batch that cannot be stored. As a value it is not
+    rotated: bytes hold it, and BF16 does not (3.4e38 is above 2^128 - 2^119)."""
+    p = Served(kind, QWEN, 16, [most], [most], seed=33)
+    rng = np.random.default_rng(4)
+    x = (1 + rng.random((p.rows, 16 * 128))).astype(np.float32)
+    row, head = int(p.starts[0]) + 2, 13 if which == "key" else 15
+    x[row, head * 128:(head + 1) * 128] = 3.4e38
+    p.rotate(x, (None, None, 1e-6, 1e6, 128))
+    side = 0 if which == "key" else 1
+    lost = which == "key" or kind != BYTES
+    assert p.flags() == (1 if lost else 0)
+    host, scales = p.get()
+    page = int(p.table[0, 0])
+    stored = host[side][page, :, 2]  # the row's two heads
+    stored = stored.astype(np.float64) * scales[side][page, :, 2, None] if kind == BYTES else widen(stored)
+    assert np.all(stored[0] != 0) if which == "value" else np.any(stored[0] != 0)
+    if lost:
+        assert np.all(stored[1] == 0)
+        if kind == BYTES:
+            assert scales[side][page, 1, 2] == 1
+    else:
+        assert np.all(np.abs(stored[1] / float(np.float32(3.4e38)) - 1) <= 2.0**-22)
+    for j in (1, 3):  # the rows beside it
+        assert np.any(host[side][page, 1, j] != 0)
+    p.free()
