@@ -9,7 +9,7 @@
 // 64-bit: the choice of pages (paged_sparse.cu) and the codes of a stored row go by values next to borders.
 //
 // What bounds it: 21,149 rows of 12 query heads and 2 of keys and of values, byte rows, take 78 us, their bytes 48: 160
-// instructions a head's row (24 of them FP64, 8 conversions), at 60 % of the issue slots. Without norm and rotation it is
+// instructions a head's row (24 of them FP64, 8 conversions), at 64 % of the issue slots. Without norm and rotation it is
 // 51. With eight rows a tile and 24 warps an SM it took 92, without the prefetch 83, at 9 or 10 CTAs an SM, in fewer
 // registers, 81 and 86. A single token takes 5 us, of which 3 are its sequence's extent, its page and the row one after another.
 #include "paged_host.cuh"

@@ -11,7 +11,8 @@ Stored rows are the codec's of the FP32 row, checked bit for bit through gpu_pag
 
 Bounds and the choice of pages are exact: the oracle's scores are 64-bit sums in another order, and a choice between
 scores closer than 2^-40 of their terms' sum would be reported as a tie of the test's own making (none is).
-The attention over what was chosen is held to the bound of test_gpu_paged.py, whose kernel does it.
+The attention over what was chosen is held to the bound of test_gpu_paged.py: a kernel of its own does it, with the parts
+and sums of that file's few-row kernel.
 """
 import numpy as np
 import pytest
